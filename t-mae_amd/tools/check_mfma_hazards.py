@@ -139,7 +139,8 @@ def _per_file_flags(hip_file):
     spec = importlib.util.spec_from_file_location('_tmae_build', os.path.join(PKG, 'build.py'))
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)
-    return list(mod.PER_FILE_FLAGS.get(os.path.basename(hip_file), []))
+    feature = mod.FLAGS.index('-target-feature')                # ... and without packed float32, as the build compiles
+    return mod.FLAGS[feature - 1:feature + 3] + list(mod.PER_FILE_FLAGS.get(os.path.basename(hip_file), []))
 
 
 def compile_to_asm(hip_file, out_file):
