@@ -40,7 +40,7 @@ extern "C" {
  * entry point does with its arguments; tmae_abi_hash() is the fingerprint of THIS header's prototypes (name, return class and
  * argument classes in order: tmae_amd/_abi.py) that the build compiled in.  The Python binding compares both at import, so a
  * stale library, or a binding row that disagrees with its prototype, fails there and not inside a launch. */
-#define TMAE_ABI_VERSION 25
+#define TMAE_ABI_VERSION 26
 int tmae_abi_version(void);
 int tmae_abi_hash(void);
 
@@ -612,6 +612,29 @@ int tmae_frame_prepare_boxes(const float* points, int row, int64_t n, const doub
                              int flip_x, int flip_y, float cosa, float sina, float scale, float xmin, float ymin, float xmax,
                              float ymax, int batch_idx, const double* remove_boxes, int n_boxes, float* out, int32_t* count,
                              void* ws, size_t ws_bytes, void* stream);
+
+/* ---- rotary positions with several axes; norms of queries and keys for each head with the rotation in the same pass -----------
+ * x [n, h, dh] (row pitch ldx, head pitch hpx, in elements; channels contiguous), y / dy / dx contiguous [n, h, dh].  Channel pair i
+ * < P = sum of `sections` (host array of `axes` <= 4 counts, 2 P <= dh <= 512) turns by theta = positions[n, axis(i)] * inv_freq[i]
+ * (inv_freq [P] float64, the product and its reduction in float64): pair i = channels (2i, 2i+1) if `interleaved`, else (i, i + P);
+ * axis(i) by the sections in order; channels >= 2 P pass.  positions [n, axes] with row pitch ldpos: pos_kind 0 int32, 1 int64,
+ * 2 float32.  inverse: by -theta (the gradient of the rotation).  x and y do not overlap. */
+int tmae_rotary_axes(const void* x, int64_t ldx, int64_t hpx, int dtype, int64_t n, int h, int dh, const void* positions, int pos_kind,
+                     int64_t ldpos, const double* inv_freq, const int32_t* sections, int axes, int interleaved, int inverse, void* y,
+                     void* stream);
+/* y = rotate(gain * x rsqrt(mean_c x^2 + eps)): the first q_heads heads with q_gain, the others with k_gain (float32 [dh], or
+ * [heads of the side, dh] with gain_per_head; NULL: no gain). */
+int tmae_qk_norm_rotary_fwd(const void* x, int64_t ldx, int64_t hpx, int dtype, int64_t n, int h, int q_heads, int dh,
+                            const float* q_gain, const float* k_gain, int gain_per_head, float eps, const void* positions, int pos_kind,
+                            int64_t ldpos, const double* inv_freq, const int32_t* sections, int axes, int interleaved, void* y,
+                            void* stream);
+/* dx, and the gradients of the gains (shapes of the gains; NULL: not wanted; both NULL: no workspace is needed).  The gradients are
+ * summed in a fixed order.  pairs = P. */
+size_t tmae_qk_norm_rotary_bwd_workspace(int64_t n, int h, int dh, int pairs, int gain_per_head);
+int tmae_qk_norm_rotary_bwd(const void* x, int64_t ldx, int64_t hpx, const void* dy, int dtype, int64_t n, int h, int q_heads, int dh,
+                            const float* q_gain, const float* k_gain, int gain_per_head, float eps, const void* positions, int pos_kind,
+                            int64_t ldpos, const double* inv_freq, const int32_t* sections, int axes, int interleaved, void* dx,
+                            float* dq_gain, float* dk_gain, void* ws, size_t ws_bytes, void* stream);
 
 /* ---- box calibration probes (bench.py `peak_measured`; SURVEY.md section 7: measured achievable peaks on the box next
  * to the spec peaks -- no reference counterpart).  tmae_probe_copy: a 16-bytes-per-lane streaming copy of `bytes` (a

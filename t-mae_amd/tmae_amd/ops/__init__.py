@@ -5,6 +5,7 @@ pytorch3d -- same argument meaning, but every call lands in a han
 No tensor math happens here besides allocation and dense GEMMs handed to hipBLASLt via torch.
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .._lib import lib, check, PinnedStager
@@ -1750,6 +1751,188 @@ class _WinAttn(torch.autograd.Function):
 def win_attn(a, b, c, tau, grid_q, grid_k, nhead, batch, ny, nx, do_shift, tau_min, worklist=None, covered=False):
     """covered: see _WinAttn.forward (cross attention with a work list: zero only the orphan rows)."""
     return _WinAttn.apply(a, b, c, tau, grid_q, grid_k, worklist, nhead, batch, ny, nx, do_shift, tau_min, bool(covered))
+
+
+# ----------------------------------------------------------------------------- rotary positions, q / k norms
+
+class _Launch:
+    """The device and stream a call on `t` launches on: the tensors' own device, that device's current stream."""
+    __slots__ = ('dev', 'prev')
+
+    def __init__(self, t):
+        self.dev = t.device.index
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.dev:
+            torch.cuda.set_device(self.dev)
+        return _s()
+
+    def __exit__(self, *exc):
+        if self.prev != self.dev:
+            torch.cuda.set_device(self.prev)
+
+
+def _grad_on(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+_POS_KIND = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+def rotary_freqs(sections, base=10000.0, device=None):
+    """[sum(sections)] float64: every axis has a ladder of frequencies of its own, base ** (-j / p) for the j-th of its p channel
+    pairs."""
+    if not sections or any(int(p) < 1 for p in sections) or not float(base) > 0.0:
+        raise ValueError(f'rotary_freqs: sections {tuple(sections)}, base {base}')
+    return torch.cat([float(base) ** (-torch.arange(int(p), dtype=torch.float64) / int(p)) for p in sections]).to(device)
+
+
+def _rotary_args(name, x, positions, inv_freq, sections):
+    """Checks the arguments the two rotary operators share; returns (x, positions, inv_freq, C array of the sections, P)."""
+    import ctypes as C
+    if x.dim() != 3:
+        raise ValueError(f'{name}: x [tokens, heads, channels] expected, got {tuple(x.shape)}')
+    _dt(x)
+    n, h, dh = x.shape
+    sections = tuple(int(p) for p in sections)
+    P = sum(sections)
+    if not 1 <= len(sections) <= 4 or min(sections) < 1 or 2 * P > dh or dh > 512 or not 1 <= h <= 65535:
+        raise ValueError(f'{name}: sections {sections} for {h} heads of {dh} channels (1 to 4 axes, at most {dh // 2} pairs, at most '
+                         f'512 channels)')
+    if tuple(positions.shape) != (n, len(sections)):
+        raise ValueError(f'{name}: positions {tuple(positions.shape)}, expected {(n, len(sections))}')
+    if positions.dtype not in _POS_KIND:
+        raise TypeError(f'{name}: positions are int32, int64 or float32, got {positions.dtype}')
+    if inv_freq.dtype != torch.float64 or tuple(inv_freq.shape) != (P,):
+        raise ValueError(f'{name}: inv_freq [{P}] float64 expected, got {tuple(inv_freq.shape)} {inv_freq.dtype}')
+    if positions.device != x.device or inv_freq.device != x.device:
+        raise ValueError(f'{name}: x on {x.device}, positions on {positions.device}, inv_freq on {inv_freq.device}')
+    if positions.requires_grad or inv_freq.requires_grad:
+        raise ValueError(f'{name}: positions and inv_freq have no gradient')
+    if x.stride(2) != 1 and dh > 1:
+        x = x.contiguous()
+    if positions.stride(1) != 1 and len(sections) > 1 or positions.stride(0) < len(sections):
+        positions = positions.contiguous()
+    return x, positions, inv_freq.contiguous(), (C.c_int32 * len(sections))(*sections), P
+
+
+def _rotary_launch(x, positions, inv_freq, arr, interleaved, inverse):
+    n, h, dh = x.shape
+    y = torch.empty((n, h, dh), dtype=x.dtype, device=x.device)
+    with _Launch(x) as s:
+        check(lib.tmae_rotary_axes(_p(x), x.stride(0), x.stride(1), _dt(x), n, h, dh, _p(positions), _POS_KIND[positions.dtype],
+                                   positions.stride(0), _p(inv_freq), arr, len(arr), interleaved, inverse, _p(y), s),
+              'tmae_rotary_axes')
+    return y
+
+
+class _RotaryAxes(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, inv_freq, arr, interleaved, inverse):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.meta = (arr, interleaved, inverse)
+        return _rotary_launch(x, positions, inv_freq, arr, interleaved, inverse)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        positions, inv_freq = ctx.saved_tensors
+        arr, interleaved, inverse = ctx.meta
+        if dy.stride(2) != 1 and dy.shape[2] > 1:
+            dy = dy.contiguous()
+        return _rotary_launch(dy, positions, inv_freq, arr, interleaved, 1 - inverse), None, None, None, None, None
+
+
+def rotary_axes(x, positions, inv_freq, sections, interleaved=False, inverse=False):
+    """Turns the heads of x [tokens, heads, channels] (float32 / bfloat16, any token and head pitch: a slice of a packed projection
+    will do) by the tokens' positions on several axes, e.g. (time, y, x): returns a contiguous tensor of x's type.
+
+    Channel pair i < P = sum(sections) turns by positions[:, axis(i)] * inv_freq[i]; the first sections[0] pairs belong to axis 0
+    and so on.  Pair i is channels (2i, 2i+1) if `interleaved`, else (i, i + P); channels from 2 P on pass unchanged.
+    positions [tokens, len(sections)] int32 / int64 / float32, inv_freq [P] float64 (rotary_freqs).  inverse: turns back."""
+    x, positions, inv_freq, arr, _ = _rotary_args('rotary_axes', x, positions, inv_freq, sections)
+    _need_cuda(x)
+    if _grad_on(x):
+        return _RotaryAxes.apply(x, positions, inv_freq, arr, int(bool(interleaved)), int(bool(inverse)))
+    return _rotary_launch(x, positions, inv_freq, arr, int(bool(interleaved)), int(bool(inverse)))
+
+
+def _qk_norm_launch(x, q_gain, k_gain, positions, inv_freq, arr, q_heads, per_head, eps, interleaved):
+    n, h, dh = x.shape
+    y = torch.empty((n, h, dh), dtype=x.dtype, device=x.device)
+    with _Launch(x) as s:
+        check(lib.tmae_qk_norm_rotary_fwd(_p(x), x.stride(0), x.stride(1), _dt(x), n, h, q_heads, dh, _p(q_gain), _p(k_gain), per_head,
+                                          eps, _p(positions), _POS_KIND[positions.dtype], positions.stride(0), _p(inv_freq), arr,
+                                          len(arr), interleaved, _p(y), s), 'tmae_qk_norm_rotary_fwd')
+    return y
+
+
+class _QkNormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, q_gain, k_gain, positions, inv_freq, arr, pairs, q_heads, per_head, eps, interleaved):
+        ctx.save_for_backward(x, q_gain, k_gain, positions, inv_freq)
+        ctx.meta = (arr, pairs, q_heads, per_head, eps, interleaved)
+        return _qk_norm_launch(x, q_gain, k_gain, positions, inv_freq, arr, q_heads, per_head, eps, interleaved)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, q_gain, k_gain, positions, inv_freq = ctx.saved_tensors
+        arr, pairs, q_heads, per_head, eps, interleaved = ctx.meta
+        n, h, dh = x.shape
+        dy = dy.contiguous()
+        dx = torch.empty((n, h, dh), dtype=x.dtype, device=x.device)
+        dq = torch.empty_like(q_gain) if q_gain is not None and ctx.needs_input_grad[1] else None
+        dk = torch.empty_like(k_gain) if k_gain is not None and ctx.needs_input_grad[2] else None
+        ws, wsb = None, 0
+        if dq is not None or dk is not None:
+            wsb = lib.tmae_qk_norm_rotary_bwd_workspace(n, h, dh, pairs, per_head)
+            ws = _ws(wsb, x.device)
+        with _Launch(x) as s:
+            check(lib.tmae_qk_norm_rotary_bwd(_p(x), x.stride(0), x.stride(1), _p(dy), _dt(x), n, h, q_heads, dh, _p(q_gain), _p(k_gain),
+                                              per_head, eps, _p(positions), _POS_KIND[positions.dtype], positions.stride(0),
+                                              _p(inv_freq), arr, len(arr), interleaved, _p(dx), _p(dq), _p(dk), _p(ws), wsb, s),
+                  'tmae_qk_norm_rotary_bwd')
+        return dx, dq, dk, None, None, None, None, None, None, None, None
+
+
+def qk_norm_rotary(x, q_gain, k_gain, positions, inv_freq, sections, q_heads=None, eps=1e-6, interleaved=False):
+    """The norm of every head of x [tokens, heads, channels] and the rotation of rotary_axes in one pass:
+    rotate(gain * x * rsqrt(mean(x^2) + eps)), statistics in float32, one rounding to x's type.
+
+    The first q_heads heads are queries (q_gain), the others keys (k_gain); q_heads defaults to half of them, or to all of them where
+    k_gain is None (one side alone: queries and keys of different tokens).  A gain is float32 [channels], one for all heads of its
+    side, or [heads of the side, channels] (both sides alike); None: no gain."""
+    name = 'qk_norm_rotary'
+    x, positions, inv_freq, arr, pairs = _rotary_args(name, x, positions, inv_freq, sections)
+    h, dh = x.shape[1], x.shape[2]
+    if q_heads is None:
+        if k_gain is not None and h % 2:
+            raise ValueError(f'{name}: q_heads is needed for {h} heads')
+        q_heads = h if k_gain is None else h // 2
+    q_heads = int(q_heads)
+    if not 0 <= q_heads <= h:
+        raise ValueError(f'{name}: q_heads {q_heads} of {h} heads')
+    if not 0.0 <= float(eps) < float('inf'):
+        raise ValueError(f'{name}: eps {eps}')
+    per_head = {g.dim() for g in (q_gain, k_gain) if g is not None}
+    if len(per_head) > 1:
+        raise ValueError(f'{name}: gains of one kind, [channels] or [heads, channels], for both sides')
+    per_head = int(per_head == {2})
+    gains = []
+    for side, gain, heads in (('q_gain', q_gain, q_heads), ('k_gain', k_gain, h - q_heads)):
+        if gain is not None:
+            if gain.dtype != torch.float32 or gain.device != x.device:
+                raise TypeError(f'{name}: {side} is float32 on {x.device}, got {gain.dtype} on {gain.device}')
+            if tuple(gain.shape) != ((heads, dh) if per_head else (dh,)):
+                raise ValueError(f'{name}: {side} {tuple(gain.shape)} for {heads} heads of {dh} channels')
+            gain = gain.contiguous()
+        gains.append(gain)
+    _need_cuda(x)
+    if _grad_on(x, *gains):
+        return _QkNormRotary.apply(x, *gains, positions, inv_freq, arr, pairs, q_heads, per_head, float(eps), int(bool(interleaved)))
+    return _qk_norm_launch(x, *gains, positions, inv_freq, arr, q_heads, per_head, float(eps), int(bool(interleaved)))
 
 
 # ----------------------------------------------------------------------------- sparse conv (A9)
