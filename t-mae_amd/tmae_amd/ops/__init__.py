@@ -1935,6 +1935,93 @@ def qk_norm_rotary(x, q_gain, k_gain, positions, inv_freq, sections, q_heads=Non
     return _qk_norm_launch(x, *gains, positions, inv_freq, arr, q_heads, per_head, float(eps), int(bool(interleaved)))
 
 
+class _WinAttnDot(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, a, b, c, grid_q, grid_k, worklist, meta):
+        out, lse = _win_attn_dot_launch(a, b, c, grid_q, grid_k, worklist, meta)
+        ctx.save_for_backward(a, b, c if torch.is_tensor(c) else None, grid_q, grid_k, worklist, lse)
+        ctx.meta, ctx.packed_kv = meta, isinstance(c, str)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        a, b, c, grid_q, grid_k, worklist, lse = ctx.saved_tensors
+        c = 'kv' if ctx.packed_kv else c
+        d, nhead, batch, ny, nx, do_shift, scale, covered = ctx.meta
+        mq, mk = a.shape[0], (a if b is None else b).shape[0]
+        dout = dout.contiguous()
+        alloc = torch.empty_like if covered else torch.zeros_like
+        da = alloc(a)
+        db = alloc(b) if b is not None else None
+        dc = alloc(c) if torch.is_tensor(c) else c
+        dq, lddq, dk, lddk, dv, lddv = _WinAttn._ptrs(da, db, dc, d)
+        with _Launch(a) as s:
+            check(lib.tmae_win_attn_dot_bwd(*_WinAttn._ptrs(a, b, c, d), _p(dout), d, _p(lse), _dt(a), mq, mk, nhead, d // nhead,
+                                            _p(grid_q), _p(grid_k), batch, ny, nx, do_shift, scale, dq, lddq, dk, lddk, dv, lddv,
+                                            _p(worklist), s), 'tmae_win_attn_dot_bwd')
+        return da, db, (dc if torch.is_tensor(dc) else None), None, None, None, None
+
+
+def _win_attn_dot_launch(a, b, c, grid_q, grid_k, worklist, meta):
+    d, nhead, batch, ny, nx, do_shift, scale, covered = meta
+    mq, mk = a.shape[0], (a if b is None else b).shape[0]
+    out = (torch.empty if covered else torch.zeros)((mq, d), dtype=a.dtype, device=a.device)
+    lse = torch.empty((mq, nhead), dtype=torch.float32, device=a.device)        # read back in the windows that wrote it only
+    with _Launch(a) as s:
+        check(lib.tmae_win_attn_dot_fwd(*_WinAttn._ptrs(a, b, c, d), _dt(a), mq, mk, nhead, d // nhead, _p(grid_q), _p(grid_k), batch,
+                                        ny, nx, do_shift, scale, _p(out), d, _p(lse), _p(worklist), s), 'tmae_win_attn_dot_fwd')
+    return out, lse
+
+
+def win_attn_dot(a, b, c, grid_q, grid_k, nhead, batch, ny, nx, do_shift, scale=None, worklist=None, covered=False):
+    """Scaled-dot-product attention inside the 8x8 windows of win_attn, over projected rows (float32 / bfloat16) in its layouts:
+    a = packed [m, 3 d] (q|k|v), b and c None; a = packed [m, 2 d] (q|k), b = v [m, d], c None; a = q [mq, d], b = k and c = v [mk, d];
+    a = q, b = packed [mk, 2 d] (k|v), c = 'kv'.  Heads of 16, 32 or 64 channels, any number of them; the logits are scale * q . k
+    (default: channels ** -0.5).  Queries whose window holds no key get zero rows.
+
+    grid_q, grid_k [batch * ny * nx] int32: row numbers of the queries and keys, -1 where a cell is empty (index_grid); a row stands
+    in one cell.  worklist: window_worklist of the same grids and shift; without one every window is visited.  covered: the caller's
+    promise that every row stands in the grids -- without it the results start from zeros and the others stay zero."""
+    name = 'win_attn_dot'
+    layout = 'qkv' if b is None else 'qk_v' if c is None else 'q_kv' if isinstance(c, str) else 'q_k_v'
+    if (b is None and c is not None) or (layout == 'q_kv' and c != 'kv'):
+        raise ValueError(f'{name}: a, b and c are (q|k|v), (q|k, v), (q, k, v) or (q, k|v, "kv")')
+    tensors = [t for t in (a, b, c) if torch.is_tensor(t)]
+    if any(t.dim() != 2 or t.dtype != a.dtype or t.device != a.device for t in tensors):
+        raise ValueError(f'{name}: rows of one type on one device expected, got '
+                         f'{[(tuple(t.shape), t.dtype, str(t.device)) for t in tensors]}')
+    _dt(a)
+    d = a.shape[1] // {'qkv': 3, 'qk_v': 2}.get(layout, 1)
+    want = {'qkv': (3 * d,), 'qk_v': (2 * d, d), 'q_kv': (d, 2 * d), 'q_k_v': (d, d, d)}[layout]
+    if tuple(t.shape[1] for t in tensors) != want or (layout == 'qk_v' and a.shape[0] != b.shape[0]) or \
+            (layout == 'q_k_v' and b.shape[0] != c.shape[0]):
+        raise ValueError(f'{name}: {[tuple(t.shape) for t in tensors]} are not the rows of {layout}')
+    nhead, batch, ny, nx = int(nhead), int(batch), int(ny), int(nx)
+    if nhead < 1 or nhead > 4096 or d not in (16 * nhead, 32 * nhead, 64 * nhead):
+        raise ValueError(f'{name}: {d} channels for {nhead} heads; heads have 16, 32 or 64')
+    scale = float((d // nhead) ** -0.5 if scale is None else scale)
+    if not 0.0 < scale <= 3e38:
+        raise ValueError(f'{name}: scale {scale}')
+    if batch < 1 or ny < 1 or nx < 1 or batch * ny * nx >= 1 << 31 or max(t.shape[0] for t in tensors) >= 1 << 31:
+        raise ValueError(f'{name}: batch {batch}, grid {ny} x {nx}')
+    for g, what in ((grid_q, 'grid_q'), (grid_k, 'grid_k')):
+        if g.dtype != torch.int32 or g.numel() != batch * ny * nx or not g.is_contiguous() or g.device != a.device:
+            raise ValueError(f'{name}: {what} [{batch * ny * nx}] int32 on {a.device} expected, got {tuple(g.shape)} {g.dtype} on {g.device}')
+    if worklist is not None:
+        if worklist.dtype != torch.int32 or not worklist.is_contiguous() or worklist.device != a.device or \
+                worklist.numel() != lib.tmae_window_worklist_size(batch, ny, nx):
+            raise ValueError(f'{name}: the work list is not one of {batch} grids of {ny} x {nx}')
+    _need_cuda(a)
+    a = a.contiguous()
+    b = None if b is None else b.contiguous()
+    c = c.contiguous() if torch.is_tensor(c) else c
+    meta = (d, nhead, batch, ny, nx, 1 if do_shift else 0, scale, bool(covered))
+    if _grad_on(*tensors):
+        return _WinAttnDot.apply(a, b, c, grid_q, grid_k, worklist, meta)
+    return _win_attn_dot_launch(a, b, c, grid_q, grid_k, worklist, meta)[0]
+
+
 # ----------------------------------------------------------------------------- sparse conv (A9)
 
 def spconv_down_outputs(grid_in, batch, ny, nx):

@@ -1,0 +1,336 @@
+"""Scaled-dot-product attention inside 8x8 windows (ops.win_attn_dot) against the definition in 64 bits, and the chain
+q/k norms + rotation -> attention as an encoder layer runs it.
+
+Tolerances (u = 2^-24, e = eps / 2 of the stored type, bf16 2^-8; T = 64 tokens of a window at most).  Per query, A = the largest
+scale * sum |q_c k_c| of its keys:
+ * a logit is off by (dh + 4) u A; the exponent's argument and the saved logarithm round once more each (of a size up to A + 6): a
+   probability is off by rho = 2 (dh + 8) u (A + 6) + (T + 16) u of itself, and by e more where it is rounded to the type for a product;
+ * out: (rho + e + 4 T u) sum_j P |v| + e |out|;          dv: the same with sum_i P |dO|;
+ * dS = scale P (dP - D), with G = sum |dO v| per pair and Dm = sum_j P G: off by
+   eta = (2 rho + (dh + T + 8) u + e) scale P (G + Dm);    dq: sum_j (eta + T u |dS|) |k| + e |dq|;    dk: sum_i of the same with |q|."""
+import ctypes
+
+import pytest
+import torch
+
+U = 2.0 ** -24
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2 if dtype == torch.bfloat16 else 0.0
+
+
+def within(got, want, tol, what):
+    got = got.detach().double().cpu()
+    assert torch.isfinite(want).all() and torch.isfinite(got).all(), what
+    bad = ~((got - want).abs() <= tol + 1e-37)
+    assert not bad.any(), f'{what}: {int(bad.sum())} of {bad.numel()}, worst {((got - want).abs() / tol.clamp_min(1e-300)).max():.3g} of the tolerance'
+
+
+def place(counts, batch, ny, nx, g, shuffle=False):
+    """counts: occupied cells of every frame -> the grid (-1: empty), and each row's (frame, y, x)"""
+    grid = torch.full((batch, ny * nx), -1, dtype=torch.int32)
+    cells = [torch.randperm(ny * nx, generator=g)[:c].sort().values for c in counts]
+    flat = torch.cat([c + b * ny * nx for b, c in enumerate(cells)])
+    rows = torch.randperm(flat.numel(), generator=g) if shuffle else torch.arange(flat.numel())
+    grid.view(-1)[flat] = rows.int()
+    at = torch.empty_like(flat)
+    at[rows] = flat
+    return grid.view(-1), torch.stack([at // (ny * nx), at % (ny * nx) // nx, at % nx], 1)
+
+
+def window_of(at, shift):
+    s = 4 if shift else 8
+    return at[:, 0] * 10 ** 8 + (at[:, 1] + s) // 8 * 10 ** 4 + (at[:, 2] + s) // 8
+
+
+def reference(q, k, v, do, same, nhead, scale):
+    """[tokens, d] float64 and the mask of pairs that share a window -> results and tolerances without the rounding of the type"""
+    if not q.shape[0] or not k.shape[0]:                                               # nothing attends to anything
+        zeros = [torch.zeros_like(t) for t in (q, q, k, v)]
+        return zeros, lambda e: zeros
+    split = lambda t: t.view(t.shape[0], nhead, -1).transpose(0, 1)                    # noqa: E731
+    join = lambda t: t.transpose(0, 1).reshape(t.shape[1], -1)                         # noqa: E731
+    q, k, v, do = split(q), split(k), split(v), split(do)
+    dh = q.shape[-1]
+    logits = (q @ k.transpose(1, 2) * scale).masked_fill(~same, -float('inf'))
+    top = logits.amax(-1, keepdim=True).clamp_min(-1e300)
+    p = (logits - top).exp()
+    total = p.sum(-1, keepdim=True)
+    p = p / total.clamp_min(1e-300) * (total > 0)
+    dp = do @ v.transpose(1, 2)
+    ds = scale * p * (dp - (p * dp).sum(-1, keepdim=True))
+    out = [join(t) for t in (p @ v, ds @ k, ds.transpose(1, 2) @ q, p.transpose(1, 2) @ do)]
+    A = (q.abs() @ k.abs().transpose(1, 2) * scale).masked_fill(~same, 0).amax(-1, keepdim=True)
+
+    def tolerances(e):
+        T = 64
+        rho = 2 * (dh + 8) * U * (A + 6) + (T + 16) * U
+        gsum = (do.abs() @ v.abs().transpose(1, 2)) * same
+        eta = (2 * rho + (dh + T + 8) * U + e) * scale * p * (gsum + (p * gsum).sum(-1, keepdim=True)) + T * U * ds.abs()
+        wp = p * (rho + e + 4 * T * U)
+        tols = [join(t) for t in (wp @ v.abs(), eta @ k.abs(), eta.transpose(1, 2) @ q.abs(), wp.transpose(1, 2) @ do.abs())]
+        return [t + (e + 2 * U) * o.abs() for t, o in zip(tols, out)]
+    return out, tolerances
+
+
+CASES = [  # name, batch, ny, nx, queries, keys (None: self), heads, dh, shift, dtype, layout, work list, scale
+    ('one_token', 1, 3, 5, [1], None, 1, 16, False, 'bf16', 'qkv', True, None),
+    ('one_token_f32', 1, 1, 1, [1], None, 3, 64, True, 'f32', 'qk_v', False, None),
+    ('full_window', 1, 8, 8, [64], None, 2, 32, False, 'bf16', 'qk_v', True, None),
+    ('full_windows_shifted', 2, 24, 17, [408, 408], None, 4, 16, True, 'bf16', 'qkv', True, None),
+    ('full_windows_64', 1, 16, 16, [256], None, 5, 64, False, 'bf16', 'qk_v', True, None),
+    ('full_windows_f32', 1, 19, 21, [399], None, 3, 32, True, 'f32', 'qk_v', True, None),
+    ('full_windows_f32_64', 1, 16, 16, [256], None, 1, 64, False, 'f32', 'qkv', True, None),
+    ('sparse', 2, 70, 45, [160, 31], None, 8, 16, False, 'bf16', 'qk_v', True, None),
+    ('sparse_dense_launch', 2, 70, 45, [160, 31], None, 8, 16, True, 'bf16', 'qk_v', False, None),
+    ('ragged', 3, 40, 41, [900, 0, 333], None, 8, 32, True, 'bf16', 'qk_v', True, 0.4),
+    ('ragged_f32', 2, 40, 41, [900, 333], None, 8, 16, False, 'f32', 'qkv', True, 0.03),
+    ('seven_heads', 1, 33, 50, [700], None, 7, 16, True, 'bf16', 'qkv', True, None),
+    ('cross', 2, 40, 41, [120, 300], [800, 13], 8, 32, True, 'bf16', 'q_k_v', True, None),
+    ('cross_packed', 2, 40, 41, [120, 300], [800, 13], 8, 16, False, 'bf16', 'q_kv', True, None),
+    ('cross_64', 1, 40, 41, [1100], [700], 2, 64, False, 'bf16', 'q_k_v', True, None),
+    ('cross_f32', 2, 40, 41, [50, 900], [1600, 20], 5, 32, False, 'f32', 'q_kv', True, None),
+    ('cross_dense_launch', 2, 40, 41, [50, 900], [1600, 20], 4, 16, True, 'bf16', 'q_k_v', False, None),
+    ('cross_no_keys', 1, 20, 20, [90], [0], 4, 16, False, 'bf16', 'q_k_v', True, None),
+    ('cross_no_queries', 1, 20, 20, [0], [90], 4, 16, False, 'f32', 'q_k_v', True, None),
+    ('large_logits', 1, 30, 30, [600], None, 4, 32, False, 'bf16', 'qk_v', True, 9.0),
+]
+
+
+def make(case):
+    name, batch, ny, nx, nq, nk, heads, dh, shift, dtype, layout, wl, scale = case
+    g = torch.Generator().manual_seed(len(name) * 7 + ny)
+    dt = {'bf16': torch.bfloat16, 'f32': torch.float32}[dtype]
+    d = heads * dh
+    grid_q, at_q = place(nq, batch, ny, nx, g, shuffle=True)
+    grid_k, at_k = (grid_q, at_q) if nk is None else place(nk, batch, ny, nx, g)
+    mq, mk = at_q.shape[0], at_k.shape[0]
+    q, do = (torch.randn(mq, d, generator=g).to(dt) for _ in range(2))
+    k, v = (torch.randn(mk, d, generator=g).to(dt) for _ in range(2))
+    same = window_of(at_q, shift)[:, None] == window_of(at_k, shift)[None]
+    return q, k, v, do, grid_q, grid_k, same
+
+
+def pack(layout, q, k, v):
+    return {'qkv': lambda: (torch.cat([q, k, v], 1), None, None), 'qk_v': lambda: (torch.cat([q, k], 1), v, None),
+            'q_k_v': lambda: (q, k, v), 'q_kv': lambda: (q, torch.cat([k, v], 1), 'kv')}[layout]()
+
+
+def unpack(layout, grads, d):
+    if layout == 'qkv':
+        return grads[0].split(d, 1)
+    if layout == 'qk_v':
+        return (*grads[0].split(d, 1), grads[1])
+    return grads if layout == 'q_k_v' else (grads[0], *grads[1].split(d, 1))
+
+
+# --------------------------------------------------------------------------------------------------------------- the CPU
+
+def test_refusals():
+    from tmae_amd import ops
+    grid = torch.full((2 * 9 * 9,), -1, dtype=torch.int32)
+    x, v = torch.zeros(10, 64), torch.zeros(10, 32)
+
+    def call(a=x, b=v, c=None, gq=grid, gk=grid, nhead=2, batch=2, ny=9, nx=9, **k):
+        return ops.win_attn_dot(a, b, c, gq, gk, nhead, batch, ny, nx, False, **k)
+    with pytest.raises(RuntimeError, match='GPU only'):
+        call()
+    for kind, match, bad in (
+            (ValueError, r'q\|k', dict(b=None, c=v)), (ValueError, 'kv', dict(c='vk')), (ValueError, 'one type', dict(b=v.bfloat16())),
+            (TypeError, 'float32 / bfloat16', dict(a=x.half(), b=v.half())), (ValueError, 'rows of', dict(b=v[:, :16])),
+            (ValueError, 'rows of', dict(b=v[:9])), (ValueError, 'rows of', dict(a=v, b=v, c=v[:3])), (ValueError, '16, 32 or 64', dict(nhead=4)),
+            (ValueError, '16, 32 or 64', dict(nhead=0)), (ValueError, 'scale', dict(scale=0.0)), (ValueError, 'scale', dict(scale=-1.0)),
+            (ValueError, 'scale', dict(scale=float('nan'))), (ValueError, 'scale', dict(scale=float('inf'))), (ValueError, 'grid', dict(batch=0)),
+            (ValueError, 'grid_q', dict(gq=grid[:-1])), (ValueError, 'grid_k', dict(gk=grid.long())), (ValueError, 'grid_q', dict(nx=8)),
+            (ValueError, 'work list', dict(worklist=torch.zeros(5, dtype=torch.int32)))):
+        with pytest.raises(kind, match=match):
+            call(**bad)
+
+
+def test_c_entries_refuse_bad_arguments():
+    from tmae_amd._lib import lib
+    one = ctypes.c_void_p(16)
+
+    def fwd(q=one, ldq=64, k=one, v=one, dtype=1, mq=4, mk=4, nhead=4, dh=16, gq=one, gk=one, batch=1, ny=8, nx=8, scale=1.0, out=one, ldo=64,
+            lse=one, wl=None):
+        return lib.tmae_win_attn_dot_fwd(q, ldq, k, 64, v, 64, dtype, mq, mk, nhead, dh, gq, gk, batch, ny, nx, 0, scale, out, ldo, lse, wl, None)
+    assert fwd(mq=0) == 0 and fwd(dtype=3) == -3
+    for bad in (dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(lse=None), dict(gq=None), dict(gk=None), dict(mq=-1), dict(mk=-1),
+                dict(mq=1 << 31), dict(nhead=0), dict(nhead=4097), dict(dh=8), dict(dh=48), dict(batch=0), dict(ny=0), dict(nx=0), dict(scale=0.0),
+                dict(scale=-1.0), dict(scale=float('nan')), dict(scale=float('inf')), dict(ldq=63), dict(ldq=56), dict(ldo=68 + 2),
+                dict(q=ctypes.c_void_p(8)), dict(batch=1 << 20, ny=1 << 10, nx=1 << 10), dict(wl=one, ny=2041)):
+        assert fwd(**bad) == -1, bad
+
+    def bwd(dq=one, dk=one, dv=one, do=one, lse=one, lddq=64):
+        return lib.tmae_win_attn_dot_bwd(one, 64, one, 64, one, 64, do, 64, lse, 1, 4, 4, 4, 16, one, one, 1, 8, 8, 0, 1.0, dq, lddq, dk, 64, dv,
+                                         64, None, None)
+    for bad in (dict(dq=None), dict(dk=None), dict(dv=None), dict(do=None), dict(lse=None), dict(lddq=60)):
+        assert bwd(**bad) == -1, bad
+
+
+# --------------------------------------------------------------------------------------------------------------- the GPU
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('case', CASES, ids=lambda c: c[0])
+def test_attention_and_its_gradients(case):
+    from tmae_amd import ops
+    name, batch, ny, nx, nq, nk, heads, dh, shift, dtype, layout, wl, scale = case
+    q, k, v, do, grid_q, grid_k, same = make(case)
+    d, e = heads * dh, half_step(q.dtype)
+    want, tolerances = reference(q.double(), k.double(), v.double(), do.double(), same, heads, scale or dh ** -0.5)
+    gq = grid_q.cuda()
+    gk = gq if nk is None else grid_k.cuda()
+    args = [t.cuda().requires_grad_() if torch.is_tensor(t) else t for t in pack(layout, q, k, v)]
+    worklist = ops.window_worklist(gq, gk, batch, ny, nx, shift) if wl else None
+    for covered in (True, False):
+        o = ops.win_attn_dot(*args, gq, gk, heads, batch, ny, nx, shift, scale=scale, worklist=worklist, covered=covered)
+        grads = torch.autograd.grad(o, [t for t in args if torch.is_tensor(t)], do.cuda())
+        for what, got, w, t in zip(('out', 'dq', 'dk', 'dv'), (o, *unpack(layout, grads, d)), want, tolerances(e)):
+            assert got.dtype == q.dtype
+            within(got, w, t, f'{name} {what}')
+        with torch.no_grad():
+            assert torch.equal(ops.win_attn_dot(*args, gq, gk, heads, batch, ny, nx, shift, scale=scale, worklist=worklist, covered=covered), o)
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences():
+    """The float32 gradients along a direction against differences of the 64-bit definition."""
+    from tmae_amd import ops
+    case = ('differences', 2, 40, 41, [120, 300], [800, 13], 4, 16, True, 'f32', 'q_k_v', True, None)
+    q, k, v, do, grid_q, grid_k, same = make(case)
+    g = torch.Generator().manual_seed(5)
+    ways = [torch.randn(t.shape, generator=g).double() for t in (q, k, v)]
+    h = 1e-6
+    hi, lo = ((reference(*(t.double() + s * h * w for t, w in zip((q, k, v), ways)), do.double(), same, 4, 0.25)[0][0] * do.double()).sum()
+              for s in (1, -1))
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    gq, gk = grid_q.cuda(), grid_k.cuda()
+    o = ops.win_attn_dot(*leaves, gq, gk, 4, 2, 40, 41, True, worklist=ops.window_worklist(gq, gk, 2, 40, 41, True))
+    grads = torch.autograd.grad(o, leaves, do.cuda())
+    along = sum((gr.double().cpu() * w).sum() for gr, w in zip(grads, ways))
+    size = sum((gr.double().cpu() * w).abs().sum() for gr, w in zip(grads, ways))
+    assert abs((hi - lo) / (2 * h) - along) <= 1e-5 * size
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_rows_outside_the_grids(dtype):
+    """Rows that stand in no cell (dropped tokens) stay zero, entries that are no row count as empty cells, with and without a list."""
+    from tmae_amd import ops
+    g = torch.Generator().manual_seed(2)
+    grid, at = place([300], 1, 24, 24, g)
+    q, k, v, do = (torch.randn(300, 64, generator=g).to(dtype) for _ in range(4))
+    gone = torch.randperm(300, generator=g)[:80]
+    kept = torch.ones(300, dtype=torch.bool)
+    kept[gone] = False
+    masked = torch.where(grid >= 0, torch.where(kept[grid.clamp(min=0).long()], grid, torch.full_like(grid, -1)), grid)
+    odd = torch.where((grid >= 0) & (masked < 0), torch.full_like(grid, 300) + (torch.arange(grid.numel()) % 2) * 2 ** 30, masked).int()
+    same = (window_of(at, False)[:, None] == window_of(at, False)[None]) & kept[:, None] & kept[None]
+    want, tolerances = reference(q.double(), k.double(), v.double(), do.double(), same, 4, 0.25)
+    for gr in (masked, odd):
+        for other in (False, True):
+            gq = gr.cuda()
+            gk = gr.cuda() if other else gq
+            for worklist in (None, ops.window_worklist(masked.cuda(), masked.cuda(), 1, 24, 24, False)):
+                leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+                o = ops.win_attn_dot(*leaves, gq, gk, 4, 1, 24, 24, False, worklist=worklist)
+                grads = torch.autograd.grad(o, leaves, do.cuda())
+                for what, got, w, t in zip(('out', 'dq', 'dk', 'dv'), (o, *grads), want, tolerances(half_step(dtype))):
+                    within(got, w, t, what)
+                    assert not got[gone.cuda()].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('value', [float('nan'), float('inf'), -float('inf')])
+def test_a_bad_token_stays_in_its_window_and_head(dtype, value):
+    """What a NaN or an infinity reaches ends at its window and head, in every output, whichever tensor holds it."""
+    from tmae_amd import ops
+    g = torch.Generator().manual_seed(4)
+    for counts, ny in (([60], 40), ([700], 40), ([1600], 40)):
+        grid, at = place(counts, 1, ny, ny, g)
+        n, h, dh = counts[0], 6, 16
+        gr = grid.cuda()
+        wl = ops.window_worklist(gr, gr, 1, ny, ny, True)
+        win = window_of(at, True)
+        for which in range(4):
+            tensors = [torch.randn(n, h * dh, generator=g) for _ in range(4)]
+            tensors[which][n // 2, 2 * dh + 3] = value
+            q, k, v, do = (t.to(dtype).cuda() for t in tensors)
+            leaves = [t.requires_grad_() for t in (q, k, v)]
+            o = ops.win_attn_dot(*leaves, gr, gr, h, 1, ny, ny, True, worklist=wl, covered=True)
+            for t in (o, *torch.autograd.grad(o, leaves, do)):
+                fine = torch.isfinite(t.detach().float().view(n, h, dh)).all(-1).cpu()
+                touched = torch.zeros(n, h, dtype=torch.bool)
+                touched[win == win[n // 2], 2] = True
+                assert fine[~touched].all()
+            # (a key's infinity gives a logit of -inf where the query's channel has the other sign: probability 0, and all is finite)
+            assert which == 3 or value == value or not torch.isfinite(o[n // 2]).all()
+
+
+@pytest.mark.gpu
+def test_norms_rotation_and_attention_together():
+    """As an encoder layer uses them: one packed projection, norms and rotation, attention, all gradients -- against autograd through
+    the definition in 64 bits; the same bits again on another stream and from a captured graph on new inputs."""
+    from tmae_amd import ops
+    g = torch.Generator().manual_seed(9)
+    batch, ny, nx, h, dh, sec = 2, 40, 41, 8, 16, (2, 3, 3)
+    grid, at = place([500, 301], batch, ny, nx, g)
+    n, d = at.shape[0], h * dh
+    same = window_of(at, True)[:, None] == window_of(at, True)[None]
+    pos = torch.cat([torch.zeros(n, 1, dtype=torch.int64), at[:, 1:]], 1).int()
+    f = ops.rotary_freqs(sec, 100.0)
+    gq, gk = (1 + 0.2 * torch.randn(dh, generator=g) for _ in range(2))
+    qk, v, do = (torch.randn(n, w, generator=g) for w in (2 * d, d, d))
+
+    def definition(qk, gq, gk, v):
+        x = qk.view(n, 2 * h, dh)
+        x = x * (x.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+        x = torch.cat([x[:, :h] * gq, x[:, h:] * gk], 1)
+        theta = (pos.double()[:, torch.repeat_interleave(torch.arange(3), torch.tensor(sec))] * f)[:, None]
+        a, b = x[..., :8], x[..., 8:]
+        x = torch.cat([a * theta.cos() - b * theta.sin(), a * theta.sin() + b * theta.cos()], -1)
+        q, k = x[:, :h].transpose(0, 1), x[:, h:].transpose(0, 1)
+        p = torch.softmax((q @ k.transpose(1, 2) * dh ** -0.5).masked_fill(~same, -float('inf')), -1)
+        return (p @ v.view(n, h, dh).transpose(0, 1)).transpose(0, 1).reshape(n, d)
+
+    gr, posg, fg = grid.cuda(), pos.cuda(), f.cuda()
+    wl = ops.window_worklist(gr, gr, batch, ny, nx, True)
+
+    def run(qk, gq, gk, v, do):
+        y = ops.qk_norm_rotary(qk.view(n, 2 * h, dh), gq, gk, posg, fg, sec)
+        o = ops.win_attn_dot(y.view(n, 2 * d), v, None, gr, gr, h, batch, ny, nx, True, worklist=wl, covered=True)
+        return (o.detach(), *torch.autograd.grad(o, (qk, gq, gk, v), do))
+
+    # bf16: the rows between the two operators are rounded once more each way (2^-8 of a unit-size row, through logits of size ~ 4 and
+    # sums of mixed signs: 2-norms within 4 roundings); float32: every step within a few hundred u
+    for dtype, bound in ((torch.float32, 400 * U), (torch.bfloat16, 4 * 2.0 ** -8)):
+        rounded = [t.to(dtype) for t in (qk, v, do)]
+        ref_in = [rounded[0].double().requires_grad_(), gq.double().requires_grad_(), gk.double().requires_grad_(), rounded[1].double().requires_grad_()]
+        ref = definition(*ref_in)
+        want = (ref.detach(), *torch.autograd.grad(ref, ref_in, rounded[2].double()))
+        gpu = [rounded[0].cuda().requires_grad_(), gq.cuda().requires_grad_(), gk.cuda().requires_grad_(), rounded[1].cuda().requires_grad_()]
+        got = run(*gpu, rounded[2].cuda())
+        for i, (a, b) in enumerate(zip(got, want)):
+            assert (a.double().cpu() - b).norm() <= bound * b.norm(), (dtype, i, float((a.double().cpu() - b).norm() / b.norm()))
+    # another stream, then a graph replayed on new inputs with eager work between
+    dog = do.bfloat16().cuda()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = run(*gpu, dog)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(again, got))
+    held = [t.detach().clone().requires_grad_() for t in gpu]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(*held, dog)
+    for k in range(4):
+        fresh = [torch.randn(t.shape, generator=g).to(t.dtype).cuda().requires_grad_() for t in gpu]
+        with torch.no_grad():
+            for a, b in zip(held, fresh):
+                a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, run(*fresh, dog))), k
