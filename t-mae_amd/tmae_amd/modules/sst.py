@@ -40,22 +40,69 @@ def pos_embed_table(feat_dim, window_shape, pos_temperature, normalize_pos=False
     return table
 
 
+class HeadNorm(nn.Module):
+    """The gain of the norm of queries or keys, [channels of a head].  A module of its own: the optimizer's groups hold the
+    parameters of leaf modules (train/optim.py)."""
+
+    def __init__(self, head_dim):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(head_dim))
+
+
 class CosineMultiheadAttention(nn.Module):
     """Parameter container with nn.MultiheadAttention's names (cosine_msa.py:441-458): packed in-proj,
     out_proj, learnable temperature tau clamped at tau_min: (1,1,1) shared by the heads, or (1, num_heads, 1, 1) with
-    non_shared_tau (cosine_msa.py:453-456)."""
+    non_shared_tau (cosine_msa.py:453-456).
 
-    def __init__(self, embed_dim, num_heads, dropout=0.0, tau_min=0.01, cosine=True, non_shared_tau=False):
+    cosine False: scaled dot products (ops.win_attn_dot) and no temperature.  rotary {'SECTIONS': (y, x) or (time, y, x) channel
+    pairs of a head, 'BASE': 100.0}: queries and keys turn by the voxel's position (ops.rotary_axes) and the additive position
+    table is not used; qk_norm: their heads are normalised with a learned gain in the same pass (ops.qk_norm_rotary)."""
+
+    def __init__(self, embed_dim, num_heads, dropout=0.0, tau_min=0.01, cosine=True, non_shared_tau=False, rotary=None, qk_norm=False):
         super().__init__()
-        if dropout != 0.0 or not cosine:
-            raise NotImplementedError('T-MAE configs use cosine attention, dropout 0')
-        self.embed_dim, self.num_heads, self.tau_min = embed_dim, num_heads, tau_min
+        if dropout != 0.0:
+            raise NotImplementedError('T-MAE configs use dropout 0')
+        if qk_norm and not rotary:
+            raise NotImplementedError('LAYER_CFG.qk_norm comes with the rotation: set LAYER_CFG.rotary')
+        self.embed_dim, self.num_heads, self.tau_min, self.cosine = embed_dim, num_heads, tau_min, bool(cosine)
+        self.head_dim = embed_dim // num_heads
+        self.sections = None
+        if rotary:
+            self.sections = tuple(int(p) for p in rotary['SECTIONS'])
+            if len(self.sections) not in (2, 3) or min(self.sections) < 1 or 2 * sum(self.sections) > self.head_dim:
+                raise ValueError(f'LAYER_CFG.rotary.SECTIONS {self.sections}: channel pairs for (y, x) or (time, y, x), at most '
+                                 f'{self.head_dim // 2} for heads of {self.head_dim} channels')
+            self.base = float(rotary.get('BASE', 100.0))
+            self._freqs = {}                 # device -> ops.rotary_freqs (float64: no buffer, so that .half() / .float() leave it alone)
         self.in_proj_weight = nn.Parameter(torch.empty(3 * embed_dim, embed_dim))
         self.in_proj_bias = nn.Parameter(torch.zeros(3 * embed_dim))
         self.out_proj = nn.Linear(embed_dim, embed_dim)
-        self.tau = nn.Parameter(torch.ones(1, num_heads, 1, 1) if non_shared_tau else torch.ones(1, 1, 1))
+        if self.cosine:
+            self.tau = nn.Parameter(torch.ones(1, num_heads, 1, 1) if non_shared_tau else torch.ones(1, 1, 1))
+        if qk_norm:
+            self.q_norm, self.k_norm = HeadNorm(self.head_dim), HeadNorm(self.head_dim)
+        self.qk_norm = bool(qk_norm)
         nn.init.xavier_uniform_(self.in_proj_weight)
         nn.init.constant_(self.out_proj.bias, 0.0)
+
+    def turn(self, rows, plan, queries, keys, time=0):
+        """rows [m, d] (queries or keys) or [m, 2 d] (both) of plan's voxels, normalised and turned by their positions."""
+        f = self._freqs.get(rows.device)
+        if f is None:
+            f = self._freqs[rows.device] = ops.rotary_freqs(self.sections, self.base, rows.device)
+        heads = rows.view(rows.shape[0], rows.shape[1] // self.head_dim, self.head_dim)
+        pos = plan.positions(len(self.sections), time)
+        if not self.qk_norm:
+            return ops.rotary_axes(heads, pos, f, self.sections).view(rows.shape)
+        y = ops.qk_norm_rotary(heads, self.q_norm.weight if queries else None, self.k_norm.weight if keys else None, pos, f,
+                               self.sections, q_heads=self.num_heads if queries else 0)
+        return y.view(rows.shape)
+
+
+def _attention_params(d_model, nhead, dropout, layer_cfg):
+    return CosineMultiheadAttention(d_model, nhead, dropout=dropout, tau_min=layer_cfg.get('tau_min', 0.01),
+                                    cosine=layer_cfg.get('cosine', False), non_shared_tau=layer_cfg.get('non_shared_tau', False),
+                                    rotary=layer_cfg.get('rotary', None), qk_norm=layer_cfg.get('qk_norm', False))
 
 
 class WindowPlan:
@@ -69,6 +116,7 @@ class WindowPlan:
         self.key_grid = self.grid if other is None else other.grid
         self._wl = {}
         self._cells = {}
+        self._positions = {}
         self._shift_grids = {}           # shift -> (query grid, key grid) with dropped tokens masked out (token dropping)
 
     def set_shift_grids(self, shift, grid_q, grid_k):
@@ -94,6 +142,17 @@ class WindowPlan:
             self._wl[shift] = ops.window_worklist(self.grid_q(shift), self.grid_k(shift), self.batch, self.ny, self.nx, shift)
         return self._wl[shift]
 
+    def positions(self, axes, time=0):
+        """(y, x) or (time, y, x) of the voxels on the whole grid, int32: a rotation depends on differences only, so both shifts and
+        every window share them.  time: the frame's, 0 the current one."""
+        if axes == 2:
+            return self.indices[:, 1:]
+        if time not in self._positions:
+            p = self.indices.clone()
+            p[:, 0] = time
+            self._positions[time] = p
+        return self._positions[time]
+
     def cells(self, shift, window_shape):
         """cell bytes of the tokens for this shift (ops.window_cells), shared by the layers of the stage."""
         shift = bool(shift)
@@ -115,41 +174,42 @@ class WindowAttention(nn.Module):
     def __init__(self, d_model, nhead, dropout, layer_cfg):
         super().__init__()
         self.nhead = nhead
-        if not layer_cfg.get('cosine', False):
-            raise NotImplementedError('non-cosine window attention is not on the T-MAE path')
-        self.self_attn = CosineMultiheadAttention(d_model, nhead, dropout=dropout,
-                                                  tau_min=layer_cfg.get('tau_min', 0.01),
-                                                  non_shared_tau=layer_cfg.get('non_shared_tau', False))
+        self.self_attn = _attention_params(d_model, nhead, dropout, layer_cfg)
 
     def forward(self, x, plan, pos_table, window_shape, shift):
         """q = k = x + pos, v = x (sst_basic_block.py:22-54), windows of `shift` read from plan.grid.
         Returns (attention output, x's alias for the residual branch): see ops.proj_fork."""
         a = self.self_attn
         d = a.embed_dim
-        if _POS_FOLD and ops._pos_proj_ok(x, d, 3 * d):
+        if a.sections is None and _POS_FOLD and ops._pos_proj_ok(x, d, 3 * d):
             qkv, x_res = ops.pos_proj(x, a.in_proj_weight, a.in_proj_bias, 0, 3 * d, 0, 2 * d,
                                       plan.cells(shift, window_shape), ops.pos_axes(pos_table, window_shape), fork=True,
                                       inplace_dx=True)
-            o = ops.win_attn(qkv, None, None, a.tau, plan.grid, plan.grid, self.nhead, plan.batch, plan.ny, plan.nx,
-                             shift, a.tau_min, worklist=plan.worklist(shift))
+            o = self._attend(qkv, None, plan, shift)
             return ops.linear(o, a.out_proj.weight, a.out_proj.bias), x_res
-        qk, v, x_res = ops.proj_fork(x, a.in_proj_weight, a.in_proj_bias, ((0, 2 * d, True), (2 * d, 3 * d, False)),
+        table = a.sections is None                # a rotation takes the place of the additive position table
+        qk, v, x_res = ops.proj_fork(x, a.in_proj_weight, a.in_proj_bias, ((0, 2 * d, table), (2 * d, 3 * d, False)),
                                      pos=(plan.indices, pos_table, window_shape, shift), fork=True,
                                      inplace_dx=True)
-        o = ops.win_attn(qk, v, None, a.tau, plan.grid, plan.grid, self.nhead, plan.batch, plan.ny, plan.nx,
-                         shift, a.tau_min, worklist=plan.worklist(shift))
+        if not table:
+            qk = a.turn(qk, plan, True, True)
+        o = self._attend(qk, v, plan, shift)
         return ops.linear(o, a.out_proj.weight, a.out_proj.bias), x_res
+
+    def _attend(self, qk, v, plan, shift):
+        a = self.self_attn
+        if a.cosine:
+            return ops.win_attn(qk, v, None, a.tau, plan.grid, plan.grid, self.nhead, plan.batch, plan.ny, plan.nx,
+                                shift, a.tau_min, worklist=plan.worklist(shift))
+        return ops.win_attn_dot(qk, v, None, plan.grid, plan.grid, self.nhead, plan.batch, plan.ny, plan.nx, shift,
+                                worklist=plan.worklist(shift), covered=True)
 
 
 class WindowCrossAttention(nn.Module):
     def __init__(self, d_model, nhead, dropout, layer_cfg):
         super().__init__()
         self.nhead = nhead
-        if not layer_cfg.get('cosine', False):
-            raise NotImplementedError('non-cosine window attention is not on the T-MAE path')
-        self.cross_attn = CosineMultiheadAttention(d_model, nhead, dropout=dropout,
-                                                   tau_min=layer_cfg.get('tau_min', 0.01),
-                                                   non_shared_tau=layer_cfg.get('non_shared_tau', False))
+        self.cross_attn = _attention_params(d_model, nhead, dropout, layer_cfg)
 
     def forward(self, x, plan, x_prv, plan_prv, pos_table, window_shape, shift, prv_alias=False):
         """q = cur + pos, k = prev + pos_prev, v = prev (wca_block.py:26-67).  Query tokens whose window is
@@ -159,21 +219,30 @@ class WindowCrossAttention(nn.Module):
         a = self.cross_attn
         d = a.embed_dim
         w, b = a.in_proj_weight, a.in_proj_bias
-        if _POS_FOLD and ops._pos_proj_ok(x, d, d) and ops._pos_proj_ok(x_prv, d, 2 * d):
+        if a.sections is None and _POS_FOLD and ops._pos_proj_ok(x, d, d) and ops._pos_proj_ok(x_prv, d, 2 * d):
             E = ops.pos_axes(pos_table, window_shape)
             res = ops.pos_proj_cross(x, x_prv, w, b, plan.cells(shift, window_shape),
                                      plan_prv.cells(shift, window_shape), E, inplace_dx=True, kv_alias=prv_alias)
             q, kv, x_res = res[:3]
-            o = ops.win_attn(q, kv, 'kv', a.tau, plan.grid_q(shift), plan.grid_k(shift), self.nhead, plan.batch, plan.ny,
-                             plan.nx, shift, a.tau_min, worklist=plan.worklist(shift), covered=plan.covered(shift))
+            o = self._attend(q, kv, 'kv', plan, shift)
             return (o, x_res, res[3]) if prv_alias else (o, x_res)
-        q, x_res = ops.proj_fork(x, w, b, ((0, d, True),), pos=(plan.indices, pos_table, window_shape, shift), fork=True,
+        table = a.sections is None
+        q, x_res = ops.proj_fork(x, w, b, ((0, d, table),), pos=(plan.indices, pos_table, window_shape, shift), fork=True,
                                  inplace_dx=True)
-        k, v = ops.proj_fork(x_prv, w, b, ((d, 2 * d, True), (2 * d, 3 * d, False)),
+        k, v = ops.proj_fork(x_prv, w, b, ((d, 2 * d, table), (2 * d, 3 * d, False)),
                              pos=(plan_prv.indices, pos_table, window_shape, shift))
-        o = ops.win_attn(q, k, v, a.tau, plan.grid_q(shift), plan.grid_k(shift), self.nhead, plan.batch, plan.ny, plan.nx,
-                         shift, a.tau_min, worklist=plan.worklist(shift), covered=plan.covered(shift))
+        if not table:
+            q, k = a.turn(q, plan, True, False), a.turn(k, plan_prv, False, True, time=-1)
+        o = self._attend(q, k, v, plan, shift)
         return (o, x_res, x_prv) if prv_alias else (o, x_res)
+
+    def _attend(self, q, k, v, plan, shift):
+        a = self.cross_attn
+        if a.cosine:
+            return ops.win_attn(q, k, v, a.tau, plan.grid_q(shift), plan.grid_k(shift), self.nhead, plan.batch, plan.ny, plan.nx,
+                                shift, a.tau_min, worklist=plan.worklist(shift), covered=plan.covered(shift))
+        return ops.win_attn_dot(q, k, v, plan.grid_q(shift), plan.grid_k(shift), self.nhead, plan.batch, plan.ny, plan.nx, shift,
+                                worklist=plan.worklist(shift), covered=plan.covered(shift))
 
 
 def _activation(name):

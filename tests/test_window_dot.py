@@ -334,3 +334,135 @@ def test_norms_rotation_and_attention_together():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, run(*fresh, dog))), k
+
+
+# ------------------------------------------------------------------------------------------------ the layers that call them
+
+OPTIONS = [{'cosine': False}, {'cosine': True, 'tau_min': 0.01, 'rotary': {'SECTIONS': [4, 4]}},
+           {'cosine': False, 'rotary': {'SECTIONS': [2, 3, 3], 'BASE': 50.0}},
+           {'cosine': False, 'rotary': {'SECTIONS': [2, 3, 3], 'BASE': 50.0}, 'qk_norm': True}]
+
+
+def test_options_build_and_train_their_gains():
+    from tmae_amd.modules.sst import WindowAttention, WindowCrossAttention
+    from tmae_amd.train.optim import reference_param_groups
+    for opt in OPTIONS:
+        m = WindowAttention(128, 8, 0.0, opt).self_attn
+        names = set(dict(m.named_parameters()))
+        assert ('tau' in names) == opt['cosine'] and ('q_norm.weight' in names) == bool(opt.get('qk_norm'))
+        if opt.get('qk_norm'):
+            plain, _, rest = reference_param_groups(m)
+            assert any(p is m.q_norm.weight for p in plain) and any(p is m.k_norm.weight for p in plain)
+    for bad, kind in (({'cosine': False, 'qk_norm': True}, NotImplementedError), ({'rotary': {'SECTIONS': [8]}}, ValueError),
+                      ({'rotary': {'SECTIONS': [4, 5]}}, ValueError), ({'rotary': {'SECTIONS': [0, 5]}}, ValueError)):
+        with pytest.raises(kind):
+            WindowCrossAttention(128, 8, 0.0, bad)
+
+
+def layer_reference(a, W, b, x, x_kv, at_q, at_k, tq, tk, table, shift, opt, tau):
+    """q, k, v from the packed in-projection -> attention rows before the out-projection, float64"""
+    d, h, dh = 128, 8, 16
+    s = 4 if shift else 8
+    cell = lambda at: (at[:, 1] + s) % 8 * 8 + (at[:, 2] + s) % 8                      # noqa: E731
+    rot = opt.get('rotary')
+    q_in, k_in = (x, x_kv) if rot else (x + table[cell(at_q)], x_kv + table[cell(at_k)])
+    q = (q_in @ W[:d].t() + b[:d]).view(-1, h, dh)
+    k = (k_in @ W[d:2 * d].t() + b[d:2 * d]).view(-1, h, dh)
+    v = (x_kv @ W[2 * d:].t() + b[2 * d:]).view(-1, h, dh)
+    if opt.get('qk_norm'):
+        q = q * (q.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * a['q_norm.weight']
+        k = k * (k.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * a['k_norm.weight']
+    if rot:
+        sec = rot['SECTIONS']
+        axis = torch.repeat_interleave(torch.arange(len(sec)), torch.tensor(sec))
+        f = torch.cat([torch.tensor(float(rot.get('BASE', 100.0)), dtype=torch.float64) ** (-torch.arange(p).double() / p) for p in sec])
+
+        def turned(t, at, time):
+            pos = at.clone().double()
+            pos[:, 0] = time
+            th = (pos[:, 3 - len(sec):][:, axis] * f)[:, None]
+            p = th.shape[-1]
+            lo, hi = t[..., :p], t[..., p:2 * p]
+            return torch.cat([lo * th.cos() - hi * th.sin(), lo * th.sin() + hi * th.cos(), t[..., 2 * p:]], -1)
+        q, k = turned(q, at_q, tq), turned(k, at_k, tk)
+    scale = dh ** -0.5
+    if opt['cosine']:
+        q, k, scale = q / q.norm(dim=-1, keepdim=True), k / k.norm(dim=-1, keepdim=True), 1.0 / a['tau'].view(())
+    same = window_of(at_q, shift)[:, None] == window_of(at_k, shift)[None]
+    logits = (q.transpose(0, 1) @ k.permute(1, 2, 0) * scale).masked_fill(~same, -1e30)
+    p = torch.softmax(logits, -1) * same
+    return (p @ v.transpose(0, 1)).transpose(0, 1).reshape(-1, d)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('cross', [False, True])
+@pytest.mark.parametrize('opt', OPTIONS, ids=['dot', 'cosine_rotary', 'dot_rotary', 'dot_rotary_norm'])
+def test_layers_with_the_options(opt, cross):
+    """Self and cross attention layers in float32, outputs and every gradient against autograd through the definition in 64 bits.
+    2-norms: projections over 128 channels (128 u each way), norms, rotation and attention (400 u, above), the weight gradients' sums
+    over 800 rows (800 u) -- within 1500 u together."""
+    from tmae_amd.modules.sparse import SparseConvTensor
+    from tmae_amd.modules.sst import WindowAttention, WindowCrossAttention, WindowPlan, pos_embed_table
+    g = torch.Generator().manual_seed(21)
+    ny, nx = 40, 41
+    (_, at_q), (_, at_k) = place([500, 300], 2, ny, nx, g), place([90, 700], 2, ny, nx, g)
+    table = pos_embed_table(128, [8, 8, 1], 1000)
+    x, x_kv = (torch.randn(t.shape[0], 128, generator=g) for t in (at_q, at_k))
+    do = torch.randn(800, 128, generator=g)
+    torch.manual_seed(3)
+    layer = (WindowCrossAttention if cross else WindowAttention)(128, 8, 0.0, opt)
+    params = layer.cross_attn if cross else layer.self_attn
+    with torch.no_grad():
+        for n, t in params.named_parameters():
+            if 'norm' in n or 'bias' in n:
+                t.add_(0.2 * torch.randn(t.shape))
+    names = [n for n, _ in params.named_parameters() if not (cross and n.startswith('out_proj'))]
+    ref = {n: t.detach().double().requires_grad_() for n, t in params.named_parameters()}
+    layer.cuda()
+    for shift in (False, True):
+        xr, kr = x.double().requires_grad_(), x_kv.double().requires_grad_()
+        kv = kr if cross else xr
+        o = layer_reference(ref, ref['in_proj_weight'], ref['in_proj_bias'], xr, kv, at_q, at_k if cross else at_q, 0, -1 if cross else 0,
+                            table.double(), shift, opt, None)
+        if not cross:
+            o = o @ ref['out_proj.weight'].t() + ref['out_proj.bias']
+        leaves = [xr] + ([kr] if cross else []) + [ref[n] for n in names]
+        want = [o.detach(), *torch.autograd.grad(o, leaves, do.double())]
+        xg, kg = x.cuda().requires_grad_(), x_kv.cuda().requires_grad_()
+        plan_k = WindowPlan(SparseConvTensor(kg, at_k.int().cuda(), [ny, nx], 2))
+        plan = WindowPlan(SparseConvTensor(xg, at_q.int().cuda(), [ny, nx], 2), other=plan_k if cross else None)
+        args = (xg, plan, kg, plan_k) if cross else (xg, plan)
+        og = layer(*args, table.cuda(), [8, 8, 1], shift)[0]
+        got = [og.detach(), *torch.autograd.grad(og, [xg] + ([kg] if cross else []) + [dict(params.named_parameters())[n] for n in names],
+                                                 do.cuda())]
+        for n, a, b in zip(['out', 'dx'] + (['dx_kv'] if cross else []) + names, got, want):
+            off = float((a.double().cpu() - b).norm())
+            assert off <= 1500 * U * float(b.norm()) + 1e-6 * (n == 'tau'), (n, shift, off / float(b.norm()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('amp', [False, True])
+def test_model_step_with_the_options(amp):
+    """A training step of the model built with the options: every parameter of the layers gets a finite gradient that is not zero."""
+    from conftest import build_product_model
+    from pcdet.models import model_fn_decorator
+
+    def edit(c):
+        for blk in c.MODEL.BACKBONE_3D.SST_BLOCK_LIST:
+            pairs = blk.ENCODER.D_MODEL // blk.ENCODER.NHEAD // 2
+            blk.ENCODER.LAYER_CFG = {'cosine': False, 'qk_norm': True, 'rotary': {'SECTIONS': [pairs // 4, pairs // 4, pairs // 2], 'BASE': 100.0}}
+    torch.manual_seed(0)
+    model, _, ds = build_product_model(2, device='cuda', n_points=6000, cfg_edit=edit)
+    model.train()
+    with torch.autocast('cuda', dtype=torch.bfloat16, enabled=amp):
+        loss = model_fn_decorator()(model, ds.batch(0)).loss
+    loss.backward()
+    assert torch.isfinite(loss)
+    seen = 0
+    for n, p in model.named_parameters():
+        if 'win_attn' in n:
+            assert p.grad is not None and torch.isfinite(p.grad).all(), n
+            seen += int('norm.weight' in n)
+            # (a bias of all keys moves every logit of a query alike where no rotation stands between: not so here)
+            assert p.grad.abs().max() > 0, n
+    assert seen >= 16
