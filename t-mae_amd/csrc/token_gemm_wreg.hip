@@ -16,8 +16,9 @@
 //    with 4 * NTC CONSECUTIVE columns of one token: 16-byte stores, four lanes per 128-byte line (token_gemm.hip).
 //  * vmcnt bookkeeping: DMA pieces and stores retire in order.  Step q issues DMA(q+3) right after its barrier and its
 //    stores at its end, so when step q+1 waits for DMA(q+1) the younger operations are stores(q-2), DMA(q+2),
-//    stores(q-1), DMA(q+3), stores(q): vmcnt(3 NST + 2 ND).  The prologue issues dropped dummy stores so that the count
-//    is uniform from step 0, and the tail issues out-of-range DMAs (zeros, no traffic) for the same reason.
+//    stores(q-1), DMA(q+3), stores(q): vmcnt(3 NST + 2 ND).  The prologue waits for its DMAs outright (until then nothing
+//    was stored, so the count would let the first step's own pieces stay in flight; stores that only fill the count up do not
+//    survive the compiler, which merges them), and the tail issues out-of-range DMAs (zeros, no traffic) to keep it uniform.
 #include "common.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -163,11 +164,6 @@ __global__ __launch_bounds__(512, 2) void token_gemm_wreg_kernel(const __hip_bfl
       }
     }
   };
-  auto dummy_stores = [&]() {
-#pragma unroll
-    for (int q = 0; q < NST; ++q)
-      __builtin_amdgcn_raw_buffer_store_b128(u32x4{0u, 0u, 0u, 0u}, yr, (int)TGW_OOB, 0, 0);
-  };
 
   // ---- prologue: this wave's W fragments (tile ct, row i of the tile = column 4 NTC (i >> 2) + 4 ct + (i & 3)) and bias
   u32x4 wf[NTC][KS];
@@ -184,10 +180,7 @@ __global__ __launch_bounds__(512, 2) void token_gemm_wreg_kernel(const __hip_bfl
 #pragma unroll
     for (int r = 0; r < 4; ++r) bl[ct][r] = __bfloat162float(bias[colbase + 4 * NTC * g + 4 * ct + r]);
 #pragma unroll
-  for (int q = 0; q < NS - 1; ++q) {
-    issue(q);
-    dummy_stores();
-  }
+  for (int q = 0; q < NS - 1; ++q) issue(q);
   // LDS read addresses of this lane's B fragments: row i of a token group, chunk (4 ks + g) ^ i
   int ardr[4];
 #pragma unroll
@@ -303,6 +296,7 @@ __global__ __launch_bounds__(512, 2) void token_gemm_wreg_kernel(const __hip_bfl
       }
     }
   };
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // the first NS - 1 steps are in LDS
   for (int q = 0; q < mine; ++q) {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(WAITN) : "memory");
     __builtin_amdgcn_s_barrier();
