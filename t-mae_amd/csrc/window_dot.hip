@@ -117,7 +117,7 @@ __device__ __forceinline__ void order_lds() {
 }
 
 template <class T, int DH>
-__global__ __launch_bounds__(256) void dot_fwd_kernel(DotArgs a, int cls) {
+__global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a, int cls) {
   constexpr int KD = DH / 4, CT = DH / 16;
   __shared__ int toks[2][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(256) void dot_fwd_kernel(DotArgs a, int cls) {
 }
 
 template <class T, int DH>
-__global__ __launch_bounds__(256) void dot_bwd_kernel(DotArgs a, int cls) {
+__global__ __launch_bounds__(256, 2) void dot_bwd_kernel(DotArgs a, int cls) {
   constexpr int KD = DH / 4, CT = DH / 16;
   __shared__ int toks[2][64];
   __shared__ float lse[4][64], dot[4][64];               // of the query slots: saved log2 denominator, sum_j P dP
@@ -294,6 +294,347 @@ __global__ __launch_bounds__(256) void dot_bwd_kernel(DotArgs a, int cls) {
   }
 }
 
+// ------------------------------------------------------------------------------------------------------------------ bfloat16
+// The same products on the bfloat16 matrix instructions.  A lane's piece of a token row -- FR = DH / 4 channels -- is as loaded the
+// operand of the products over the channels (logits, dP).  The products over tokens need a tile by columns: its rows go through LDS
+// (ds_read_b64_tr_b16 returns four rows of one column).  In the image of a row, position 4 a + b of 16-channel tile ct holds channel
+// FR a + 4 ct + b, so that a lane ends with FR consecutive channels of one token and stores them at once.
+//
+// P and dS enter their products rounded to bfloat16 (2^-8 of each; sums, maxima and everything else stay float32): their error is
+// that of the results' own rounding.
+//
+// A wave holds the NK key tiles of its window and walks the query tiles; NK is a template parameter, so no branch stands between a
+// matrix instruction and its reader.  Windows of at most 16 tokens (three quarters of an outdoor scene's, with two fifths of the tokens):
+// one wave takes HG heads of the window, whose rows it requests together.
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int HG = 4;
+constexpr int TILE_PITCH = 40;             // bytes per row of a 16x16 bfloat16 tile in LDS
+
+__device__ __forceinline__ unsigned pack2(float a, float b) {
+  return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{a, b}, bf16x2));
+}
+__device__ __forceinline__ s16x4 pack4(const f32x4& v) { return __builtin_bit_cast(s16x4, u32x2{pack2(v[0], v[1]), pack2(v[2], v[3])}); }
+__device__ __forceinline__ s16x4 read_columns(const char* lds) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)lds);
+}
+// sum / maximum over the 4 lanes that share a column, in every one of them
+__device__ __forceinline__ float column_sum(float v) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+__device__ __forceinline__ float column_max(float v) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+template <int FR> struct Piece { unsigned u[FR / 2]; };          // FR channels of a token
+template <int FR> __device__ __forceinline__ Piece<FR> load_piece(const char* p) {
+  Piece<FR> f;
+  if constexpr (FR == 4) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    f.u[0] = v.x; f.u[1] = v.y;
+  } else {
+#pragma unroll
+    for (int j = 0; j < FR / 8; ++j) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[j];
+      f.u[4 * j] = v.x; f.u[4 * j + 1] = v.y; f.u[4 * j + 2] = v.z; f.u[4 * j + 3] = v.w;
+    }
+  }
+  return f;
+}
+template <int FR> __device__ __forceinline__ void store_piece(char* p, const f32x4* v, float by) {
+  unsigned u[FR / 2];
+#pragma unroll
+  for (int ct = 0; ct < FR / 4; ++ct) {
+    u[2 * ct] = pack2(v[ct][0] * by, v[ct][1] * by);
+    u[2 * ct + 1] = pack2(v[ct][2] * by, v[ct][3] * by);
+  }
+  if constexpr (FR == 4) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < FR / 8; ++j) reinterpret_cast<uint4*>(p)[j] = make_uint4(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
+  }
+}
+template <int FR> __device__ __forceinline__ f32x4 over_channels(const Piece<FR>& a, const Piece<FR>& b, f32x4 c) {
+  if constexpr (FR == 4) {
+    c = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int j = 0; j < FR / 8; ++j)
+      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+          __builtin_bit_cast(bf16x8, u32x4{a.u[4 * j], a.u[4 * j + 1], a.u[4 * j + 2], a.u[4 * j + 3]}),
+          __builtin_bit_cast(bf16x8, u32x4{b.u[4 * j], b.u[4 * j + 1], b.u[4 * j + 2], b.u[4 * j + 3]}), c, 0, 0, 0);
+  }
+  return c;
+}
+// c += A B over the 16 tokens of one tile, or over the 32 of two (a third tile rides with zeros: one accumulator goes through products
+// of one shape only -- a 16x16x16 right behind the 16x16x32 that it continues has read wrong values)
+__device__ __forceinline__ f32x4 over_tokens(const s16x4& a, const s16x4& b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 over_tokens(const s16x4& a0, const s16x4& a1, const s16x4& b0, const s16x4& b1, f32x4 c) {
+  const s16x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7), b = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <int DH> struct Image {            // rows of a head by token, read by columns
+  static constexpr int FR = DH / 4, CT = DH / 16, PITCH = DH * 2 + 16, TILE = 16 * PITCH;
+  static __device__ __forceinline__ void put(char* tile, int g, int i, const Piece<FR>& f) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) *reinterpret_cast<uint2*>(tile + i * PITCH + 32 * ct + 8 * g) = make_uint2(f.u[2 * ct], f.u[2 * ct + 1]);
+  }
+  static __device__ __forceinline__ s16x4 get(const char* tile, int g, int i, int ct) {
+    return read_columns(tile + (4 * g + (i >> 2)) * PITCH + 32 * ct + 8 * (i & 3));
+  }
+};
+
+// One window, one head: NK key tiles against nq query tiles.  toks: the window's token lists in LDS; lds: 16 NK rows of an image.
+template <int DH, int NK>
+__device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq_, const int* tk_, int Tq, int Tk, int head, char* lds) {
+  using Im = Image<DH>;
+  constexpr int FR = Im::FR, CT = Im::CT;
+  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+  const int64_t col = (int64_t)head * DH * 2 + FR * 2 * g;
+  const char *q = (const char*)a.q + col, *k = (const char*)a.k + col, *v = (const char*)a.v + col;
+  char* out = (char*)a.o + col;
+  const int nq = (Tq + 15) >> 4;
+  Piece<FR> kf[NK], vf[NK];
+#pragma unroll
+  for (int kt = 0; kt < NK; ++kt) {
+    const int64_t t = tk_[kt * 16 + i];
+    kf[kt] = load_piece<FR>(k + t * a.ldk * 2);
+    vf[kt] = load_piece<FR>(v + t * a.ldv * 2);
+  }
+  int64_t tq = tq_[i];
+  Piece<FR> qf = load_piece<FR>(q + tq * a.ldq * 2);
+#pragma unroll
+  for (int kt = 0; kt < NK; ++kt) Im::put(lds + kt * Im::TILE, g, i, vf[kt]);
+  order_lds();
+  s16x4 vc[NK][CT];
+#pragma unroll
+  for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) vc[kt][ct] = Im::get(lds + kt * Im::TILE, g, i, ct);
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  f32x4 absent;                              // of the last key tile: -inf where there is no key
+#pragma unroll
+  for (int r = 0; r < 4; ++r) absent[r] = (NK - 1) * 16 + 4 * g + r < Tk ? 0.f : -INFINITY;
+  const float c = a.scale * LOG2E;
+  for (int qt = 0; qt < nq; ++qt) {
+    const int64_t tnext = tq_[(qt + 1 < nq ? qt + 1 : qt) * 16 + i];
+    const Piece<FR> qnext = load_piece<FR>(q + tnext * a.ldq * 2);
+    f32x4 st[NK];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < NK; ++kt) st[kt] = over_channels<FR>(kf[kt], qf, kt == NK - 1 ? absent : zero);
+#pragma unroll
+    for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[kt][r]);
+    mx = column_max(mx) * c;
+    float l = 0.f;
+    s16x4 p[NK];
+#pragma unroll
+    for (int kt = 0; kt < NK; ++kt) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        st[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[kt][r], c, -mx));
+        l += st[kt][r];
+      }
+      p[kt] = pack4(st[kt]);
+    }
+    l = column_sum(l);
+    f32x4 o[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      o[ct] = zero;
+      if constexpr (NK >= 2) o[ct] = over_tokens(vc[0][ct], vc[1][ct], p[0], p[1], o[ct]);
+      if constexpr (NK == 4) o[ct] = over_tokens(vc[2][ct], vc[3][ct], p[2], p[3], o[ct]);
+      if constexpr (NK == 3) o[ct] = over_tokens(vc[2][ct], s16x4{0, 0, 0, 0}, p[2], s16x4{0, 0, 0, 0}, o[ct]);
+      if constexpr (NK == 1) o[ct] = over_tokens(vc[0][ct], p[0], o[ct]);
+    }
+    const float inv = __builtin_amdgcn_rcpf(l);
+    if (qt * 16 + i < Tq) {
+      store_piece<FR>(out + tq * a.ldo * 2, o, inv);
+      if (g == 0) a.lse[tq * a.nhead + head] = mx + __builtin_amdgcn_logf(l);
+    }
+    tq = tnext;
+    qf = qnext;
+  }
+}
+
+template <int DH, int NK>
+__device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq_, const int* tk_, int Tq, int Tk, int head, char* lds) {
+  using Im = Image<DH>;
+  constexpr int FR = Im::FR, CT = Im::CT, TP = TILE_PITCH;
+  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+  const int64_t col = (int64_t)head * DH * 2 + FR * 2 * g;
+  const char *q = (const char*)a.q + col, *k = (const char*)a.k + col, *v = (const char*)a.v + col, *gr = (const char*)a.g + col;
+  const int nq = (Tq + 15) >> 4;
+  Piece<FR> kf[NK], vf[NK];
+#pragma unroll
+  for (int kt = 0; kt < NK; ++kt) {
+    const int64_t t = tk_[kt * 16 + i];
+    kf[kt] = load_piece<FR>(k + t * a.ldk * 2);
+    vf[kt] = load_piece<FR>(v + t * a.ldv * 2);
+  }
+  int64_t tq = tq_[i];
+  Piece<FR> qf = load_piece<FR>(q + tq * a.ldq * 2), gf = load_piece<FR>(gr + tq * a.ldg * 2);
+  float ls = a.lse[tq * a.nhead + head];
+#pragma unroll
+  for (int kt = 0; kt < NK; ++kt) Im::put(lds + kt * Im::TILE, g, i, kf[kt]);
+  order_lds();
+  s16x4 kc[NK][CT];
+#pragma unroll
+  for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) kc[kt][ct] = Im::get(lds + kt * Im::TILE, g, i, ct);
+  order_lds();
+  // from here on: the query tile's q and dO rows, and the P and dS tiles of every key tile
+  char *qimg = lds, *gimg = lds + Im::TILE, *tiles = lds + 2 * Im::TILE;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  f32x4 absent;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) absent[r] = (NK - 1) * 16 + 4 * g + r < Tk ? 0.f : -INFINITY;
+  const float c = a.scale * LOG2E;
+  f32x4 dk[NK][CT], dv[NK][CT];
+#pragma unroll
+  for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) dk[kt][ct] = dv[kt][ct] = zero;
+  for (int qt = 0; qt < nq; ++qt) {
+    const int64_t tnext = tq_[(qt + 1 < nq ? qt + 1 : qt) * 16 + i];
+    const Piece<FR> qnext = load_piece<FR>(q + tnext * a.ldq * 2), gnext = load_piece<FR>(gr + tnext * a.ldg * 2);
+    const float lsnext = a.lse[tnext * a.nhead + head];
+    Im::put(qimg, g, i, qf);
+    Im::put(gimg, g, i, gf);
+    order_lds();
+    s16x4 qc[CT], gc[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      qc[ct] = Im::get(qimg, g, i, ct);
+      gc[ct] = Im::get(gimg, g, i, ct);
+    }
+    order_lds();
+    const float le = qt * 16 + i < Tq ? ls : INFINITY;           // no query: P = 0
+    f32x4 p[NK], dp[NK];
+    float d = 0.f;
+#pragma unroll
+    for (int kt = 0; kt < NK; ++kt) {
+      p[kt] = over_channels<FR>(kf[kt], qf, kt == NK - 1 ? absent : zero);           // rows = keys, column = query i
+      dp[kt] = over_channels<FR>(vf[kt], gf, zero);
+    }
+#pragma unroll
+    for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        p[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[kt][r], c, -le));
+        d = __builtin_fmaf(p[kt][r], dp[kt][r], d);
+      }
+    d = column_sum(d);
+    s16x4 ds[NK];
+#pragma unroll
+    for (int kt = 0; kt < NK; ++kt) {
+      f32x4 t;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) t[r] = p[kt][r] * (dp[kt][r] - d);
+      ds[kt] = pack4(t);
+      *reinterpret_cast<s16x4*>(tiles + (2 * kt) * 16 * TP + i * TP + 8 * g) = pack4(p[kt]);
+      *reinterpret_cast<s16x4*>(tiles + (2 * kt + 1) * 16 * TP + i * TP + 8 * g) = ds[kt];
+    }
+    order_lds();
+    f32x4 dq[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      dq[ct] = zero;
+      if constexpr (NK >= 2) dq[ct] = over_tokens(kc[0][ct], kc[1][ct], ds[0], ds[1], dq[ct]);
+      if constexpr (NK == 4) dq[ct] = over_tokens(kc[2][ct], kc[3][ct], ds[2], ds[3], dq[ct]);
+      if constexpr (NK == 3) dq[ct] = over_tokens(kc[2][ct], s16x4{0, 0, 0, 0}, ds[2], s16x4{0, 0, 0, 0}, dq[ct]);
+      if constexpr (NK == 1) dq[ct] = over_tokens(kc[0][ct], ds[0], dq[ct]);
+    }
+#pragma unroll
+    for (int kt = 0; kt < NK; ++kt) {
+      const s16x4 pt = read_columns(tiles + (2 * kt) * 16 * TP + (4 * g + (i >> 2)) * TP + 8 * (i & 3));            // queries 4g.. of key i
+      const s16x4 dt = read_columns(tiles + (2 * kt + 1) * 16 * TP + (4 * g + (i >> 2)) * TP + 8 * (i & 3));
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        dv[kt][ct] = over_tokens(gc[ct], pt, dv[kt][ct]);
+        dk[kt][ct] = over_tokens(qc[ct], dt, dk[kt][ct]);
+      }
+    }
+    order_lds();
+    if (qt * 16 + i < Tq) store_piece<FR>((char*)a.dq + col + tq * a.lddq * 2, dq, a.scale);
+    tq = tnext;
+    qf = qnext;
+    gf = gnext;
+    ls = lsnext;
+  }
+#pragma unroll
+  for (int kt = 0; kt < NK; ++kt)
+    if (kt * 16 + i < Tk) {
+      const int64_t t = tk_[kt * 16 + i];
+      store_piece<FR>((char*)a.dk + col + t * a.lddk * 2, dk[kt], a.scale);
+      store_piece<FR>((char*)a.dv + col + t * a.lddv * 2, dv[kt], 1.f);
+    }
+}
+
+template <int DH, int NT> constexpr int lds_bytes(bool bwd) {            // of one wave
+  const int image = NT * Image<DH>::TILE, rest = 2 * Image<DH>::TILE + NT * 2 * 16 * TILE_PITCH;
+  return !bwd || image > rest ? image : rest;
+}
+
+// A window of up to 16 NT tokens per workgroup, a head per wave; without a work list (NT = 4) every window, empty ones included.
+// Two waves per SIMD as the bound: 256 registers at most, and the matrix instructions then write plain vector registers.
+template <int DH, int NT, bool BWD>
+__global__ __launch_bounds__(256, 2) void dot_window_kernel(DotArgs a, int cls) {
+  constexpr int BYTES = lds_bytes<DH, NT>(BWD);
+  __shared__ int toks[2][64];
+  __shared__ __attribute__((aligned(16))) char lds[4][BYTES];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  Window win;
+  if (!find_window(a, cls, toks, win)) return;
+  __syncthreads();
+  const int head = blockIdx.y * 4 + w;
+  if (head >= a.nhead) return;
+  const int Tq = win.Tq < NT * 16 ? win.Tq : NT * 16, Tk = win.Tk < NT * 16 ? win.Tk : NT * 16;
+  if (Tq == 0 || Tk == 0) {
+    const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+    if (lane < Tq) {
+      uint4* o = reinterpret_cast<uint4*>(BWD ? (char*)a.dq + (toks[0][lane] * a.lddq + head * DH) * 2 : (char*)a.o + (toks[0][lane] * a.ldo + head * DH) * 2);
+      for (int c = 0; c < DH / 8; ++c) o[c] = z;
+    }
+    if (BWD && lane < Tk) {
+      uint4 *p = reinterpret_cast<uint4*>((char*)a.dk + (toks[1][lane] * a.lddk + head * DH) * 2),
+            *r = reinterpret_cast<uint4*>((char*)a.dv + (toks[1][lane] * a.lddv + head * DH) * 2);
+      for (int c = 0; c < DH / 8; ++c) { p[c] = z; r[c] = z; }
+    }
+    return;
+  }
+  const int nk = (Tk + 15) >> 4;
+#define ONE(NK)                                                                     \
+  if constexpr (BWD) bwd_window<DH, NK>(a, toks[0], toks[1], Tq, Tk, head, lds[w]); \
+  else fwd_window<DH, NK>(a, toks[0], toks[1], Tq, Tk, head, lds[w])
+  if (nk == 1) { ONE(1); }
+  else if (NT == 2 || nk == 2) { ONE(2); }
+  else if constexpr (NT == 4) {
+    if (nk == 3) { ONE(3); } else { ONE(4); }
+  }
+#undef ONE
+}
+
 // The windows that are in no list: zero rows for queries without a key (out, or dq) and for keys without a query (dk, dv).  One wave per
 // window, a lane per cell.
 __global__ __launch_bounds__(256) void dot_orphan_kernel(DotArgs a, char* q0, int64_t ldq0, char* k0, int64_t ldk0, char* k1, int64_t ldk1,
@@ -346,15 +687,26 @@ int fill(DotArgs& a, int dtype, int64_t mq, int64_t mk, int nhead, int dh, const
   return TMAE_OK;
 }
 
-template <class F> void by_head(int dtype, int dh, F&& f) {
-  auto with = [&](auto t) {
-    using T = decltype(t);
-    if (dh == 16) f(T(), std::integral_constant<int, 16>());
-    else if (dh == 32) f(T(), std::integral_constant<int, 32>());
-    else f(T(), std::integral_constant<int, 64>());
-  };
-  if (dtype == TMAE_BF16) with(__hip_bfloat16()); else with(0.f);
+template <class F> void by_head(int dh, F&& f) {
+  if (dh == 16) f(std::integral_constant<int, 16>());
+  else if (dh == 32) f(std::integral_constant<int, 32>());
+  else f(std::integral_constant<int, 64>());
 }
+template <int DH, bool BWD> void launch_bf16(const DotArgs& a, hipStream_t stream) {
+  const unsigned gy = (unsigned)((a.nhead + 3) / 4);
+  if (!a.wl) {
+    hipLaunchKernelGGL((dot_window_kernel<DH, 4, BWD>), dim3((unsigned)a.nwin, gy), dim3(256), 0, stream, a, 0);
+    return;
+  }
+  const int64_t b3 = class_blocks(3, a.nwin, a.mq, a.mk), b2 = class_blocks(2, a.nwin, a.mq, a.mk);
+  if (b3 > 0) hipLaunchKernelGGL((dot_window_kernel<DH, 4, BWD>), dim3((unsigned)b3, gy), dim3(256), 0, stream, a, 3);
+  if (b2 > 0) hipLaunchKernelGGL((dot_window_kernel<DH, 2, BWD>), dim3((unsigned)b2, gy), dim3(256), 0, stream, a, 2);
+  for (int cls = 1; cls >= 0; --cls) {
+    const int64_t b = class_blocks(cls, a.nwin, a.mq, a.mk);
+    if (b > 0) hipLaunchKernelGGL((dot_window_kernel<DH, 2, BWD>), dim3((unsigned)b, gy), dim3(256), 0, stream, a, cls);
+  }
+}
+
 template <class F> void by_class(const DotArgs& a, F&& f) {
   const unsigned gy = (unsigned)((a.nhead + 3) / 4);
   if (!a.wl) { f(dim3((unsigned)a.nwin, gy), 0); return; }
@@ -380,10 +732,13 @@ int tmae_win_attn_dot_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk
   if (worklist && grid_q != grid_k)
     hipLaunchKernelGGL(dot_orphan_kernel, dim3(tmae_cdiv(a.nwin, 4)), dim3(256), 0, (hipStream_t)stream, a, (char*)out, ldo * es, nullptr,
                        (int64_t)0, nullptr, (int64_t)0, d * es / 16);
-  by_head(dtype, dh, [&](auto t, auto w) {
-    by_class(a, [&](dim3 grid, int cls) {
-      hipLaunchKernelGGL((dot_fwd_kernel<decltype(t), decltype(w)::value>), grid, dim3(256), 0, (hipStream_t)stream, a, cls);
-    });
+  by_head(dh, [&](auto w) {
+    constexpr int DH = decltype(w)::value;
+    if (dtype == TMAE_BF16) launch_bf16<DH, false>(a, (hipStream_t)stream);
+    else
+      by_class(a, [&](dim3 grid, int cls) {
+        hipLaunchKernelGGL((dot_fwd_kernel<float, DH>), grid, dim3(256), 0, (hipStream_t)stream, a, cls);
+      });
   });
   return tmae_launch_status();
 }
@@ -405,10 +760,13 @@ int tmae_win_attn_dot_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk
   if (worklist && grid_q != grid_k)
     hipLaunchKernelGGL(dot_orphan_kernel, dim3(tmae_cdiv(a.nwin, 4)), dim3(256), 0, (hipStream_t)stream, a, (char*)dq, lddq * es,
                        (char*)dk, lddk * es, (char*)dv, lddv * es, d * es / 16);
-  by_head(dtype, dh, [&](auto t, auto w) {
-    by_class(a, [&](dim3 grid, int cls) {
-      hipLaunchKernelGGL((dot_bwd_kernel<decltype(t), decltype(w)::value>), grid, dim3(256), 0, (hipStream_t)stream, a, cls);
-    });
+  by_head(dh, [&](auto w) {
+    constexpr int DH = decltype(w)::value;
+    if (dtype == TMAE_BF16) launch_bf16<DH, true>(a, (hipStream_t)stream);
+    else
+      by_class(a, [&](dim3 grid, int cls) {
+        hipLaunchKernelGGL((dot_bwd_kernel<float, DH>), grid, dim3(256), 0, (hipStream_t)stream, a, cls);
+      });
   });
   return tmae_launch_status();
 }

@@ -15,7 +15,7 @@ previous statement -- -inf for an absent query, hence 0 * -inf = NaN in dK and g
 
 What is checked: for every v_mfma, every path of instructions that follows it (both sides of conditional branches) until the
 required number of wait states has passed; an instruction on such a path that names a VGPR of the MFMA's destination is reported
-(a dependent MFMA is checked for SrcA / SrcB only: SrcC and back-to-back accumulation are interlocked).  A taken branch is counted
+(a dependent MFMA of the same shape is checked for SrcA / SrcB only: SrcC and back-to-back accumulation are interlocked).  A taken branch is counted
 as ONE wait state, like the compiler does.  Required wait states per MFMA shape: what the compiler pads with in straight-line
 code (need_states)."""
 import glob
@@ -41,17 +41,22 @@ def need_states(op):
     return {4: 5, 16: 8, 32: 12}.get(mm, 19)
 
 
-_VREG = re.compile(r'\bv\[(\d+):(\d+)\]|\bv(\d+)\b')
+_VREG = re.compile(r'\b([va])\[(\d+):(\d+)\]|\b([va])(\d+)\b')
 
 
 def vregs(text):
+    """the vector registers named: v as their numbers, a (accumulation registers) from 1000 on"""
     out = set()
-    for a, b, c in _VREG.findall(text):
+    for f, a, b, f1, c in _VREG.findall(text):
         if c:
-            out.add(int(c))
+            out.add(int(c) + (1000 if f1 == 'a' else 0))
         else:
-            out.update(range(int(a), int(b) + 1))
+            out.update(r + (1000 if f == 'a' else 0) for r in range(int(a), int(b) + 1))
     return out
+
+
+def _shape(op):
+    return re.match(r'v_s?mfma\w*?_(\d+x\d+x\d+)', op).group(1)
 
 
 def parse_functions(asm_text):
@@ -103,7 +108,9 @@ def check_function(name, ins):
                     break
                 if o2.startswith('v_mfma'):
                     ops = [x.strip() for x in a2.split(',')]
-                    touched = vregs(','.join(ops[1:3])) & dst          # SrcA / SrcB only
+                    # SrcA / SrcB; SrcC too where the shape differs (an accumulation across shapes, right behind the first product and
+                    # with its registers reused behind the second, has given wrong values: it is kept apart like any other reader)
+                    touched = vregs(','.join(ops[1:3 if _shape(o2) == _shape(op) else 4])) & dst
                 elif o2.startswith(('s_', ';')):
                     touched = set()
                 else:
