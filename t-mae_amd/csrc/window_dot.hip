@@ -305,7 +305,7 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_kernel(DotArgs a, int cls) {
 //
 // A wave holds the NK key tiles of its window and walks the query tiles; NK is a template parameter, so no branch stands between a
 // matrix instruction and its reader.  Windows of at most 16 tokens (three quarters of an outdoor scene's, with two fifths of the tokens):
-// one wave takes HG heads of the window, whose rows it requests together.
+// one wave takes up to four heads of the window at once, whose rows it requests together.
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -315,7 +315,6 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int HG = 4;
 constexpr int TILE_PITCH = 40;             // bytes per row of a 16x16 bfloat16 tile in LDS
 
 __device__ __forceinline__ unsigned pack2(float a, float b) {
@@ -635,6 +634,176 @@ __global__ __launch_bounds__(256, 2) void dot_window_kernel(DotArgs a, int cls) 
 #undef ONE
 }
 
+// Windows of at most 16 tokens: a window per wave, HG heads of it at a time.  Nothing is shared between the waves of a workgroup.
+template <int DH> constexpr int heads_at_once() { return DH == 16 ? 4 : DH == 32 ? 2 : 1; }
+
+template <int DH, bool BWD>
+__global__ __launch_bounds__(256, 2) void dot_small_kernel(DotArgs a) {
+  using Im = Image<DH>;
+  constexpr int FR = Im::FR, CT = Im::CT, HG = heads_at_once<DH>(), TP = TILE_PITCH;
+  constexpr int PER_HEAD = (BWD ? 3 : 1) * Im::TILE > (BWD ? 2 * 16 * TP : 0) ? (BWD ? 3 : 1) * Im::TILE : 2 * 16 * TP;
+  __shared__ int toks_[4][2][16];
+  __shared__ __attribute__((aligned(16))) char lds_[4][HG * PER_HEAD];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
+  // list 1 first (9 to 16 tokens), then list 0
+  const int64_t e = (int64_t)blockIdx.x * 4 + w, n1 = a.wl[1] < a.nwin ? a.wl[1] : a.nwin, n0 = a.wl[0] < a.nwin ? a.wl[0] : a.nwin;
+  if (e >= n1 + n0) return;
+  const int packed = a.wl[WL_HDR + (e < n1 ? a.nwin + e : e - n1)];
+  const int b = packed >> 16, wcx = (packed >> 8) & 255, wcy = packed & 255;
+  const int y = wcy * WIN - a.s + (lane >> 3), x = wcx * WIN - a.s + (lane & 7);
+  const bool in = b >= 0 && b < a.batch && y >= 0 && y < a.ny && x >= 0 && x < a.nx;
+  const int64_t cell = ((int64_t)b * a.ny + y) * a.nx + x;
+  int t0 = in ? a.grid_q[cell] : -1, t1 = in ? a.grid_k[cell] : -1;
+  if (t0 >= a.mq) t0 = -1;
+  if (t1 >= a.mk) t1 = -1;
+  const unsigned long long m0 = __ballot(t0 >= 0), m1 = __ballot(t1 >= 0), below = (1ull << lane) - 1ull;
+  const int Tq = min(__popcll(m0), 16), Tk = min(__popcll(m1), 16);
+  if (Tq == 0 || Tk == 0) return;                        // (in no list: the rows are zeroed elsewhere)
+  int (*toks)[16] = toks_[w];
+  char* lds = lds_[w];
+  const int f0 = __shfl(t0, __ffsll(m0) - 1, 64), f1 = __shfl(t1, __ffsll(m1) - 1, 64);
+  if (lane < 16) { toks[0][lane] = f0; toks[1][lane] = f1; }
+  order_lds();
+  const int r0 = __popcll(m0 & below), r1 = __popcll(m1 & below);
+  if (t0 >= 0 && r0 < 16) toks[0][r0] = t0;
+  if (t1 >= 0 && r1 < 16) toks[1][r1] = t1;
+  order_lds();
+  const int64_t tq = toks[0][i], tk = toks[1][i];
+  const float c = a.scale * LOG2E;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  f32x4 absent;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) absent[r] = 4 * g + r < Tk ? 0.f : -INFINITY;
+  const int64_t at = FR * 2 * g;
+  const char *q = (const char*)a.q + tq * a.ldq * 2 + at, *k = (const char*)a.k + tk * a.ldk * 2 + at, *v = (const char*)a.v + tk * a.ldv * 2 + at;
+  const char* gr = BWD ? (const char*)a.g + tq * a.ldg * 2 + at : nullptr;
+  for (int h0 = 0; h0 < a.nhead; h0 += HG) {
+    Piece<FR> kf[HG], vf[HG], qf[HG], gf[HG];
+    float ls[HG];
+#pragma unroll
+    for (int h = 0; h < HG; ++h) {
+      const int hh = h0 + h < a.nhead ? h0 + h : a.nhead - 1;            // a head behind the last one: read twice, stored once
+      kf[h] = load_piece<FR>(k + hh * DH * 2);
+      vf[h] = load_piece<FR>(v + hh * DH * 2);
+      qf[h] = load_piece<FR>(q + hh * DH * 2);
+      if constexpr (BWD) {
+        gf[h] = load_piece<FR>(gr + hh * DH * 2);
+        ls[h] = a.lse[tq * a.nhead + hh];
+      }
+    }
+    if constexpr (!BWD) {
+#pragma unroll
+      for (int h = 0; h < HG; ++h) Im::put(lds + h * PER_HEAD, g, i, vf[h]);
+      order_lds();
+      s16x4 vc[HG][CT], p[HG];
+#pragma unroll
+      for (int h = 0; h < HG; ++h)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) vc[h][ct] = Im::get(lds + h * PER_HEAD, g, i, ct);
+      order_lds();
+      f32x4 st[HG];
+      float mx[HG], l[HG];
+#pragma unroll
+      for (int h = 0; h < HG; ++h) st[h] = over_channels<FR>(kf[h], qf[h], absent);
+#pragma unroll
+      for (int h = 0; h < HG; ++h) {
+        mx[h] = column_max(fmaxf(fmaxf(st[h][0], st[h][1]), fmaxf(st[h][2], st[h][3]))) * c;
+        l[h] = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          st[h][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[h][r], c, -mx[h]));
+          l[h] += st[h][r];
+        }
+        p[h] = pack4(st[h]);
+      }
+#pragma unroll
+      for (int h = 0; h < HG; ++h) {
+        f32x4 o[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) o[ct] = over_tokens(vc[h][ct], p[h], zero);
+        const float s = column_sum(l[h]);
+        if (i < Tq && h0 + h < a.nhead) {
+          store_piece<FR>((char*)a.o + tq * a.ldo * 2 + (h0 + h) * DH * 2 + at, o, __builtin_amdgcn_rcpf(s));
+          if (g == 0) a.lse[tq * a.nhead + h0 + h] = mx[h] + __builtin_amdgcn_logf(s);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < HG; ++h) {
+        char* im = lds + h * PER_HEAD;
+        Im::put(im, g, i, kf[h]);
+        Im::put(im + Im::TILE, g, i, qf[h]);
+        Im::put(im + 2 * Im::TILE, g, i, gf[h]);
+      }
+      order_lds();
+      s16x4 kc[HG][CT], qc[HG][CT], gc[HG][CT], ds[HG], pb[HG];
+#pragma unroll
+      for (int h = 0; h < HG; ++h) {
+        const char* im = lds + h * PER_HEAD;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          kc[h][ct] = Im::get(im, g, i, ct);
+          qc[h][ct] = Im::get(im + Im::TILE, g, i, ct);
+          gc[h][ct] = Im::get(im + 2 * Im::TILE, g, i, ct);
+        }
+      }
+      order_lds();
+      f32x4 p[HG], dp[HG];
+#pragma unroll
+      for (int h = 0; h < HG; ++h) {
+        p[h] = over_channels<FR>(kf[h], qf[h], absent);
+        dp[h] = over_channels<FR>(vf[h], gf[h], zero);
+      }
+#pragma unroll
+      for (int h = 0; h < HG; ++h) {
+        const float le = i < Tq ? ls[h] : INFINITY;
+        float d = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          p[h][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[h][r], c, -le));
+          d = __builtin_fmaf(p[h][r], dp[h][r], d);
+        }
+        d = column_sum(d);
+        f32x4 t;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t[r] = p[h][r] * (dp[h][r] - d);
+        ds[h] = pack4(t);
+        pb[h] = pack4(p[h]);
+        char* im = lds + h * PER_HEAD;
+        *reinterpret_cast<s16x4*>(im + i * TP + 8 * g) = pb[h];
+        *reinterpret_cast<s16x4*>(im + 16 * TP + i * TP + 8 * g) = ds[h];
+      }
+      order_lds();
+      s16x4 pt[HG], dt[HG];
+#pragma unroll
+      for (int h = 0; h < HG; ++h) {
+        const char* im = lds + h * PER_HEAD;
+        pt[h] = read_columns(im + (4 * g + (i >> 2)) * TP + 8 * (i & 3));
+        dt[h] = read_columns(im + 16 * TP + (4 * g + (i >> 2)) * TP + 8 * (i & 3));
+      }
+      order_lds();
+#pragma unroll
+      for (int h = 0; h < HG; ++h) {
+        f32x4 dq[CT], dk[CT], dv[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          dq[ct] = over_tokens(kc[h][ct], ds[h], zero);
+          dv[ct] = over_tokens(gc[h][ct], pt[h], zero);
+          dk[ct] = over_tokens(qc[h][ct], dt[h], zero);
+        }
+        const int64_t hcol = (int64_t)(h0 + h) * DH * 2 + at;
+        if (h0 + h < a.nhead) {
+          if (i < Tq) store_piece<FR>((char*)a.dq + tq * a.lddq * 2 + hcol, dq, a.scale);
+          if (i < Tk) {
+            store_piece<FR>((char*)a.dk + tk * a.lddk * 2 + hcol, dk, a.scale);
+            store_piece<FR>((char*)a.dv + tk * a.lddv * 2 + hcol, dv, 1.f);
+          }
+        }
+      }
+    }
+  }
+}
+
 // The windows that are in no list: zero rows for queries without a key (out, or dq) and for keys without a query (dk, dv).  One wave per
 // window, a lane per cell.
 __global__ __launch_bounds__(256) void dot_orphan_kernel(DotArgs a, char* q0, int64_t ldq0, char* k0, int64_t ldk0, char* k1, int64_t ldk1,
@@ -701,10 +870,9 @@ template <int DH, bool BWD> void launch_bf16(const DotArgs& a, hipStream_t strea
   const int64_t b3 = class_blocks(3, a.nwin, a.mq, a.mk), b2 = class_blocks(2, a.nwin, a.mq, a.mk);
   if (b3 > 0) hipLaunchKernelGGL((dot_window_kernel<DH, 4, BWD>), dim3((unsigned)b3, gy), dim3(256), 0, stream, a, 3);
   if (b2 > 0) hipLaunchKernelGGL((dot_window_kernel<DH, 2, BWD>), dim3((unsigned)b2, gy), dim3(256), 0, stream, a, 2);
-  for (int cls = 1; cls >= 0; --cls) {
-    const int64_t b = class_blocks(cls, a.nwin, a.mq, a.mk);
-    if (b > 0) hipLaunchKernelGGL((dot_window_kernel<DH, 2, BWD>), dim3((unsigned)b, gy), dim3(256), 0, stream, a, cls);
-  }
+  int64_t small = a.mq < a.mk ? a.mq : a.mk;             // a listed window holds a query and a key
+  if (small > a.nwin) small = a.nwin;
+  if (small > 0) hipLaunchKernelGGL((dot_small_kernel<DH, BWD>), dim3(tmae_cdiv(small, 4)), dim3(256), 0, stream, a);
 }
 
 template <class F> void by_class(const DotArgs& a, F&& f) {
