@@ -33,40 +33,89 @@ struct DotArgs {
   float scale;
 };
 
-struct Window { int Tq, Tk; };
-
-// The window's tokens in cell order, into toks[0] (queries) and toks[1] (keys); slots behind the last token repeat the first one.
-// A row number outside the tensors counts as an empty cell.  False: the block has no window.
-__device__ __forceinline__ bool find_window(const DotArgs& a, int cls, int (*toks)[64], Window& w) {
-  const int lane = threadIdx.x & 63;
-  int b, wcy, wcx;
-  if (a.wl) {
-    const int64_t cnt = a.wl[cls];
-    if ((int64_t)blockIdx.x >= cnt || (int64_t)blockIdx.x >= a.nwin) return false;
-    const int p = a.wl[WL_HDR + cls * a.nwin + blockIdx.x];
-    b = p >> 16; wcx = (p >> 8) & 255; wcy = p & 255;
-  } else {
-    const unsigned u = blockIdx.x;
-    wcy = (int)(u % (unsigned)a.Wy); wcx = (int)((u / (unsigned)a.Wy) % (unsigned)a.Wx); b = (int)(u / (unsigned)(a.Wy * a.Wx));
-  }
-  const int y = wcy * WIN - a.s + (lane >> 3), x = wcx * WIN - a.s + (lane & 7);
-  const bool in = b >= 0 && b < a.batch && y >= 0 && y < a.ny && x >= 0 && x < a.nx;
-  const int64_t cell = ((int64_t)b * a.ny + y) * a.nx + x;
-  int tq = in ? a.grid_q[cell] : -1, tk = in ? a.grid_k[cell] : -1;
-  if (tq >= a.mq) tq = -1;
-  if (tk >= a.mk) tk = -1;
-  const unsigned long long mq = __ballot(tq >= 0), mk = __ballot(tk >= 0), below = (1ull << lane) - 1ull;
-  w.Tq = __popcll(mq);
-  w.Tk = __popcll(mk);
-  const int fq = mq ? __shfl(tq, __ffsll(mq) - 1, 64) : -1, fk = mk ? __shfl(tk, __ffsll(mk) - 1, 64) : -1;
-  if (threadIdx.x < 64) {
-    if (lane >= w.Tq) toks[0][lane] = fq;
-    if (lane >= w.Tk) toks[1][lane] = fk;
-    if (tq >= 0) toks[0][__popcll(mq & below)] = tq;
-    if (tk >= 0) toks[1][__popcll(mk & below)] = tk;
-  }
-  return true;
+// LDS operations of a wave execute in order: this keeps the compiler to the order they are written in.  Every wave works in a piece of
+// LDS of its own; no workgroup barrier is needed anywhere.
+__device__ __forceinline__ void order_lds() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
+
+// The windows of a launch: those of the work list's classes `from`, `from` - 1, ... `to` one after the other (larger windows first), or
+// every window of the grids where there is no list.  A wave takes every step-th one and requests the cells of the next one before it
+// works on the present one: the list's entry, the cells and the rows are three loads that wait for each other.
+struct Walk {
+  int64_t n, e, step;
+  int from, to;
+  int tq, tk;                              // this lane's cell of the present window: row numbers, -1 where it is empty
+  int nq, nk;                              // ... of the next one
+  int entry;                               // the list's entry behind that
+
+  __device__ __forceinline__ int entry_at(const DotArgs& a, int64_t e) const {
+    int cls = from;
+    for (; cls > to; --cls) {
+      const int64_t c = count(a, cls);
+      if (e < c) break;
+      e -= c;
+    }
+    return a.wl[WL_HDR + cls * a.nwin + e];
+  }
+  __device__ __forceinline__ static int64_t count(const DotArgs& a, int cls) {
+    const int64_t c = a.wl[cls];
+    return c < 0 ? 0 : c < a.nwin ? c : a.nwin;
+  }
+  // the cells of window e (its list entry, where there is a list); a row number outside the tensors counts as an empty cell
+  __device__ __forceinline__ void cells(const DotArgs& a, int64_t e, int entry, int& q, int& k) const {
+    const int lane = threadIdx.x & 63;
+    int b, wcy, wcx;
+    if (a.wl) {
+      b = entry >> 16; wcx = (entry >> 8) & 255; wcy = entry & 255;
+    } else {
+      const unsigned u = (unsigned)e;
+      wcy = (int)(u % (unsigned)a.Wy); wcx = (int)((u / (unsigned)a.Wy) % (unsigned)a.Wx); b = (int)(u / (unsigned)(a.Wy * a.Wx));
+    }
+    const int y = wcy * WIN - a.s + (lane >> 3), x = wcx * WIN - a.s + (lane & 7);
+    const bool in = b >= 0 && b < a.batch && y >= 0 && y < a.ny && x >= 0 && x < a.nx;
+    const int64_t cell = ((int64_t)b * a.ny + y) * a.nx + x;
+    q = in ? a.grid_q[cell] : -1;
+    k = in ? a.grid_k[cell] : -1;
+  }
+  __device__ __forceinline__ Walk(const DotArgs& a, int from_, int to_, int64_t first, int64_t step_) : e(first), step(step_), from(from_), to(to_) {
+    n = a.nwin;
+    if (a.wl) {
+      n = 0;
+      for (int c = from; c >= to; --c) n += count(a, c);
+    }
+    tq = tk = nq = nk = -1;
+    entry = 0;
+    if (e < n) cells(a, e, a.wl ? entry_at(a, e) : 0, nq, nk);
+    if (a.wl && e + step < n) entry = entry_at(a, e + step);
+    e -= step;
+  }
+  __device__ __forceinline__ bool next(const DotArgs& a) {
+    e += step;
+    if (e >= n) return false;
+    tq = nq < a.mq ? nq : -1;
+    tk = nk < a.mk ? nk : -1;
+    if (e + step < n) cells(a, e + step, entry, nq, nk);
+    if (a.wl && e + 2 * step < n) entry = entry_at(a, e + 2 * step);
+    return true;
+  }
+  // the tokens in cell order into toks[0] (queries) and toks[1] (keys), at most `most` of each; the slots behind repeat the first one
+  __device__ __forceinline__ void tokens(int (*toks)[64], int most, int& Tq, int& Tk) const {
+    const int lane = threadIdx.x & 63;
+    const unsigned long long q = __ballot(tq >= 0), k = __ballot(tk >= 0), below = (1ull << lane) - 1ull;
+    Tq = min(__popcll(q), most);
+    Tk = min(__popcll(k), most);
+    const int fq = q ? __shfl(tq, __ffsll(q) - 1, 64) : -1, fk = k ? __shfl(tk, __ffsll(k) - 1, 64) : -1;
+    order_lds();
+    if (lane >= Tq) toks[0][lane] = fq;
+    if (lane >= Tk) toks[1][lane] = fk;
+    if (tq >= 0 && __popcll(q & below) < most) toks[0][__popcll(q & below)] = tq;
+    if (tk >= 0 && __popcll(k & below) < most) toks[1][__popcll(k & below)] = tk;
+    order_lds();
+  }
+};
 
 // channels KD g .. KD g + KD - 1 of a token's head: what the lane contributes to a product over the channels
 template <class T, int KD> __device__ __forceinline__ void load_frag(const T* p, float* f);
@@ -110,31 +159,25 @@ __device__ __forceinline__ void accumulate(const T* base, int64_t ld, const int*
     for (int ct = 0; ct < CT; ++ct) c[ct] = __builtin_amdgcn_mfma_f32_16x16x4f32(ld_f<T>(row + 16 * ct), b[r], c[ct], 0, 0, 0);
   }
 }
-__device__ __forceinline__ void order_lds() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 template <class T, int DH>
-__global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a, int cls) {
+__global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
   constexpr int KD = DH / 4, CT = DH / 16;
-  __shared__ int toks[2][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
-  Window win;
-  if (!find_window(a, cls, toks, win)) return;
-  __syncthreads();
+  __shared__ int toks_[4][2][64];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
+  int (*toks)[64] = toks_[w];
   const int head = blockIdx.y * 4 + w;
-  if (head >= a.nhead || win.Tq == 0) return;
+  if (head >= a.nhead) return;
   const int hoff = head * DH;
   T* out = (T*)a.o + hoff;
+  for (Walk walk(a, 3, 0, blockIdx.x, gridDim.x); walk.next(a);) {
+  struct { int Tq, Tk; } win;
+  walk.tokens(toks, 64, win.Tq, win.Tk);
   if (win.Tk == 0) {
     if (lane < win.Tq) {
       T* o = out + (int64_t)toks[0][lane] * a.ldo;
       for (int c = 0; c < DH; ++c) st_f<T>(o + c, 0.f);
-      a.lse[(int64_t)toks[0][lane] * a.nhead + head] = 0.f;
     }
-    return;
+    continue;
   }
   const T *q = (const T*)a.q + hoff, *k = (const T*)a.k + hoff, *v = (const T*)a.v + hoff;
   const int nq = (win.Tq + 15) >> 4, nk = (win.Tk + 15) >> 4;
@@ -183,21 +226,23 @@ __global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a, int cls) {
       if (g == 0) a.lse[tq * a.nhead + head] = mx + __builtin_amdgcn_logf(l);          // v_log_f32: the logarithm to base 2
     }
   }
+  }
 }
 
 template <class T, int DH>
-__global__ __launch_bounds__(256, 2) void dot_bwd_kernel(DotArgs a, int cls) {
+__global__ __launch_bounds__(256, 2) void dot_bwd_kernel(DotArgs a) {
   constexpr int KD = DH / 4, CT = DH / 16;
-  __shared__ int toks[2][64];
+  __shared__ int toks_[4][2][64];
   __shared__ float lse[4][64], dot[4][64];               // of the query slots: saved log2 denominator, sum_j P dP
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
-  Window win;
-  if (!find_window(a, cls, toks, win)) return;
-  __syncthreads();
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
+  int (*toks)[64] = toks_[w];
   const int head = blockIdx.y * 4 + w;
   if (head >= a.nhead) return;
   const int hoff = head * DH;
   T *dq = (T*)a.dq + hoff, *dk = (T*)a.dk + hoff, *dv = (T*)a.dv + hoff;
+  for (Walk walk(a, 3, 0, blockIdx.x, gridDim.x); walk.next(a);) {
+  struct { int Tq, Tk; } win;
+  walk.tokens(toks, 64, win.Tq, win.Tk);
   if (win.Tq == 0 || win.Tk == 0) {
     if (lane < win.Tq) {
       T* p = dq + (int64_t)toks[0][lane] * a.lddq;
@@ -207,7 +252,7 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_kernel(DotArgs a, int cls) {
       T *p = dk + (int64_t)toks[1][lane] * a.lddk, *r = dv + (int64_t)toks[1][lane] * a.lddv;
       for (int c = 0; c < DH; ++c) { st_f<T>(p + c, 0.f); st_f<T>(r + c, 0.f); }
     }
-    return;
+    continue;
   }
   const T *q = (const T*)a.q + hoff, *k = (const T*)a.k + hoff, *v = (const T*)a.v + hoff, *gr = (const T*)a.g + hoff;
   const int nq = (win.Tq + 15) >> 4, nk = (win.Tk + 15) >> 4;
@@ -292,20 +337,19 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_kernel(DotArgs a, int cls) {
       }
     }
   }
+  }
 }
 
 // ------------------------------------------------------------------------------------------------------------------ bfloat16
-// The same products on the bfloat16 matrix instructions.  A lane's piece of a token row -- FR = DH / 4 channels -- is as loaded the
-// operand of the products over the channels (logits, dP).  The products over tokens need a tile by columns: its rows go through LDS
-// (ds_read_b64_tr_b16 returns four rows of one column).  In the image of a row, position 4 a + b of 16-channel tile ct holds channel
-// FR a + 4 ct + b, so that a lane ends with FR consecutive channels of one token and stores them at once.
+// The same products on the bfloat16 matrix instructions.  Their operands want the 16 rows of a tile in 16 neighbouring lanes: loaded that
+// way straight from the tensors, each instruction touches 16 lines per 16 lanes and the cache's tag port is what the kernels wait for
+// (44 accesses per instruction, busy 2/3 of the time; 8-byte pieces of 16 rows).  So rows travel in 16-byte chunks, neighbouring lanes
+// on neighbouring chunks, into row images in LDS, and the operands are read there: pieces of a row for the products over the channels
+// (logits, dP), columns (ds_read_b64_tr_b16 returns four rows of one column) for the products over tokens.  Results go back the same
+// way: into the image, and out in whole rows.
 //
 // P and dS enter their products rounded to bfloat16 (2^-8 of each; sums, maxima and everything else stay float32): their error is
 // that of the results' own rounding.
-//
-// A wave holds the NK key tiles of its window and walks the query tiles; NK is a template parameter, so no branch stands between a
-// matrix instruction and its reader.  Windows of at most 16 tokens (three quarters of an outdoor scene's, with two fifths of the tokens):
-// one wave takes up to four heads of the window at once, whose rows it requests together.
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -315,7 +359,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int TILE_PITCH = 40;             // bytes per row of a 16x16 bfloat16 tile in LDS
+constexpr int TILE_PITCH = 40, TILE_BYTES = 16 * TILE_PITCH;             // a 16x16 bfloat16 tile in LDS
 
 __device__ __forceinline__ unsigned pack2(float a, float b) {
   return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{a, b}, bf16x2));
@@ -338,47 +382,47 @@ __device__ __forceinline__ float column_max(float v) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-template <int FR> struct Piece { unsigned u[FR / 2]; };          // FR channels of a token
-template <int FR> __device__ __forceinline__ Piece<FR> load_piece(const char* p) {
-  Piece<FR> f;
-  if constexpr (FR == 4) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    f.u[0] = v.x; f.u[1] = v.y;
-  } else {
+// One head's columns of a row image, 16 rows (a tile) at a time.
+template <int DH, int PITCH> struct Rows {
+  static constexpr int FR = DH / 4, CT = DH / 16;
+  struct Piece { unsigned u[FR / 2]; };    // of row i: channels 4g.. (DH 16), 8g.. (32), 8g.. and 32 + 8g.. (64)
+  static __device__ __forceinline__ Piece piece(const char* tile, int g, int i) {
+    Piece f;
+    if constexpr (FR == 4) {
+      const uint2 v = *reinterpret_cast<const uint2*>(tile + i * PITCH + 8 * g);
+      f.u[0] = v.x; f.u[1] = v.y;
+    } else {
 #pragma unroll
-    for (int j = 0; j < FR / 8; ++j) {
-      const uint4 v = reinterpret_cast<const uint4*>(p)[j];
-      f.u[4 * j] = v.x; f.u[4 * j + 1] = v.y; f.u[4 * j + 2] = v.z; f.u[4 * j + 3] = v.w;
+      for (int j = 0; j < FR / 8; ++j) {
+        const uint4 v = *reinterpret_cast<const uint4*>(tile + i * PITCH + 64 * j + 16 * g);
+        f.u[4 * j] = v.x; f.u[4 * j + 1] = v.y; f.u[4 * j + 2] = v.z; f.u[4 * j + 3] = v.w;
+      }
     }
+    return f;
   }
-  return f;
-}
-template <int FR> __device__ __forceinline__ void store_piece(char* p, const f32x4* v, float by) {
-  unsigned u[FR / 2];
+  // rows 4g .. 4g + 3 of channel 16 ct + i
+  static __device__ __forceinline__ s16x4 columns(const char* tile, int g, int i, int ct) {
+    return read_columns(tile + (4 * g + (i >> 2)) * PITCH + 32 * ct + 8 * (i & 3));
+  }
+  // the accumulators' layout: channels 16 ct + 4g .. + 3 of row i
+  static __device__ __forceinline__ void put(char* tile, int g, int i, const f32x4* v, float by) {
 #pragma unroll
-  for (int ct = 0; ct < FR / 4; ++ct) {
-    u[2 * ct] = pack2(v[ct][0] * by, v[ct][1] * by);
-    u[2 * ct + 1] = pack2(v[ct][2] * by, v[ct][3] * by);
+    for (int ct = 0; ct < CT; ++ct)
+      *reinterpret_cast<uint2*>(tile + i * PITCH + 32 * ct + 8 * g) = make_uint2(pack2(v[ct][0] * by, v[ct][1] * by), pack2(v[ct][2] * by, v[ct][3] * by));
   }
-  if constexpr (FR == 4) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
-  } else {
+  static __device__ __forceinline__ f32x4 over_channels(const Piece& a, const Piece& b, f32x4 c) {
+    if constexpr (FR == 4) {
+      c = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+    } else {
 #pragma unroll
-    for (int j = 0; j < FR / 8; ++j) reinterpret_cast<uint4*>(p)[j] = make_uint4(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
+      for (int j = 0; j < FR / 8; ++j)
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            __builtin_bit_cast(bf16x8, u32x4{a.u[4 * j], a.u[4 * j + 1], a.u[4 * j + 2], a.u[4 * j + 3]}),
+            __builtin_bit_cast(bf16x8, u32x4{b.u[4 * j], b.u[4 * j + 1], b.u[4 * j + 2], b.u[4 * j + 3]}), c, 0, 0, 0);
+    }
+    return c;
   }
-}
-template <int FR> __device__ __forceinline__ f32x4 over_channels(const Piece<FR>& a, const Piece<FR>& b, f32x4 c) {
-  if constexpr (FR == 4) {
-    c = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
-  } else {
-#pragma unroll
-    for (int j = 0; j < FR / 8; ++j)
-      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-          __builtin_bit_cast(bf16x8, u32x4{a.u[4 * j], a.u[4 * j + 1], a.u[4 * j + 2], a.u[4 * j + 3]}),
-          __builtin_bit_cast(bf16x8, u32x4{b.u[4 * j], b.u[4 * j + 1], b.u[4 * j + 2], b.u[4 * j + 3]}), c, 0, 0, 0);
-  }
-  return c;
-}
+};
 // c += A B over the 16 tokens of one tile, or over the 32 of two (a third tile rides with zeros: one accumulator goes through products
 // of one shape only -- a 16x16x16 right behind the 16x16x32 that it continues has read wrong values)
 __device__ __forceinline__ f32x4 over_tokens(const s16x4& a, const s16x4& b, f32x4 c) {
@@ -389,56 +433,38 @@ __device__ __forceinline__ f32x4 over_tokens(const s16x4& a0, const s16x4& a1, c
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-template <int DH> struct Image {            // rows of a head by token, read by columns
-  static constexpr int FR = DH / 4, CT = DH / 16, PITCH = DH * 2 + 16, TILE = 16 * PITCH;
-  static __device__ __forceinline__ void put(char* tile, int g, int i, const Piece<FR>& f) {
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) *reinterpret_cast<uint2*>(tile + i * PITCH + 32 * ct + 8 * g) = make_uint2(f.u[2 * ct], f.u[2 * ct + 1]);
-  }
-  static __device__ __forceinline__ s16x4 get(const char* tile, int g, int i, int ct) {
-    return read_columns(tile + (4 * g + (i >> 2)) * PITCH + 32 * ct + 8 * (i & 3));
-  }
-};
+// ---- windows of more than 16 tokens: a workgroup per (window, group of heads), a head per wave.  The row images -- K, V, Q and in the
+// backward dO, 16 NT rows of the group's columns -- are the workgroup's; each wave reads and overwrites its own head's columns only.
+template <int DH> constexpr int group_heads() { return DH == 64 ? 2 : 4; }
+template <int DH> constexpr int group_pitch() { return group_heads<DH>() * DH * 2 + 16; }
 
-// One window, one head: NK key tiles against nq query tiles.  toks: the window's token lists in LDS; lds: 16 NK rows of an image.
+// One head: NK key tiles against nq query tiles.  NK is a template parameter, so that no branch stands between a matrix instruction and
+// its reader.  K, V, Q: the head's columns of the images; out replaces Q, lse [slot, heads of the group].
 template <int DH, int NK>
-__device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq_, const int* tk_, int Tq, int Tk, int head, char* lds) {
-  using Im = Image<DH>;
-  constexpr int FR = Im::FR, CT = Im::CT;
+__device__ __forceinline__ void fwd_window(float scale, int Tk, int nq, const char* K, const char* V, char* Q, float* lse) {
+  constexpr int PITCH = group_pitch<DH>(), TILE = 16 * PITCH;
+  using R = Rows<DH, PITCH>;
+  constexpr int CT = R::CT;
   const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
-  const int64_t col = (int64_t)head * DH * 2 + FR * 2 * g;
-  const char *q = (const char*)a.q + col, *k = (const char*)a.k + col, *v = (const char*)a.v + col;
-  char* out = (char*)a.o + col;
-  const int nq = (Tq + 15) >> 4;
-  Piece<FR> kf[NK], vf[NK];
-#pragma unroll
-  for (int kt = 0; kt < NK; ++kt) {
-    const int64_t t = tk_[kt * 16 + i];
-    kf[kt] = load_piece<FR>(k + t * a.ldk * 2);
-    vf[kt] = load_piece<FR>(v + t * a.ldv * 2);
-  }
-  int64_t tq = tq_[i];
-  Piece<FR> qf = load_piece<FR>(q + tq * a.ldq * 2);
-#pragma unroll
-  for (int kt = 0; kt < NK; ++kt) Im::put(lds + kt * Im::TILE, g, i, vf[kt]);
-  order_lds();
+  typename R::Piece kf[NK];
   s16x4 vc[NK][CT];
 #pragma unroll
-  for (int kt = 0; kt < NK; ++kt)
+  for (int kt = 0; kt < NK; ++kt) {
+    kf[kt] = R::piece(K + kt * TILE, g, i);
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) vc[kt][ct] = Im::get(lds + kt * Im::TILE, g, i, ct);
+    for (int ct = 0; ct < CT; ++ct) vc[kt][ct] = R::columns(V + kt * TILE, g, i, ct);
+  }
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   f32x4 absent;                              // of the last key tile: -inf where there is no key
 #pragma unroll
   for (int r = 0; r < 4; ++r) absent[r] = (NK - 1) * 16 + 4 * g + r < Tk ? 0.f : -INFINITY;
-  const float c = a.scale * LOG2E;
+  const float c = scale * LOG2E;
   for (int qt = 0; qt < nq; ++qt) {
-    const int64_t tnext = tq_[(qt + 1 < nq ? qt + 1 : qt) * 16 + i];
-    const Piece<FR> qnext = load_piece<FR>(q + tnext * a.ldq * 2);
+    const typename R::Piece qf = R::piece(Q + qt * TILE, g, i);
     f32x4 st[NK];
     float mx = -INFINITY;
 #pragma unroll
-    for (int kt = 0; kt < NK; ++kt) st[kt] = over_channels<FR>(kf[kt], qf, kt == NK - 1 ? absent : zero);
+    for (int kt = 0; kt < NK; ++kt) st[kt] = R::over_channels(kf[kt], qf, kt == NK - 1 ? absent : zero);
 #pragma unroll
     for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
@@ -465,76 +491,53 @@ __device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq_, con
       if constexpr (NK == 3) o[ct] = over_tokens(vc[2][ct], s16x4{0, 0, 0, 0}, p[2], s16x4{0, 0, 0, 0}, o[ct]);
       if constexpr (NK == 1) o[ct] = over_tokens(vc[0][ct], p[0], o[ct]);
     }
-    const float inv = __builtin_amdgcn_rcpf(l);
-    if (qt * 16 + i < Tq) {
-      store_piece<FR>(out + tq * a.ldo * 2, o, inv);
-      if (g == 0) a.lse[tq * a.nhead + head] = mx + __builtin_amdgcn_logf(l);
-    }
-    tq = tnext;
-    qf = qnext;
+    R::put(Q + qt * TILE, g, i, o, __builtin_amdgcn_rcpf(l));
+    if (g == 0) lse[(qt * 16 + i) * group_heads<DH>()] = mx + __builtin_amdgcn_logf(l);       // v_log_f32: to base 2
   }
 }
 
+// dq replaces Q, dk K and dv V; tiles: the wave's own P and dS tiles, two of each
 template <int DH, int NK>
-__device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq_, const int* tk_, int Tq, int Tk, int head, char* lds) {
-  using Im = Image<DH>;
-  constexpr int FR = Im::FR, CT = Im::CT, TP = TILE_PITCH;
+__device__ __forceinline__ void bwd_window(float scale, int Tq, int Tk, int nq, char* K, char* V, char* Q, const char* G, const float* lse,
+                                           char* tiles) {
+  constexpr int PITCH = group_pitch<DH>(), TILE = 16 * PITCH, TP = TILE_PITCH;
+  using R = Rows<DH, PITCH>;
+  constexpr int CT = R::CT;
   const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
-  const int64_t col = (int64_t)head * DH * 2 + FR * 2 * g;
-  const char *q = (const char*)a.q + col, *k = (const char*)a.k + col, *v = (const char*)a.v + col, *gr = (const char*)a.g + col;
-  const int nq = (Tq + 15) >> 4;
-  Piece<FR> kf[NK], vf[NK];
-#pragma unroll
-  for (int kt = 0; kt < NK; ++kt) {
-    const int64_t t = tk_[kt * 16 + i];
-    kf[kt] = load_piece<FR>(k + t * a.ldk * 2);
-    vf[kt] = load_piece<FR>(v + t * a.ldv * 2);
-  }
-  int64_t tq = tq_[i];
-  Piece<FR> qf = load_piece<FR>(q + tq * a.ldq * 2), gf = load_piece<FR>(gr + tq * a.ldg * 2);
-  float ls = a.lse[tq * a.nhead + head];
-#pragma unroll
-  for (int kt = 0; kt < NK; ++kt) Im::put(lds + kt * Im::TILE, g, i, kf[kt]);
-  order_lds();
+  typename R::Piece kf[NK], vf[NK];
   s16x4 kc[NK][CT];
 #pragma unroll
-  for (int kt = 0; kt < NK; ++kt)
+  for (int kt = 0; kt < NK; ++kt) {
+    kf[kt] = R::piece(K + kt * TILE, g, i);
+    vf[kt] = R::piece(V + kt * TILE, g, i);
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) kc[kt][ct] = Im::get(lds + kt * Im::TILE, g, i, ct);
-  order_lds();
-  // from here on: the query tile's q and dO rows, and the P and dS tiles of every key tile
-  char *qimg = lds, *gimg = lds + Im::TILE, *tiles = lds + 2 * Im::TILE;
+    for (int ct = 0; ct < CT; ++ct) kc[kt][ct] = R::columns(K + kt * TILE, g, i, ct);
+  }
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   f32x4 absent;
 #pragma unroll
   for (int r = 0; r < 4; ++r) absent[r] = (NK - 1) * 16 + 4 * g + r < Tk ? 0.f : -INFINITY;
-  const float c = a.scale * LOG2E;
+  const float c = scale * LOG2E;
   f32x4 dk[NK][CT], dv[NK][CT];
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) dk[kt][ct] = dv[kt][ct] = zero;
   for (int qt = 0; qt < nq; ++qt) {
-    const int64_t tnext = tq_[(qt + 1 < nq ? qt + 1 : qt) * 16 + i];
-    const Piece<FR> qnext = load_piece<FR>(q + tnext * a.ldq * 2), gnext = load_piece<FR>(gr + tnext * a.ldg * 2);
-    const float lsnext = a.lse[tnext * a.nhead + head];
-    Im::put(qimg, g, i, qf);
-    Im::put(gimg, g, i, gf);
-    order_lds();
+    const typename R::Piece qf = R::piece(Q + qt * TILE, g, i), gf = R::piece(G + qt * TILE, g, i);
     s16x4 qc[CT], gc[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      qc[ct] = Im::get(qimg, g, i, ct);
-      gc[ct] = Im::get(gimg, g, i, ct);
+      qc[ct] = R::columns(Q + qt * TILE, g, i, ct);
+      gc[ct] = R::columns(G + qt * TILE, g, i, ct);
     }
-    order_lds();
-    const float le = qt * 16 + i < Tq ? ls : INFINITY;           // no query: P = 0
+    const float le = qt * 16 + i < Tq ? lse[(qt * 16 + i) * group_heads<DH>()] : INFINITY;           // no query: P = 0
     f32x4 p[NK], dp[NK];
     float d = 0.f;
 #pragma unroll
     for (int kt = 0; kt < NK; ++kt) {
-      p[kt] = over_channels<FR>(kf[kt], qf, kt == NK - 1 ? absent : zero);           // rows = keys, column = query i
-      dp[kt] = over_channels<FR>(vf[kt], gf, zero);
+      p[kt] = R::over_channels(kf[kt], qf, kt == NK - 1 ? absent : zero);           // rows = keys, column = query i
+      dp[kt] = R::over_channels(vf[kt], gf, zero);
     }
 #pragma unroll
     for (int kt = 0; kt < NK; ++kt)
@@ -546,15 +549,30 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq_, con
     d = column_sum(d);
     s16x4 ds[NK];
 #pragma unroll
-    for (int kt = 0; kt < NK; ++kt) {
-      f32x4 t;
+    for (int k0 = 0; k0 < NK; k0 += 2) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) t[r] = p[kt][r] * (dp[kt][r] - d);
-      ds[kt] = pack4(t);
-      *reinterpret_cast<s16x4*>(tiles + (2 * kt) * 16 * TP + i * TP + 8 * g) = pack4(p[kt]);
-      *reinterpret_cast<s16x4*>(tiles + (2 * kt + 1) * 16 * TP + i * TP + 8 * g) = ds[kt];
+      for (int kt = k0; kt < (k0 + 2 < NK ? k0 + 2 : NK); ++kt) {
+        f32x4 t;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t[r] = p[kt][r] * (dp[kt][r] - d);
+        ds[kt] = pack4(t);
+        char* tile = tiles + (kt - k0) * 2 * TILE_BYTES;
+        *reinterpret_cast<s16x4*>(tile + i * TP + 8 * g) = pack4(p[kt]);
+        *reinterpret_cast<s16x4*>(tile + TILE_BYTES + i * TP + 8 * g) = ds[kt];
+      }
+      order_lds();
+#pragma unroll
+      for (int kt = k0; kt < (k0 + 2 < NK ? k0 + 2 : NK); ++kt) {
+        const char* tile = tiles + (kt - k0) * 2 * TILE_BYTES + (4 * g + (i >> 2)) * TP + 8 * (i & 3);
+        const s16x4 pt = read_columns(tile), dt = read_columns(tile + TILE_BYTES);               // queries 4g .. of key i
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          dv[kt][ct] = over_tokens(gc[ct], pt, dv[kt][ct]);
+          dk[kt][ct] = over_tokens(qc[ct], dt, dk[kt][ct]);
+        }
+      }
+      order_lds();
     }
-    order_lds();
     f32x4 dq[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
@@ -564,147 +582,190 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq_, con
       if constexpr (NK == 3) dq[ct] = over_tokens(kc[2][ct], s16x4{0, 0, 0, 0}, ds[2], s16x4{0, 0, 0, 0}, dq[ct]);
       if constexpr (NK == 1) dq[ct] = over_tokens(kc[0][ct], ds[0], dq[ct]);
     }
+    R::put(Q + qt * TILE, g, i, dq, scale);
+  }
+  order_lds();
 #pragma unroll
-    for (int kt = 0; kt < NK; ++kt) {
-      const s16x4 pt = read_columns(tiles + (2 * kt) * 16 * TP + (4 * g + (i >> 2)) * TP + 8 * (i & 3));            // queries 4g.. of key i
-      const s16x4 dt = read_columns(tiles + (2 * kt + 1) * 16 * TP + (4 * g + (i >> 2)) * TP + 8 * (i & 3));
+  for (int kt = 0; kt < NK; ++kt) {
+    R::put(K + kt * TILE, g, i, dk[kt], scale);
+    R::put(V + kt * TILE, g, i, dv[kt], 1.f);
+  }
+}
+
+template <int DH, int NT, bool BWD> constexpr int window_lds() {
+  return (BWD ? 4 : 3) * NT * 16 * group_pitch<DH>() + NT * 16 * group_heads<DH>() * 4 + (BWD ? group_heads<DH>() * 4 * TILE_BYTES : 0) +
+         group_heads<DH>() * 2 * 64 * 4;
+}
+
+// Windows of up to 16 NT tokens; without a work list (NT = 4) every window, empty ones included.  Two waves per SIMD as the bound: 256
+// registers at most, and the matrix instructions then write plain vector registers (the backward of 64 channels by 64 tokens needs more).
+template <int DH, int NT, bool BWD>
+__global__ __launch_bounds__(64 * group_heads<DH>(), DH == 64 && NT == 4 && BWD ? 1 : 2) void dot_window_kernel(DotArgs a) {
+  constexpr int HPB = group_heads<DH>(), THREADS = 64 * HPB, PITCH = group_pitch<DH>(), IMAGE = NT * 16 * PITCH, NI = BWD ? 4 : 3;
+  constexpr int CHUNKS = HPB * DH / 8, PASS = THREADS / CHUNKS, PASSES = NT * 16 / PASS;      // 16-byte chunks of a row, rows at once
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  float* lse = reinterpret_cast<float*>(lds + NI * IMAGE);
+  char* after = lds + NI * IMAGE + NT * 16 * HPB * 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  char* tiles = after + w * 4 * TILE_BYTES;
+  int (*toks)[64] = reinterpret_cast<int (*)[64]>(after + (BWD ? HPB * 4 * TILE_BYTES : 0) + w * 512);
+  const int head0 = blockIdx.y * HPB;
+  const int r0 = threadIdx.x / CHUNKS, ch = threadIdx.x % CHUNKS;
+  const bool in_row = head0 * DH + ch * 8 < a.nhead * DH;          // a group behind the last head: its columns are read from column 0
+  const int64_t col = in_row ? (int64_t)head0 * DH * 2 + ch * 16 : 0;
+  for (Walk walk(a, NT == 4 ? 3 : 2, NT == 4 ? 3 : 2, blockIdx.x, gridDim.x); walk.next(a);) {
+    int Tq, Tk;
+    walk.tokens(toks, NT * 16, Tq, Tk);
+    if (Tq == 0 || Tk == 0) {
+      const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+      if (in_row) {
+        for (int r = r0; r < Tq; r += PASS)
+          *reinterpret_cast<uint4*>(BWD ? (char*)a.dq + toks[0][r] * a.lddq * 2 + col : (char*)a.o + toks[0][r] * a.ldo * 2 + col) = z;
+        if (BWD)
+          for (int r = r0; r < Tk; r += PASS) {
+            *reinterpret_cast<uint4*>((char*)a.dk + toks[1][r] * a.lddk * 2 + col) = z;
+            *reinterpret_cast<uint4*>((char*)a.dv + toks[1][r] * a.lddv * 2 + col) = z;
+          }
+      }
+      continue;
+    }
+    const int nq = (Tq + 15) >> 4, nk = (Tk + 15) >> 4;
+    // every row of the window is requested before the first one is laid down
+    uint4 rows[NI][PASSES];
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        dv[kt][ct] = over_tokens(gc[ct], pt, dv[kt][ct]);
-        dk[kt][ct] = over_tokens(qc[ct], dt, dk[kt][ct]);
+    for (int s = 0; s < PASSES; ++s) {
+      const int r = s * PASS + r0;
+      if (s * PASS < nk * 16) {
+        const int64_t t = toks[1][r];
+        rows[0][s] = *reinterpret_cast<const uint4*>((const char*)a.k + t * a.ldk * 2 + col);
+        rows[1][s] = *reinterpret_cast<const uint4*>((const char*)a.v + t * a.ldv * 2 + col);
+      }
+      if (s * PASS < nq * 16) {
+        const int64_t t = toks[0][r];
+        rows[2][s] = *reinterpret_cast<const uint4*>((const char*)a.q + t * a.ldq * 2 + col);
+        if constexpr (BWD) rows[3][s] = *reinterpret_cast<const uint4*>((const char*)a.g + t * a.ldg * 2 + col);
       }
     }
-    order_lds();
-    if (qt * 16 + i < Tq) store_piece<FR>((char*)a.dq + col + tq * a.lddq * 2, dq, a.scale);
-    tq = tnext;
-    qf = qnext;
-    gf = gnext;
-    ls = lsnext;
-  }
+    float ls = 0.f;
+    const int lr = threadIdx.x / HPB, lh = threadIdx.x % HPB;                // (64 rows of HPB heads: one value a thread)
+    if (BWD && lr < Tq && head0 + lh < a.nhead) ls = a.lse[(int64_t)toks[0][lr] * a.nhead + head0 + lh];
+    __syncthreads();                         // the window before is stored
 #pragma unroll
-  for (int kt = 0; kt < NK; ++kt)
-    if (kt * 16 + i < Tk) {
-      const int64_t t = tk_[kt * 16 + i];
-      store_piece<FR>((char*)a.dk + col + t * a.lddk * 2, dk[kt], a.scale);
-      store_piece<FR>((char*)a.dv + col + t * a.lddv * 2, dv[kt], 1.f);
+    for (int s = 0; s < PASSES; ++s) {
+      char* at = lds + (s * PASS + r0) * PITCH + ch * 16;
+      if (s * PASS < nk * 16) {
+        *reinterpret_cast<uint4*>(at) = rows[0][s];
+        *reinterpret_cast<uint4*>(at + IMAGE) = rows[1][s];
+      }
+      if (s * PASS < nq * 16) {
+        *reinterpret_cast<uint4*>(at + 2 * IMAGE) = rows[2][s];
+        if constexpr (BWD) *reinterpret_cast<uint4*>(at + 3 * IMAGE) = rows[3][s];
+      }
     }
-}
-
-template <int DH, int NT> constexpr int lds_bytes(bool bwd) {            // of one wave
-  const int image = NT * Image<DH>::TILE, rest = 2 * Image<DH>::TILE + NT * 2 * 16 * TILE_PITCH;
-  return !bwd || image > rest ? image : rest;
-}
-
-// A window of up to 16 NT tokens per workgroup, a head per wave; without a work list (NT = 4) every window, empty ones included.
-// Two waves per SIMD as the bound: 256 registers at most, and the matrix instructions then write plain vector registers.
-template <int DH, int NT, bool BWD>
-__global__ __launch_bounds__(256, 2) void dot_window_kernel(DotArgs a, int cls) {
-  constexpr int BYTES = lds_bytes<DH, NT>(BWD);
-  __shared__ int toks[2][64];
-  __shared__ __attribute__((aligned(16))) char lds[4][BYTES];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  Window win;
-  if (!find_window(a, cls, toks, win)) return;
-  __syncthreads();
-  const int head = blockIdx.y * 4 + w;
-  if (head >= a.nhead) return;
-  const int Tq = win.Tq < NT * 16 ? win.Tq : NT * 16, Tk = win.Tk < NT * 16 ? win.Tk : NT * 16;
-  if (Tq == 0 || Tk == 0) {
-    const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-    if (lane < Tq) {
-      uint4* o = reinterpret_cast<uint4*>(BWD ? (char*)a.dq + (toks[0][lane] * a.lddq + head * DH) * 2 : (char*)a.o + (toks[0][lane] * a.ldo + head * DH) * 2);
-      for (int c = 0; c < DH / 8; ++c) o[c] = z;
-    }
-    if (BWD && lane < Tk) {
-      uint4 *p = reinterpret_cast<uint4*>((char*)a.dk + (toks[1][lane] * a.lddk + head * DH) * 2),
-            *r = reinterpret_cast<uint4*>((char*)a.dv + (toks[1][lane] * a.lddv + head * DH) * 2);
-      for (int c = 0; c < DH / 8; ++c) { p[c] = z; r[c] = z; }
-    }
-    return;
-  }
-  const int nk = (Tk + 15) >> 4;
-#define ONE(NK)                                                                     \
-  if constexpr (BWD) bwd_window<DH, NK>(a, toks[0], toks[1], Tq, Tk, head, lds[w]); \
-  else fwd_window<DH, NK>(a, toks[0], toks[1], Tq, Tk, head, lds[w])
-  if (nk == 1) { ONE(1); }
-  else if (NT == 2 || nk == 2) { ONE(2); }
-  else if constexpr (NT == 4) {
-    if (nk == 3) { ONE(3); } else { ONE(4); }
-  }
+    if (BWD && lr < NT * 16) lse[threadIdx.x] = ls;
+    __syncthreads();
+    if (head0 + w < a.nhead) {
+      char *K = lds + w * DH * 2, *V = K + IMAGE, *Q = K + 2 * IMAGE, *G = K + 3 * IMAGE;
+#define ONE(NK)                                                                              \
+  if constexpr (BWD) bwd_window<DH, NK>(a.scale, Tq, Tk, nq, K, V, Q, G, lse + w, tiles);    \
+  else fwd_window<DH, NK>(a.scale, Tk, nq, K, V, Q, lse + w)
+      if (nk == 1) { ONE(1); }
+      else if (NT == 2 || nk == 2) { ONE(2); }
+      else if constexpr (NT == 4) {
+        if (nk == 3) { ONE(3); } else { ONE(4); }
+      }
 #undef ONE
+    }
+    __syncthreads();
+    if (in_row) {
+      char* o = BWD ? (char*)a.dq : (char*)a.o;
+      const int64_t ldo = BWD ? a.lddq : a.ldo;
+#pragma unroll
+      for (int s = 0; s < PASSES; ++s) {
+        const int r = s * PASS + r0;
+        const char* at = lds + r * PITCH + ch * 16;
+        if (r < Tq) *reinterpret_cast<uint4*>(o + toks[0][r] * ldo * 2 + col) = *reinterpret_cast<const uint4*>(at + 2 * IMAGE);
+        if (BWD && r < Tk) {
+          *reinterpret_cast<uint4*>((char*)a.dk + toks[1][r] * a.lddk * 2 + col) = *reinterpret_cast<const uint4*>(at);
+          *reinterpret_cast<uint4*>((char*)a.dv + toks[1][r] * a.lddv * 2 + col) = *reinterpret_cast<const uint4*>(at + IMAGE);
+        }
+      }
+    }
+    if (!BWD && lr < Tq && head0 + lh < a.nhead) a.lse[(int64_t)toks[0][lr] * a.nhead + head0 + lh] = lse[threadIdx.x];
+  }
 }
 
-// Windows of at most 16 tokens: a window per wave, HG heads of it at a time.  Nothing is shared between the waves of a workgroup.
-template <int DH> constexpr int heads_at_once() { return DH == 16 ? 4 : DH == 32 ? 2 : 1; }
+// ---- windows of at most 16 tokens: a wave per (window, 64 channels), all heads of the 64 channels at once.  Nothing is shared between the
+// waves of a workgroup.
+constexpr int SMALL_PITCH = 144;           // 128 bytes of a row
 
 template <int DH, bool BWD>
 __global__ __launch_bounds__(256, 2) void dot_small_kernel(DotArgs a) {
-  using Im = Image<DH>;
-  constexpr int FR = Im::FR, CT = Im::CT, HG = heads_at_once<DH>(), TP = TILE_PITCH;
-  constexpr int PER_HEAD = (BWD ? 3 : 1) * Im::TILE > (BWD ? 2 * 16 * TP : 0) ? (BWD ? 3 : 1) * Im::TILE : 2 * 16 * TP;
-  __shared__ int toks_[4][2][16];
-  __shared__ __attribute__((aligned(16))) char lds_[4][HG * PER_HEAD];
+  constexpr int HG = 64 / DH, PITCH = SMALL_PITCH, IMAGE = 16 * PITCH, NI = BWD ? 4 : 3, TP = TILE_PITCH;
+  using R = Rows<DH, PITCH>;
+  constexpr int CT = R::CT;
+  static_assert(HG * 2 * TILE_BYTES <= NI * IMAGE || !BWD, "the P and dS tiles take the images' place");
+  __shared__ int toks_[4][2][64];
+  __shared__ __attribute__((aligned(16))) char lds_[4][NI * IMAGE];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
-  // list 1 first (9 to 16 tokens), then list 0
-  const int64_t e = (int64_t)blockIdx.x * 4 + w, n1 = a.wl[1] < a.nwin ? a.wl[1] : a.nwin, n0 = a.wl[0] < a.nwin ? a.wl[0] : a.nwin;
-  if (e >= n1 + n0) return;
-  const int packed = a.wl[WL_HDR + (e < n1 ? a.nwin + e : e - n1)];
-  const int b = packed >> 16, wcx = (packed >> 8) & 255, wcy = packed & 255;
-  const int y = wcy * WIN - a.s + (lane >> 3), x = wcx * WIN - a.s + (lane & 7);
-  const bool in = b >= 0 && b < a.batch && y >= 0 && y < a.ny && x >= 0 && x < a.nx;
-  const int64_t cell = ((int64_t)b * a.ny + y) * a.nx + x;
-  int t0 = in ? a.grid_q[cell] : -1, t1 = in ? a.grid_k[cell] : -1;
-  if (t0 >= a.mq) t0 = -1;
-  if (t1 >= a.mk) t1 = -1;
-  const unsigned long long m0 = __ballot(t0 >= 0), m1 = __ballot(t1 >= 0), below = (1ull << lane) - 1ull;
-  const int Tq = min(__popcll(m0), 16), Tk = min(__popcll(m1), 16);
-  if (Tq == 0 || Tk == 0) return;                        // (in no list: the rows are zeroed elsewhere)
-  int (*toks)[16] = toks_[w];
-  char* lds = lds_[w];
-  const int f0 = __shfl(t0, __ffsll(m0) - 1, 64), f1 = __shfl(t1, __ffsll(m1) - 1, 64);
-  if (lane < 16) { toks[0][lane] = f0; toks[1][lane] = f1; }
-  order_lds();
-  const int r0 = __popcll(m0 & below), r1 = __popcll(m1 & below);
-  if (t0 >= 0 && r0 < 16) toks[0][r0] = t0;
-  if (t1 >= 0 && r1 < 16) toks[1][r1] = t1;
-  order_lds();
-  const int64_t tq = toks[0][i], tk = toks[1][i];
+  int (*toks)[64] = toks_[w];
+  char *K = lds_[w], *V = K + IMAGE, *Q = K + 2 * IMAGE, *G = K + 3 * IMAGE;
   const float c = a.scale * LOG2E;
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  f32x4 absent;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) absent[r] = 4 * g + r < Tk ? 0.f : -INFINITY;
-  const int64_t at = FR * 2 * g;
-  const char *q = (const char*)a.q + tq * a.ldq * 2 + at, *k = (const char*)a.k + tk * a.ldk * 2 + at, *v = (const char*)a.v + tk * a.ldv * 2 + at;
-  const char* gr = BWD ? (const char*)a.g + tq * a.ldg * 2 + at : nullptr;
-  for (int h0 = 0; h0 < a.nhead; h0 += HG) {
-    Piece<FR> kf[HG], vf[HG], qf[HG], gf[HG];
-    float ls[HG];
-#pragma unroll
-    for (int h = 0; h < HG; ++h) {
-      const int hh = h0 + h < a.nhead ? h0 + h : a.nhead - 1;            // a head behind the last one: read twice, stored once
-      kf[h] = load_piece<FR>(k + hh * DH * 2);
-      vf[h] = load_piece<FR>(v + hh * DH * 2);
-      qf[h] = load_piece<FR>(q + hh * DH * 2);
-      if constexpr (BWD) {
-        gf[h] = load_piece<FR>(gr + hh * DH * 2);
-        ls[h] = a.lse[tq * a.nhead + hh];
-      }
+  const int head0 = blockIdx.y * HG;
+  const int r8 = lane >> 3, ch = lane & 7;
+  const bool in_row = head0 * DH + ch * 8 < a.nhead * DH;
+  const int64_t col = in_row ? (int64_t)head0 * DH * 2 + ch * 16 : 0;
+  for (Walk walk(a, 1, 0, (int64_t)blockIdx.x * 4 + w, (int64_t)gridDim.x * 4); walk.next(a);) {
+    int Tq, Tk;
+    walk.tokens(toks, 16, Tq, Tk);
+    if (Tq == 0 || Tk == 0) continue;                    // (in no list: the rows are zeroed elsewhere)
+    const bool more_q = Tq > 8, more_k = Tk > 8;
+    uint4 rows[NI][2];
+    {
+      const int64_t tk = toks[1][r8], tq = toks[0][r8];
+      rows[0][0] = *reinterpret_cast<const uint4*>((const char*)a.k + tk * a.ldk * 2 + col);
+      rows[1][0] = *reinterpret_cast<const uint4*>((const char*)a.v + tk * a.ldv * 2 + col);
+      rows[2][0] = *reinterpret_cast<const uint4*>((const char*)a.q + tq * a.ldq * 2 + col);
+      if constexpr (BWD) rows[3][0] = *reinterpret_cast<const uint4*>((const char*)a.g + tq * a.ldg * 2 + col);
     }
+    if (more_k) {
+      const int64_t tk = toks[1][r8 + 8];
+      rows[0][1] = *reinterpret_cast<const uint4*>((const char*)a.k + tk * a.ldk * 2 + col);
+      rows[1][1] = *reinterpret_cast<const uint4*>((const char*)a.v + tk * a.ldv * 2 + col);
+    } else {
+      rows[0][1] = rows[0][0];               // (rows that are no tokens hold anything finite that the window holds)
+      rows[1][1] = rows[1][0];
+    }
+    if (more_q) {
+      const int64_t tq = toks[0][r8 + 8];
+      rows[2][1] = *reinterpret_cast<const uint4*>((const char*)a.q + tq * a.ldq * 2 + col);
+      if constexpr (BWD) rows[3][1] = *reinterpret_cast<const uint4*>((const char*)a.g + tq * a.ldg * 2 + col);
+    } else {
+      rows[2][1] = rows[2][0];
+      if constexpr (BWD) rows[3][1] = rows[3][0];
+    }
+    // lane (g, i): the saved logarithm of query i, head g
+    float ls = INFINITY;                     // no query: P = 0
+    if (BWD && i < Tq && g < HG && head0 + g < a.nhead) ls = a.lse[(int64_t)toks[0][i] * a.nhead + head0 + g];
+#pragma unroll
+    for (int t = 0; t < NI; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) *reinterpret_cast<uint4*>(K + t * IMAGE + (r8 + 8 * u) * PITCH + ch * 16) = rows[t][u];
+    order_lds();
+    f32x4 absent;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) absent[r] = 4 * g + r < Tk ? 0.f : -INFINITY;
     if constexpr (!BWD) {
-#pragma unroll
-      for (int h = 0; h < HG; ++h) Im::put(lds + h * PER_HEAD, g, i, vf[h]);
-      order_lds();
       s16x4 vc[HG][CT], p[HG];
-#pragma unroll
-      for (int h = 0; h < HG; ++h)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) vc[h][ct] = Im::get(lds + h * PER_HEAD, g, i, ct);
-      order_lds();
       f32x4 st[HG];
-      float mx[HG], l[HG];
+      float mx[HG], l[HG], out_lse = 0.f;
 #pragma unroll
-      for (int h = 0; h < HG; ++h) st[h] = over_channels<FR>(kf[h], qf[h], absent);
+      for (int h = 0; h < HG; ++h) {
+        st[h] = R::over_channels(R::piece(K + h * DH * 2, g, i), R::piece(Q + h * DH * 2, g, i), absent);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) vc[h][ct] = R::columns(V + h * DH * 2, g, i, ct);
+      }
 #pragma unroll
       for (int h = 0; h < HG; ++h) {
         mx[h] = column_max(fmaxf(fmaxf(st[h][0], st[h][1]), fmaxf(st[h][2], st[h][3]))) * c;
@@ -722,41 +783,37 @@ __global__ __launch_bounds__(256, 2) void dot_small_kernel(DotArgs a) {
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) o[ct] = over_tokens(vc[h][ct], p[h], zero);
         const float s = column_sum(l[h]);
-        if (i < Tq && h0 + h < a.nhead) {
-          store_piece<FR>((char*)a.o + tq * a.ldo * 2 + (h0 + h) * DH * 2 + at, o, __builtin_amdgcn_rcpf(s));
-          if (g == 0) a.lse[tq * a.nhead + h0 + h] = mx[h] + __builtin_amdgcn_logf(s);
+        R::put(Q + h * DH * 2, g, i, o, __builtin_amdgcn_rcpf(s));
+        if (g == h) out_lse = mx[h] + __builtin_amdgcn_logf(s);
+      }
+      order_lds();
+      if (in_row) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int r = r8 + 8 * u;
+          if (r < Tq) *reinterpret_cast<uint4*>((char*)a.o + toks[0][r] * a.ldo * 2 + col) = *reinterpret_cast<const uint4*>(Q + r * PITCH + ch * 16);
         }
       }
+      if (i < Tq && g < HG && head0 + g < a.nhead) a.lse[(int64_t)toks[0][i] * a.nhead + head0 + g] = out_lse;
     } else {
-#pragma unroll
-      for (int h = 0; h < HG; ++h) {
-        char* im = lds + h * PER_HEAD;
-        Im::put(im, g, i, kf[h]);
-        Im::put(im + Im::TILE, g, i, qf[h]);
-        Im::put(im + 2 * Im::TILE, g, i, gf[h]);
-      }
-      order_lds();
-      s16x4 kc[HG][CT], qc[HG][CT], gc[HG][CT], ds[HG], pb[HG];
-#pragma unroll
-      for (int h = 0; h < HG; ++h) {
-        const char* im = lds + h * PER_HEAD;
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          kc[h][ct] = Im::get(im, g, i, ct);
-          qc[h][ct] = Im::get(im + Im::TILE, g, i, ct);
-          gc[h][ct] = Im::get(im + 2 * Im::TILE, g, i, ct);
-        }
-      }
-      order_lds();
+      s16x4 kc[HG][CT], qc[HG][CT], gc[HG][CT], ds[HG];
       f32x4 p[HG], dp[HG];
 #pragma unroll
       for (int h = 0; h < HG; ++h) {
-        p[h] = over_channels<FR>(kf[h], qf[h], absent);
-        dp[h] = over_channels<FR>(vf[h], gf[h], zero);
+        const int at = h * DH * 2;
+        p[h] = R::over_channels(R::piece(K + at, g, i), R::piece(Q + at, g, i), absent);
+        dp[h] = R::over_channels(R::piece(V + at, g, i), R::piece(G + at, g, i), zero);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          kc[h][ct] = R::columns(K + at, g, i, ct);
+          qc[h][ct] = R::columns(Q + at, g, i, ct);
+          gc[h][ct] = R::columns(G + at, g, i, ct);
+        }
       }
+      order_lds();
 #pragma unroll
       for (int h = 0; h < HG; ++h) {
-        const float le = i < Tq ? ls[h] : INFINITY;
+        const float le = HG == 1 ? __shfl(ls, i, 64) : __shfl(ls, 16 * h + i, 64);
         float d = 0.f;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -768,18 +825,17 @@ __global__ __launch_bounds__(256, 2) void dot_small_kernel(DotArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) t[r] = p[h][r] * (dp[h][r] - d);
         ds[h] = pack4(t);
-        pb[h] = pack4(p[h]);
-        char* im = lds + h * PER_HEAD;
-        *reinterpret_cast<s16x4*>(im + i * TP + 8 * g) = pb[h];
-        *reinterpret_cast<s16x4*>(im + 16 * TP + i * TP + 8 * g) = ds[h];
+        char* tile = K + h * 2 * TILE_BYTES;
+        *reinterpret_cast<s16x4*>(tile + i * TP + 8 * g) = pack4(p[h]);
+        *reinterpret_cast<s16x4*>(tile + TILE_BYTES + i * TP + 8 * g) = ds[h];
       }
       order_lds();
       s16x4 pt[HG], dt[HG];
 #pragma unroll
       for (int h = 0; h < HG; ++h) {
-        const char* im = lds + h * PER_HEAD;
-        pt[h] = read_columns(im + (4 * g + (i >> 2)) * TP + 8 * (i & 3));
-        dt[h] = read_columns(im + 16 * TP + (4 * g + (i >> 2)) * TP + 8 * (i & 3));
+        const char* tile = K + h * 2 * TILE_BYTES + (4 * g + (i >> 2)) * TP + 8 * (i & 3);
+        pt[h] = read_columns(tile);
+        dt[h] = read_columns(tile + TILE_BYTES);
       }
       order_lds();
 #pragma unroll
@@ -791,16 +847,25 @@ __global__ __launch_bounds__(256, 2) void dot_small_kernel(DotArgs a) {
           dv[ct] = over_tokens(gc[h][ct], pt[h], zero);
           dk[ct] = over_tokens(qc[h][ct], dt[h], zero);
         }
-        const int64_t hcol = (int64_t)(h0 + h) * DH * 2 + at;
-        if (h0 + h < a.nhead) {
-          if (i < Tq) store_piece<FR>((char*)a.dq + tq * a.lddq * 2 + hcol, dq, a.scale);
-          if (i < Tk) {
-            store_piece<FR>((char*)a.dk + tk * a.lddk * 2 + hcol, dk, a.scale);
-            store_piece<FR>((char*)a.dv + tk * a.lddv * 2 + hcol, dv, 1.f);
+        R::put(Q + h * DH * 2, g, i, dq, a.scale);
+        R::put(K + h * DH * 2, g, i, dk, a.scale);
+        R::put(V + h * DH * 2, g, i, dv, 1.f);
+      }
+      order_lds();
+      if (in_row) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int r = r8 + 8 * u;
+          const char* at = K + r * PITCH + ch * 16;
+          if (r < Tq) *reinterpret_cast<uint4*>((char*)a.dq + toks[0][r] * a.lddq * 2 + col) = *reinterpret_cast<const uint4*>(at + 2 * IMAGE);
+          if (r < Tk) {
+            *reinterpret_cast<uint4*>((char*)a.dk + toks[1][r] * a.lddk * 2 + col) = *reinterpret_cast<const uint4*>(at);
+            *reinterpret_cast<uint4*>((char*)a.dv + toks[1][r] * a.lddv * 2 + col) = *reinterpret_cast<const uint4*>(at + IMAGE);
           }
         }
       }
     }
+    order_lds();
   }
 }
 
@@ -829,10 +894,17 @@ __global__ __launch_bounds__(256) void dot_orphan_kernel(DotArgs a, char* q0, in
     }
 }
 
-// blocks of a work list's class: class c > 0 windows hold more than 8 * 2^(c-1) tokens of one of the two frames
-int64_t class_blocks(int cls, int64_t nwin, int64_t mq, int64_t mk) {
-  const int64_t most = cls == 0 ? nwin : (mq + mk) / (cls == 1 ? 9 : cls == 2 ? 17 : 33);
-  return most < nwin ? most : nwin;
+// workgroups along the windows: what the windows can need, at most so many that each CU has `per_cu` of them in all
+unsigned walkers(int64_t windows, int per_group, unsigned gy, int per_cu) {
+  const int64_t need = (windows + per_group - 1) / per_group;
+  int64_t most = (int64_t)tmae_num_cus() * per_cu / gy;
+  if (most < 1) most = 1;
+  return (unsigned)(need < most ? need : most);
+}
+// windows that a class of a work list can hold: class c > 0 windows hold more than 8 * 2^(c-1) tokens of one of the two frames
+int64_t class_windows(const DotArgs& a, int cls) {
+  const int64_t most = (a.mq + a.mk) / (cls == 0 ? 2 : cls == 1 ? 9 : cls == 2 ? 17 : 33);
+  return most < a.nwin ? most : a.nwin;
 }
 
 bool rows_ok(const void* p, int64_t ld, int width, int es) {
@@ -861,27 +933,33 @@ template <class F> void by_head(int dh, F&& f) {
   else if (dh == 32) f(std::integral_constant<int, 32>());
   else f(std::integral_constant<int, 64>());
 }
-template <int DH, bool BWD> void launch_bf16(const DotArgs& a, hipStream_t stream) {
-  const unsigned gy = (unsigned)((a.nhead + 3) / 4);
-  if (!a.wl) {
-    hipLaunchKernelGGL((dot_window_kernel<DH, 4, BWD>), dim3((unsigned)a.nwin, gy), dim3(256), 0, stream, a, 0);
-    return;
-  }
-  const int64_t b3 = class_blocks(3, a.nwin, a.mq, a.mk), b2 = class_blocks(2, a.nwin, a.mq, a.mk);
-  if (b3 > 0) hipLaunchKernelGGL((dot_window_kernel<DH, 4, BWD>), dim3((unsigned)b3, gy), dim3(256), 0, stream, a, 3);
-  if (b2 > 0) hipLaunchKernelGGL((dot_window_kernel<DH, 2, BWD>), dim3((unsigned)b2, gy), dim3(256), 0, stream, a, 2);
-  int64_t small = a.mq < a.mk ? a.mq : a.mk;             // a listed window holds a query and a key
-  if (small > a.nwin) small = a.nwin;
-  if (small > 0) hipLaunchKernelGGL((dot_small_kernel<DH, BWD>), dim3(tmae_cdiv(small, 4)), dim3(256), 0, stream, a);
+template <int DH, int NT, bool BWD> int launch_windows(const DotArgs& a, int64_t windows, hipStream_t stream) {
+  constexpr int HPB = group_heads<DH>(), LDS = window_lds<DH, NT, BWD>();
+  if (windows == 0) return TMAE_OK;
+  static TmaeLdsAttr attr;
+  if (LDS > 65536)
+    if (int e = tmae_allow_lds(attr, (const void*)dot_window_kernel<DH, NT, BWD>, LDS)) return e;
+  const unsigned gy = (unsigned)((a.nhead + HPB - 1) / HPB);
+  hipLaunchKernelGGL((dot_window_kernel<DH, NT, BWD>), dim3(walkers(windows, 1, gy, 8), gy), dim3(64 * HPB), LDS, stream, a);
+  return TMAE_OK;
 }
-
-template <class F> void by_class(const DotArgs& a, F&& f) {
+template <int DH, bool BWD> int launch_bf16(const DotArgs& a, hipStream_t stream) {
+  if (!a.wl) return launch_windows<DH, 4, BWD>(a, a.nwin, stream);
+  int rc = launch_windows<DH, 4, BWD>(a, class_windows(a, 3), stream);
+  if (rc == TMAE_OK) rc = launch_windows<DH, 2, BWD>(a, class_windows(a, 2), stream);
+  if (rc != TMAE_OK) return rc;
+  const unsigned gy = (unsigned)((a.nhead * DH + 63) / 64);
+  const int64_t small = class_windows(a, 0);
+  if (small > 0) hipLaunchKernelGGL((dot_small_kernel<DH, BWD>), dim3(walkers(small, 4, gy, 8), gy), dim3(256), 0, stream, a);
+  return TMAE_OK;
+}
+template <int DH, bool BWD> void launch_f32(const DotArgs& a, hipStream_t stream) {
   const unsigned gy = (unsigned)((a.nhead + 3) / 4);
-  if (!a.wl) { f(dim3((unsigned)a.nwin, gy), 0); return; }
-  for (int cls = 3; cls >= 0; --cls) {
-    const int64_t blocks = class_blocks(cls, a.nwin, a.mq, a.mk);
-    if (blocks > 0) f(dim3((unsigned)blocks, gy), cls);
-  }
+  const int64_t windows = a.wl ? class_windows(a, 0) : a.nwin;
+  if (windows == 0) return;
+  const dim3 grid(walkers(windows, 1, gy, 8), gy);
+  if constexpr (BWD) hipLaunchKernelGGL((dot_bwd_kernel<float, DH>), grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((dot_fwd_kernel<float, DH>), grid, dim3(256), 0, stream, a);
 }
 
 }  // namespace
@@ -900,15 +978,13 @@ int tmae_win_attn_dot_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk
   if (worklist && grid_q != grid_k)
     hipLaunchKernelGGL(dot_orphan_kernel, dim3(tmae_cdiv(a.nwin, 4)), dim3(256), 0, (hipStream_t)stream, a, (char*)out, ldo * es, nullptr,
                        (int64_t)0, nullptr, (int64_t)0, d * es / 16);
+  int failed = TMAE_OK;
   by_head(dh, [&](auto w) {
     constexpr int DH = decltype(w)::value;
-    if (dtype == TMAE_BF16) launch_bf16<DH, false>(a, (hipStream_t)stream);
-    else
-      by_class(a, [&](dim3 grid, int cls) {
-        hipLaunchKernelGGL((dot_fwd_kernel<float, DH>), grid, dim3(256), 0, (hipStream_t)stream, a, cls);
-      });
+    if (dtype == TMAE_BF16) failed = launch_bf16<DH, false>(a, (hipStream_t)stream);
+    else launch_f32<DH, false>(a, (hipStream_t)stream);
   });
-  return tmae_launch_status();
+  return failed != TMAE_OK ? failed : tmae_launch_status();
 }
 
 int tmae_win_attn_dot_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, const void* dout,
@@ -928,13 +1004,11 @@ int tmae_win_attn_dot_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk
   if (worklist && grid_q != grid_k)
     hipLaunchKernelGGL(dot_orphan_kernel, dim3(tmae_cdiv(a.nwin, 4)), dim3(256), 0, (hipStream_t)stream, a, (char*)dq, lddq * es,
                        (char*)dk, lddk * es, (char*)dv, lddv * es, d * es / 16);
+  int failed = TMAE_OK;
   by_head(dh, [&](auto w) {
     constexpr int DH = decltype(w)::value;
-    if (dtype == TMAE_BF16) launch_bf16<DH, true>(a, (hipStream_t)stream);
-    else
-      by_class(a, [&](dim3 grid, int cls) {
-        hipLaunchKernelGGL((dot_bwd_kernel<float, DH>), grid, dim3(256), 0, (hipStream_t)stream, a, cls);
-      });
+    if (dtype == TMAE_BF16) failed = launch_bf16<DH, true>(a, (hipStream_t)stream);
+    else launch_f32<DH, true>(a, (hipStream_t)stream);
   });
-  return tmae_launch_status();
+  return failed != TMAE_OK ? failed : tmae_launch_status();
 }
