@@ -42,63 +42,72 @@ __device__ __forceinline__ void order_lds() {
 }
 
 // The windows of a launch: those of the work list's classes `from`, `from` - 1, ... `to` one after the other (larger windows first), or
-// every window of the grids where there is no list.  A wave takes every step-th one and requests the cells of the next one before it
-// works on the present one: the list's entry, the cells and the rows are three loads that wait for each other.
+// every window of the grids where there is no list.  A wave takes every step-th one.  The list's entry, the cells and the rows are three
+// loads that wait for each other: a wave reads 64 of its entries at once (a lane each), and requests the cells of the next window before
+// it works on the present one.  No load stands behind a branch -- it would be waited for there -- so places that do not exist are
+// replaced by ones that do.
 struct Walk {
-  int64_t n, e, step;
-  int from, to;
+  int n, e, step, from, to;                // windows in all, the present one
+  int entries, at;                         // this lane's entry of the 64, the next window's among them
   int tq, tk;                              // this lane's cell of the present window: row numbers, -1 where it is empty
-  int nq, nk;                              // ... of the next one
-  int entry;                               // the list's entry behind that
+  int nq, nk;                              // ... of the next one, if it is a cell of the grid
+  bool nin;
 
-  __device__ __forceinline__ int entry_at(const DotArgs& a, int64_t e) const {
-    int cls = from;
-    for (; cls > to; --cls) {
-      const int64_t c = count(a, cls);
-      if (e < c) break;
-      e -= c;
+  __device__ __forceinline__ static int count(const DotArgs& a, int cls) {
+    const int c = a.wl[cls];
+    return c < 0 ? 0 : c < (int)a.nwin ? c : (int)a.nwin;
+  }
+  __device__ __forceinline__ void read_entries(const DotArgs& a, int first) {
+    int x = first + (int)(threadIdx.x & 63) * step;
+    if (x >= n || x < first) x = n - 1;
+    entries = x;
+    at = 0;
+    if (a.wl) {
+      int cls = from;
+      for (int c = from; c > to; --c) {
+        const int k = count(a, c);
+        if (cls == c && x >= k) { x -= k; cls = c - 1; }
+      }
+      entries = a.wl[WL_HDR + cls * a.nwin + x];
+      asm volatile("" : "+v"(entries));      // waited for here, once in 64 windows, and not where the two ways meet again
     }
-    return a.wl[WL_HDR + cls * a.nwin + e];
   }
-  __device__ __forceinline__ static int64_t count(const DotArgs& a, int cls) {
-    const int64_t c = a.wl[cls];
-    return c < 0 ? 0 : c < a.nwin ? c : a.nwin;
-  }
-  // the cells of window e (its list entry, where there is a list); a row number outside the tensors counts as an empty cell
-  __device__ __forceinline__ void cells(const DotArgs& a, int64_t e, int entry, int& q, int& k) const {
-    const int lane = threadIdx.x & 63;
+  __device__ __forceinline__ void request_cells(const DotArgs& a) {
+    const int lane = threadIdx.x & 63, u = __builtin_amdgcn_readlane(entries, at);
     int b, wcy, wcx;
     if (a.wl) {
-      b = entry >> 16; wcx = (entry >> 8) & 255; wcy = entry & 255;
+      b = u >> 16; wcx = (u >> 8) & 255; wcy = u & 255;
     } else {
-      const unsigned u = (unsigned)e;
-      wcy = (int)(u % (unsigned)a.Wy); wcx = (int)((u / (unsigned)a.Wy) % (unsigned)a.Wx); b = (int)(u / (unsigned)(a.Wy * a.Wx));
+      wcy = u % a.Wy; wcx = u / a.Wy % a.Wx; b = u / (a.Wy * a.Wx);
     }
     const int y = wcy * WIN - a.s + (lane >> 3), x = wcx * WIN - a.s + (lane & 7);
     const bool in = b >= 0 && b < a.batch && y >= 0 && y < a.ny && x >= 0 && x < a.nx;
-    const int64_t cell = ((int64_t)b * a.ny + y) * a.nx + x;
-    q = in ? a.grid_q[cell] : -1;
-    k = in ? a.grid_k[cell] : -1;
+    int cell = in ? (b * a.ny + y) * a.nx + x : 0;                   // batch * ny * nx < 2^31
+    asm volatile("" : "+v"(cell));           // (the loads stay outside of the condition)
+    nq = a.grid_q[cell];
+    nk = a.grid_k[cell];
+    nin = in;
   }
-  __device__ __forceinline__ Walk(const DotArgs& a, int from_, int to_, int64_t first, int64_t step_) : e(first), step(step_), from(from_), to(to_) {
-    n = a.nwin;
+  __device__ __forceinline__ Walk(const DotArgs& a, int from_, int to_, int first, int step_) : e(first - step_), step(step_), from(from_), to(to_) {
+    n = (int)a.nwin;
     if (a.wl) {
       n = 0;
       for (int c = from; c >= to; --c) n += count(a, c);
     }
     tq = tk = nq = nk = -1;
-    entry = 0;
-    if (e < n) cells(a, e, a.wl ? entry_at(a, e) : 0, nq, nk);
-    if (a.wl && e + step < n) entry = entry_at(a, e + step);
-    e -= step;
+    nin = false;
+    if (first < n) {
+      read_entries(a, first);
+      request_cells(a);
+    }
   }
   __device__ __forceinline__ bool next(const DotArgs& a) {
+    if (e >= n - step) return false;
     e += step;
-    if (e >= n) return false;
-    tq = nq < a.mq ? nq : -1;
-    tk = nk < a.mk ? nk : -1;
-    if (e + step < n) cells(a, e + step, entry, nq, nk);
-    if (a.wl && e + 2 * step < n) entry = entry_at(a, e + 2 * step);
+    tq = nin && nq < a.mq ? nq : -1;       // a row number outside the tensors counts as an empty cell
+    tk = nin && nk < a.mk ? nk : -1;
+    if (++at == 64) read_entries(a, e < n - step ? e + step : e);
+    request_cells(a);                      // (behind the last window: once more some window of the list)
     return true;
   }
   // the tokens in cell order into toks[0] (queries) and toks[1] (keys), at most `most` of each; the slots behind repeat the first one
@@ -107,12 +116,12 @@ struct Walk {
     const unsigned long long q = __ballot(tq >= 0), k = __ballot(tk >= 0), below = (1ull << lane) - 1ull;
     Tq = min(__popcll(q), most);
     Tk = min(__popcll(k), most);
-    const int fq = q ? __shfl(tq, __ffsll(q) - 1, 64) : -1, fk = k ? __shfl(tk, __ffsll(k) - 1, 64) : -1;
+    const int fq = __builtin_amdgcn_readlane(tq, q ? __ffsll(q) - 1 : 0), fk = __builtin_amdgcn_readlane(tk, k ? __ffsll(k) - 1 : 0);
+    // every lane writes one slot of each list: the tokens' ranks first, then the others the slots behind (a full list has none)
+    const int rq = __popcll(q & below), rk = __popcll(k & below), sq = __popcll(q), sk = __popcll(k);
     order_lds();
-    if (lane >= Tq) toks[0][lane] = fq;
-    if (lane >= Tk) toks[1][lane] = fk;
-    if (tq >= 0 && __popcll(q & below) < most) toks[0][__popcll(q & below)] = tq;
-    if (tk >= 0 && __popcll(k & below) < most) toks[1][__popcll(k & below)] = tk;
+    toks[0][tq >= 0 ? rq : sq + lane - rq] = tq >= 0 ? tq : fq;
+    toks[1][tk >= 0 ? rk : sk + lane - rk] = tk >= 0 ? tk : fk;
     order_lds();
   }
 };
@@ -169,7 +178,7 @@ __global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
   if (head >= a.nhead) return;
   const int hoff = head * DH;
   T* out = (T*)a.o + hoff;
-  for (Walk walk(a, 3, 0, blockIdx.x, gridDim.x); walk.next(a);) {
+  for (Walk walk(a, 3, 0, (int)blockIdx.x, (int)gridDim.x); walk.next(a);) {
   struct { int Tq, Tk; } win;
   walk.tokens(toks, 64, win.Tq, win.Tk);
   if (win.Tk == 0) {
@@ -240,7 +249,7 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_kernel(DotArgs a) {
   if (head >= a.nhead) return;
   const int hoff = head * DH;
   T *dq = (T*)a.dq + hoff, *dk = (T*)a.dk + hoff, *dv = (T*)a.dv + hoff;
-  for (Walk walk(a, 3, 0, blockIdx.x, gridDim.x); walk.next(a);) {
+  for (Walk walk(a, 3, 0, (int)blockIdx.x, (int)gridDim.x); walk.next(a);) {
   struct { int Tq, Tk; } win;
   walk.tokens(toks, 64, win.Tq, win.Tk);
   if (win.Tq == 0 || win.Tk == 0) {
@@ -433,34 +442,66 @@ __device__ __forceinline__ f32x4 over_tokens(const s16x4& a0, const s16x4& a1, c
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// ---- windows of more than 16 tokens: a workgroup per (window, group of heads), a head per wave.  The row images -- K, V, Q and in the
-// backward dO, 16 NT rows of the group's columns -- are the workgroup's; each wave reads and overwrites its own head's columns only.
-template <int DH> constexpr int group_heads() { return DH == 64 ? 2 : 4; }
-template <int DH> constexpr int group_pitch() { return group_heads<DH>() * DH * 2 + 16; }
-
-// One head: NK key tiles against nq query tiles.  NK is a template parameter, so that no branch stands between a matrix instruction and
-// its reader.  K, V, Q: the head's columns of the images; out replaces Q, lse [slot, heads of the group].
-template <int DH, int NK>
-__device__ __forceinline__ void fwd_window(float scale, int Tk, int nq, const char* K, const char* V, char* Q, float* lse) {
-  constexpr int PITCH = group_pitch<DH>(), TILE = 16 * PITCH;
+// ---- windows of more than 16 tokens: a wave per (window, head), four heads in a workgroup so that their pieces of a line meet in the cache.
+// All rows of the window are requested at once.  K and V go through the wave's two images into registers, then Q (and dO) take their place;
+// results replace Q, and at the end dK and dV follow.
+template <int DH, int NT> struct Window {
+  static constexpr int PITCH = DH * 2 + 16, TILE = 16 * PITCH, IMAGE = NT * TILE;
+  static constexpr int CHUNKS = DH / 8, RPI = 64 / CHUNKS, LOADS = NT * 16 / RPI;             // 16-byte chunks of a row, rows of a load
   using R = Rows<DH, PITCH>;
-  constexpr int CT = R::CT;
-  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+  static constexpr int CT = R::CT;
+
+  static __device__ __forceinline__ void request(uint4* rows, const void* base, int64_t ld, const int* toks, int64_t col) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int s = 0; s < LOADS; ++s)
+      rows[s] = *reinterpret_cast<const uint4*>((const char*)base + (int64_t)toks[s * RPI + lane / CHUNKS] * ld * 2 + col + (lane % CHUNKS) * 16);
+  }
+  static __device__ __forceinline__ void lay(char* image, const uint4* rows) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int s = 0; s < LOADS; ++s) *reinterpret_cast<uint4*>(image + (s * RPI + lane / CHUNKS) * PITCH + (lane % CHUNKS) * 16) = rows[s];
+  }
+  static __device__ __forceinline__ void store(void* base, int64_t ld, const int* toks, int T, int64_t col, const char* image) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int s = 0; s < LOADS; ++s) {
+      const int r = s * RPI + lane / CHUNKS;
+      if (r < T)
+        *reinterpret_cast<uint4*>((char*)base + (int64_t)toks[r] * ld * 2 + col + (lane % CHUNKS) * 16) =
+            *reinterpret_cast<const uint4*>(image + r * PITCH + (lane % CHUNKS) * 16);
+    }
+  }
+};
+
+// NK key tiles against nq query tiles.  NK is a template parameter, so that no branch stands between a matrix instruction and its reader.
+template <int DH, int NT, int NK>
+__device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq, const int* tk, int Tq, int Tk, int head, char* A, const uint4* qrows) {
+  using W = Window<DH, NT>;
+  using R = typename W::R;
+  constexpr int CT = W::CT, TILE = W::TILE;
+  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15, nq = (Tq + 15) >> 4;
+  const int64_t col = (int64_t)head * DH * 2;
+  const char* V = A + W::IMAGE;
   typename R::Piece kf[NK];
   s16x4 vc[NK][CT];
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt) {
-    kf[kt] = R::piece(K + kt * TILE, g, i);
+    kf[kt] = R::piece(A + kt * TILE, g, i);
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) vc[kt][ct] = R::columns(V + kt * TILE, g, i, ct);
   }
+  order_lds();
+  W::lay(A, qrows);
+  order_lds();
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   f32x4 absent;                              // of the last key tile: -inf where there is no key
 #pragma unroll
   for (int r = 0; r < 4; ++r) absent[r] = (NK - 1) * 16 + 4 * g + r < Tk ? 0.f : -INFINITY;
-  const float c = scale * LOG2E;
+  const float c = a.scale * LOG2E;
+  float my_lse = 0.f;                        // lane (g, i): of query 16 g + i
   for (int qt = 0; qt < nq; ++qt) {
-    const typename R::Piece qf = R::piece(Q + qt * TILE, g, i);
+    const typename R::Piece qf = R::piece(A + qt * TILE, g, i);
     f32x4 st[NK];
     float mx = -INFINITY;
 #pragma unroll
@@ -491,47 +532,55 @@ __device__ __forceinline__ void fwd_window(float scale, int Tk, int nq, const ch
       if constexpr (NK == 3) o[ct] = over_tokens(vc[2][ct], s16x4{0, 0, 0, 0}, p[2], s16x4{0, 0, 0, 0}, o[ct]);
       if constexpr (NK == 1) o[ct] = over_tokens(vc[0][ct], p[0], o[ct]);
     }
-    R::put(Q + qt * TILE, g, i, o, __builtin_amdgcn_rcpf(l));
-    if (g == 0) lse[(qt * 16 + i) * group_heads<DH>()] = mx + __builtin_amdgcn_logf(l);       // v_log_f32: to base 2
+    R::put(A + qt * TILE, g, i, o, __builtin_amdgcn_rcpf(l));
+    if (g == qt) my_lse = mx + __builtin_amdgcn_logf(l);                 // v_log_f32: to base 2
   }
+  order_lds();
+  W::store(a.o, a.ldo, tq, Tq, col, A);
+  if (lane < Tq) a.lse[(int64_t)tq[lane] * a.nhead + head] = my_lse;
 }
 
-// dq replaces Q, dk K and dv V; tiles: the wave's own P and dS tiles, two of each
-template <int DH, int NK>
-__device__ __forceinline__ void bwd_window(float scale, int Tq, int Tk, int nq, char* K, char* V, char* Q, const char* G, const float* lse,
-                                           char* tiles) {
-  constexpr int PITCH = group_pitch<DH>(), TILE = 16 * PITCH, TP = TILE_PITCH;
-  using R = Rows<DH, PITCH>;
-  constexpr int CT = R::CT;
-  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+template <int DH, int NT, int NK>
+__device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, const int* tk, int Tq, int Tk, int head, char* A, const uint4* qrows,
+                                           const uint4* grows, float ls, char* tiles) {
+  using W = Window<DH, NT>;
+  using R = typename W::R;
+  constexpr int CT = W::CT, TILE = W::TILE, TP = TILE_PITCH;
+  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15, nq = (Tq + 15) >> 4;
+  const int64_t col = (int64_t)head * DH * 2;
+  char* B = A + W::IMAGE;
   typename R::Piece kf[NK], vf[NK];
   s16x4 kc[NK][CT];
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt) {
-    kf[kt] = R::piece(K + kt * TILE, g, i);
-    vf[kt] = R::piece(V + kt * TILE, g, i);
+    kf[kt] = R::piece(A + kt * TILE, g, i);
+    vf[kt] = R::piece(B + kt * TILE, g, i);
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) kc[kt][ct] = R::columns(K + kt * TILE, g, i, ct);
+    for (int ct = 0; ct < CT; ++ct) kc[kt][ct] = R::columns(A + kt * TILE, g, i, ct);
   }
+  order_lds();
+  W::lay(A, qrows);
+  W::lay(B, grows);
+  order_lds();
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   f32x4 absent;
 #pragma unroll
   for (int r = 0; r < 4; ++r) absent[r] = (NK - 1) * 16 + 4 * g + r < Tk ? 0.f : -INFINITY;
-  const float c = scale * LOG2E;
+  const float c = a.scale * LOG2E;
   f32x4 dk[NK][CT], dv[NK][CT];
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) dk[kt][ct] = dv[kt][ct] = zero;
   for (int qt = 0; qt < nq; ++qt) {
-    const typename R::Piece qf = R::piece(Q + qt * TILE, g, i), gf = R::piece(G + qt * TILE, g, i);
+    const typename R::Piece qf = R::piece(A + qt * TILE, g, i), gf = R::piece(B + qt * TILE, g, i);
     s16x4 qc[CT], gc[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      qc[ct] = R::columns(Q + qt * TILE, g, i, ct);
-      gc[ct] = R::columns(G + qt * TILE, g, i, ct);
+      qc[ct] = R::columns(A + qt * TILE, g, i, ct);
+      gc[ct] = R::columns(B + qt * TILE, g, i, ct);
     }
-    const float le = qt * 16 + i < Tq ? lse[(qt * 16 + i) * group_heads<DH>()] : INFINITY;           // no query: P = 0
+    const float le = __shfl(ls, qt * 16 + i, 64);                // +inf where there is no query: P = 0
     f32x4 p[NK], dp[NK];
     float d = 0.f;
 #pragma unroll
@@ -582,116 +631,75 @@ __device__ __forceinline__ void bwd_window(float scale, int Tq, int Tk, int nq, 
       if constexpr (NK == 3) dq[ct] = over_tokens(kc[2][ct], s16x4{0, 0, 0, 0}, ds[2], s16x4{0, 0, 0, 0}, dq[ct]);
       if constexpr (NK == 1) dq[ct] = over_tokens(kc[0][ct], ds[0], dq[ct]);
     }
-    R::put(Q + qt * TILE, g, i, dq, scale);
+    R::put(A + qt * TILE, g, i, dq, a.scale);
   }
+  order_lds();
+  W::store(a.dq, a.lddq, tq, Tq, col, A);
   order_lds();
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt) {
-    R::put(K + kt * TILE, g, i, dk[kt], scale);
-    R::put(V + kt * TILE, g, i, dv[kt], 1.f);
+    R::put(A + kt * TILE, g, i, dk[kt], a.scale);
+    R::put(B + kt * TILE, g, i, dv[kt], 1.f);
   }
-}
-
-template <int DH, int NT, bool BWD> constexpr int window_lds() {
-  return (BWD ? 4 : 3) * NT * 16 * group_pitch<DH>() + NT * 16 * group_heads<DH>() * 4 + (BWD ? group_heads<DH>() * 4 * TILE_BYTES : 0) +
-         group_heads<DH>() * 2 * 64 * 4;
+  order_lds();
+  W::store(a.dk, a.lddk, tk, Tk, col, A);
+  W::store(a.dv, a.lddv, tk, Tk, col, B);
 }
 
 // Windows of up to 16 NT tokens; without a work list (NT = 4) every window, empty ones included.  Two waves per SIMD as the bound: 256
 // registers at most, and the matrix instructions then write plain vector registers (the backward of 64 channels by 64 tokens needs more).
+template <int DH, int NT, bool BWD> constexpr int window_lds() { return 2 * Window<DH, NT>::IMAGE + (BWD ? 4 * TILE_BYTES : 0); }
 template <int DH, int NT, bool BWD>
-__global__ __launch_bounds__(64 * group_heads<DH>(), DH == 64 && NT == 4 && BWD ? 1 : 2) void dot_window_kernel(DotArgs a) {
-  constexpr int HPB = group_heads<DH>(), THREADS = 64 * HPB, PITCH = group_pitch<DH>(), IMAGE = NT * 16 * PITCH, NI = BWD ? 4 : 3;
-  constexpr int CHUNKS = HPB * DH / 8, PASS = THREADS / CHUNKS, PASSES = NT * 16 / PASS;      // 16-byte chunks of a row, rows at once
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  float* lse = reinterpret_cast<float*>(lds + NI * IMAGE);
-  char* after = lds + NI * IMAGE + NT * 16 * HPB * 4;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  char* tiles = after + w * 4 * TILE_BYTES;
-  int (*toks)[64] = reinterpret_cast<int (*)[64]>(after + (BWD ? HPB * 4 * TILE_BYTES : 0) + w * 512);
-  const int head0 = blockIdx.y * HPB;
-  const int r0 = threadIdx.x / CHUNKS, ch = threadIdx.x % CHUNKS;
-  const bool in_row = head0 * DH + ch * 8 < a.nhead * DH;          // a group behind the last head: its columns are read from column 0
-  const int64_t col = in_row ? (int64_t)head0 * DH * 2 + ch * 16 : 0;
-  for (Walk walk(a, NT == 4 ? 3 : 2, NT == 4 ? 3 : 2, blockIdx.x, gridDim.x); walk.next(a);) {
+__global__ __launch_bounds__(256, DH == 64 && NT == 4 && BWD ? 1 : 2) void dot_window_kernel(DotArgs a) {
+  using W = Window<DH, NT>;
+  extern __shared__ __attribute__((aligned(16))) char lds_[];
+  __shared__ int toks_[4][2][64];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int (*toks)[64] = toks_[w];
+  char* A = lds_ + w * window_lds<DH, NT, BWD>();
+  const int head = blockIdx.y * 4 + w;
+  if (head >= a.nhead) return;
+  const int64_t col = (int64_t)head * DH * 2;
+  for (Walk walk(a, NT == 4 ? 3 : 2, NT == 4 ? 3 : 2, (int)blockIdx.x, (int)gridDim.x); walk.next(a);) {
     int Tq, Tk;
     walk.tokens(toks, NT * 16, Tq, Tk);
     if (Tq == 0 || Tk == 0) {
       const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-      if (in_row) {
-        for (int r = r0; r < Tq; r += PASS)
-          *reinterpret_cast<uint4*>(BWD ? (char*)a.dq + toks[0][r] * a.lddq * 2 + col : (char*)a.o + toks[0][r] * a.ldo * 2 + col) = z;
-        if (BWD)
-          for (int r = r0; r < Tk; r += PASS) {
-            *reinterpret_cast<uint4*>((char*)a.dk + toks[1][r] * a.lddk * 2 + col) = z;
-            *reinterpret_cast<uint4*>((char*)a.dv + toks[1][r] * a.lddv * 2 + col) = z;
-          }
+      if (lane < Tq) {
+        uint4* o = reinterpret_cast<uint4*>(BWD ? (char*)a.dq + toks[0][lane] * a.lddq * 2 + col : (char*)a.o + toks[0][lane] * a.ldo * 2 + col);
+        for (int c = 0; c < DH / 8; ++c) o[c] = z;
+      }
+      if (BWD && lane < Tk) {
+        uint4 *p = reinterpret_cast<uint4*>((char*)a.dk + toks[1][lane] * a.lddk * 2 + col),
+              *r = reinterpret_cast<uint4*>((char*)a.dv + toks[1][lane] * a.lddv * 2 + col);
+        for (int c = 0; c < DH / 8; ++c) { p[c] = z; r[c] = z; }
       }
       continue;
     }
-    const int nq = (Tq + 15) >> 4, nk = (Tk + 15) >> 4;
-    // every row of the window is requested before the first one is laid down
-    uint4 rows[NI][PASSES];
-#pragma unroll
-    for (int s = 0; s < PASSES; ++s) {
-      const int r = s * PASS + r0;
-      if (s * PASS < nk * 16) {
-        const int64_t t = toks[1][r];
-        rows[0][s] = *reinterpret_cast<const uint4*>((const char*)a.k + t * a.ldk * 2 + col);
-        rows[1][s] = *reinterpret_cast<const uint4*>((const char*)a.v + t * a.ldv * 2 + col);
-      }
-      if (s * PASS < nq * 16) {
-        const int64_t t = toks[0][r];
-        rows[2][s] = *reinterpret_cast<const uint4*>((const char*)a.q + t * a.ldq * 2 + col);
-        if constexpr (BWD) rows[3][s] = *reinterpret_cast<const uint4*>((const char*)a.g + t * a.ldg * 2 + col);
-      }
-    }
+    uint4 krows[W::LOADS], vrows[W::LOADS], qrows[W::LOADS], grows[W::LOADS];
+    W::request(krows, a.k, a.ldk, toks[1], col);
+    W::request(vrows, a.v, a.ldv, toks[1], col);
+    W::request(qrows, a.q, a.ldq, toks[0], col);
     float ls = 0.f;
-    const int lr = threadIdx.x / HPB, lh = threadIdx.x % HPB;                // (64 rows of HPB heads: one value a thread)
-    if (BWD && lr < Tq && head0 + lh < a.nhead) ls = a.lse[(int64_t)toks[0][lr] * a.nhead + head0 + lh];
-    __syncthreads();                         // the window before is stored
-#pragma unroll
-    for (int s = 0; s < PASSES; ++s) {
-      char* at = lds + (s * PASS + r0) * PITCH + ch * 16;
-      if (s * PASS < nk * 16) {
-        *reinterpret_cast<uint4*>(at) = rows[0][s];
-        *reinterpret_cast<uint4*>(at + IMAGE) = rows[1][s];
-      }
-      if (s * PASS < nq * 16) {
-        *reinterpret_cast<uint4*>(at + 2 * IMAGE) = rows[2][s];
-        if constexpr (BWD) *reinterpret_cast<uint4*>(at + 3 * IMAGE) = rows[3][s];
-      }
+    if constexpr (BWD) {
+      W::request(grows, a.g, a.ldg, toks[0], col);
+      ls = a.lse[(int64_t)toks[0][lane] * a.nhead + head];
+      if (lane >= Tq) ls = INFINITY;
     }
-    if (BWD && lr < NT * 16) lse[threadIdx.x] = ls;
-    __syncthreads();
-    if (head0 + w < a.nhead) {
-      char *K = lds + w * DH * 2, *V = K + IMAGE, *Q = K + 2 * IMAGE, *G = K + 3 * IMAGE;
-#define ONE(NK)                                                                              \
-  if constexpr (BWD) bwd_window<DH, NK>(a.scale, Tq, Tk, nq, K, V, Q, G, lse + w, tiles);    \
-  else fwd_window<DH, NK>(a.scale, Tk, nq, K, V, Q, lse + w)
-      if (nk == 1) { ONE(1); }
-      else if (NT == 2 || nk == 2) { ONE(2); }
-      else if constexpr (NT == 4) {
-        if (nk == 3) { ONE(3); } else { ONE(4); }
-      }
+    W::lay(A, krows);
+    W::lay(A + W::IMAGE, vrows);
+    order_lds();
+    const int nk = (Tk + 15) >> 4;
+#define ONE(NK)                                                                                                                            \
+  if constexpr (BWD) bwd_window<DH, NT, NK>(a, toks[0], toks[1], Tq, Tk, head, A, qrows, grows, ls, A + 2 * W::IMAGE);                     \
+  else fwd_window<DH, NT, NK>(a, toks[0], toks[1], Tq, Tk, head, A, qrows)
+    if (nk == 1) { ONE(1); }
+    else if (NT == 2 || nk == 2) { ONE(2); }
+    else if constexpr (NT == 4) {
+      if (nk == 3) { ONE(3); } else { ONE(4); }
+    }
 #undef ONE
-    }
-    __syncthreads();
-    if (in_row) {
-      char* o = BWD ? (char*)a.dq : (char*)a.o;
-      const int64_t ldo = BWD ? a.lddq : a.ldo;
-#pragma unroll
-      for (int s = 0; s < PASSES; ++s) {
-        const int r = s * PASS + r0;
-        const char* at = lds + r * PITCH + ch * 16;
-        if (r < Tq) *reinterpret_cast<uint4*>(o + toks[0][r] * ldo * 2 + col) = *reinterpret_cast<const uint4*>(at + 2 * IMAGE);
-        if (BWD && r < Tk) {
-          *reinterpret_cast<uint4*>((char*)a.dk + toks[1][r] * a.lddk * 2 + col) = *reinterpret_cast<const uint4*>(at);
-          *reinterpret_cast<uint4*>((char*)a.dv + toks[1][r] * a.lddv * 2 + col) = *reinterpret_cast<const uint4*>(at + IMAGE);
-        }
-      }
-    }
-    if (!BWD && lr < Tq && head0 + lh < a.nhead) a.lse[(int64_t)toks[0][lr] * a.nhead + head0 + lh] = lse[threadIdx.x];
+    order_lds();
   }
 }
 
@@ -699,55 +707,43 @@ __global__ __launch_bounds__(64 * group_heads<DH>(), DH == 64 && NT == 4 && BWD 
 // waves of a workgroup.
 constexpr int SMALL_PITCH = 144;           // 128 bytes of a row
 
-template <int DH, bool BWD>
-__global__ __launch_bounds__(256, 2) void dot_small_kernel(DotArgs a) {
+// HALF: at most 8 tokens, one load brings a tensor's rows (rows 8 .. 15 then hold them once more)
+template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_windows(const DotArgs& a, int (*toks)[64], char* K) {
   constexpr int HG = 64 / DH, PITCH = SMALL_PITCH, IMAGE = 16 * PITCH, NI = BWD ? 4 : 3, TP = TILE_PITCH;
   using R = Rows<DH, PITCH>;
   constexpr int CT = R::CT;
-  static_assert(HG * 2 * TILE_BYTES <= NI * IMAGE || !BWD, "the P and dS tiles take the images' place");
-  __shared__ int toks_[4][2][64];
-  __shared__ __attribute__((aligned(16))) char lds_[4][NI * IMAGE];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
-  int (*toks)[64] = toks_[w];
-  char *K = lds_[w], *V = K + IMAGE, *Q = K + 2 * IMAGE, *G = K + 3 * IMAGE;
+  char *V = K + IMAGE, *Q = K + 2 * IMAGE, *G = K + 3 * IMAGE;
   const float c = a.scale * LOG2E;
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   const int head0 = blockIdx.y * HG;
   const int r8 = lane >> 3, ch = lane & 7;
   const bool in_row = head0 * DH + ch * 8 < a.nhead * DH;
   const int64_t col = in_row ? (int64_t)head0 * DH * 2 + ch * 16 : 0;
-  for (Walk walk(a, 1, 0, (int64_t)blockIdx.x * 4 + w, (int64_t)gridDim.x * 4); walk.next(a);) {
+  const int lhead = g < HG && head0 + g < a.nhead ? head0 + g : 0;
+  for (Walk walk(a, HALF ? 0 : 1, HALF ? 0 : 1, (int)blockIdx.x * 4 + w, (int)gridDim.x * 4); walk.next(a);) {
     int Tq, Tk;
-    walk.tokens(toks, 16, Tq, Tk);
+    walk.tokens(toks, HALF ? 8 : 16, Tq, Tk);
     if (Tq == 0 || Tk == 0) continue;                    // (in no list: the rows are zeroed elsewhere)
-    const bool more_q = Tq > 8, more_k = Tk > 8;
     uint4 rows[NI][2];
-    {
-      const int64_t tk = toks[1][r8], tq = toks[0][r8];
-      rows[0][0] = *reinterpret_cast<const uint4*>((const char*)a.k + tk * a.ldk * 2 + col);
-      rows[1][0] = *reinterpret_cast<const uint4*>((const char*)a.v + tk * a.ldv * 2 + col);
-      rows[2][0] = *reinterpret_cast<const uint4*>((const char*)a.q + tq * a.ldq * 2 + col);
-      if constexpr (BWD) rows[3][0] = *reinterpret_cast<const uint4*>((const char*)a.g + tq * a.ldg * 2 + col);
+#pragma unroll
+    for (int u = 0; u < (HALF ? 1 : 2); ++u) {
+      const int64_t tk = toks[1][r8 + 8 * u], tq = toks[0][r8 + 8 * u];
+      rows[0][u] = *reinterpret_cast<const uint4*>((const char*)a.k + tk * a.ldk * 2 + col);
+      rows[1][u] = *reinterpret_cast<const uint4*>((const char*)a.v + tk * a.ldv * 2 + col);
+      rows[2][u] = *reinterpret_cast<const uint4*>((const char*)a.q + tq * a.ldq * 2 + col);
+      if constexpr (BWD) rows[3][u] = *reinterpret_cast<const uint4*>((const char*)a.g + tq * a.ldg * 2 + col);
     }
-    if (more_k) {
-      const int64_t tk = toks[1][r8 + 8];
-      rows[0][1] = *reinterpret_cast<const uint4*>((const char*)a.k + tk * a.ldk * 2 + col);
-      rows[1][1] = *reinterpret_cast<const uint4*>((const char*)a.v + tk * a.ldv * 2 + col);
-    } else {
-      rows[0][1] = rows[0][0];               // (rows that are no tokens hold anything finite that the window holds)
-      rows[1][1] = rows[1][0];
-    }
-    if (more_q) {
-      const int64_t tq = toks[0][r8 + 8];
-      rows[2][1] = *reinterpret_cast<const uint4*>((const char*)a.q + tq * a.ldq * 2 + col);
-      if constexpr (BWD) rows[3][1] = *reinterpret_cast<const uint4*>((const char*)a.g + tq * a.ldg * 2 + col);
-    } else {
-      rows[2][1] = rows[2][0];
-      if constexpr (BWD) rows[3][1] = rows[3][0];
+    if constexpr (HALF) {
+#pragma unroll
+      for (int t = 0; t < NI; ++t) rows[t][1] = rows[t][0];
     }
     // lane (g, i): the saved logarithm of query i, head g
-    float ls = INFINITY;                     // no query: P = 0
-    if (BWD && i < Tq && g < HG && head0 + g < a.nhead) ls = a.lse[(int64_t)toks[0][i] * a.nhead + head0 + g];
+    float ls = 0.f;
+    if constexpr (BWD) {
+      ls = a.lse[(int64_t)toks[0][i] * a.nhead + lhead];
+      if (i >= Tq) ls = INFINITY;            // no query: P = 0
+    }
 #pragma unroll
     for (int t = 0; t < NI; ++t)
 #pragma unroll
@@ -789,7 +785,7 @@ __global__ __launch_bounds__(256, 2) void dot_small_kernel(DotArgs a) {
       order_lds();
       if (in_row) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < (HALF ? 1 : 2); ++u) {
           const int r = r8 + 8 * u;
           if (r < Tq) *reinterpret_cast<uint4*>((char*)a.o + toks[0][r] * a.ldo * 2 + col) = *reinterpret_cast<const uint4*>(Q + r * PITCH + ch * 16);
         }
@@ -854,7 +850,7 @@ __global__ __launch_bounds__(256, 2) void dot_small_kernel(DotArgs a) {
       order_lds();
       if (in_row) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < (HALF ? 1 : 2); ++u) {
           const int r = r8 + 8 * u;
           const char* at = K + r * PITCH + ch * 16;
           if (r < Tq) *reinterpret_cast<uint4*>((char*)a.dq + toks[0][r] * a.lddq * 2 + col) = *reinterpret_cast<const uint4*>(at + 2 * IMAGE);
@@ -867,6 +863,17 @@ __global__ __launch_bounds__(256, 2) void dot_small_kernel(DotArgs a) {
     }
     order_lds();
   }
+}
+
+template <int DH, bool BWD>
+__global__ __launch_bounds__(256, 2) void dot_small_kernel(DotArgs a) {
+  constexpr int IMAGE = 16 * SMALL_PITCH, NI = BWD ? 4 : 3;
+  static_assert(64 / DH * 2 * TILE_BYTES <= NI * IMAGE || !BWD, "the P and dS tiles take the images' place");
+  __shared__ int toks[4][2][64];
+  __shared__ __attribute__((aligned(16))) char lds[4][NI * IMAGE];
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  small_windows<DH, BWD, false>(a, toks[w], lds[w]);
+  small_windows<DH, BWD, true>(a, toks[w], lds[w]);
 }
 
 // The windows that are in no list: zero rows for queries without a key (out, or dq) and for keys without a query (dk, dv).  One wave per
@@ -934,13 +941,13 @@ template <class F> void by_head(int dh, F&& f) {
   else f(std::integral_constant<int, 64>());
 }
 template <int DH, int NT, bool BWD> int launch_windows(const DotArgs& a, int64_t windows, hipStream_t stream) {
-  constexpr int HPB = group_heads<DH>(), LDS = window_lds<DH, NT, BWD>();
+  constexpr int LDS = 4 * window_lds<DH, NT, BWD>();
   if (windows == 0) return TMAE_OK;
   static TmaeLdsAttr attr;
-  if (LDS > 65536)
+  if (LDS + 2048 > 65536)
     if (int e = tmae_allow_lds(attr, (const void*)dot_window_kernel<DH, NT, BWD>, LDS)) return e;
-  const unsigned gy = (unsigned)((a.nhead + HPB - 1) / HPB);
-  hipLaunchKernelGGL((dot_window_kernel<DH, NT, BWD>), dim3(walkers(windows, 1, gy, 8), gy), dim3(64 * HPB), LDS, stream, a);
+  const unsigned gy = (unsigned)((a.nhead + 3) / 4);
+  hipLaunchKernelGGL((dot_window_kernel<DH, NT, BWD>), dim3(walkers(windows, 1, gy, 8), gy), dim3(256), LDS, stream, a);
   return TMAE_OK;
 }
 template <int DH, bool BWD> int launch_bf16(const DotArgs& a, hipStream_t stream) {
