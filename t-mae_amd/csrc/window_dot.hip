@@ -26,7 +26,7 @@ struct DotArgs {
   int64_t ldq, ldk, ldv, ldg;
   void *o, *dq, *dk, *dv;
   int64_t ldo, lddq, lddk, lddv;
-  float* lse;                              // [mq, nhead]: log2 of sum_j 2^(c q.k_j), c = scale * log2(e)
+  float* lse;                              // [nhead, mq]: log2 of sum_j 2^(c q.k_j), c = scale * log2(e)
   const int32_t *grid_q, *grid_k, *wl;
   int64_t mq, mk, nwin;
   int nhead, batch, ny, nx, Wy, Wx, s;
@@ -174,11 +174,11 @@ __global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
   __shared__ int toks_[4][2][64];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
   int (*toks)[64] = toks_[w];
-  const int head = blockIdx.y * 4 + w;
+  const int head = blockIdx.x * 4 + w;
   if (head >= a.nhead) return;
   const int hoff = head * DH;
   T* out = (T*)a.o + hoff;
-  for (Walk walk(a, 3, 0, (int)blockIdx.x, (int)gridDim.x); walk.next(a);) {
+  for (Walk walk(a, 3, 0, (int)blockIdx.y, (int)gridDim.y); walk.next(a);) {
   struct { int Tq, Tk; } win;
   walk.tokens(toks, 64, win.Tq, win.Tk);
   if (win.Tk == 0) {
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
       const float inv = 1.f / l;
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) store_four<T>(out + tq * a.ldo + 16 * ct + 4 * g, o[ct] * inv);
-      if (g == 0) a.lse[tq * a.nhead + head] = mx + __builtin_amdgcn_logf(l);          // v_log_f32: the logarithm to base 2
+      if (g == 0) a.lse[(int64_t)head * a.mq + tq] = mx + __builtin_amdgcn_logf(l);          // v_log_f32: the logarithm to base 2
     }
   }
   }
@@ -245,11 +245,11 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_kernel(DotArgs a) {
   __shared__ float lse[4][64], dot[4][64];               // of the query slots: saved log2 denominator, sum_j P dP
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
   int (*toks)[64] = toks_[w];
-  const int head = blockIdx.y * 4 + w;
+  const int head = blockIdx.x * 4 + w;
   if (head >= a.nhead) return;
   const int hoff = head * DH;
   T *dq = (T*)a.dq + hoff, *dk = (T*)a.dk + hoff, *dv = (T*)a.dv + hoff;
-  for (Walk walk(a, 3, 0, (int)blockIdx.x, (int)gridDim.x); walk.next(a);) {
+  for (Walk walk(a, 3, 0, (int)blockIdx.y, (int)gridDim.y); walk.next(a);) {
   struct { int Tq, Tk; } win;
   walk.tokens(toks, 64, win.Tq, win.Tk);
   if (win.Tq == 0 || win.Tk == 0) {
@@ -266,7 +266,7 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_kernel(DotArgs a) {
   const T *q = (const T*)a.q + hoff, *k = (const T*)a.k + hoff, *v = (const T*)a.v + hoff, *gr = (const T*)a.g + hoff;
   const int nq = (win.Tq + 15) >> 4, nk = (win.Tk + 15) >> 4;
   const float c = a.scale * LOG2E;
-  lse[w][lane] = a.lse[(int64_t)toks[0][lane] * a.nhead + head];
+  lse[w][lane] = a.lse[(int64_t)head * a.mq + toks[0][lane]];
   order_lds();
   // dQ: the query in the column
   for (int qt = 0; qt < nq; ++qt) {
@@ -451,16 +451,19 @@ template <int DH, int NT> struct Window {
   using R = Rows<DH, PITCH>;
   static constexpr int CT = R::CT;
 
-  static __device__ __forceinline__ void request(uint4* rows, const void* base, int64_t ld, const int* toks, int64_t col) {
+  struct Loaded { u32x4 row[LOADS]; };
+  static __device__ __forceinline__ Loaded request(const void* base, int64_t ld, const int* toks, int64_t col) {
     const int lane = threadIdx.x & 63;
+    Loaded l;
 #pragma unroll
     for (int s = 0; s < LOADS; ++s)
-      rows[s] = *reinterpret_cast<const uint4*>((const char*)base + (int64_t)toks[s * RPI + lane / CHUNKS] * ld * 2 + col + (lane % CHUNKS) * 16);
+      l.row[s] = *reinterpret_cast<const u32x4*>((const char*)base + (int64_t)toks[s * RPI + lane / CHUNKS] * ld * 2 + col + (lane % CHUNKS) * 16);
+    return l;
   }
-  static __device__ __forceinline__ void lay(char* image, const uint4* rows) {
+  static __device__ __forceinline__ void lay(char* image, Loaded l) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int s = 0; s < LOADS; ++s) *reinterpret_cast<uint4*>(image + (s * RPI + lane / CHUNKS) * PITCH + (lane % CHUNKS) * 16) = rows[s];
+    for (int s = 0; s < LOADS; ++s) *reinterpret_cast<u32x4*>(image + (s * RPI + lane / CHUNKS) * PITCH + (lane % CHUNKS) * 16) = l.row[s];
   }
   static __device__ __forceinline__ void store(void* base, int64_t ld, const int* toks, int T, int64_t col, const char* image) {
     const int lane = threadIdx.x & 63;
@@ -476,7 +479,8 @@ template <int DH, int NT> struct Window {
 
 // NK key tiles against nq query tiles.  NK is a template parameter, so that no branch stands between a matrix instruction and its reader.
 template <int DH, int NT, int NK>
-__device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq, const int* tk, int Tq, int Tk, int head, char* A, const uint4* qrows) {
+__device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq, const int* tk, int Tq, int Tk, int head, char* A,
+                                           typename Window<DH, NT>::Loaded qrows) {
   using W = Window<DH, NT>;
   using R = typename W::R;
   constexpr int CT = W::CT, TILE = W::TILE;
@@ -537,12 +541,12 @@ __device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq, cons
   }
   order_lds();
   W::store(a.o, a.ldo, tq, Tq, col, A);
-  if (lane < Tq) a.lse[(int64_t)tq[lane] * a.nhead + head] = my_lse;
+  if (lane < Tq) a.lse[(int64_t)head * a.mq + tq[lane]] = my_lse;
 }
 
 template <int DH, int NT, int NK>
-__device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, const int* tk, int Tq, int Tk, int head, char* A, const uint4* qrows,
-                                           const uint4* grows, float ls, char* tiles) {
+__device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, const int* tk, int Tq, int Tk, int head, char* A,
+                                           typename Window<DH, NT>::Loaded qrows, typename Window<DH, NT>::Loaded grows, float ls, char* tiles) {
   using W = Window<DH, NT>;
   using R = typename W::R;
   constexpr int CT = W::CT, TILE = W::TILE, TP = TILE_PITCH;
@@ -657,10 +661,10 @@ __global__ __launch_bounds__(256, DH == 64 && NT == 4 && BWD ? 1 : 2) void dot_w
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int (*toks)[64] = toks_[w];
   char* A = lds_ + w * window_lds<DH, NT, BWD>();
-  const int head = blockIdx.y * 4 + w;
+  const int head = blockIdx.x * 4 + w;
   if (head >= a.nhead) return;
   const int64_t col = (int64_t)head * DH * 2;
-  for (Walk walk(a, NT == 4 ? 3 : 2, NT == 4 ? 3 : 2, (int)blockIdx.x, (int)gridDim.x); walk.next(a);) {
+  for (Walk walk(a, NT == 4 ? 3 : 2, NT == 4 ? 3 : 2, (int)blockIdx.y, (int)gridDim.y); walk.next(a);) {
     int Tq, Tk;
     walk.tokens(toks, NT * 16, Tq, Tk);
     if (Tq == 0 || Tk == 0) {
@@ -676,14 +680,13 @@ __global__ __launch_bounds__(256, DH == 64 && NT == 4 && BWD ? 1 : 2) void dot_w
       }
       continue;
     }
-    uint4 krows[W::LOADS], vrows[W::LOADS], qrows[W::LOADS], grows[W::LOADS];
-    W::request(krows, a.k, a.ldk, toks[1], col);
-    W::request(vrows, a.v, a.ldv, toks[1], col);
-    W::request(qrows, a.q, a.ldq, toks[0], col);
+    const typename W::Loaded krows = W::request(a.k, a.ldk, toks[1], col), vrows = W::request(a.v, a.ldv, toks[1], col),
+                             qrows = W::request(a.q, a.ldq, toks[0], col);
+    typename W::Loaded grows;
     float ls = 0.f;
     if constexpr (BWD) {
-      W::request(grows, a.g, a.ldg, toks[0], col);
-      ls = a.lse[(int64_t)toks[0][lane] * a.nhead + head];
+      grows = W::request(a.g, a.ldg, toks[0], col);
+      ls = a.lse[(int64_t)head * a.mq + toks[0][lane]];
       if (lane >= Tq) ls = INFINITY;
     }
     W::lay(A, krows);
@@ -716,12 +719,12 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
   char *V = K + IMAGE, *Q = K + 2 * IMAGE, *G = K + 3 * IMAGE;
   const float c = a.scale * LOG2E;
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  const int head0 = blockIdx.y * HG;
+  const int head0 = blockIdx.x * HG;
   const int r8 = lane >> 3, ch = lane & 7;
   const bool in_row = head0 * DH + ch * 8 < a.nhead * DH;
   const int64_t col = in_row ? (int64_t)head0 * DH * 2 + ch * 16 : 0;
   const int lhead = g < HG && head0 + g < a.nhead ? head0 + g : 0;
-  for (Walk walk(a, HALF ? 0 : 1, HALF ? 0 : 1, (int)blockIdx.x * 4 + w, (int)gridDim.x * 4); walk.next(a);) {
+  for (Walk walk(a, HALF ? 0 : 1, HALF ? 0 : 1, (int)blockIdx.y * 4 + w, (int)gridDim.y * 4); walk.next(a);) {
     int Tq, Tk;
     walk.tokens(toks, HALF ? 8 : 16, Tq, Tk);
     if (Tq == 0 || Tk == 0) continue;                    // (in no list: the rows are zeroed elsewhere)
@@ -741,7 +744,7 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
     // lane (g, i): the saved logarithm of query i, head g
     float ls = 0.f;
     if constexpr (BWD) {
-      ls = a.lse[(int64_t)toks[0][i] * a.nhead + lhead];
+      ls = a.lse[(int64_t)lhead * a.mq + toks[0][i]];
       if (i >= Tq) ls = INFINITY;            // no query: P = 0
     }
 #pragma unroll
@@ -790,7 +793,7 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
           if (r < Tq) *reinterpret_cast<uint4*>((char*)a.o + toks[0][r] * a.ldo * 2 + col) = *reinterpret_cast<const uint4*>(Q + r * PITCH + ch * 16);
         }
       }
-      if (i < Tq && g < HG && head0 + g < a.nhead) a.lse[(int64_t)toks[0][i] * a.nhead + head0 + g] = out_lse;
+      if (i < Tq && g < HG && head0 + g < a.nhead) a.lse[(int64_t)(head0 + g) * a.mq + toks[0][i]] = out_lse;
     } else {
       s16x4 kc[HG][CT], qc[HG][CT], gc[HG][CT], ds[HG];
       f32x4 p[HG], dp[HG];
@@ -947,7 +950,7 @@ template <int DH, int NT, bool BWD> int launch_windows(const DotArgs& a, int64_t
   if (LDS + 2048 > 65536)
     if (int e = tmae_allow_lds(attr, (const void*)dot_window_kernel<DH, NT, BWD>, LDS)) return e;
   const unsigned gy = (unsigned)((a.nhead + 3) / 4);
-  hipLaunchKernelGGL((dot_window_kernel<DH, NT, BWD>), dim3(walkers(windows, 1, gy, 8), gy), dim3(256), LDS, stream, a);
+  hipLaunchKernelGGL((dot_window_kernel<DH, NT, BWD>), dim3(gy, walkers(windows, 1, gy, 8)), dim3(256), LDS, stream, a);
   return TMAE_OK;
 }
 template <int DH, bool BWD> int launch_bf16(const DotArgs& a, hipStream_t stream) {
@@ -957,14 +960,14 @@ template <int DH, bool BWD> int launch_bf16(const DotArgs& a, hipStream_t stream
   if (rc != TMAE_OK) return rc;
   const unsigned gy = (unsigned)((a.nhead * DH + 63) / 64);
   const int64_t small = class_windows(a, 0);
-  if (small > 0) hipLaunchKernelGGL((dot_small_kernel<DH, BWD>), dim3(walkers(small, 4, gy, 8), gy), dim3(256), 0, stream, a);
+  if (small > 0) hipLaunchKernelGGL((dot_small_kernel<DH, BWD>), dim3(gy, walkers(small, 4, gy, 8)), dim3(256), 0, stream, a);
   return TMAE_OK;
 }
 template <int DH, bool BWD> void launch_f32(const DotArgs& a, hipStream_t stream) {
   const unsigned gy = (unsigned)((a.nhead + 3) / 4);
   const int64_t windows = a.wl ? class_windows(a, 0) : a.nwin;
   if (windows == 0) return;
-  const dim3 grid(walkers(windows, 1, gy, 8), gy);
+  const dim3 grid(gy, walkers(windows, 1, gy, 8));
   if constexpr (BWD) hipLaunchKernelGGL((dot_bwd_kernel<float, DH>), grid, dim3(256), 0, stream, a);
   else hipLaunchKernelGGL((dot_fwd_kernel<float, DH>), grid, dim3(256), 0, stream, a);
 }

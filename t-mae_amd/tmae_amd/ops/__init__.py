@@ -1967,7 +1967,7 @@ def _win_attn_dot_launch(a, b, c, grid_q, grid_k, worklist, meta):
     d, nhead, batch, ny, nx, do_shift, scale, covered = meta
     mq, mk = a.shape[0], (a if b is None else b).shape[0]
     out = (torch.empty if covered else torch.zeros)((mq, d), dtype=a.dtype, device=a.device)
-    lse = torch.empty((mq, nhead), dtype=torch.float32, device=a.device)        # read back in the windows that wrote it only
+    lse = torch.empty((nhead, mq), dtype=torch.float32, device=a.device)        # read back in the windows that wrote it only
     with _Launch(a) as s:
         check(lib.tmae_win_attn_dot_fwd(*_WinAttn._ptrs(a, b, c, d), _dt(a), mq, mk, nhead, d // nhead, _p(grid_q), _p(grid_k), batch,
                                         ny, nx, do_shift, scale, _p(out), d, _p(lse), _p(worklist), s), 'tmae_win_attn_dot_fwd')
