@@ -40,7 +40,7 @@ extern "C" {
  * entry point does with its arguments; tmae_abi_hash() is the fingerprint of THIS header's prototypes (name, return class and
  * argument classes in order: tmae_amd/_abi.py) that the build compiled in.  The Python binding compares both at import, so a
  * stale library, or a binding row that disagrees with its prototype, fails there and not inside a launch. */
-#define TMAE_ABI_VERSION 27
+#define TMAE_ABI_VERSION 28
 int tmae_abi_version(void);
 int tmae_abi_hash(void);
 
@@ -638,14 +638,14 @@ int tmae_qk_norm_rotary_bwd(const void* x, int64_t ldx, int64_t hpx, const void*
 
 /* ---- scaled-dot-product attention inside 8x8 windows -- layouts, grids, shift and work list of tmae_win_attn_fwd / _bwd; the logits
  * are scale * q . k (scale > 0), any number of heads, dh in {16, 32, 64}.  Every
- * base and row pitch is a multiple of 16 bytes.  lse [nhead, mq] f32 (log2 of the softmax's denominator) is kept for the backward.
+ * base and row pitch is a multiple of 16 bytes.  The backward needs the forward's inputs only.
  * Every row that stands in a grid is written: zero rows where its window has no key (for dk / dv: no query).  A grid entry that is no
  * row of its tensor counts as an empty cell.  worklist (may be NULL: every window is visited) is of these grids and this shift. */
 int tmae_win_attn_dot_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, int dtype, int64_t mq,
                           int64_t mk, int nhead, int dh, const int32_t* grid_q, const int32_t* grid_k, int batch, int ny, int nx,
-                          int do_shift, float scale, void* out, int64_t ldo, float* lse, const int32_t* worklist, void* stream);
+                          int do_shift, float scale, void* out, int64_t ldo, const int32_t* worklist, void* stream);
 int tmae_win_attn_dot_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, const void* dout,
-                          int64_t lddo, const float* lse, int dtype, int64_t mq, int64_t mk, int nhead, int dh, const int32_t* grid_q,
+                          int64_t lddo, int dtype, int64_t mq, int64_t mk, int nhead, int dh, const int32_t* grid_q,
                           const int32_t* grid_k, int batch, int ny, int nx, int do_shift, float scale, void* dq, int64_t lddq, void* dk,
                           int64_t lddk, void* dv, int64_t lddv, const int32_t* worklist, void* stream);
 

@@ -1,7 +1,8 @@
 // Scaled-dot-product attention inside 8x8 windows of the token grid.
 //
 //   P_ij = softmax_j(scale q_i . k_j) over the keys j of the query's window,  o_i = sum_j P_ij v_j;  a window without keys: o_i = 0
-//   backward, P recomputed from the saved log2 of the softmax's denominator:
+//   backward, P recomputed from q and k (nothing is kept of the forward but its inputs: a log-sum-exp a row and head, 4 bytes at a time in
+//   rows that lie apart, took longer to write and read than the row maxima and sums take to compute again):
 //   dV_j = sum_i P_ij dO_i,  dP_ij = dO_i . v_j,  dS_ij = scale P_ij (dP_ij - sum_j P_ij dP_ij),  dQ_i = sum_j dS_ij k_j,  dK_j = sum_i dS_ij q_i
 //
 // One wavefront per (window, head), tiles of 16 tokens on the float32 matrix instruction 16x16x4.  Its accumulator layout -- lane
@@ -26,7 +27,6 @@ struct DotArgs {
   int64_t ldq, ldk, ldv, ldg;
   void *o, *dq, *dk, *dv;
   int64_t ldo, lddq, lddk, lddv;
-  float* lse;                              // [nhead, mq]: log2 of sum_j 2^(c q.k_j), c = scale * log2(e)
   const int32_t *grid_q, *grid_k, *wl;
   int64_t mq, mk, nwin;
   int nhead, batch, ny, nx, Wy, Wx, s;
@@ -232,7 +232,6 @@ __global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
       const float inv = 1.f / l;
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) store_four<T>(out + tq * a.ldo + 16 * ct + 4 * g, o[ct] * inv);
-      if (g == 0) a.lse[(int64_t)head * a.mq + tq] = mx + __builtin_amdgcn_logf(l);          // v_log_f32: the logarithm to base 2
     }
   }
   }
@@ -242,7 +241,7 @@ template <class T, int DH>
 __global__ __launch_bounds__(256, 2) void dot_bwd_kernel(DotArgs a) {
   constexpr int KD = DH / 4, CT = DH / 16;
   __shared__ int toks_[4][2][64];
-  __shared__ float lse[4][64], dot[4][64];               // of the query slots: saved log2 denominator, sum_j P dP
+  __shared__ float top[4][64], inv[4][64], dot[4][64];   // of the query slots: c * the largest logit, 1 / sum_j, sum_j P dP
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
   int (*toks)[64] = toks_[w];
   const int head = blockIdx.x * 4 + w;
@@ -266,35 +265,45 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_kernel(DotArgs a) {
   const T *q = (const T*)a.q + hoff, *k = (const T*)a.k + hoff, *v = (const T*)a.v + hoff, *gr = (const T*)a.g + hoff;
   const int nq = (win.Tq + 15) >> 4, nk = (win.Tk + 15) >> 4;
   const float c = a.scale * LOG2E;
-  lse[w][lane] = a.lse[(int64_t)head * a.mq + toks[0][lane]];
-  order_lds();
   // dQ: the query in the column
   for (int qt = 0; qt < nq; ++qt) {
     const int64_t tq = toks[0][qt * 16 + i];
-    const float ls = lse[w][qt * 16 + i];
     float qf[KD], gf[KD];
     load_frag<T, KD>(q + tq * a.ldq + KD * g, qf);
     load_frag<T, KD>(gr + tq * a.ldg + KD * g, gf);
     f32x4 p[4], dp[4], acc[CT];
-    float d = 0.f;
+    float d = 0.f, l = 0.f, mx = -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
       if (kt < nk) {
         const int64_t tk = toks[1][kt * 16 + i];
         float f[KD];
         load_frag<T, KD>(k + tk * a.ldk + KD * g, f);
-        const f32x4 s = product<KD>(f, qf);
+        p[kt] = product<KD>(f, qf);
         load_frag<T, KD>(v + tk * a.ldv + KD * g, f);
         dp[kt] = product<KD>(f, gf);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          p[kt][r] = kt * 16 + 4 * g + r < win.Tk ? __builtin_amdgcn_exp2f(fmaf(s[r], c, -ls)) : 0.f;
+          if (kt * 16 + 4 * g + r >= win.Tk) p[kt][r] = -INFINITY;
+          mx = fmaxf(mx, p[kt][r]);
+        }
+      }
+    }
+    mx = lanes4_max(mx) * c;
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+      if (kt < nk) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          p[kt][r] = kt * 16 + 4 * g + r < win.Tk ? __builtin_amdgcn_exp2f(fmaf(p[kt][r], c, -mx)) : 0.f;
+          l += p[kt][r];
           d += p[kt][r] * dp[kt][r];
         }
       }
     }
-    d = lanes4_sum(d);
-    if (g == 0) dot[w][qt * 16 + i] = d;
+    const float il = 1.f / lanes4_sum(l);
+    d = lanes4_sum(d) * il;
+    if (g == 0) { dot[w][qt * 16 + i] = d; top[w][qt * 16 + i] = mx; inv[w][qt * 16 + i] = il; }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) acc[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -302,7 +311,7 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_kernel(DotArgs a) {
       if (kt < nk) {
         f32x4 ds;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) ds[r] = a.scale * p[kt][r] * (dp[kt][r] - d);
+        for (int r = 0; r < 4; ++r) ds[r] = a.scale * (p[kt][r] * il) * (dp[kt][r] - d);
         accumulate<T, CT>(k, a.ldk, toks[1] + kt * 16, ds, acc, g, i);
       }
     }
@@ -332,7 +341,7 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_kernel(DotArgs a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int slot = qt * 16 + 4 * g + r;
-        p[r] = slot < win.Tq ? __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse[w][slot])) : 0.f;
+        p[r] = slot < win.Tq ? __builtin_amdgcn_exp2f(fmaf(s[r], c, -top[w][slot])) * inv[w][slot] : 0.f;
         ds[r] = a.scale * p[r] * (dp[r] - dot[w][slot]);
       }
       accumulate<T, CT>(gr, a.ldg, toks[0] + qt * 16, p, av, g, i);
@@ -503,7 +512,6 @@ __device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq, cons
 #pragma unroll
   for (int r = 0; r < 4; ++r) absent[r] = (NK - 1) * 16 + 4 * g + r < Tk ? 0.f : -INFINITY;
   const float c = a.scale * LOG2E;
-  float my_lse = 0.f;                        // lane (g, i): of query 16 g + i
   for (int qt = 0; qt < nq; ++qt) {
     const typename R::Piece qf = R::piece(A + qt * TILE, g, i);
     f32x4 st[NK];
@@ -537,16 +545,14 @@ __device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq, cons
       if constexpr (NK == 1) o[ct] = over_tokens(vc[0][ct], p[0], o[ct]);
     }
     R::put(A + qt * TILE, g, i, o, __builtin_amdgcn_rcpf(l));
-    if (g == qt) my_lse = mx + __builtin_amdgcn_logf(l);                 // v_log_f32: to base 2
   }
   order_lds();
   W::store(a.o, a.ldo, tq, Tq, col, A);
-  if (lane < Tq) a.lse[(int64_t)head * a.mq + tq[lane]] = my_lse;
 }
 
 template <int DH, int NT, int NK>
 __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, const int* tk, int Tq, int Tk, int head, char* A,
-                                           typename Window<DH, NT>::Loaded qrows, typename Window<DH, NT>::Loaded grows, float ls, char* tiles) {
+                                           typename Window<DH, NT>::Loaded qrows, typename Window<DH, NT>::Loaded grows, char* tiles) {
   using W = Window<DH, NT>;
   using R = typename W::R;
   constexpr int CT = W::CT, TILE = W::TILE, TP = TILE_PITCH;
@@ -584,9 +590,8 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
       qc[ct] = R::columns(A + qt * TILE, g, i, ct);
       gc[ct] = R::columns(B + qt * TILE, g, i, ct);
     }
-    const float le = __shfl(ls, qt * 16 + i, 64);                // +inf where there is no query: P = 0
     f32x4 p[NK], dp[NK];
-    float d = 0.f;
+    float d = 0.f, l = 0.f, mx = -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < NK; ++kt) {
       p[kt] = R::over_channels(kf[kt], qf, kt == NK - 1 ? absent : zero);           // rows = keys, column = query i
@@ -595,11 +600,18 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
 #pragma unroll
     for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
+      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, p[kt][r]);
+    mx = column_max(mx) * c;
+#pragma unroll
+    for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
       for (int r = 0; r < 4; ++r) {
-        p[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[kt][r], c, -le));
+        p[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[kt][r], c, -mx));
+        l += p[kt][r];
         d = __builtin_fmaf(p[kt][r], dp[kt][r], d);
       }
-    d = column_sum(d);
+    const float il = qt * 16 + i < Tq ? __builtin_amdgcn_rcpf(column_sum(l)) : 0.f;             // no query: P = 0
+    d = column_sum(d) * il;
     s16x4 ds[NK];
 #pragma unroll
     for (int k0 = 0; k0 < NK; k0 += 2) {
@@ -607,7 +619,10 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
       for (int kt = k0; kt < (k0 + 2 < NK ? k0 + 2 : NK); ++kt) {
         f32x4 t;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) t[r] = p[kt][r] * (dp[kt][r] - d);
+        for (int r = 0; r < 4; ++r) {
+          p[kt][r] *= il;
+          t[r] = p[kt][r] * (dp[kt][r] - d);
+        }
         ds[kt] = pack4(t);
         char* tile = tiles + (kt - k0) * 2 * TILE_BYTES;
         *reinterpret_cast<s16x4*>(tile + i * TP + 8 * g) = pack4(p[kt]);
@@ -653,8 +668,11 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
 // Windows of up to 16 NT tokens; without a work list (NT = 4) every window, empty ones included.  Two waves per SIMD as the bound: 256
 // registers at most, and the matrix instructions then write plain vector registers (the backward of 64 channels by 64 tokens needs more).
 template <int DH, int NT, bool BWD> constexpr int window_lds() { return 2 * Window<DH, NT>::IMAGE + (BWD ? 4 * TILE_BYTES : 0); }
+template <int DH, int NT, bool BWD> constexpr int window_waves() {        // waves per SIMD that the registers allow
+  return DH == 16 ? (BWD ? (NT == 4 ? 3 : 4) : (NT == 4 ? 5 : 8)) : DH == 32 ? (BWD ? (NT == 4 ? 2 : 3) : (NT == 4 ? 4 : 5)) : BWD && NT == 4 ? 1 : 2;
+}
 template <int DH, int NT, bool BWD>
-__global__ __launch_bounds__(256, DH == 64 && NT == 4 && BWD ? 1 : 2) void dot_window_kernel(DotArgs a) {
+__global__ __launch_bounds__(256, (window_waves<DH, NT, BWD>())) void dot_window_kernel(DotArgs a) {
   using W = Window<DH, NT>;
   extern __shared__ __attribute__((aligned(16))) char lds_[];
   __shared__ int toks_[4][2][64];
@@ -682,19 +700,16 @@ __global__ __launch_bounds__(256, DH == 64 && NT == 4 && BWD ? 1 : 2) void dot_w
     }
     const typename W::Loaded krows = W::request(a.k, a.ldk, toks[1], col), vrows = W::request(a.v, a.ldv, toks[1], col),
                              qrows = W::request(a.q, a.ldq, toks[0], col);
+    constexpr bool LATE = DH * NT >= 128;                // registers: dO is requested when K and V have left theirs
     typename W::Loaded grows;
-    float ls = 0.f;
-    if constexpr (BWD) {
-      grows = W::request(a.g, a.ldg, toks[0], col);
-      ls = a.lse[(int64_t)head * a.mq + toks[0][lane]];
-      if (lane >= Tq) ls = INFINITY;
-    }
+    if constexpr (BWD && !LATE) grows = W::request(a.g, a.ldg, toks[0], col);
     W::lay(A, krows);
     W::lay(A + W::IMAGE, vrows);
     order_lds();
+    if constexpr (BWD && LATE) grows = W::request(a.g, a.ldg, toks[0], col);
     const int nk = (Tk + 15) >> 4;
 #define ONE(NK)                                                                                                                            \
-  if constexpr (BWD) bwd_window<DH, NT, NK>(a, toks[0], toks[1], Tq, Tk, head, A, qrows, grows, ls, A + 2 * W::IMAGE);                     \
+  if constexpr (BWD) bwd_window<DH, NT, NK>(a, toks[0], toks[1], Tq, Tk, head, A, qrows, grows, A + 2 * W::IMAGE);                         \
   else fwd_window<DH, NT, NK>(a, toks[0], toks[1], Tq, Tk, head, A, qrows)
     if (nk == 1) { ONE(1); }
     else if (NT == 2 || nk == 2) { ONE(2); }
@@ -711,11 +726,11 @@ __global__ __launch_bounds__(256, DH == 64 && NT == 4 && BWD ? 1 : 2) void dot_w
 constexpr int SMALL_PITCH = 144;           // 128 bytes of a row
 
 // HALF: at most 8 tokens, one load brings a tensor's rows (rows 8 .. 15 then hold them once more)
-template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_windows(const DotArgs& a, int (*toks)[64], char* K) {
+template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_window(const DotArgs& a, const int (*toks)[64], int Tq, int Tk, char* K) {
   constexpr int HG = 64 / DH, PITCH = SMALL_PITCH, IMAGE = 16 * PITCH, NI = BWD ? 4 : 3, TP = TILE_PITCH;
   using R = Rows<DH, PITCH>;
   constexpr int CT = R::CT;
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
+  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
   char *V = K + IMAGE, *Q = K + 2 * IMAGE, *G = K + 3 * IMAGE;
   const float c = a.scale * LOG2E;
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
@@ -723,148 +738,138 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
   const int r8 = lane >> 3, ch = lane & 7;
   const bool in_row = head0 * DH + ch * 8 < a.nhead * DH;
   const int64_t col = in_row ? (int64_t)head0 * DH * 2 + ch * 16 : 0;
-  const int lhead = g < HG && head0 + g < a.nhead ? head0 + g : 0;
-  for (Walk walk(a, HALF ? 0 : 1, HALF ? 0 : 1, (int)blockIdx.y * 4 + w, (int)gridDim.y * 4); walk.next(a);) {
-    int Tq, Tk;
-    walk.tokens(toks, HALF ? 8 : 16, Tq, Tk);
-    if (Tq == 0 || Tk == 0) continue;                    // (in no list: the rows are zeroed elsewhere)
-    uint4 rows[NI][2];
+  u32x4 rows[NI][2];
 #pragma unroll
-    for (int u = 0; u < (HALF ? 1 : 2); ++u) {
-      const int64_t tk = toks[1][r8 + 8 * u], tq = toks[0][r8 + 8 * u];
-      rows[0][u] = *reinterpret_cast<const uint4*>((const char*)a.k + tk * a.ldk * 2 + col);
-      rows[1][u] = *reinterpret_cast<const uint4*>((const char*)a.v + tk * a.ldv * 2 + col);
-      rows[2][u] = *reinterpret_cast<const uint4*>((const char*)a.q + tq * a.ldq * 2 + col);
-      if constexpr (BWD) rows[3][u] = *reinterpret_cast<const uint4*>((const char*)a.g + tq * a.ldg * 2 + col);
+  for (int u = 0; u < (HALF ? 1 : 2); ++u) {
+    const int64_t tk = toks[1][r8 + 8 * u], tq = toks[0][r8 + 8 * u];
+    rows[0][u] = *reinterpret_cast<const u32x4*>((const char*)a.k + tk * a.ldk * 2 + col);
+    rows[1][u] = *reinterpret_cast<const u32x4*>((const char*)a.v + tk * a.ldv * 2 + col);
+    rows[2][u] = *reinterpret_cast<const u32x4*>((const char*)a.q + tq * a.ldq * 2 + col);
+    if constexpr (BWD) rows[3][u] = *reinterpret_cast<const u32x4*>((const char*)a.g + tq * a.ldg * 2 + col);
+  }
+  if constexpr (HALF) {
+#pragma unroll
+    for (int t = 0; t < NI; ++t) rows[t][1] = rows[t][0];
+  }
+#pragma unroll
+  for (int t = 0; t < NI; ++t)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) *reinterpret_cast<u32x4*>(K + t * IMAGE + (r8 + 8 * u) * PITCH + ch * 16) = rows[t][u];
+  order_lds();
+  f32x4 absent;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) absent[r] = 4 * g + r < Tk ? 0.f : -INFINITY;
+  if constexpr (!BWD) {
+    s16x4 vc[HG][CT], p[HG];
+    f32x4 st[HG];
+    float mx[HG], l[HG];
+#pragma unroll
+    for (int h = 0; h < HG; ++h) {
+      st[h] = R::over_channels(R::piece(K + h * DH * 2, g, i), R::piece(Q + h * DH * 2, g, i), absent);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) vc[h][ct] = R::columns(V + h * DH * 2, g, i, ct);
     }
-    if constexpr (HALF) {
 #pragma unroll
-      for (int t = 0; t < NI; ++t) rows[t][1] = rows[t][0];
+    for (int h = 0; h < HG; ++h) {
+      mx[h] = column_max(fmaxf(fmaxf(st[h][0], st[h][1]), fmaxf(st[h][2], st[h][3]))) * c;
+      l[h] = 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        st[h][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[h][r], c, -mx[h]));
+        l[h] += st[h][r];
+      }
+      p[h] = pack4(st[h]);
     }
-    // lane (g, i): the saved logarithm of query i, head g
-    float ls = 0.f;
-    if constexpr (BWD) {
-      ls = a.lse[(int64_t)lhead * a.mq + toks[0][i]];
-      if (i >= Tq) ls = INFINITY;            // no query: P = 0
+#pragma unroll
+    for (int h = 0; h < HG; ++h) {
+      f32x4 o[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) o[ct] = over_tokens(vc[h][ct], p[h], zero);
+      const float s = column_sum(l[h]);
+      R::put(Q + h * DH * 2, g, i, o, __builtin_amdgcn_rcpf(s));
     }
-#pragma unroll
-    for (int t = 0; t < NI; ++t)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) *reinterpret_cast<uint4*>(K + t * IMAGE + (r8 + 8 * u) * PITCH + ch * 16) = rows[t][u];
     order_lds();
-    f32x4 absent;
+    if (in_row) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) absent[r] = 4 * g + r < Tk ? 0.f : -INFINITY;
-    if constexpr (!BWD) {
-      s16x4 vc[HG][CT], p[HG];
-      f32x4 st[HG];
-      float mx[HG], l[HG], out_lse = 0.f;
-#pragma unroll
-      for (int h = 0; h < HG; ++h) {
-        st[h] = R::over_channels(R::piece(K + h * DH * 2, g, i), R::piece(Q + h * DH * 2, g, i), absent);
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) vc[h][ct] = R::columns(V + h * DH * 2, g, i, ct);
+      for (int u = 0; u < (HALF ? 1 : 2); ++u) {
+        const int r = r8 + 8 * u;
+        if (r < Tq) *reinterpret_cast<uint4*>((char*)a.o + toks[0][r] * a.ldo * 2 + col) = *reinterpret_cast<const uint4*>(Q + r * PITCH + ch * 16);
       }
+    }
+  } else {
+    s16x4 kc[HG][CT], qc[HG][CT], gc[HG][CT], ds[HG];
+    f32x4 p[HG], dp[HG];
 #pragma unroll
-      for (int h = 0; h < HG; ++h) {
-        mx[h] = column_max(fmaxf(fmaxf(st[h][0], st[h][1]), fmaxf(st[h][2], st[h][3]))) * c;
-        l[h] = 0.f;
+    for (int h = 0; h < HG; ++h) {
+      const int at = h * DH * 2;
+      p[h] = R::over_channels(R::piece(K + at, g, i), R::piece(Q + at, g, i), absent);
+      dp[h] = R::over_channels(R::piece(V + at, g, i), R::piece(G + at, g, i), zero);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          st[h][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[h][r], c, -mx[h]));
-          l[h] += st[h][r];
-        }
-        p[h] = pack4(st[h]);
-      }
-#pragma unroll
-      for (int h = 0; h < HG; ++h) {
-        f32x4 o[CT];
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) o[ct] = over_tokens(vc[h][ct], p[h], zero);
-        const float s = column_sum(l[h]);
-        R::put(Q + h * DH * 2, g, i, o, __builtin_amdgcn_rcpf(s));
-        if (g == h) out_lse = mx[h] + __builtin_amdgcn_logf(s);
-      }
-      order_lds();
-      if (in_row) {
-#pragma unroll
-        for (int u = 0; u < (HALF ? 1 : 2); ++u) {
-          const int r = r8 + 8 * u;
-          if (r < Tq) *reinterpret_cast<uint4*>((char*)a.o + toks[0][r] * a.ldo * 2 + col) = *reinterpret_cast<const uint4*>(Q + r * PITCH + ch * 16);
-        }
-      }
-      if (i < Tq && g < HG && head0 + g < a.nhead) a.lse[(int64_t)(head0 + g) * a.mq + toks[0][i]] = out_lse;
-    } else {
-      s16x4 kc[HG][CT], qc[HG][CT], gc[HG][CT], ds[HG];
-      f32x4 p[HG], dp[HG];
-#pragma unroll
-      for (int h = 0; h < HG; ++h) {
-        const int at = h * DH * 2;
-        p[h] = R::over_channels(R::piece(K + at, g, i), R::piece(Q + at, g, i), absent);
-        dp[h] = R::over_channels(R::piece(V + at, g, i), R::piece(G + at, g, i), zero);
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          kc[h][ct] = R::columns(K + at, g, i, ct);
-          qc[h][ct] = R::columns(Q + at, g, i, ct);
-          gc[h][ct] = R::columns(G + at, g, i, ct);
-        }
-      }
-      order_lds();
-#pragma unroll
-      for (int h = 0; h < HG; ++h) {
-        const float le = HG == 1 ? __shfl(ls, i, 64) : __shfl(ls, 16 * h + i, 64);
-        float d = 0.f;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          p[h][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[h][r], c, -le));
-          d = __builtin_fmaf(p[h][r], dp[h][r], d);
-        }
-        d = column_sum(d);
-        f32x4 t;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) t[r] = p[h][r] * (dp[h][r] - d);
-        ds[h] = pack4(t);
-        char* tile = K + h * 2 * TILE_BYTES;
-        *reinterpret_cast<s16x4*>(tile + i * TP + 8 * g) = pack4(p[h]);
-        *reinterpret_cast<s16x4*>(tile + TILE_BYTES + i * TP + 8 * g) = ds[h];
-      }
-      order_lds();
-      s16x4 pt[HG], dt[HG];
-#pragma unroll
-      for (int h = 0; h < HG; ++h) {
-        const char* tile = K + h * 2 * TILE_BYTES + (4 * g + (i >> 2)) * TP + 8 * (i & 3);
-        pt[h] = read_columns(tile);
-        dt[h] = read_columns(tile + TILE_BYTES);
-      }
-      order_lds();
-#pragma unroll
-      for (int h = 0; h < HG; ++h) {
-        f32x4 dq[CT], dk[CT], dv[CT];
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          dq[ct] = over_tokens(kc[h][ct], ds[h], zero);
-          dv[ct] = over_tokens(gc[h][ct], pt[h], zero);
-          dk[ct] = over_tokens(qc[h][ct], dt[h], zero);
-        }
-        R::put(Q + h * DH * 2, g, i, dq, a.scale);
-        R::put(K + h * DH * 2, g, i, dk, a.scale);
-        R::put(V + h * DH * 2, g, i, dv, 1.f);
-      }
-      order_lds();
-      if (in_row) {
-#pragma unroll
-        for (int u = 0; u < (HALF ? 1 : 2); ++u) {
-          const int r = r8 + 8 * u;
-          const char* at = K + r * PITCH + ch * 16;
-          if (r < Tq) *reinterpret_cast<uint4*>((char*)a.dq + toks[0][r] * a.lddq * 2 + col) = *reinterpret_cast<const uint4*>(at + 2 * IMAGE);
-          if (r < Tk) {
-            *reinterpret_cast<uint4*>((char*)a.dk + toks[1][r] * a.lddk * 2 + col) = *reinterpret_cast<const uint4*>(at);
-            *reinterpret_cast<uint4*>((char*)a.dv + toks[1][r] * a.lddv * 2 + col) = *reinterpret_cast<const uint4*>(at + IMAGE);
-          }
-        }
+      for (int ct = 0; ct < CT; ++ct) {
+        kc[h][ct] = R::columns(K + at, g, i, ct);
+        qc[h][ct] = R::columns(Q + at, g, i, ct);
+        gc[h][ct] = R::columns(G + at, g, i, ct);
       }
     }
     order_lds();
+#pragma unroll
+    for (int h = 0; h < HG; ++h) {
+      const float mx = column_max(fmaxf(fmaxf(p[h][0], p[h][1]), fmaxf(p[h][2], p[h][3]))) * c;
+      float d = 0.f, l = 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        p[h][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[h][r], c, -mx));
+        l += p[h][r];
+        d = __builtin_fmaf(p[h][r], dp[h][r], d);
+      }
+      const float il = i < Tq ? __builtin_amdgcn_rcpf(column_sum(l)) : 0.f;                   // no query: P = 0
+      d = column_sum(d) * il;
+      f32x4 t;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        p[h][r] *= il;
+        t[r] = p[h][r] * (dp[h][r] - d);
+      }
+      ds[h] = pack4(t);
+      char* tile = K + h * 2 * TILE_BYTES;
+      *reinterpret_cast<s16x4*>(tile + i * TP + 8 * g) = pack4(p[h]);
+      *reinterpret_cast<s16x4*>(tile + TILE_BYTES + i * TP + 8 * g) = ds[h];
+    }
+    order_lds();
+    s16x4 pt[HG], dt[HG];
+#pragma unroll
+    for (int h = 0; h < HG; ++h) {
+      const char* tile = K + h * 2 * TILE_BYTES + (4 * g + (i >> 2)) * TP + 8 * (i & 3);
+      pt[h] = read_columns(tile);
+      dt[h] = read_columns(tile + TILE_BYTES);
+    }
+    order_lds();
+#pragma unroll
+    for (int h = 0; h < HG; ++h) {
+      f32x4 dq[CT], dk[CT], dv[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        dq[ct] = over_tokens(kc[h][ct], ds[h], zero);
+        dv[ct] = over_tokens(gc[h][ct], pt[h], zero);
+        dk[ct] = over_tokens(qc[h][ct], dt[h], zero);
+      }
+      R::put(Q + h * DH * 2, g, i, dq, a.scale);
+      R::put(K + h * DH * 2, g, i, dk, a.scale);
+      R::put(V + h * DH * 2, g, i, dv, 1.f);
+    }
+    order_lds();
+    if (in_row) {
+#pragma unroll
+      for (int u = 0; u < (HALF ? 1 : 2); ++u) {
+        const int r = r8 + 8 * u;
+        const char* at = K + r * PITCH + ch * 16;
+        if (r < Tq) *reinterpret_cast<uint4*>((char*)a.dq + toks[0][r] * a.lddq * 2 + col) = *reinterpret_cast<const uint4*>(at + 2 * IMAGE);
+        if (r < Tk) {
+          *reinterpret_cast<uint4*>((char*)a.dk + toks[1][r] * a.lddk * 2 + col) = *reinterpret_cast<const uint4*>(at);
+          *reinterpret_cast<uint4*>((char*)a.dv + toks[1][r] * a.lddv * 2 + col) = *reinterpret_cast<const uint4*>(at + IMAGE);
+        }
+      }
+    }
   }
 }
 
@@ -875,8 +880,14 @@ __global__ __launch_bounds__(256, 2) void dot_small_kernel(DotArgs a) {
   __shared__ int toks[4][2][64];
   __shared__ __attribute__((aligned(16))) char lds[4][NI * IMAGE];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  small_windows<DH, BWD, false>(a, toks[w], lds[w]);
-  small_windows<DH, BWD, true>(a, toks[w], lds[w]);
+  for (Walk walk(a, 1, 0, (int)blockIdx.y * 4 + w, (int)gridDim.y * 4); walk.next(a);) {
+    int Tq, Tk;
+    walk.tokens(toks[w], 16, Tq, Tk);
+    if (Tq == 0 || Tk == 0) continue;                    // (in no list: the rows are zeroed elsewhere)
+    if (Tq <= 8 && Tk <= 8) small_window<DH, BWD, true>(a, toks[w], Tq, Tk, lds[w]);
+    else small_window<DH, BWD, false>(a, toks[w], Tq, Tk, lds[w]);
+    order_lds();
+  }
 }
 
 // The windows that are in no list: zero rows for queries without a key (out, or dq) and for keys without a query (dk, dv).  One wave per
@@ -904,10 +915,11 @@ __global__ __launch_bounds__(256) void dot_orphan_kernel(DotArgs a, char* q0, in
     }
 }
 
-// workgroups along the windows: what the windows can need, at most so many that each CU has `per_cu` of them in all
-unsigned walkers(int64_t windows, int per_group, unsigned gy, int per_cu) {
+// Workgroups along the windows: what the windows can need, at most `per_cu` per CU in all -- a few times what is resident at
+// once.  Fewer leave the last windows to a few workgroups; more spend their time on workgroups that find no window.
+unsigned walkers(int64_t windows, int per_group, unsigned gx, int per_cu = 12) {
   const int64_t need = (windows + per_group - 1) / per_group;
-  int64_t most = (int64_t)tmae_num_cus() * per_cu / gy;
+  int64_t most = (int64_t)tmae_num_cus() * per_cu / gx;
   if (most < 1) most = 1;
   return (unsigned)(need < most ? need : most);
 }
@@ -949,8 +961,9 @@ template <int DH, int NT, bool BWD> int launch_windows(const DotArgs& a, int64_t
   static TmaeLdsAttr attr;
   if (LDS + 2048 > 65536)
     if (int e = tmae_allow_lds(attr, (const void*)dot_window_kernel<DH, NT, BWD>, LDS)) return e;
-  const unsigned gy = (unsigned)((a.nhead + 3) / 4);
-  hipLaunchKernelGGL((dot_window_kernel<DH, NT, BWD>), dim3(gy, walkers(windows, 1, gy, 8)), dim3(256), LDS, stream, a);
+  const unsigned gx = (unsigned)((a.nhead + 3) / 4);
+  hipLaunchKernelGGL((dot_window_kernel<DH, NT, BWD>), dim3(gx, walkers(windows, 1, gx)), dim3(256), LDS,
+                     stream, a);
   return TMAE_OK;
 }
 template <int DH, bool BWD> int launch_bf16(const DotArgs& a, hipStream_t stream) {
@@ -958,33 +971,35 @@ template <int DH, bool BWD> int launch_bf16(const DotArgs& a, hipStream_t stream
   int rc = launch_windows<DH, 4, BWD>(a, class_windows(a, 3), stream);
   if (rc == TMAE_OK) rc = launch_windows<DH, 2, BWD>(a, class_windows(a, 2), stream);
   if (rc != TMAE_OK) return rc;
-  const unsigned gy = (unsigned)((a.nhead * DH + 63) / 64);
+  const unsigned gx = (unsigned)((a.nhead * DH + 63) / 64);
   const int64_t small = class_windows(a, 0);
-  if (small > 0) hipLaunchKernelGGL((dot_small_kernel<DH, BWD>), dim3(gy, walkers(small, 4, gy, 8)), dim3(256), 0, stream, a);
+  if (small > 0)
+    hipLaunchKernelGGL((dot_small_kernel<DH, BWD>), dim3(gx, walkers(small, 4, gx)), dim3(256), 0, stream, a);
   return TMAE_OK;
 }
 template <int DH, bool BWD> void launch_f32(const DotArgs& a, hipStream_t stream) {
-  const unsigned gy = (unsigned)((a.nhead + 3) / 4);
+  const unsigned gx = (unsigned)((a.nhead + 3) / 4);
   const int64_t windows = a.wl ? class_windows(a, 0) : a.nwin;
   if (windows == 0) return;
-  const dim3 grid(gy, walkers(windows, 1, gy, 8));
-  if constexpr (BWD) hipLaunchKernelGGL((dot_bwd_kernel<float, DH>), grid, dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((dot_fwd_kernel<float, DH>), grid, dim3(256), 0, stream, a);
+  if constexpr (BWD)
+    hipLaunchKernelGGL((dot_bwd_kernel<float, DH>), dim3(gx, walkers(windows, 1, gx)), dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((dot_fwd_kernel<float, DH>), dim3(gx, walkers(windows, 1, gx)), dim3(256), 0, stream, a);
 }
 
 }  // namespace
 
 int tmae_win_attn_dot_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, int dtype, int64_t mq,
                           int64_t mk, int nhead, int dh, const int32_t* grid_q, const int32_t* grid_k, int batch, int ny, int nx,
-                          int do_shift, float scale, void* out, int64_t ldo, float* lse, const int32_t* worklist, void* stream) {
+                          int do_shift, float scale, void* out, int64_t ldo, const int32_t* worklist, void* stream) {
   (void)hipGetLastError();
   DotArgs a = {};
   const int rc = fill(a, dtype, mq, mk, nhead, dh, grid_q, grid_k, batch, ny, nx, do_shift, scale, worklist);
   if (rc != TMAE_OK) return rc;
   if (mq == 0) return TMAE_OK;
   const int es = dtype == TMAE_BF16 ? 2 : 4, d = nhead * dh;
-  if (!rows_ok(q, ldq, d, es) || !rows_ok(out, ldo, d, es) || !lse || (mk && (!rows_ok(k, ldk, d, es) || !rows_ok(v, ldv, d, es)))) return TMAE_EARG;
-  a.q = q; a.ldq = ldq; a.k = k; a.ldk = ldk; a.v = v; a.ldv = ldv; a.o = out; a.ldo = ldo; a.lse = lse;
+  if (!rows_ok(q, ldq, d, es) || !rows_ok(out, ldo, d, es) || (mk && (!rows_ok(k, ldk, d, es) || !rows_ok(v, ldv, d, es)))) return TMAE_EARG;
+  a.q = q; a.ldq = ldq; a.k = k; a.ldk = ldk; a.v = v; a.ldv = ldv; a.o = out; a.ldo = ldo;
   if (worklist && grid_q != grid_k)
     hipLaunchKernelGGL(dot_orphan_kernel, dim3(tmae_cdiv(a.nwin, 4)), dim3(256), 0, (hipStream_t)stream, a, (char*)out, ldo * es, nullptr,
                        (int64_t)0, nullptr, (int64_t)0, d * es / 16);
@@ -998,7 +1013,7 @@ int tmae_win_attn_dot_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk
 }
 
 int tmae_win_attn_dot_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, const void* dout,
-                          int64_t lddo, const float* lse, int dtype, int64_t mq, int64_t mk, int nhead, int dh, const int32_t* grid_q,
+                          int64_t lddo, int dtype, int64_t mq, int64_t mk, int nhead, int dh, const int32_t* grid_q,
                           const int32_t* grid_k, int batch, int ny, int nx, int do_shift, float scale, void* dq, int64_t lddq, void* dk,
                           int64_t lddk, void* dv, int64_t lddv, const int32_t* worklist, void* stream) {
   (void)hipGetLastError();
@@ -1007,9 +1022,9 @@ int tmae_win_attn_dot_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk
   if (rc != TMAE_OK) return rc;
   if (mq == 0 && mk == 0) return TMAE_OK;
   const int es = dtype == TMAE_BF16 ? 2 : 4, d = nhead * dh;
-  if (mq && (!rows_ok(q, ldq, d, es) || !rows_ok(dout, lddo, d, es) || !rows_ok(dq, lddq, d, es) || !lse)) return TMAE_EARG;
+  if (mq && (!rows_ok(q, ldq, d, es) || !rows_ok(dout, lddo, d, es) || !rows_ok(dq, lddq, d, es))) return TMAE_EARG;
   if (mk && (!rows_ok(k, ldk, d, es) || !rows_ok(v, ldv, d, es) || !rows_ok(dk, lddk, d, es) || !rows_ok(dv, lddv, d, es))) return TMAE_EARG;
-  a.q = q; a.ldq = ldq; a.k = k; a.ldk = ldk; a.v = v; a.ldv = ldv; a.g = dout; a.ldg = lddo; a.lse = const_cast<float*>(lse);
+  a.q = q; a.ldq = ldq; a.k = k; a.ldk = ldk; a.v = v; a.ldv = ldv; a.g = dout; a.ldg = lddo;
   a.dq = dq; a.lddq = lddq; a.dk = dk; a.lddk = lddk; a.dv = dv; a.lddv = lddv;
   if (worklist && grid_q != grid_k)
     hipLaunchKernelGGL(dot_orphan_kernel, dim3(tmae_cdiv(a.nwin, 4)), dim3(256), 0, (hipStream_t)stream, a, (char*)dq, lddq * es,

@@ -124,8 +124,8 @@ SIGNATURES = {
     'tmae_qk_norm_rotary_fwd': (I, [P, L, L, I, L, I, I, I, P, P, I, F, P, I, L, P, P, I, I, P, P]),
     'tmae_qk_norm_rotary_bwd_workspace': (Z, [L, I, I, I, I]),
     'tmae_qk_norm_rotary_bwd': (I, [P, L, L, P, I, L, I, I, I, P, P, I, F, P, I, L, P, P, I, I, P, P, P, P, Z, P]),
-    'tmae_win_attn_dot_fwd': (I, [P, L, P, L, P, L, I, L, L, I, I, P, P, I, I, I, I, F, P, L, P, P, P]),
-    'tmae_win_attn_dot_bwd': (I, [P, L, P, L, P, L, P, L, P, I, L, L, I, I, P, P, I, I, I, I, F, P, L, P, L, P, L, P, P]),
+    'tmae_win_attn_dot_fwd': (I, [P, L, P, L, P, L, I, L, L, I, I, P, P, I, I, I, I, F, P, L, P, P]),
+    'tmae_win_attn_dot_bwd': (I, [P, L, P, L, P, L, P, L, I, L, L, I, I, P, P, I, I, I, I, F, P, L, P, L, P, L, P, P]),
     'tmae_probe_copy': (I, [P, P, L, I, P]),
     'tmae_probe_mfma': (I, [I, P, P, P]),
 }
@@ -154,7 +154,7 @@ for _name, (_res, _args) in SIGNATURES.items():
     _fn.argtypes = _args
     setattr(lib, _name, _strict(_fn, _name, len(_args)))
 
-ABI_VERSION = 27            # = TMAE_ABI_VERSION of include/tmae_hip.h (hand-bumped with every change of the export list / a signature)
+ABI_VERSION = 28            # = TMAE_ABI_VERSION of include/tmae_hip.h (hand-bumped with every change of the export list / a signature)
 if lib.tmae_abi_version() != ABI_VERSION:
     raise ImportError(f'libtmae_hip.so ABI version {lib.tmae_abi_version()} != binding {ABI_VERSION}; rebuild with '
                       f't-mae_amd/build.py')

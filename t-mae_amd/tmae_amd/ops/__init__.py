@@ -1938,15 +1938,14 @@ def qk_norm_rotary(x, q_gain, k_gain, positions, inv_freq, sections, q_heads=Non
 class _WinAttnDot(torch.autograd.Function):
     @staticmethod
     def forward(ctx, a, b, c, grid_q, grid_k, worklist, meta):
-        out, lse = _win_attn_dot_launch(a, b, c, grid_q, grid_k, worklist, meta)
-        ctx.save_for_backward(a, b, c if torch.is_tensor(c) else None, grid_q, grid_k, worklist, lse)
+        ctx.save_for_backward(a, b, c if torch.is_tensor(c) else None, grid_q, grid_k, worklist)
         ctx.meta, ctx.packed_kv = meta, isinstance(c, str)
-        return out
+        return _win_attn_dot_launch(a, b, c, grid_q, grid_k, worklist, meta)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        a, b, c, grid_q, grid_k, worklist, lse = ctx.saved_tensors
+        a, b, c, grid_q, grid_k, worklist = ctx.saved_tensors
         c = 'kv' if ctx.packed_kv else c
         d, nhead, batch, ny, nx, do_shift, scale, covered = ctx.meta
         mq, mk = a.shape[0], (a if b is None else b).shape[0]
@@ -1957,7 +1956,7 @@ class _WinAttnDot(torch.autograd.Function):
         dc = alloc(c) if torch.is_tensor(c) else c
         dq, lddq, dk, lddk, dv, lddv = _WinAttn._ptrs(da, db, dc, d)
         with _Launch(a) as s:
-            check(lib.tmae_win_attn_dot_bwd(*_WinAttn._ptrs(a, b, c, d), _p(dout), d, _p(lse), _dt(a), mq, mk, nhead, d // nhead,
+            check(lib.tmae_win_attn_dot_bwd(*_WinAttn._ptrs(a, b, c, d), _p(dout), d, _dt(a), mq, mk, nhead, d // nhead,
                                             _p(grid_q), _p(grid_k), batch, ny, nx, do_shift, scale, dq, lddq, dk, lddk, dv, lddv,
                                             _p(worklist), s), 'tmae_win_attn_dot_bwd')
         return da, db, (dc if torch.is_tensor(dc) else None), None, None, None, None
@@ -1967,11 +1966,10 @@ def _win_attn_dot_launch(a, b, c, grid_q, grid_k, worklist, meta):
     d, nhead, batch, ny, nx, do_shift, scale, covered = meta
     mq, mk = a.shape[0], (a if b is None else b).shape[0]
     out = (torch.empty if covered else torch.zeros)((mq, d), dtype=a.dtype, device=a.device)
-    lse = torch.empty((nhead, mq), dtype=torch.float32, device=a.device)        # read back in the windows that wrote it only
     with _Launch(a) as s:
         check(lib.tmae_win_attn_dot_fwd(*_WinAttn._ptrs(a, b, c, d), _dt(a), mq, mk, nhead, d // nhead, _p(grid_q), _p(grid_k), batch,
-                                        ny, nx, do_shift, scale, _p(out), d, _p(lse), _p(worklist), s), 'tmae_win_attn_dot_fwd')
-    return out, lse
+                                        ny, nx, do_shift, scale, _p(out), d, _p(worklist), s), 'tmae_win_attn_dot_fwd')
+    return out
 
 
 def win_attn_dot(a, b, c, grid_q, grid_k, nhead, batch, ny, nx, do_shift, scale=None, worklist=None, covered=False):
@@ -2019,7 +2017,7 @@ def win_attn_dot(a, b, c, grid_q, grid_k, nhead, batch, ny, nx, do_shift, scale=
     meta = (d, nhead, batch, ny, nx, 1 if do_shift else 0, scale, bool(covered))
     if _grad_on(*tensors):
         return _WinAttnDot.apply(a, b, c, grid_q, grid_k, worklist, meta)
-    return _win_attn_dot_launch(a, b, c, grid_q, grid_k, worklist, meta)[0]
+    return _win_attn_dot_launch(a, b, c, grid_q, grid_k, worklist, meta)
 
 
 # ----------------------------------------------------------------------------- sparse conv (A9)

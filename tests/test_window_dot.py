@@ -152,20 +152,19 @@ def test_c_entries_refuse_bad_arguments():
     from tmae_amd._lib import lib
     one = ctypes.c_void_p(16)
 
-    def fwd(q=one, ldq=64, k=one, v=one, dtype=1, mq=4, mk=4, nhead=4, dh=16, gq=one, gk=one, batch=1, ny=8, nx=8, scale=1.0, out=one, ldo=64,
-            lse=one, wl=None):
-        return lib.tmae_win_attn_dot_fwd(q, ldq, k, 64, v, 64, dtype, mq, mk, nhead, dh, gq, gk, batch, ny, nx, 0, scale, out, ldo, lse, wl, None)
+    def fwd(q=one, ldq=64, k=one, v=one, dtype=1, mq=4, mk=4, nhead=4, dh=16, gq=one, gk=one, batch=1, ny=8, nx=8, scale=1.0, out=one, ldo=64, wl=None):
+        return lib.tmae_win_attn_dot_fwd(q, ldq, k, 64, v, 64, dtype, mq, mk, nhead, dh, gq, gk, batch, ny, nx, 0, scale, out, ldo, wl, None)
     assert fwd(mq=0) == 0 and fwd(dtype=3) == -3
-    for bad in (dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(lse=None), dict(gq=None), dict(gk=None), dict(mq=-1), dict(mk=-1),
+    for bad in (dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(gq=None), dict(gk=None), dict(mq=-1), dict(mk=-1),
                 dict(mq=1 << 31), dict(nhead=0), dict(nhead=4097), dict(dh=8), dict(dh=48), dict(batch=0), dict(ny=0), dict(nx=0), dict(scale=0.0),
                 dict(scale=-1.0), dict(scale=float('nan')), dict(scale=float('inf')), dict(ldq=63), dict(ldq=56), dict(ldo=68 + 2),
                 dict(q=ctypes.c_void_p(8)), dict(batch=1 << 20, ny=1 << 10, nx=1 << 10), dict(wl=one, ny=2041)):
         assert fwd(**bad) == -1, bad
 
-    def bwd(dq=one, dk=one, dv=one, do=one, lse=one, lddq=64):
-        return lib.tmae_win_attn_dot_bwd(one, 64, one, 64, one, 64, do, 64, lse, 1, 4, 4, 4, 16, one, one, 1, 8, 8, 0, 1.0, dq, lddq, dk, 64, dv,
+    def bwd(dq=one, dk=one, dv=one, do=one, lddq=64):
+        return lib.tmae_win_attn_dot_bwd(one, 64, one, 64, one, 64, do, 64, 1, 4, 4, 4, 16, one, one, 1, 8, 8, 0, 1.0, dq, lddq, dk, 64, dv,
                                          64, None, None)
-    for bad in (dict(dq=None), dict(dk=None), dict(dv=None), dict(do=None), dict(lse=None), dict(lddq=60)):
+    for bad in (dict(dq=None), dict(dk=None), dict(dv=None), dict(do=None), dict(lddq=60)):
         assert bwd(**bad) == -1, bad
 
 
