@@ -452,8 +452,9 @@ __device__ __forceinline__ f32x4 over_tokens(const s16x4& a0, const s16x4& a1, c
 }
 
 // ---- windows of more than 16 tokens: a wave per (window, head), four heads in a workgroup so that their pieces of a line meet in the cache.
-// All rows of the window are requested at once.  K and V go through the wave's two images into registers, then Q (and dO) take their place;
-// results replace Q, and at the end dK and dV follow.
+// All rows of the window are requested at once.  Forward: K and V go through the wave's two images into registers, Q takes K's place, the
+// output Q's.  Backward: K, V and Q have images; V goes into registers and dO takes its place; at the end dQ, dK and dV stand where Q, K
+// and dO stood.
 template <int DH, int NT> struct Window {
   static constexpr int PITCH = DH * 2 + 16, TILE = 16 * PITCH, IMAGE = NT * TILE;
   static constexpr int CHUNKS = DH / 8, RPI = 64 / CHUNKS, LOADS = NT * 16 / RPI;             // 16-byte chunks of a row, rows of a load
@@ -552,24 +553,20 @@ __device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq, cons
 
 template <int DH, int NT, int NK>
 __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, const int* tk, int Tq, int Tk, int head, char* A,
-                                           typename Window<DH, NT>::Loaded qrows, typename Window<DH, NT>::Loaded grows, char* tiles) {
+                                           typename Window<DH, NT>::Loaded grows, char* tiles) {
   using W = Window<DH, NT>;
   using R = typename W::R;
   constexpr int CT = W::CT, TILE = W::TILE, TP = TILE_PITCH;
   const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15, nq = (Tq + 15) >> 4;
   const int64_t col = (int64_t)head * DH * 2;
-  char* B = A + W::IMAGE;
+  char *B = A + W::IMAGE, *C = B + W::IMAGE;
   typename R::Piece kf[NK], vf[NK];
-  s16x4 kc[NK][CT];
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt) {
     kf[kt] = R::piece(A + kt * TILE, g, i);
     vf[kt] = R::piece(B + kt * TILE, g, i);
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) kc[kt][ct] = R::columns(A + kt * TILE, g, i, ct);
   }
   order_lds();
-  W::lay(A, qrows);
   W::lay(B, grows);
   order_lds();
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
@@ -583,11 +580,11 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) dk[kt][ct] = dv[kt][ct] = zero;
   for (int qt = 0; qt < nq; ++qt) {
-    const typename R::Piece qf = R::piece(A + qt * TILE, g, i), gf = R::piece(B + qt * TILE, g, i);
+    const typename R::Piece qf = R::piece(C + qt * TILE, g, i), gf = R::piece(B + qt * TILE, g, i);
     s16x4 qc[CT], gc[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      qc[ct] = R::columns(A + qt * TILE, g, i, ct);
+      qc[ct] = R::columns(C + qt * TILE, g, i, ct);
       gc[ct] = R::columns(B + qt * TILE, g, i, ct);
     }
     f32x4 p[NK], dp[NK];
@@ -645,15 +642,16 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       dq[ct] = zero;
-      if constexpr (NK >= 2) dq[ct] = over_tokens(kc[0][ct], kc[1][ct], ds[0], ds[1], dq[ct]);
-      if constexpr (NK == 4) dq[ct] = over_tokens(kc[2][ct], kc[3][ct], ds[2], ds[3], dq[ct]);
-      if constexpr (NK == 3) dq[ct] = over_tokens(kc[2][ct], s16x4{0, 0, 0, 0}, ds[2], s16x4{0, 0, 0, 0}, dq[ct]);
-      if constexpr (NK == 1) dq[ct] = over_tokens(kc[0][ct], ds[0], dq[ct]);
+      s16x4 kc[NK];
+#pragma unroll
+      for (int kt = 0; kt < NK; ++kt) kc[kt] = R::columns(A + kt * TILE, g, i, ct);
+      if constexpr (NK >= 2) dq[ct] = over_tokens(kc[0], kc[1], ds[0], ds[1], dq[ct]);
+      if constexpr (NK == 4) dq[ct] = over_tokens(kc[2], kc[3], ds[2], ds[3], dq[ct]);
+      if constexpr (NK == 3) dq[ct] = over_tokens(kc[2], s16x4{0, 0, 0, 0}, ds[2], s16x4{0, 0, 0, 0}, dq[ct]);
+      if constexpr (NK == 1) dq[ct] = over_tokens(kc[0], ds[0], dq[ct]);
     }
-    R::put(A + qt * TILE, g, i, dq, a.scale);
+    R::put(C + qt * TILE, g, i, dq, a.scale);
   }
-  order_lds();
-  W::store(a.dq, a.lddq, tq, Tq, col, A);
   order_lds();
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt) {
@@ -661,13 +659,14 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
     R::put(B + kt * TILE, g, i, dv[kt], 1.f);
   }
   order_lds();
+  W::store(a.dq, a.lddq, tq, Tq, col, C);
   W::store(a.dk, a.lddk, tk, Tk, col, A);
   W::store(a.dv, a.lddv, tk, Tk, col, B);
 }
 
 // Windows of up to 16 NT tokens; without a work list (NT = 4) every window, empty ones included.  Two waves per SIMD as the bound: 256
 // registers at most, and the matrix instructions then write plain vector registers (the backward of 64 channels by 64 tokens needs more).
-template <int DH, int NT, bool BWD> constexpr int window_lds() { return 2 * Window<DH, NT>::IMAGE + (BWD ? 4 * TILE_BYTES : 0); }
+template <int DH, int NT, bool BWD> constexpr int window_lds() { return (BWD ? 3 : 2) * Window<DH, NT>::IMAGE + (BWD ? 4 * TILE_BYTES : 0); }
 template <int DH, int NT, bool BWD> constexpr int window_waves() {        // waves per SIMD that the registers allow
   return DH == 16 ? (BWD ? (NT == 4 ? 3 : 4) : (NT == 4 ? 5 : 8)) : DH == 32 ? (BWD ? (NT == 4 ? 2 : 3) : (NT == 4 ? 4 : 5)) : BWD && NT == 4 ? 1 : 2;
 }
@@ -705,11 +704,12 @@ __global__ __launch_bounds__(256, (window_waves<DH, NT, BWD>())) void dot_window
     if constexpr (BWD && !LATE) grows = W::request(a.g, a.ldg, toks[0], col);
     W::lay(A, krows);
     W::lay(A + W::IMAGE, vrows);
+    if constexpr (BWD) W::lay(A + 2 * W::IMAGE, qrows);
     order_lds();
     if constexpr (BWD && LATE) grows = W::request(a.g, a.ldg, toks[0], col);
     const int nk = (Tk + 15) >> 4;
 #define ONE(NK)                                                                                                                            \
-  if constexpr (BWD) bwd_window<DH, NT, NK>(a, toks[0], toks[1], Tq, Tk, head, A, qrows, grows, A + 2 * W::IMAGE);                         \
+  if constexpr (BWD) bwd_window<DH, NT, NK>(a, toks[0], toks[1], Tq, Tk, head, A, grows, A + 3 * W::IMAGE);                                \
   else fwd_window<DH, NT, NK>(a, toks[0], toks[1], Tq, Tk, head, A, qrows)
     if (nk == 1) { ONE(1); }
     else if (NT == 2 || nk == 2) { ONE(2); }
@@ -904,14 +904,18 @@ __global__ __launch_bounds__(256) void dot_orphan_kernel(DotArgs a, char* q0, in
   int tq = in ? a.grid_q[cell] : -1, tk = in ? a.grid_k[cell] : -1;
   if (tq >= a.mq) tq = -1;
   if (tk >= a.mk) tk = -1;
-  const bool some_q = __ballot(tq >= 0) != 0, some_k = __ballot(tk >= 0) != 0;
+  const unsigned long long q = __ballot(tq >= 0), k = __ballot(tk >= 0);
   const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-  if (q0 && !some_k && tq >= 0)
-    for (int c = 0; c < row16; ++c) reinterpret_cast<uint4*>(q0 + tq * ldq0)[c] = z;
-  if (k0 && !some_q && tk >= 0)
-    for (int c = 0; c < row16; ++c) {
-      reinterpret_cast<uint4*>(k0 + tk * ldk0)[c] = z;
-      reinterpret_cast<uint4*>(k1 + tk * ldk1)[c] = z;
+  if (q0 && !k)
+    for (unsigned long long m = q; m; m &= m - 1) {
+      uint4* r = reinterpret_cast<uint4*>(q0 + (int64_t)__builtin_amdgcn_readlane(tq, __ffsll(m) - 1) * ldq0);
+      for (int c = lane; c < row16; c += 64) r[c] = z;
+    }
+  if (k0 && !q)
+    for (unsigned long long m = k; m; m &= m - 1) {
+      const int64_t t = __builtin_amdgcn_readlane(tk, __ffsll(m) - 1);
+      uint4 *r = reinterpret_cast<uint4*>(k0 + t * ldk0), *v = reinterpret_cast<uint4*>(k1 + t * ldk1);
+      for (int c = lane; c < row16; c += 64) { r[c] = z; v[c] = z; }
     }
 }
 
