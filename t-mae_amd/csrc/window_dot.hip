@@ -358,6 +358,38 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_kernel(DotArgs a) {
   }
 }
 
+// The windows that are in no list: zero rows for queries without a key (out, or dq) and for keys without a query (dk, dv).  A wave per
+// window, a lane per cell, whole rows at a time.
+struct Orphans { char *q; int64_t ldq; char *k, *v; int64_t ldk, ldv; int row16; };        // pitches in bytes, 16-byte pieces of a row
+__device__ __forceinline__ void orphan_role(const DotArgs& a, const Orphans& z, int64_t first, int64_t step) {
+  const int lane = threadIdx.x & 63;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  for (int64_t u = first; u < a.nwin; u += step) {
+    const int e = (int)u, wcy = e % a.Wy, wcx = e / a.Wy % a.Wx, b = e / (a.Wy * a.Wx);
+    const int y = wcy * WIN - a.s + (lane >> 3), x = wcx * WIN - a.s + (lane & 7);
+    const bool in = y >= 0 && y < a.ny && x >= 0 && x < a.nx;
+    const int cell = in ? (b * a.ny + y) * a.nx + x : 0;
+    int tq = a.grid_q[cell], tk = a.grid_k[cell];
+    if (!in || tq >= a.mq) tq = -1;
+    if (!in || tk >= a.mk) tk = -1;
+    const unsigned long long q = __ballot(tq >= 0), k = __ballot(tk >= 0);
+    if (z.q && !k)
+      for (unsigned long long m = q; m; m &= m - 1) {
+        uint4* r = reinterpret_cast<uint4*>(z.q + (int64_t)__builtin_amdgcn_readlane(tq, __ffsll(m) - 1) * z.ldq);
+        for (int c = lane; c < z.row16; c += 64) r[c] = zero;
+      }
+    if (z.k && !q)
+      for (unsigned long long m = k; m; m &= m - 1) {
+        const int64_t t = __builtin_amdgcn_readlane(tk, __ffsll(m) - 1);
+        uint4 *r = reinterpret_cast<uint4*>(z.k + t * z.ldk), *v = reinterpret_cast<uint4*>(z.v + t * z.ldv);
+        for (int c = lane; c < z.row16; c += 64) { r[c] = zero; v[c] = zero; }
+      }
+  }
+}
+__global__ __launch_bounds__(256) void dot_orphan_kernel(DotArgs a, Orphans z) {
+  orphan_role(a, z, (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), (int64_t)gridDim.x * 4);
+}
+
 // ------------------------------------------------------------------------------------------------------------------ bfloat16
 // The same products on the bfloat16 matrix instructions.  Their operands want the 16 rows of a tile in 16 neighbouring lanes: loaded that
 // way straight from the tensors, each instruction touches 16 lines per 16 lanes and the cache's tag port is what the kernels wait for
@@ -667,21 +699,12 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
 // Windows of up to 16 NT tokens; without a work list (NT = 4) every window, empty ones included.  Two waves per SIMD as the bound: 256
 // registers at most, and the matrix instructions then write plain vector registers (the backward of 64 channels by 64 tokens needs more).
 template <int DH, int NT, bool BWD> constexpr int window_lds() { return (BWD ? 3 : 2) * Window<DH, NT>::IMAGE + (BWD ? 4 * TILE_BYTES : 0); }
-template <int DH, int NT, bool BWD> constexpr int window_waves() {        // waves per SIMD that the registers allow
-  return DH == 16 ? (BWD ? (NT == 4 ? 3 : 4) : (NT == 4 ? 5 : 8)) : DH == 32 ? (BWD ? (NT == 4 ? 2 : 3) : (NT == 4 ? 4 : 5)) : BWD && NT == 4 ? 1 : 2;
-}
-template <int DH, int NT, bool BWD>
-__global__ __launch_bounds__(256, (window_waves<DH, NT, BWD>())) void dot_window_kernel(DotArgs a) {
+template <int DH, int NT, bool BWD> __device__ __forceinline__ void window_role(const DotArgs& a, int first, int step, int head, int (*toks)[64], char* A) {
   using W = Window<DH, NT>;
-  extern __shared__ __attribute__((aligned(16))) char lds_[];
-  __shared__ int toks_[4][2][64];
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int (*toks)[64] = toks_[w];
-  char* A = lds_ + w * window_lds<DH, NT, BWD>();
-  const int head = blockIdx.x * 4 + w;
+  const int lane = threadIdx.x & 63;
   if (head >= a.nhead) return;
   const int64_t col = (int64_t)head * DH * 2;
-  for (Walk walk(a, NT == 4 ? 3 : 2, NT == 4 ? 3 : 2, (int)blockIdx.y, (int)gridDim.y); walk.next(a);) {
+  for (Walk walk(a, NT == 4 ? 3 : 2, NT == 4 ? 3 : 2, first, step); walk.next(a);) {
     int Tq, Tk;
     walk.tokens(toks, NT * 16, Tq, Tk);
     if (Tq == 0 || Tk == 0) {
@@ -726,7 +749,7 @@ __global__ __launch_bounds__(256, (window_waves<DH, NT, BWD>())) void dot_window
 constexpr int SMALL_PITCH = 144;           // 128 bytes of a row
 
 // HALF: at most 8 tokens, one load brings a tensor's rows (rows 8 .. 15 then hold them once more)
-template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_window(const DotArgs& a, const int (*toks)[64], int Tq, int Tk, char* K) {
+template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_window(const DotArgs& a, const int (*toks)[64], int Tq, int Tk, int head0, char* K) {
   constexpr int HG = 64 / DH, PITCH = SMALL_PITCH, IMAGE = 16 * PITCH, NI = BWD ? 4 : 3, TP = TILE_PITCH;
   using R = Rows<DH, PITCH>;
   constexpr int CT = R::CT;
@@ -734,7 +757,6 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
   char *V = K + IMAGE, *Q = K + 2 * IMAGE, *G = K + 3 * IMAGE;
   const float c = a.scale * LOG2E;
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  const int head0 = blockIdx.x * HG;
   const int r8 = lane >> 3, ch = lane & 7;
   const bool in_row = head0 * DH + ch * 8 < a.nhead * DH;
   const int64_t col = in_row ? (int64_t)head0 * DH * 2 + ch * 16 : 0;
@@ -873,50 +895,60 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
   }
 }
 
-template <int DH, bool BWD>
-__global__ __launch_bounds__(256, 2) void dot_small_kernel(DotArgs a) {
-  constexpr int IMAGE = 16 * SMALL_PITCH, NI = BWD ? 4 : 3;
-  static_assert(64 / DH * 2 * TILE_BYTES <= NI * IMAGE || !BWD, "the P and dS tiles take the images' place");
-  __shared__ int toks[4][2][64];
-  __shared__ __attribute__((aligned(16))) char lds[4][NI * IMAGE];
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  for (Walk walk(a, 1, 0, (int)blockIdx.y * 4 + w, (int)gridDim.y * 4); walk.next(a);) {
+template <int DH, bool BWD> constexpr int small_lds() { return (BWD ? 4 : 3) * 16 * SMALL_PITCH; }             // of one wave
+template <int DH, bool BWD> __device__ __forceinline__ void small_role(const DotArgs& a, int first, int step, int head0, int (*toks)[64], char* lds) {
+  static_assert(64 / DH * 2 * TILE_BYTES <= small_lds<DH, BWD>() || !BWD, "the P and dS tiles take the images' place");
+  for (Walk walk(a, 1, 0, first, step); walk.next(a);) {
     int Tq, Tk;
-    walk.tokens(toks[w], 16, Tq, Tk);
+    walk.tokens(toks, 16, Tq, Tk);
     if (Tq == 0 || Tk == 0) continue;                    // (in no list: the rows are zeroed elsewhere)
-    if (Tq <= 8 && Tk <= 8) small_window<DH, BWD, true>(a, toks[w], Tq, Tk, lds[w]);
-    else small_window<DH, BWD, false>(a, toks[w], Tq, Tk, lds[w]);
+    if (Tq <= 8 && Tk <= 8) small_window<DH, BWD, true>(a, toks, Tq, Tk, head0, lds);
+    else small_window<DH, BWD, false>(a, toks, Tq, Tk, head0, lds);
     order_lds();
   }
 }
 
-// The windows that are in no list: zero rows for queries without a key (out, or dq) and for keys without a query (dk, dv).  One wave per
-// window, a lane per cell.
-__global__ __launch_bounds__(256) void dot_orphan_kernel(DotArgs a, char* q0, int64_t ldq0, char* k0, int64_t ldk0, char* k1, int64_t ldk1,
-                                                        int row16) {
-  const int lane = threadIdx.x & 63;
-  const int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (u >= a.nwin) return;
-  const int wcy = (int)(u % a.Wy), wcx = (int)((u / a.Wy) % a.Wx), b = (int)(u / ((int64_t)a.Wy * a.Wx));
-  const int y = wcy * WIN - a.s + (lane >> 3), x = wcx * WIN - a.s + (lane & 7);
-  const bool in = y >= 0 && y < a.ny && x >= 0 && x < a.nx;
-  const int64_t cell = ((int64_t)b * a.ny + y) * a.nx + x;
-  int tq = in ? a.grid_q[cell] : -1, tk = in ? a.grid_k[cell] : -1;
-  if (tq >= a.mq) tq = -1;
-  if (tk >= a.mk) tk = -1;
-  const unsigned long long q = __ballot(tq >= 0), k = __ballot(tk >= 0);
-  const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-  if (q0 && !k)
-    for (unsigned long long m = q; m; m &= m - 1) {
-      uint4* r = reinterpret_cast<uint4*>(q0 + (int64_t)__builtin_amdgcn_readlane(tq, __ffsll(m) - 1) * ldq0);
-      for (int c = lane; c < row16; c += 64) r[c] = z;
+// The workgroups of a launch: n4 walk the windows of 33 to 64 tokens (or every window, where there is no list), n2 those of 17 to 32, n1
+// the others, each of them with its group of heads; those behind them zero the rows of the windows that are in no list.
+struct Roles { int n4, n2, n1, n0, heads, columns; };                   // heads: groups of four; columns: groups of 64 channels
+constexpr int ROLE4 = 1, ROLE2 = 2, ROLE1 = 4;
+template <int DH, bool BWD, int ROLES> constexpr int kernel_lds() {
+  const int l4 = ROLES & ROLE4 ? window_lds<DH, 4, BWD>() : 0, l2 = ROLES & ROLE2 ? window_lds<DH, 2, BWD>() : 0,
+            l1 = ROLES & ROLE1 ? small_lds<DH, BWD>() : 0;
+  return 4 * (l4 > l2 ? (l4 > l1 ? l4 : l1) : (l2 > l1 ? l2 : l1));
+}
+template <int DH, bool BWD, int ROLES> constexpr int kernel_waves() {    // waves per SIMD that the registers allow
+  return ROLES & ROLE4 ? (DH == 16 ? (BWD ? 3 : 5) : DH == 32 ? (BWD ? 2 : 4) : BWD ? 1 : 2) : (DH == 16 ? (BWD ? 4 : 6) : DH == 32 ? (BWD ? 3 : 5) : BWD ? 2 : 4);
+}
+template <int DH, bool BWD, int ROLES>
+__global__ __launch_bounds__(256, (kernel_waves<DH, BWD, ROLES>())) void dot_kernel(DotArgs a, Roles n, Orphans z) {
+  extern __shared__ __attribute__((aligned(16))) char lds_[];
+  __shared__ int toks_[4][2][64];
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int (*toks)[64] = toks_[w];
+  int u = blockIdx.x;
+  if constexpr (ROLES & ROLE4) {
+    if (u < n.n4 * n.heads) {
+      window_role<DH, 4, BWD>(a, u / n.heads, n.n4, u % n.heads * 4 + w, toks, lds_ + w * window_lds<DH, 4, BWD>());
+      return;
     }
-  if (k0 && !q)
-    for (unsigned long long m = k; m; m &= m - 1) {
-      const int64_t t = __builtin_amdgcn_readlane(tk, __ffsll(m) - 1);
-      uint4 *r = reinterpret_cast<uint4*>(k0 + t * ldk0), *v = reinterpret_cast<uint4*>(k1 + t * ldk1);
-      for (int c = lane; c < row16; c += 64) { r[c] = z; v[c] = z; }
+    u -= n.n4 * n.heads;
+  }
+  if constexpr (ROLES & ROLE2) {
+    if (u < n.n2 * n.heads) {
+      window_role<DH, 2, BWD>(a, u / n.heads, n.n2, u % n.heads * 4 + w, toks, lds_ + w * window_lds<DH, 2, BWD>());
+      return;
     }
+    u -= n.n2 * n.heads;
+  }
+  if constexpr (ROLES & ROLE1) {
+    if (u < n.n1 * n.columns) {
+      small_role<DH, BWD>(a, u / n.columns * 4 + w, n.n1 * 4, u % n.columns * (64 / DH), toks, lds_ + w * small_lds<DH, BWD>());
+      return;
+    }
+    u -= n.n1 * n.columns;
+    orphan_role(a, z, u * 4 + w, n.n0 * 4);
+  }
 }
 
 // Workgroups along the windows: what the windows can need, at most `per_cu` per CU in all -- a few times what is resident at
@@ -959,29 +991,35 @@ template <class F> void by_head(int dh, F&& f) {
   else if (dh == 32) f(std::integral_constant<int, 32>());
   else f(std::integral_constant<int, 64>());
 }
-template <int DH, int NT, bool BWD> int launch_windows(const DotArgs& a, int64_t windows, hipStream_t stream) {
-  constexpr int LDS = 4 * window_lds<DH, NT, BWD>();
-  if (windows == 0) return TMAE_OK;
+template <int DH, bool BWD, int ROLES> int launch_roles(const DotArgs& a, const Orphans& z, int64_t w4, int64_t w2, int64_t w1, hipStream_t stream) {
+  constexpr int LDS = kernel_lds<DH, BWD, ROLES>();
   static TmaeLdsAttr attr;
   if (LDS + 2048 > 65536)
-    if (int e = tmae_allow_lds(attr, (const void*)dot_window_kernel<DH, NT, BWD>, LDS)) return e;
-  const unsigned gx = (unsigned)((a.nhead + 3) / 4);
-  hipLaunchKernelGGL((dot_window_kernel<DH, NT, BWD>), dim3(gx, walkers(windows, 1, gx)), dim3(256), LDS,
-                     stream, a);
+    if (int e = tmae_allow_lds(attr, (const void*)dot_kernel<DH, BWD, ROLES>, LDS)) return e;
+  Roles n;
+  n.heads = (a.nhead + 3) / 4;
+  n.columns = (a.nhead * DH + 63) / 64;
+  n.n4 = ROLES & ROLE4 ? (int)walkers(w4, 1, n.heads) : 0;
+  n.n2 = ROLES & ROLE2 ? (int)walkers(w2, 1, n.heads) : 0;
+  n.n1 = ROLES & ROLE1 ? (int)walkers(w1, 4, n.columns) : 0;
+  n.n0 = ROLES & ROLE1 && z.row16 ? (int)walkers(a.nwin, 16, 1, 1) : 0;
+  const int64_t blocks = (int64_t)(n.n4 + n.n2) * n.heads + (int64_t)n.n1 * n.columns + n.n0;
+  if (blocks > 0) hipLaunchKernelGGL((dot_kernel<DH, BWD, ROLES>), dim3((unsigned)blocks), dim3(256), LDS, stream, a, n, z);
   return TMAE_OK;
 }
-template <int DH, bool BWD> int launch_bf16(const DotArgs& a, hipStream_t stream) {
-  if (!a.wl) return launch_windows<DH, 4, BWD>(a, a.nwin, stream);
-  int rc = launch_windows<DH, 4, BWD>(a, class_windows(a, 3), stream);
-  if (rc == TMAE_OK) rc = launch_windows<DH, 2, BWD>(a, class_windows(a, 2), stream);
-  if (rc != TMAE_OK) return rc;
-  const unsigned gx = (unsigned)((a.nhead * DH + 63) / 64);
-  const int64_t small = class_windows(a, 0);
-  if (small > 0)
-    hipLaunchKernelGGL((dot_small_kernel<DH, BWD>), dim3(gx, walkers(small, 4, gx)), dim3(256), 0, stream, a);
-  return TMAE_OK;
+// One launch for all windows, or one for those of more than 32 tokens and one for the others.  One overlaps the ends of the parts and
+// costs a launch less, but every workgroup then has the registers and LDS of the largest part.  Eight frames at stage 1 (375 k tokens, 8
+// heads of 16): forward 109 us in one launch against 114, backward 206 against 193; stage 2 (8 heads of 32): forward 45 against 42,
+// backward 90 against 84.  Few tokens: the launch counts.
+template <int DH, bool BWD> int launch_bf16(const DotArgs& a, const Orphans& z, hipStream_t stream) {
+  if (!a.wl) return launch_roles<DH, BWD, ROLE4>(a, z, a.nwin, 0, 0, stream);
+  const int64_t w4 = class_windows(a, 3), w2 = class_windows(a, 2), w1 = class_windows(a, 0);
+  if ((DH == 16 && !BWD) || a.mq + a.mk <= 32768) return launch_roles<DH, BWD, ROLE4 | ROLE2 | ROLE1>(a, z, w4, w2, w1, stream);
+  const int rc = launch_roles<DH, BWD, ROLE4>(a, z, w4, w2, w1, stream);
+  return rc != TMAE_OK ? rc : launch_roles<DH, BWD, ROLE2 | ROLE1>(a, z, w4, w2, w1, stream);
 }
-template <int DH, bool BWD> void launch_f32(const DotArgs& a, hipStream_t stream) {
+template <int DH, bool BWD> void launch_f32(const DotArgs& a, const Orphans& z, hipStream_t stream) {
+  if (z.row16) hipLaunchKernelGGL(dot_orphan_kernel, dim3(walkers(a.nwin, 4, 1)), dim3(256), 0, stream, a, z);
   const unsigned gx = (unsigned)((a.nhead + 3) / 4);
   const int64_t windows = a.wl ? class_windows(a, 0) : a.nwin;
   if (windows == 0) return;
@@ -1004,14 +1042,13 @@ int tmae_win_attn_dot_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk
   const int es = dtype == TMAE_BF16 ? 2 : 4, d = nhead * dh;
   if (!rows_ok(q, ldq, d, es) || !rows_ok(out, ldo, d, es) || (mk && (!rows_ok(k, ldk, d, es) || !rows_ok(v, ldv, d, es)))) return TMAE_EARG;
   a.q = q; a.ldq = ldq; a.k = k; a.ldk = ldk; a.v = v; a.ldv = ldv; a.o = out; a.ldo = ldo;
-  if (worklist && grid_q != grid_k)
-    hipLaunchKernelGGL(dot_orphan_kernel, dim3(tmae_cdiv(a.nwin, 4)), dim3(256), 0, (hipStream_t)stream, a, (char*)out, ldo * es, nullptr,
-                       (int64_t)0, nullptr, (int64_t)0, d * es / 16);
+  Orphans z = {};
+  if (worklist && grid_q != grid_k) z = Orphans{(char*)out, ldo * es, nullptr, nullptr, 0, 0, d * es / 16};
   int failed = TMAE_OK;
   by_head(dh, [&](auto w) {
     constexpr int DH = decltype(w)::value;
-    if (dtype == TMAE_BF16) failed = launch_bf16<DH, false>(a, (hipStream_t)stream);
-    else launch_f32<DH, false>(a, (hipStream_t)stream);
+    if (dtype == TMAE_BF16) failed = launch_bf16<DH, false>(a, z, (hipStream_t)stream);
+    else launch_f32<DH, false>(a, z, (hipStream_t)stream);
   });
   return failed != TMAE_OK ? failed : tmae_launch_status();
 }
@@ -1030,14 +1067,13 @@ int tmae_win_attn_dot_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk
   if (mk && (!rows_ok(k, ldk, d, es) || !rows_ok(v, ldv, d, es) || !rows_ok(dk, lddk, d, es) || !rows_ok(dv, lddv, d, es))) return TMAE_EARG;
   a.q = q; a.ldq = ldq; a.k = k; a.ldk = ldk; a.v = v; a.ldv = ldv; a.g = dout; a.ldg = lddo;
   a.dq = dq; a.lddq = lddq; a.dk = dk; a.lddk = lddk; a.dv = dv; a.lddv = lddv;
-  if (worklist && grid_q != grid_k)
-    hipLaunchKernelGGL(dot_orphan_kernel, dim3(tmae_cdiv(a.nwin, 4)), dim3(256), 0, (hipStream_t)stream, a, (char*)dq, lddq * es,
-                       (char*)dk, lddk * es, (char*)dv, lddv * es, d * es / 16);
+  Orphans z = {};
+  if (worklist && grid_q != grid_k) z = Orphans{(char*)dq, lddq * es, (char*)dk, (char*)dv, lddk * es, lddv * es, d * es / 16};
   int failed = TMAE_OK;
   by_head(dh, [&](auto w) {
     constexpr int DH = decltype(w)::value;
-    if (dtype == TMAE_BF16) failed = launch_bf16<DH, true>(a, (hipStream_t)stream);
-    else launch_f32<DH, true>(a, (hipStream_t)stream);
+    if (dtype == TMAE_BF16) failed = launch_bf16<DH, true>(a, z, (hipStream_t)stream);
+    else launch_f32<DH, true>(a, z, (hipStream_t)stream);
   });
   return failed != TMAE_OK ? failed : tmae_launch_status();
 }
