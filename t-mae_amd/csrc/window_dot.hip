@@ -126,236 +126,192 @@ struct Walk {
   }
 };
 
-// channels KD g .. KD g + KD - 1 of a token's head: what the lane contributes to a product over the channels
-template <class T, int KD> __device__ __forceinline__ void load_frag(const T* p, float* f);
-template <> __device__ __forceinline__ void load_frag<float, 4>(const float* p, float* f) {
-  const float4 a = *reinterpret_cast<const float4*>(p);
-  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-}
-template <> __device__ __forceinline__ void load_frag<float, 8>(const float* p, float* f) { load8<float>(p, f); }
-template <> __device__ __forceinline__ void load_frag<float, 16>(const float* p, float* f) { load8<float>(p, f); load8<float>(p + 8, f + 8); }
-template <> __device__ __forceinline__ void load_frag<__hip_bfloat16, 4>(const __hip_bfloat16* p, float* f) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  f[0] = __uint_as_float(u.x << 16); f[1] = __uint_as_float(u.x & 0xFFFF0000u);
-  f[2] = __uint_as_float(u.y << 16); f[3] = __uint_as_float(u.y & 0xFFFF0000u);
-}
-template <> __device__ __forceinline__ void load_frag<__hip_bfloat16, 8>(const __hip_bfloat16* p, float* f) { load8<__hip_bfloat16>(p, f); }
-template <> __device__ __forceinline__ void load_frag<__hip_bfloat16, 16>(const __hip_bfloat16* p, float* f) {
-  load8<__hip_bfloat16>(p, f);
-  load8<__hip_bfloat16>(p + 8, f + 8);
-}
-template <class T> __device__ __forceinline__ void store_four(T* p, const f32x4& v) {
-#pragma unroll
-  for (int r = 0; r < 4; ++r) st_f<T>(p + r, v[r]);
-}
-
+// ------------------------------------------------------------------------------------------------------------------- float32
+// Four waves of a workgroup share the windows of up to 16 NT tokens: NT of them the tiles of one head, 4 / NT heads at a time -- 64 rows
+// of each tensor in LDS whatever the window's size.  A wave takes one tile of queries (out, dQ and the rows' maxima, sums and sum_j P dP),
+// then, in the backward, one tile of keys (dK, dV).  Operands come from LDS: pieces of rows for the products over the channels, single
+// values of four rows for those over the tokens.
 __device__ __forceinline__ float lanes4_sum(float v) { v += __shfl_xor(v, 16, 64); return v + __shfl_xor(v, 32, 64); }
 __device__ __forceinline__ float lanes4_max(float v) { v = fmaxf(v, __shfl_xor(v, 16, 64)); return fmaxf(v, __shfl_xor(v, 32, 64)); }
 
-template <int KD> __device__ __forceinline__ f32x4 product(const float* a, const float* b) {
-  f32x4 c = {0.f, 0.f, 0.f, 0.f};
+template <int DH> struct Rows32 {
+  static constexpr int PITCH = DH + 4, KD = DH / 4, CT = DH / 16, IMAGE = 64 * PITCH;      // floats
+  struct Piece { f32x4 v[KD / 4]; };         // of row i: channels 4g .. 4g + 3 of every 16
+  static __device__ __forceinline__ Piece piece(const float* tile, int g, int i) {
+    Piece p;
 #pragma unroll
-  for (int s = 0; s < KD; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], c, 0, 0, 0);
-  return c;
-}
-// c[ct] += (tokens' channels as rows) x (b as columns): rows 16 ct .. +15 of the head's channels, contraction over the tile's tokens
-template <class T, int CT>
-__device__ __forceinline__ void accumulate(const T* base, int64_t ld, const int* toks, const f32x4& b, f32x4* c, int g, int i) {
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const T* row = base + (int64_t)toks[4 * g + r] * ld + i;
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) c[ct] = __builtin_amdgcn_mfma_f32_16x16x4f32(ld_f<T>(row + 16 * ct), b[r], c[ct], 0, 0, 0);
+    for (int j = 0; j < KD / 4; ++j) p.v[j] = *reinterpret_cast<const f32x4*>(tile + i * PITCH + 16 * j + 4 * g);
+    return p;
   }
-}
-template <class T, int DH>
-__global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
-  constexpr int KD = DH / 4, CT = DH / 16;
-  __shared__ int toks_[4][2][64];
+  static __device__ __forceinline__ f32x4 over_channels(const Piece& a, const Piece& b) {
+    f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < KD / 4; ++j)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j][s], b.v[j][s], c, 0, 0, 0);
+    return c;
+  }
+  // c[ct] += channels 16 ct .. + 15 of the tile's rows (as rows of the result) x b (columns), over the tile's 16 tokens
+  static __device__ __forceinline__ void over_tokens(const float* tile, const f32x4& b, f32x4* c, int g, int i) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) c[ct] = __builtin_amdgcn_mfma_f32_16x16x4f32(tile[(4 * g + r) * PITCH + 16 * ct + i], b[r], c[ct], 0, 0, 0);
+  }
+  static __device__ __forceinline__ void store(float* row, int g, const f32x4* v, float by) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) *reinterpret_cast<f32x4*>(row + 16 * ct + 4 * g) = v[ct] * by;
+  }
+};
+
+template <int DH, int NT, bool BWD> __device__ __forceinline__ void f32_role(const DotArgs& a, int first, int step, int group, int (*toks)[64], float* lds) {
+  using R = Rows32<DH>;
+  constexpr int CT = R::CT, ROWS = NT * 16, HPB = 4 / NT, NI = BWD ? 4 : 3;
+  constexpr int LPR = DH / 4, RP = 256 / LPR, PASSES = 64 / RP, TILE = 16 * R::PITCH;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
-  int (*toks)[64] = toks_[w];
-  const int head = blockIdx.x * 4 + w;
-  if (head >= a.nhead) return;
-  const int hoff = head * DH;
-  T* out = (T*)a.o + hoff;
-  for (Walk walk(a, 3, 0, (int)blockIdx.y, (int)gridDim.y); walk.next(a);) {
-  struct { int Tq, Tk; } win;
-  walk.tokens(toks, 64, win.Tq, win.Tk);
-  if (win.Tk == 0) {
-    if (lane < win.Tq) {
-      T* o = out + (int64_t)toks[0][lane] * a.ldo;
-      for (int c = 0; c < DH; ++c) st_f<T>(o + c, 0.f);
-    }
-    continue;
-  }
-  const T *q = (const T*)a.q + hoff, *k = (const T*)a.k + hoff, *v = (const T*)a.v + hoff;
-  const int nq = (win.Tq + 15) >> 4, nk = (win.Tk + 15) >> 4;
+  const int t = w % NT, hh = w / NT, head = group * HPB + hh;
+  float *top = lds + NI * R::IMAGE, *inv = top + 64, *dot = inv + 64;           // per row: c * the largest logit, 1 / sum_j, sum_j P dP
   const float c = a.scale * LOG2E;
-  for (int qt = 0; qt < nq; ++qt) {
-    const int64_t tq = toks[0][qt * 16 + i];
-    float qf[KD];
-    load_frag<T, KD>(q + tq * a.ldq + KD * g, qf);
-    f32x4 st[4];
-    float mx = -INFINITY;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  for (Walk walk(a, NT == 4 ? 3 : NT == 2 ? 2 : 1, NT == 4 ? 3 : NT == 2 ? 2 : 0, first, step); walk.next(a);) {
+    int Tq, Tk;
+    walk.tokens(toks, ROWS, Tq, Tk);
+    if (Tq == 0 || Tk == 0) {
+      if (t == 0 && head < a.nhead) {
+        float* o = BWD ? (float*)a.dq : (float*)a.o;
+        const int64_t ldo = BWD ? a.lddq : a.ldo;
+        for (int r = lane / LPR; r < Tq; r += 64 / LPR) *reinterpret_cast<f32x4*>(o + toks[0][r] * ldo + head * DH + lane % LPR * 4) = zero;
+        if (BWD)
+          for (int r = lane / LPR; r < Tk; r += 64 / LPR) {
+            *reinterpret_cast<f32x4*>((float*)a.dk + toks[1][r] * a.lddk + head * DH + lane % LPR * 4) = zero;
+            *reinterpret_cast<f32x4*>((float*)a.dv + toks[1][r] * a.lddv + head * DH + lane % LPR * 4) = zero;
+          }
+      }
+      continue;
+    }
+    f32x4 rows[NI][PASSES];
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      if (kt < nk) {
-        float kf[KD];
-        load_frag<T, KD>(k + (int64_t)toks[1][kt * 16 + i] * a.ldk + KD * g, kf);
-        st[kt] = product<KD>(kf, qf);                                  // rows = keys, column = query i
+    for (int p = 0; p < PASSES; ++p) {
+      const int row = p * RP + (int)threadIdx.x / LPR, slot = row % ROWS;
+      int h = group * HPB + row / ROWS;
+      if (h >= a.nhead) h = a.nhead - 1;
+      const int64_t tq = toks[0][slot], tk = toks[1][slot];
+      const int col = h * DH + (int)threadIdx.x % LPR * 4;
+      rows[0][p] = *reinterpret_cast<const f32x4*>((const float*)a.k + tk * a.ldk + col);
+      rows[1][p] = *reinterpret_cast<const f32x4*>((const float*)a.v + tk * a.ldv + col);
+      rows[2][p] = *reinterpret_cast<const f32x4*>((const float*)a.q + tq * a.ldq + col);
+      if constexpr (BWD) rows[3][p] = *reinterpret_cast<const f32x4*>((const float*)a.g + tq * a.ldg + col);
+    }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (kt * 16 + 4 * g + r >= win.Tk) st[kt][r] = -INFINITY;
-          mx = fmaxf(mx, st[kt][r]);
+    for (int p = 0; p < PASSES; ++p) {       // slots without a token hold zeros: 0 times a probability of 0, whatever the tokens hold
+      const int slot = (p * RP + (int)threadIdx.x / LPR) % ROWS;
+      if (slot >= Tk) rows[0][p] = rows[1][p] = zero;
+      if (slot >= Tq) { rows[2][p] = zero; if constexpr (BWD) rows[3][p] = zero; }
+    }
+    __syncthreads();                         // the window before is done with
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p)
+#pragma unroll
+      for (int n = 0; n < NI; ++n)
+        *reinterpret_cast<f32x4*>(lds + n * R::IMAGE + (p * RP + (int)threadIdx.x / LPR) * R::PITCH + (int)threadIdx.x % LPR * 4) = rows[n][p];
+    __syncthreads();
+    const int nq = (Tq + 15) >> 4, nk = (Tk + 15) >> 4;
+    const float *K = lds + hh * ROWS * R::PITCH, *V = K + R::IMAGE, *Q = K + 2 * R::IMAGE, *G = K + 3 * R::IMAGE;
+    const bool mine = head < a.nhead;
+    if (mine && t < nq) {
+      const typename R::Piece qf = R::piece(Q + t * TILE, g, i);
+      typename R::Piece gf;
+      if constexpr (BWD) gf = R::piece(G + t * TILE, g, i);
+      f32x4 p[NT], dp[NT];
+      float mx = -INFINITY, l = 0.f, d = 0.f;
+#pragma unroll
+      for (int kt = 0; kt < NT; ++kt) {
+        if (kt < nk) {
+          p[kt] = R::over_channels(R::piece(K + kt * TILE, g, i), qf);              // rows = keys, column = query i
+          if constexpr (BWD) dp[kt] = R::over_channels(R::piece(V + kt * TILE, g, i), gf);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (kt * 16 + 4 * g + r >= Tk) p[kt][r] = -INFINITY;
+            mx = fmaxf(mx, p[kt][r]);
+          }
+        }
+      }
+      mx = lanes4_max(mx) * c;
+      f32x4 o[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) o[ct] = zero;
+#pragma unroll
+      for (int kt = 0; kt < NT; ++kt) {
+        if (kt < nk) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            p[kt][r] = __builtin_amdgcn_exp2f(fmaf(p[kt][r], c, -mx));
+            l += p[kt][r];
+            if constexpr (BWD) d += p[kt][r] * dp[kt][r];
+          }
+          if constexpr (!BWD) R::over_tokens(V + kt * TILE, p[kt], o, g, i);        // rows = channels, column = query i
+        }
+      }
+      const float il = 1.f / lanes4_sum(l);
+      const int64_t tq = toks[0][t * 16 + i];
+      if constexpr (BWD) {
+        d = lanes4_sum(d) * il;
+        const int row = hh * ROWS + t * 16 + i;
+        if (g == 0) { top[row] = mx; inv[row] = t * 16 + i < Tq ? il : 0.f; dot[row] = d; }          // no query: P = 0
+#pragma unroll
+        for (int kt = 0; kt < NT; ++kt) {
+          if (kt < nk) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) p[kt][r] = p[kt][r] * il * (dp[kt][r] - d);
+            R::over_tokens(K + kt * TILE, p[kt], o, g, i);
+          }
+        }
+        if (t * 16 + i < Tq) R::store((float*)a.dq + tq * a.lddq + head * DH, g, o, a.scale);
+      } else {
+        if (t * 16 + i < Tq) R::store((float*)a.o + tq * a.ldo + head * DH, g, o, il);
+      }
+    }
+    if constexpr (BWD) {
+      __syncthreads();
+      if (mine && t < nk) {
+        const typename R::Piece kf = R::piece(K + t * TILE, g, i), vf = R::piece(V + t * TILE, g, i);
+        f32x4 dk[CT], dv[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) dk[ct] = dv[ct] = zero;
+        for (int qt = 0; qt < nq; ++qt) {
+          f32x4 p = R::over_channels(R::piece(Q + qt * TILE, g, i), kf), ds = R::over_channels(R::piece(G + qt * TILE, g, i), vf);
+          const int row = hh * ROWS + qt * 16 + 4 * g;                              // rows = queries, column = key i
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            p[r] = inv[row + r] != 0.f ? __builtin_amdgcn_exp2f(fmaf(p[r], c, -top[row + r])) * inv[row + r] : 0.f;
+            ds[r] = p[r] * (ds[r] - dot[row + r]);
+          }
+          R::over_tokens(G + qt * TILE, p, dv, g, i);
+          R::over_tokens(Q + qt * TILE, ds, dk, g, i);
+        }
+        if (t * 16 + i < Tk) {
+          const int64_t tk = toks[1][t * 16 + i];
+          R::store((float*)a.dk + tk * a.lddk + head * DH, g, dk, a.scale);
+          R::store((float*)a.dv + tk * a.lddv + head * DH, g, dv, 1.f);
         }
       }
     }
-    mx = lanes4_max(mx) * c;
-    float l = 0.f;
-    f32x4 o[CT];
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) o[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      if (kt < nk) {
-        f32x4 p;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          p[r] = kt * 16 + 4 * g + r < win.Tk ? __builtin_amdgcn_exp2f(fmaf(st[kt][r], c, -mx)) : 0.f;
-          l += p[r];
-        }
-        accumulate<T, CT>(v, a.ldv, toks[1] + kt * 16, p, o, g, i);      // rows = channels, column = query i
-      }
-    }
-    l = lanes4_sum(l);
-    if (qt * 16 + i < win.Tq) {
-      const float inv = 1.f / l;
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) store_four<T>(out + tq * a.ldo + 16 * ct + 4 * g, o[ct] * inv);
-    }
-  }
   }
 }
 
-template <class T, int DH>
-__global__ __launch_bounds__(256, 2) void dot_bwd_kernel(DotArgs a) {
-  constexpr int KD = DH / 4, CT = DH / 16;
+struct Roles32 { int n4, n2, n1, h4, h2, h1; };      // workgroups along the windows of each size, and along the heads
+// Three workgroups a CU in the backward (10 registers of heads of 32 spilled: 59 us a frame of 16 k tokens, 67 with room for two and none spilled)
+template <int DH, bool BWD>
+__global__ __launch_bounds__(256, (BWD && DH == 64 ? 2 : 3)) void dot_f32_kernel(DotArgs a, Roles32 n) {
+  extern __shared__ __attribute__((aligned(16))) float lds32[];
   __shared__ int toks_[4][2][64];
-  __shared__ float top[4][64], inv[4][64], dot[4][64];   // of the query slots: c * the largest logit, 1 / sum_j, sum_j P dP
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
-  int (*toks)[64] = toks_[w];
-  const int head = blockIdx.x * 4 + w;
-  if (head >= a.nhead) return;
-  const int hoff = head * DH;
-  T *dq = (T*)a.dq + hoff, *dk = (T*)a.dk + hoff, *dv = (T*)a.dv + hoff;
-  for (Walk walk(a, 3, 0, (int)blockIdx.y, (int)gridDim.y); walk.next(a);) {
-  struct { int Tq, Tk; } win;
-  walk.tokens(toks, 64, win.Tq, win.Tk);
-  if (win.Tq == 0 || win.Tk == 0) {
-    if (lane < win.Tq) {
-      T* p = dq + (int64_t)toks[0][lane] * a.lddq;
-      for (int c = 0; c < DH; ++c) st_f<T>(p + c, 0.f);
-    }
-    if (lane < win.Tk) {
-      T *p = dk + (int64_t)toks[1][lane] * a.lddk, *r = dv + (int64_t)toks[1][lane] * a.lddv;
-      for (int c = 0; c < DH; ++c) { st_f<T>(p + c, 0.f); st_f<T>(r + c, 0.f); }
-    }
-    continue;
-  }
-  const T *q = (const T*)a.q + hoff, *k = (const T*)a.k + hoff, *v = (const T*)a.v + hoff, *gr = (const T*)a.g + hoff;
-  const int nq = (win.Tq + 15) >> 4, nk = (win.Tk + 15) >> 4;
-  const float c = a.scale * LOG2E;
-  // dQ: the query in the column
-  for (int qt = 0; qt < nq; ++qt) {
-    const int64_t tq = toks[0][qt * 16 + i];
-    float qf[KD], gf[KD];
-    load_frag<T, KD>(q + tq * a.ldq + KD * g, qf);
-    load_frag<T, KD>(gr + tq * a.ldg + KD * g, gf);
-    f32x4 p[4], dp[4], acc[CT];
-    float d = 0.f, l = 0.f, mx = -INFINITY;
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      if (kt < nk) {
-        const int64_t tk = toks[1][kt * 16 + i];
-        float f[KD];
-        load_frag<T, KD>(k + tk * a.ldk + KD * g, f);
-        p[kt] = product<KD>(f, qf);
-        load_frag<T, KD>(v + tk * a.ldv + KD * g, f);
-        dp[kt] = product<KD>(f, gf);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (kt * 16 + 4 * g + r >= win.Tk) p[kt][r] = -INFINITY;
-          mx = fmaxf(mx, p[kt][r]);
-        }
-      }
-    }
-    mx = lanes4_max(mx) * c;
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      if (kt < nk) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          p[kt][r] = kt * 16 + 4 * g + r < win.Tk ? __builtin_amdgcn_exp2f(fmaf(p[kt][r], c, -mx)) : 0.f;
-          l += p[kt][r];
-          d += p[kt][r] * dp[kt][r];
-        }
-      }
-    }
-    const float il = 1.f / lanes4_sum(l);
-    d = lanes4_sum(d) * il;
-    if (g == 0) { dot[w][qt * 16 + i] = d; top[w][qt * 16 + i] = mx; inv[w][qt * 16 + i] = il; }
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) acc[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      if (kt < nk) {
-        f32x4 ds;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) ds[r] = a.scale * (p[kt][r] * il) * (dp[kt][r] - d);
-        accumulate<T, CT>(k, a.ldk, toks[1] + kt * 16, ds, acc, g, i);
-      }
-    }
-    if (qt * 16 + i < win.Tq) {
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) store_four<T>(dq + tq * a.lddq + 16 * ct + 4 * g, acc[ct]);
-    }
-  }
-  order_lds();
-  // dK, dV: the key in the column
-  for (int kt = 0; kt < nk; ++kt) {
-    const int64_t tk = toks[1][kt * 16 + i];
-    float kf[KD], vf[KD];
-    load_frag<T, KD>(k + tk * a.ldk + KD * g, kf);
-    load_frag<T, KD>(v + tk * a.ldv + KD * g, vf);
-    f32x4 ak[CT], av[CT];
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) ak[ct] = av[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int qt = 0; qt < nq; ++qt) {
-      const int64_t tq = toks[0][qt * 16 + i];
-      float f[KD];
-      load_frag<T, KD>(q + tq * a.ldq + KD * g, f);
-      const f32x4 s = product<KD>(f, kf);                               // rows = queries, column = key i
-      load_frag<T, KD>(gr + tq * a.ldg + KD * g, f);
-      const f32x4 dp = product<KD>(f, vf);
-      f32x4 p, ds;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int slot = qt * 16 + 4 * g + r;
-        p[r] = slot < win.Tq ? __builtin_amdgcn_exp2f(fmaf(s[r], c, -top[w][slot])) * inv[w][slot] : 0.f;
-        ds[r] = a.scale * p[r] * (dp[r] - dot[w][slot]);
-      }
-      accumulate<T, CT>(gr, a.ldg, toks[0] + qt * 16, p, av, g, i);
-      accumulate<T, CT>(q, a.ldq, toks[0] + qt * 16, ds, ak, g, i);
-    }
-    if (kt * 16 + i < win.Tk) {
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        store_four<T>(dk + tk * a.lddk + 16 * ct + 4 * g, ak[ct]);
-        store_four<T>(dv + tk * a.lddv + 16 * ct + 4 * g, av[ct]);
-      }
-    }
-  }
-  }
+  int (*toks)[64] = toks_[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)];
+  int u = blockIdx.x;
+  if (u < n.n4 * n.h4) { f32_role<DH, 4, BWD>(a, u / n.h4, n.n4, u % n.h4, toks, lds32); return; }
+  u -= n.n4 * n.h4;
+  if (u < n.n2 * n.h2) { f32_role<DH, 2, BWD>(a, u / n.h2, n.n2, u % n.h2, toks, lds32); return; }
+  u -= n.n2 * n.h2;
+  f32_role<DH, 1, BWD>(a, u / n.h1, n.n1, u % n.h1, toks, lds32);
 }
 
 // The windows that are in no list: zero rows for queries without a key (out, or dq) and for keys without a query (dk, dv).  A wave per
@@ -1018,15 +974,21 @@ template <int DH, bool BWD> int launch_bf16(const DotArgs& a, const Orphans& z, 
   const int rc = launch_roles<DH, BWD, ROLE4>(a, z, w4, w2, w1, stream);
   return rc != TMAE_OK ? rc : launch_roles<DH, BWD, ROLE2 | ROLE1>(a, z, w4, w2, w1, stream);
 }
-template <int DH, bool BWD> void launch_f32(const DotArgs& a, const Orphans& z, hipStream_t stream) {
+template <int DH, bool BWD> int launch_f32(const DotArgs& a, const Orphans& z, hipStream_t stream) {
   if (z.row16) hipLaunchKernelGGL(dot_orphan_kernel, dim3(walkers(a.nwin, 4, 1)), dim3(256), 0, stream, a, z);
-  const unsigned gx = (unsigned)((a.nhead + 3) / 4);
-  const int64_t windows = a.wl ? class_windows(a, 0) : a.nwin;
-  if (windows == 0) return;
-  if constexpr (BWD)
-    hipLaunchKernelGGL((dot_bwd_kernel<float, DH>), dim3(gx, walkers(windows, 1, gx)), dim3(256), 0, stream, a);
-  else
-    hipLaunchKernelGGL((dot_fwd_kernel<float, DH>), dim3(gx, walkers(windows, 1, gx)), dim3(256), 0, stream, a);
+  constexpr int LDS = ((BWD ? 4 : 3) * Rows32<DH>::IMAGE + 192) * 4;
+  static TmaeLdsAttr attr;
+  if (LDS + 2048 > 65536)
+    if (int e = tmae_allow_lds(attr, (const void*)dot_f32_kernel<DH, BWD>, LDS)) return e;
+  Roles32 n;
+  n.h4 = a.nhead; n.h2 = (a.nhead + 1) / 2; n.h1 = (a.nhead + 3) / 4;
+  // three workgroups a CU for each size: 21 us forward and 48 us backward for a frame of 16 k tokens, 27 and 59 with twelve
+  n.n4 = (int)walkers(a.wl ? class_windows(a, 3) : a.nwin, 1, n.h4, 3);
+  n.n2 = a.wl ? (int)walkers(class_windows(a, 2), 1, n.h2, 3) : 0;
+  n.n1 = a.wl ? (int)walkers(class_windows(a, 0), 1, n.h1, 3) : 0;
+  const int64_t blocks = (int64_t)n.n4 * n.h4 + (int64_t)n.n2 * n.h2 + (int64_t)n.n1 * n.h1;
+  if (blocks > 0) hipLaunchKernelGGL((dot_f32_kernel<DH, BWD>), dim3((unsigned)blocks), dim3(256), LDS, stream, a, n);
+  return TMAE_OK;
 }
 
 }  // namespace
@@ -1048,7 +1010,7 @@ int tmae_win_attn_dot_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk
   by_head(dh, [&](auto w) {
     constexpr int DH = decltype(w)::value;
     if (dtype == TMAE_BF16) failed = launch_bf16<DH, false>(a, z, (hipStream_t)stream);
-    else launch_f32<DH, false>(a, z, (hipStream_t)stream);
+    else failed = launch_f32<DH, false>(a, z, (hipStream_t)stream);
   });
   return failed != TMAE_OK ? failed : tmae_launch_status();
 }
@@ -1073,7 +1035,7 @@ int tmae_win_attn_dot_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk
   by_head(dh, [&](auto w) {
     constexpr int DH = decltype(w)::value;
     if (dtype == TMAE_BF16) failed = launch_bf16<DH, true>(a, z, (hipStream_t)stream);
-    else launch_f32<DH, true>(a, z, (hipStream_t)stream);
+    else failed = launch_f32<DH, true>(a, z, (hipStream_t)stream);
   });
   return failed != TMAE_OK ? failed : tmae_launch_status();
 }
