@@ -9,10 +9,13 @@
 // Bound: HBM.  One read and one write of the rows (the backward of the norm: two reads, one write); statistics, angles and the gain
 // gradient in float32, the angle's product and reduction in float64, one rounding where a row is stored.
 //
-// A workgroup takes a tile of tokens.  It first computes the tile's cos / sin table in LDS -- once per (token, pair), not once per
-// head: 16 heads share it -- and then streams the rows: a lane owns 8 channels of one head (16-byte accesses in bf16), the lanes of a
-// head are adjacent, and a lane keeps its head from token to token, so that its gains and its share of the gain gradient stay in
-// registers.
+// A workgroup takes a tile of tokens, four rows a lane.  All of them are requested first; while they are on their way the tile's cos / sin
+// table is computed in LDS -- once per (token, pair), not once per head: 16 heads share it.  A lane owns 8 channels of one head (16-byte
+// accesses in bf16), the lanes of a head are adjacent, and a lane keeps its head from token to token, so that its gains and its share of
+// the gain gradient stay in registers.
+//
+// 375 k tokens of 16 heads of 16 in bf16 (192 MB): rotation 75 us (5.1 TB/s; 97 us with the table first and the rows after it), with the
+// norm 72 us (5.4 TB/s; 91), gradient 117 us (4.9 TB/s; 139), where a large copy runs at 5.9 TB/s.
 #include "common.h"
 #include <type_traits>
 
@@ -85,16 +88,6 @@ __device__ __forceinline__ float lanes_sum(float v, int lg) {
   return v;
 }
 
-template <class T> __device__ __forceinline__ void load4(const T* p, float* v);
-template <> __device__ __forceinline__ void load4<float>(const float* p, float* v) {
-  const float4 a = *reinterpret_cast<const float4*>(p);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-}
-template <> __device__ __forceinline__ void load4<__hip_bfloat16>(const __hip_bfloat16* p, float* v) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  v[0] = __uint_as_float(u.x << 16); v[1] = __uint_as_float(u.x & 0xFFFF0000u);
-  v[2] = __uint_as_float(u.y << 16); v[3] = __uint_as_float(u.y & 0xFFFF0000u);
-}
 template <class T> __device__ __forceinline__ void store4(T* p, const float* v);
 template <> __device__ __forceinline__ void store4<float>(float* p, const float* v) {
   *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
@@ -117,18 +110,45 @@ template <int MODE> __device__ __forceinline__ int channel_of(const RotaryArgs& 
   return 8 * u + e;
 }
 
+// a unit as it lies in memory: requested early, unpacked where it is used
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+template <class T, bool VEC> struct Raw { float v[8]; };
+template <> struct Raw<float, true> { f32x4 lo, hi; };
+template <> struct Raw<__hip_bfloat16, true> { u32x4 v; };
 template <class T, int MODE, bool VEC>
-__device__ __forceinline__ void load_unit(const T* row, const RotaryArgs& a, int u, float* v) {
-  if constexpr (VEC) {
-    if (MODE == MODE_SPLIT && 4 * u < a.P) {
-      load4<T>(row + 4 * u, v);
-      load4<T>(row + 4 * u + a.P, v + 4);
+__device__ __forceinline__ Raw<T, VEC> request_unit(const T* row, const RotaryArgs& a, int u) {
+  Raw<T, VEC> r;
+  if constexpr (VEC && sizeof(T) == 4) {
+    const bool turned = MODE == MODE_SPLIT && 4 * u < a.P;
+    const T* lo = row + (turned ? 4 * u : 8 * u);
+    r.lo = *reinterpret_cast<const f32x4*>(lo);
+    r.hi = *reinterpret_cast<const f32x4*>(lo + (turned ? a.P : 4));
+  } else if constexpr (VEC) {
+    if constexpr (MODE == MODE_SPLIT) {
+      const bool turned = 4 * u < a.P;
+      const T* lo = row + (turned ? 4 * u : 8 * u);
+      const uint2 l = *reinterpret_cast<const uint2*>(lo), h = *reinterpret_cast<const uint2*>(lo + (turned ? a.P : 4));
+      r.v = u32x4{l.x, l.y, h.x, h.y};
     } else {
-      load8<T>(row + 8 * u, v);
+      r.v = *reinterpret_cast<const u32x4*>(row + 8 * u);
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 8 * u + e < a.dh ? ld_f<T>(row + 8 * u + e) : 0.f;
+    for (int e = 0; e < 8; ++e) r.v[e] = 8 * u + e < a.dh ? ld_f<T>(row + 8 * u + e) : 0.f;
+  }
+  return r;
+}
+template <class T, bool VEC> __device__ __forceinline__ void unpack(const Raw<T, VEC>& r, float* v) {
+  if constexpr (VEC && sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { v[e] = r.lo[e]; v[4 + e] = r.hi[e]; }
+  } else if constexpr (VEC) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { v[2 * e] = __uint_as_float(r.v[e] << 16); v[2 * e + 1] = __uint_as_float(r.v[e] & 0xFFFF0000u); }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = r.v[e];
   }
 }
 template <class T, int MODE, bool VEC>
@@ -223,7 +243,7 @@ template <int MODE> __device__ __forceinline__ void load_gain(const RotaryArgs& 
   }
 }
 
-constexpr int UN = 4;                      // token rows in flight per lane
+constexpr int UN = 4;                      // token rows in flight per lane: a tile's, all requested before its table is computed
 
 template <class T, int MODE, bool VEC, bool NORM>
 __global__ __launch_bounds__(256) void rotary_fwd_kernel(RotaryArgs a) {
@@ -239,38 +259,39 @@ __global__ __launch_bounds__(256) void rotary_fwd_kernel(RotaryArgs a) {
   const float inv_dh = 1.f / (float)a.dh;
   float g[8];
   if constexpr (NORM) load_gain<MODE>(a, p, g);
+  Raw<T, VEC> raw[UN];
+#pragma unroll
+  for (int k = 0; k < UN; ++k) {
+    const int t = k * a.R + p.sub;
+    raw[k] = request_unit<T, MODE, VEC>(x + (t0 + (t < tokens ? t : tokens - 1)) * a.ldx, a, u);
+  }
   fill_table(a, t0, tokens, table);
   __syncthreads();
-  for (int j = 0; j < tokens; j += a.R * UN) {
-    float v[UN][8];
 #pragma unroll
-    for (int k = 0; k < UN; ++k) {
-      const int t = j + k * a.R + p.sub;
-      load_unit<T, MODE, VEC>(x + (t0 + (t < tokens ? t : tokens - 1)) * a.ldx, a, u, v[k]);
+  for (int k = 0; k < UN; ++k) {
+    const int t = k * a.R + p.sub, tc = t < tokens ? t : tokens - 1;
+    float v[8];
+    unpack<T, VEC>(raw[k], v);
+    if constexpr (NORM) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
+      ss = lanes_sum(p.u < a.U ? ss : 0.f, a.lgG);
+      const float r = rsqrtf(ss * inv_dh + a.eps);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= r * g[e];
     }
-#pragma unroll
-    for (int k = 0; k < UN; ++k) {
-      const int t = j + k * a.R + p.sub, tc = t < tokens ? t : tokens - 1;
-      if constexpr (NORM) {
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss += v[k][e] * v[k][e];
-        ss = lanes_sum(p.u < a.U ? ss : 0.f, a.lgG);
-        const float r = rsqrtf(ss * inv_dh + a.eps);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[k][e] *= r * g[e];
-      }
-      turn_unit<MODE>(a, p.u, table + tc * a.PT, v[k], xch + (threadIdx.x >> 6) * 512);
-      if (p.on && t < tokens) store_unit<T, MODE, VEC>(y + (t0 + t) * ldy, a, u, v[k]);
-    }
+    turn_unit<MODE>(a, p.u, table + tc * a.PT, v, xch + (threadIdx.x >> 6) * 512);
+    if (p.on && t < tokens) store_unit<T, MODE, VEC>(y + (t0 + t) * ldy, a, u, v);
   }
 }
 
 // The gradient of the norm.  Workgroups walk the tiles with the grid's stride; a lane's share of the gain gradient stays in registers
-// and leaves once, through LDS, as one partial row per workgroup (summed over the tokens in a fixed order; no atomics).
+// and leaves once, through LDS, as one partial row per workgroup (summed over the tokens in a fixed order; no atomics).  A lane's
+// registers of a row are requested again for the next tile as soon as they are unpacked.
 template <class T, int MODE, bool VEC>
-__global__ __launch_bounds__(256) void qk_norm_rotary_bwd_kernel(RotaryArgs a, int64_t tiles) {
-  __shared__ float2 table[TABLE_PAIRS];
+__global__ __launch_bounds__(256) void qk_norm_rotary_bwd_kernel(RotaryArgs a) {
+  __shared__ float2 tables[2][TABLE_PAIRS];
   __shared__ float xch[4 * 512];
   const Place p = place_of(a);
   const int u = p.on ? p.u : 0;
@@ -283,45 +304,50 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_bwd_kernel(RotaryArgs a, i
   load_gain<MODE>(a, p, g);
 #pragma unroll
   for (int e = 0; e < 8; ++e) dg[e] = 0.f;
-  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const int64_t t0 = tile * a.TB;
+  Raw<T, VEC> rx[UN], rd[UN];
+  auto request = [&](int64_t t0, int k) {
+    const int64_t row = t0 + k * a.R + p.sub;
+    const int64_t r = row < a.n ? row : a.n - 1;
+    rx[k] = request_unit<T, MODE, VEC>(x + r * a.ldx, a, u);
+    rd[k] = request_unit<T, MODE, VEC>(dy + r * ldy, a, u);
+  };
+  const int64_t step = (int64_t)gridDim.x * a.TB;
+  float2* table = tables[0];
+  float2* other = tables[1];
+#pragma unroll
+  for (int k = 0; k < UN; ++k) request((int64_t)blockIdx.x * a.TB, k);
+  for (int64_t t0 = (int64_t)blockIdx.x * a.TB; t0 < a.n; t0 += step) {
     const int tokens = (int)(a.n - t0 < a.TB ? a.n - t0 : a.TB);
-    __syncthreads();
     fill_table(a, t0, tokens, table);
-    __syncthreads();
-    for (int j = 0; j < tokens; j += a.R * 2) {
-      float v[2][8], d[2][8];
+    __syncthreads();                       // one a tile: the table of the tile after the next is this one again
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int t = j + k * a.R + p.sub;
-        const int64_t row = t0 + (t < tokens ? t : tokens - 1);
-        load_unit<T, MODE, VEC>(x + row * a.ldx, a, u, v[k]);
-        load_unit<T, MODE, VEC>(dy + row * ldy, a, u, d[k]);
+    for (int k = 0; k < UN; ++k) {
+      const int t = k * a.R + p.sub, tc = t < tokens ? t : tokens - 1;
+      float v[8], d[8];
+      unpack<T, VEC>(rx[k], v);
+      unpack<T, VEC>(rd[k], d);
+      request(t0 + step, k);               // (behind the last tile: the last row again)
+      turn_unit<MODE>(a, p.u, table + tc * a.PT, d, xch + (threadIdx.x >> 6) * 512);
+      float ss = 0.f, st = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        ss += v[e] * v[e];
+        st += g[e] * d[e] * v[e];
       }
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int t = j + k * a.R + p.sub, tc = t < tokens ? t : tokens - 1;
-        turn_unit<MODE>(a, p.u, table + tc * a.PT, d[k], xch + (threadIdx.x >> 6) * 512);
-        float ss = 0.f, st = 0.f;
+      ss = lanes_sum(p.u < a.U ? ss : 0.f, a.lgG);
+      st = lanes_sum(p.u < a.U ? st : 0.f, a.lgG);
+      const float r = rsqrtf(ss * inv_dh + a.eps), m = r * r * st * inv_dh;
+      if (p.on && t < tokens) {
+        float o[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          ss += v[k][e] * v[k][e];
-          st += g[e] * d[k][e] * v[k][e];
+          dg[e] += d[e] * v[e] * r;
+          o[e] = r * (g[e] * d[e] - v[e] * m);
         }
-        ss = lanes_sum(p.u < a.U ? ss : 0.f, a.lgG);
-        st = lanes_sum(p.u < a.U ? st : 0.f, a.lgG);
-        const float r = rsqrtf(ss * inv_dh + a.eps), m = r * r * st * inv_dh;
-        if (p.on && t < tokens) {
-          float o[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            dg[e] += d[k][e] * v[k][e] * r;
-            o[e] = r * (g[e] * d[k][e] - v[k][e] * m);
-          }
-          store_unit<T, MODE, VEC>(dx + (t0 + t) * ldy, a, u, o);
-        }
+        store_unit<T, MODE, VEC>(dx + (t0 + t) * ldy, a, u, o);
       }
     }
+    float2* const swap = table; table = other; other = swap;
   }
   if (!a.part) return;
   __syncthreads();
@@ -352,19 +378,29 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_bwd_kernel(RotaryArgs a, i
   }
 }
 
-// gradient column = the sum of the partial rows (64 strips, each in row order, then the strips in order): 16 columns a workgroup
+// gradient column = the sum of the partial rows: 4 columns a workgroup, 256 strips of rows, each in row order, then the strips in a fixed
+// order
 __global__ __launch_bounds__(1024) void gain_finish_kernel(const float* __restrict__ part, int rows, int cols, int q_cols,
                                                           float* __restrict__ dq_gain, float* __restrict__ dk_gain) {
-  __shared__ double red[64][16];
-  const int cl = threadIdx.x & 15, strip = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
+  __shared__ double red[16][4];
+  const int cl = threadIdx.x & 3, strip = threadIdx.x >> 2, c = blockIdx.x * 4 + cl;
   double s = 0.0;
-  if (c < cols)
-    for (int r = strip; r < rows; r += 64) s += (double)part[(int64_t)r * cols + c];
-  red[strip][cl] = s;
+  if (c < cols) {
+    for (int r = strip; r < rows; r += 256 * 8) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = part[(int64_t)(r + 256 * k < rows ? r + 256 * k : r) * cols + c];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += r + 256 * k < rows ? (double)v[k] : 0.0;
+    }
+  }
+#pragma unroll
+  for (int k = 4; k < 64; k *= 2) s += __shfl_xor(s, k, 64);
+  if ((threadIdx.x & 63) < 4) red[threadIdx.x >> 6][cl] = s;
   __syncthreads();
-  if (strip == 0 && c < cols) {
+  if (threadIdx.x < 4 && c < cols) {
     double t = 0.0;
-    for (int k = 0; k < 64; ++k) t += red[k][cl];
+    for (int k = 0; k < 16; ++k) t += red[k][cl];
     if (c < q_cols) { if (dq_gain) dq_gain[c] = (float)t; }
     else if (dk_gain) dk_gain[c - q_cols] = (float)t;
   }
@@ -388,7 +424,7 @@ Shape shape_of(int64_t n, int h, int dh, int PT) {
   s.R = slots / s.HB;
   const int64_t want = (n + 511) / 512;
   int64_t tb = (want + s.R - 1) / s.R * s.R;
-  const int64_t most = s.R * UN * 2;
+  const int64_t most = s.R * UN;
   if (tb > most) tb = most;
   if (tb * PT > TABLE_PAIRS) tb = TABLE_PAIRS / PT;
   s.TB = (int)(tb < 1 ? 1 : tb);
@@ -434,16 +470,16 @@ template <class T, bool NORM> void launch_fwd(const RotaryArgs& a, bool interlea
 }
 template <class T> void launch_bwd(const RotaryArgs& a, bool interleaved, bool vec, unsigned gx, hipStream_t stream) {
   const dim3 grid(gx, (unsigned)((a.h + a.HB - 1) / a.HB));
-  const int64_t tiles = (a.n + a.TB - 1) / a.TB;
   by_layout(a, interleaved, vec, [&](auto mode, auto v) {
-    hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, decltype(mode)::value, decltype(v)::value>), grid, dim3(256), 0, stream, a, tiles);
+    hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, decltype(mode)::value, decltype(v)::value>), grid, dim3(256), 0, stream, a);
   });
 }
 
-// workgroups of the backward along the tokens: as many as are resident at once (8 per CU), fewer where the heads need more than one
+// workgroups of the backward along the tokens: as many as are resident at once (3 per CU; with 4, a fourth of the float32 ones wait for a
+// place: 20 k tokens of 16 heads of 72 in 70 us, not 56), fewer where the heads need more than one
 unsigned bwd_blocks(int64_t n, int TB, int gy) {
   const int64_t tiles = (n + TB - 1) / TB;
-  int64_t most = 2048 / gy;
+  int64_t most = 768 / gy;
   if (most < 1) most = 1;
   return (unsigned)(tiles < most ? tiles : most);
 }
@@ -522,7 +558,7 @@ int tmae_qk_norm_rotary_bwd(const void* x, int64_t ldx, int64_t hpx, const void*
     else launch_bwd<float>(a, interleaved != 0, vec, gx, (hipStream_t)stream);
   }
   if (want)
-    hipLaunchKernelGGL(gain_finish_kernel, dim3(tmae_cdiv(cols, 16)), dim3(1024), 0, (hipStream_t)stream, a.part, rows, cols, q_cols,
+    hipLaunchKernelGGL(gain_finish_kernel, dim3(tmae_cdiv(cols, 4)), dim3(1024), 0, (hipStream_t)stream, a.part, rows, cols, q_cols,
                        dq_gain, dk_gain);
   return tmae_launch_status();
 }
