@@ -1755,22 +1755,17 @@ def win_attn(a, b, c, tau, grid_q, grid_k, nhead, batch, ny, nx, do_shift, tau_m
 
 # ----------------------------------------------------------------------------- rotary positions, q / k norms
 
-class _Launch:
-    """The device and stream a call on `t` launches on: the tensors' own device, that device's current stream."""
-    __slots__ = ('dev', 'prev')
-
-    def __init__(self, t):
-        self.dev = t.device.index
-
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.dev:
-            torch.cuda.set_device(self.dev)
-        return _s()
-
-    def __exit__(self, *exc):
-        if self.prev != self.dev:
-            torch.cuda.set_device(self.prev)
+def _launch(entry, t, *args):
+    """entry(*args, stream) on the device of `t` and that device's current stream.  One function, few steps: a backward pass runs in a
+    thread of its own, where every step costs several times what it does in the caller's."""
+    dev = t.get_device()
+    if dev == torch.cuda.current_device():
+        rc = entry(*args, _s())
+    else:
+        with torch.cuda.device(dev):
+            rc = entry(*args, _s())
+    if rc != 0:
+        check(rc, entry.__name__)
 
 
 def _grad_on(*tensors):
@@ -1819,11 +1814,9 @@ def _rotary_args(name, x, positions, inv_freq, sections):
 
 def _rotary_launch(x, positions, inv_freq, arr, interleaved, inverse):
     n, h, dh = x.shape
-    y = torch.empty((n, h, dh), dtype=x.dtype, device=x.device)
-    with _Launch(x) as s:
-        check(lib.tmae_rotary_axes(_p(x), x.stride(0), x.stride(1), _dt(x), n, h, dh, _p(positions), _POS_KIND[positions.dtype],
-                                   positions.stride(0), _p(inv_freq), arr, len(arr), interleaved, inverse, _p(y), s),
-              'tmae_rotary_axes')
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    _launch(lib.tmae_rotary_axes, x, x.data_ptr(), x.stride(0), x.stride(1), _dt(x), n, h, dh, positions.data_ptr(),
+            _POS_KIND[positions.dtype], positions.stride(0), inv_freq.data_ptr(), arr, len(arr), interleaved, inverse, y.data_ptr())
     return y
 
 
@@ -1860,11 +1853,10 @@ def rotary_axes(x, positions, inv_freq, sections, interleaved=False, inverse=Fal
 
 def _qk_norm_launch(x, q_gain, k_gain, positions, inv_freq, arr, q_heads, per_head, eps, interleaved):
     n, h, dh = x.shape
-    y = torch.empty((n, h, dh), dtype=x.dtype, device=x.device)
-    with _Launch(x) as s:
-        check(lib.tmae_qk_norm_rotary_fwd(_p(x), x.stride(0), x.stride(1), _dt(x), n, h, q_heads, dh, _p(q_gain), _p(k_gain), per_head,
-                                          eps, _p(positions), _POS_KIND[positions.dtype], positions.stride(0), _p(inv_freq), arr,
-                                          len(arr), interleaved, _p(y), s), 'tmae_qk_norm_rotary_fwd')
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    _launch(lib.tmae_qk_norm_rotary_fwd, x, x.data_ptr(), x.stride(0), x.stride(1), _dt(x), n, h, q_heads, dh, _p(q_gain), _p(k_gain),
+            per_head, eps, positions.data_ptr(), _POS_KIND[positions.dtype], positions.stride(0), inv_freq.data_ptr(), arr, len(arr),
+            interleaved, y.data_ptr())
     return y
 
 
@@ -1872,28 +1864,26 @@ class _QkNormRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, q_gain, k_gain, positions, inv_freq, arr, pairs, q_heads, per_head, eps, interleaved):
         ctx.save_for_backward(x, q_gain, k_gain, positions, inv_freq)
-        ctx.meta = (arr, pairs, q_heads, per_head, eps, interleaved)
+        want = ctx.needs_input_grad
+        n, h, dh = x.shape
+        wsb = lib.tmae_qk_norm_rotary_bwd_workspace(n, h, dh, pairs, per_head) if want[1] or want[2] else 0
+        ctx.meta = (arr, q_heads, per_head, eps, interleaved, q_gain is not None and want[1], k_gain is not None and want[2], wsb)
         return _qk_norm_launch(x, q_gain, k_gain, positions, inv_freq, arr, q_heads, per_head, eps, interleaved)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, q_gain, k_gain, positions, inv_freq = ctx.saved_tensors
-        arr, pairs, q_heads, per_head, eps, interleaved = ctx.meta
+        arr, q_heads, per_head, eps, interleaved, want_q, want_k, wsb = ctx.meta
         n, h, dh = x.shape
         dy = dy.contiguous()
-        dx = torch.empty((n, h, dh), dtype=x.dtype, device=x.device)
-        dq = torch.empty_like(q_gain) if q_gain is not None and ctx.needs_input_grad[1] else None
-        dk = torch.empty_like(k_gain) if k_gain is not None and ctx.needs_input_grad[2] else None
-        ws, wsb = None, 0
-        if dq is not None or dk is not None:
-            wsb = lib.tmae_qk_norm_rotary_bwd_workspace(n, h, dh, pairs, per_head)
-            ws = _ws(wsb, x.device)
-        with _Launch(x) as s:
-            check(lib.tmae_qk_norm_rotary_bwd(_p(x), x.stride(0), x.stride(1), _p(dy), _dt(x), n, h, q_heads, dh, _p(q_gain), _p(k_gain),
-                                              per_head, eps, _p(positions), _POS_KIND[positions.dtype], positions.stride(0),
-                                              _p(inv_freq), arr, len(arr), interleaved, _p(dx), _p(dq), _p(dk), _p(ws), wsb, s),
-                  'tmae_qk_norm_rotary_bwd')
+        dx = torch.empty_like(dy)
+        dq = torch.empty_like(q_gain) if want_q else None
+        dk = torch.empty_like(k_gain) if want_k else None
+        ws = _ws(wsb, x.device) if want_q or want_k else None
+        _launch(lib.tmae_qk_norm_rotary_bwd, x, x.data_ptr(), x.stride(0), x.stride(1), dy.data_ptr(), _dt(x), n, h, q_heads, dh,
+                _p(q_gain), _p(k_gain), per_head, eps, positions.data_ptr(), _POS_KIND[positions.dtype], positions.stride(0),
+                inv_freq.data_ptr(), arr, len(arr), interleaved, dx.data_ptr(), _p(dq), _p(dk), _p(ws), wsb)
         return dx, dq, dk, None, None, None, None, None, None, None, None
 
 
@@ -1954,11 +1944,8 @@ class _WinAttnDot(torch.autograd.Function):
         da = alloc(a)
         db = alloc(b) if b is not None else None
         dc = alloc(c) if torch.is_tensor(c) else c
-        dq, lddq, dk, lddk, dv, lddv = _WinAttn._ptrs(da, db, dc, d)
-        with _Launch(a) as s:
-            check(lib.tmae_win_attn_dot_bwd(*_WinAttn._ptrs(a, b, c, d), _p(dout), d, _dt(a), mq, mk, nhead, d // nhead,
-                                            _p(grid_q), _p(grid_k), batch, ny, nx, do_shift, scale, dq, lddq, dk, lddk, dv, lddv,
-                                            _p(worklist), s), 'tmae_win_attn_dot_bwd')
+        _launch(lib.tmae_win_attn_dot_bwd, a, *_WinAttn._ptrs(a, b, c, d), dout.data_ptr(), d, _dt(a), mq, mk, nhead, d // nhead,
+                grid_q.data_ptr(), grid_k.data_ptr(), batch, ny, nx, do_shift, scale, *_WinAttn._ptrs(da, db, dc, d), _p(worklist))
         return da, db, (dc if torch.is_tensor(dc) else None), None, None, None, None
 
 
@@ -1966,9 +1953,8 @@ def _win_attn_dot_launch(a, b, c, grid_q, grid_k, worklist, meta):
     d, nhead, batch, ny, nx, do_shift, scale, covered = meta
     mq, mk = a.shape[0], (a if b is None else b).shape[0]
     out = (torch.empty if covered else torch.zeros)((mq, d), dtype=a.dtype, device=a.device)
-    with _Launch(a) as s:
-        check(lib.tmae_win_attn_dot_fwd(*_WinAttn._ptrs(a, b, c, d), _dt(a), mq, mk, nhead, d // nhead, _p(grid_q), _p(grid_k), batch,
-                                        ny, nx, do_shift, scale, _p(out), d, _p(worklist), s), 'tmae_win_attn_dot_fwd')
+    _launch(lib.tmae_win_attn_dot_fwd, a, *_WinAttn._ptrs(a, b, c, d), _dt(a), mq, mk, nhead, d // nhead, grid_q.data_ptr(),
+            grid_k.data_ptr(), batch, ny, nx, do_shift, scale, out.data_ptr(), d, _p(worklist))
     return out
 
 
