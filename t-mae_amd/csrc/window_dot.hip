@@ -24,14 +24,19 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct DotArgs {
   const void *q, *k, *v, *g;               // g: dO
-  int64_t ldq, ldk, ldv, ldg;
+  unsigned pq, pk, pv, pg;                 // row pitches in bytes
   void *o, *dq, *dk, *dv;
-  int64_t ldo, lddq, lddk, lddv;
+  unsigned po, pdq, pdk, pdv;
   const int32_t *grid_q, *grid_k, *wl;
   int64_t mq, mk, nwin;
   int nhead, batch, ny, nx, Wy, Wx, s;
   float scale;
 };
+
+// row `token` of a tensor: one multiply-add of 32 x 32 bits onto 64, where a pitch of 64 bits takes three of them
+__device__ __forceinline__ char* row_of(const void* base, int token, unsigned pitch) {
+  return (char*)base + (unsigned long long)(unsigned)token * pitch;
+}
 
 // LDS operations of a wave execute in order: this keeps the compiler to the order they are written in.  Every wave works in a piece of
 // LDS of its own; no workgroup barrier is needed anywhere.
@@ -178,13 +183,13 @@ template <int DH, int NT, bool BWD> __device__ __forceinline__ void f32_role(con
     walk.tokens(toks, ROWS, Tq, Tk);
     if (Tq == 0 || Tk == 0) {
       if (t == 0 && head < a.nhead) {
-        float* o = BWD ? (float*)a.dq : (float*)a.o;
-        const int64_t ldo = BWD ? a.lddq : a.ldo;
-        for (int r = lane / LPR; r < Tq; r += 64 / LPR) *reinterpret_cast<f32x4*>(o + toks[0][r] * ldo + head * DH + lane % LPR * 4) = zero;
+        const int at = (head * DH + lane % LPR * 4) * 4;
+        for (int r = lane / LPR; r < Tq; r += 64 / LPR)
+          *reinterpret_cast<f32x4*>(row_of(BWD ? a.dq : a.o, toks[0][r], BWD ? a.pdq : a.po) + at) = zero;
         if (BWD)
           for (int r = lane / LPR; r < Tk; r += 64 / LPR) {
-            *reinterpret_cast<f32x4*>((float*)a.dk + toks[1][r] * a.lddk + head * DH + lane % LPR * 4) = zero;
-            *reinterpret_cast<f32x4*>((float*)a.dv + toks[1][r] * a.lddv + head * DH + lane % LPR * 4) = zero;
+            *reinterpret_cast<f32x4*>(row_of(a.dk, toks[1][r], a.pdk) + at) = zero;
+            *reinterpret_cast<f32x4*>(row_of(a.dv, toks[1][r], a.pdv) + at) = zero;
           }
       }
       continue;
@@ -195,12 +200,11 @@ template <int DH, int NT, bool BWD> __device__ __forceinline__ void f32_role(con
       const int row = p * RP + (int)threadIdx.x / LPR, slot = row % ROWS;
       int h = group * HPB + row / ROWS;
       if (h >= a.nhead) h = a.nhead - 1;
-      const int64_t tq = toks[0][slot], tk = toks[1][slot];
-      const int col = h * DH + (int)threadIdx.x % LPR * 4;
-      rows[0][p] = *reinterpret_cast<const f32x4*>((const float*)a.k + tk * a.ldk + col);
-      rows[1][p] = *reinterpret_cast<const f32x4*>((const float*)a.v + tk * a.ldv + col);
-      rows[2][p] = *reinterpret_cast<const f32x4*>((const float*)a.q + tq * a.ldq + col);
-      if constexpr (BWD) rows[3][p] = *reinterpret_cast<const f32x4*>((const float*)a.g + tq * a.ldg + col);
+      const int tq = toks[0][slot], tk = toks[1][slot], col = (h * DH + (int)threadIdx.x % LPR * 4) * 4;
+      rows[0][p] = *reinterpret_cast<const f32x4*>(row_of(a.k, tk, a.pk) + col);
+      rows[1][p] = *reinterpret_cast<const f32x4*>(row_of(a.v, tk, a.pv) + col);
+      rows[2][p] = *reinterpret_cast<const f32x4*>(row_of(a.q, tq, a.pq) + col);
+      if constexpr (BWD) rows[3][p] = *reinterpret_cast<const f32x4*>(row_of(a.g, tq, a.pg) + col);
     }
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {       // slots without a token hold zeros: 0 times a probability of 0, whatever the tokens hold
@@ -253,7 +257,7 @@ template <int DH, int NT, bool BWD> __device__ __forceinline__ void f32_role(con
         }
       }
       const float il = 1.f / lanes4_sum(l);
-      const int64_t tq = toks[0][t * 16 + i];
+      const int tq = toks[0][t * 16 + i];
       if constexpr (BWD) {
         d = lanes4_sum(d) * il;
         const int row = hh * ROWS + t * 16 + i;
@@ -266,9 +270,9 @@ template <int DH, int NT, bool BWD> __device__ __forceinline__ void f32_role(con
             R::over_tokens(K + kt * TILE, p[kt], o, g, i);
           }
         }
-        if (t * 16 + i < Tq) R::store((float*)a.dq + tq * a.lddq + head * DH, g, o, a.scale);
+        if (t * 16 + i < Tq) R::store((float*)row_of(a.dq, tq, a.pdq) + head * DH, g, o, a.scale);
       } else {
-        if (t * 16 + i < Tq) R::store((float*)a.o + tq * a.ldo + head * DH, g, o, il);
+        if (t * 16 + i < Tq) R::store((float*)row_of(a.o, tq, a.po) + head * DH, g, o, il);
       }
     }
     if constexpr (BWD) {
@@ -290,9 +294,9 @@ template <int DH, int NT, bool BWD> __device__ __forceinline__ void f32_role(con
           R::over_tokens(Q + qt * TILE, ds, dk, g, i);
         }
         if (t * 16 + i < Tk) {
-          const int64_t tk = toks[1][t * 16 + i];
-          R::store((float*)a.dk + tk * a.lddk + head * DH, g, dk, a.scale);
-          R::store((float*)a.dv + tk * a.lddv + head * DH, g, dv, 1.f);
+          const int tk = toks[1][t * 16 + i];
+          R::store((float*)row_of(a.dk, tk, a.pdk) + head * DH, g, dk, a.scale);
+          R::store((float*)row_of(a.dv, tk, a.pdv) + head * DH, g, dv, 1.f);
         }
       }
     }
@@ -374,18 +378,19 @@ __device__ __forceinline__ s16x4 pack4(const f32x4& v) { return __builtin_bit_ca
 __device__ __forceinline__ s16x4 read_columns(const char* lds) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)lds);
 }
-// sum / maximum over the 4 lanes that share a column, in every one of them
+// sum / maximum over the 4 lanes that share a column, in every one of them.  The sum is a product with ones: the matrix unit has time,
+// the vector unit does not.  The maximum is the median with infinity, which asks for no quieting of a NaN first (a NaN lost here is still
+// in its probability).
 __device__ __forceinline__ float column_sum(float v) {
-  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(1.f, v, zero, 0, 0, 0)[0];
 }
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
 __device__ __forceinline__ float column_max(float v) {
   auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  v = larger(__uint_as_float(a[0]), __uint_as_float(a[1]));
   auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+  return larger(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
 // One head's columns of a row image, 16 rows (a tile) at a time.
@@ -411,10 +416,9 @@ template <int DH, int PITCH> struct Rows {
     return read_columns(tile + (4 * g + (i >> 2)) * PITCH + 32 * ct + 8 * (i & 3));
   }
   // the accumulators' layout: channels 16 ct + 4g .. + 3 of row i
-  static __device__ __forceinline__ void put(char* tile, int g, int i, const f32x4* v, float by) {
+  static __device__ __forceinline__ void put(char* tile, int g, int i, const f32x4* v) {
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
-      *reinterpret_cast<uint2*>(tile + i * PITCH + 32 * ct + 8 * g) = make_uint2(pack2(v[ct][0] * by, v[ct][1] * by), pack2(v[ct][2] * by, v[ct][3] * by));
+    for (int ct = 0; ct < CT; ++ct) *reinterpret_cast<s16x4*>(tile + i * PITCH + 32 * ct + 8 * g) = pack4(v[ct]);
   }
   static __device__ __forceinline__ f32x4 over_channels(const Piece& a, const Piece& b, f32x4 c) {
     if constexpr (FR == 4) {
@@ -450,26 +454,34 @@ template <int DH, int NT> struct Window {
   static constexpr int CT = R::CT;
 
   struct Loaded { u32x4 row[LOADS]; };
-  static __device__ __forceinline__ Loaded request(const void* base, int64_t ld, const int* toks, int64_t col) {
+  static __device__ __forceinline__ Loaded request(const void* base, unsigned pitch, const int* toks, int col) {
     const int lane = threadIdx.x & 63;
     Loaded l;
 #pragma unroll
     for (int s = 0; s < LOADS; ++s)
-      l.row[s] = *reinterpret_cast<const u32x4*>((const char*)base + (int64_t)toks[s * RPI + lane / CHUNKS] * ld * 2 + col + (lane % CHUNKS) * 16);
+      l.row[s] = *reinterpret_cast<const u32x4*>(row_of(base, toks[s * RPI + lane / CHUNKS], pitch) + col + (lane % CHUNKS) * 16);
     return l;
+  }
+  // the rows from `T` on as zeros: a probability of 0 stays one beside an infinity
+  static __device__ __forceinline__ void lay(char* image, Loaded l, int T) {
+    const int lane = threadIdx.x & 63;
+    const u32x4 none = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int s = 0; s < LOADS; ++s) l.row[s] = s * RPI + lane / CHUNKS < T ? l.row[s] : none;
+    lay(image, l);
   }
   static __device__ __forceinline__ void lay(char* image, Loaded l) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int s = 0; s < LOADS; ++s) *reinterpret_cast<u32x4*>(image + (s * RPI + lane / CHUNKS) * PITCH + (lane % CHUNKS) * 16) = l.row[s];
   }
-  static __device__ __forceinline__ void store(void* base, int64_t ld, const int* toks, int T, int64_t col, const char* image) {
+  static __device__ __forceinline__ void store(void* base, unsigned pitch, const int* toks, int T, int col, const char* image) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int s = 0; s < LOADS; ++s) {
       const int r = s * RPI + lane / CHUNKS;
       if (r < T)
-        *reinterpret_cast<uint4*>((char*)base + (int64_t)toks[r] * ld * 2 + col + (lane % CHUNKS) * 16) =
+        *reinterpret_cast<uint4*>(row_of(base, toks[r], pitch) + col + (lane % CHUNKS) * 16) =
             *reinterpret_cast<const uint4*>(image + r * PITCH + (lane % CHUNKS) * 16);
     }
   }
@@ -483,7 +495,7 @@ __device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq, cons
   using R = typename W::R;
   constexpr int CT = W::CT, TILE = W::TILE;
   const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15, nq = (Tq + 15) >> 4;
-  const int64_t col = (int64_t)head * DH * 2;
+  const int col = head * DH * 2;
   const char* V = A + W::IMAGE;
   typename R::Piece kf[NK];
   s16x4 vc[NK][CT];
@@ -510,7 +522,7 @@ __device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq, cons
 #pragma unroll
     for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[kt][r]);
+      for (int r = 0; r < 4; ++r) mx = larger(mx, st[kt][r]);
     mx = column_max(mx) * c;
     float l = 0.f;
     s16x4 p[NK];
@@ -533,10 +545,13 @@ __device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq, cons
       if constexpr (NK == 3) o[ct] = over_tokens(vc[2][ct], s16x4{0, 0, 0, 0}, p[2], s16x4{0, 0, 0, 0}, o[ct]);
       if constexpr (NK == 1) o[ct] = over_tokens(vc[0][ct], p[0], o[ct]);
     }
-    R::put(A + qt * TILE, g, i, o, __builtin_amdgcn_rcpf(l));
+    const float il = __builtin_amdgcn_rcpf(l);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) o[ct] *= il;
+    R::put(A + qt * TILE, g, i, o);
   }
   order_lds();
-  W::store(a.o, a.ldo, tq, Tq, col, A);
+  W::store(a.o, a.po, tq, Tq, col, A);
 }
 
 template <int DH, int NT, int NK>
@@ -546,7 +561,7 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
   using R = typename W::R;
   constexpr int CT = W::CT, TILE = W::TILE, TP = TILE_PITCH;
   const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15, nq = (Tq + 15) >> 4;
-  const int64_t col = (int64_t)head * DH * 2;
+  const int col = head * DH * 2;
   char *B = A + W::IMAGE, *C = B + W::IMAGE;
   typename R::Piece kf[NK], vf[NK];
 #pragma unroll
@@ -555,7 +570,7 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
     vf[kt] = R::piece(B + kt * TILE, g, i);
   }
   order_lds();
-  W::lay(B, grows);
+  W::lay(B, grows, Tq);
   order_lds();
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   f32x4 absent;
@@ -585,7 +600,7 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
 #pragma unroll
     for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, p[kt][r]);
+      for (int r = 0; r < 4; ++r) mx = larger(mx, p[kt][r]);
     mx = column_max(mx) * c;
 #pragma unroll
     for (int kt = 0; kt < NK; ++kt)
@@ -595,8 +610,8 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
         l += p[kt][r];
         d = __builtin_fmaf(p[kt][r], dp[kt][r], d);
       }
-    const float il = qt * 16 + i < Tq ? __builtin_amdgcn_rcpf(column_sum(l)) : 0.f;             // no query: P = 0
-    d = column_sum(d) * il;
+    const float il = __builtin_amdgcn_rcpf(column_sum(qt * 16 + i < Tq ? l : INFINITY));        // no query: P = 0
+    d = column_sum(d) * il * -a.scale;
     s16x4 ds[NK];
 #pragma unroll
     for (int k0 = 0; k0 < NK; k0 += 2) {
@@ -606,7 +621,7 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           p[kt][r] *= il;
-          t[r] = p[kt][r] * (dp[kt][r] - d);
+          t[r] = p[kt][r] * __builtin_fmaf(dp[kt][r], a.scale, d);
         }
         ds[kt] = pack4(t);
         char* tile = tiles + (kt - k0) * 2 * TILE_BYTES;
@@ -638,18 +653,18 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
       if constexpr (NK == 3) dq[ct] = over_tokens(kc[2], s16x4{0, 0, 0, 0}, ds[2], s16x4{0, 0, 0, 0}, dq[ct]);
       if constexpr (NK == 1) dq[ct] = over_tokens(kc[0], ds[0], dq[ct]);
     }
-    R::put(C + qt * TILE, g, i, dq, a.scale);
+    R::put(C + qt * TILE, g, i, dq);
   }
   order_lds();
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt) {
-    R::put(A + kt * TILE, g, i, dk[kt], a.scale);
-    R::put(B + kt * TILE, g, i, dv[kt], 1.f);
+    R::put(A + kt * TILE, g, i, dk[kt]);
+    R::put(B + kt * TILE, g, i, dv[kt]);
   }
   order_lds();
-  W::store(a.dq, a.lddq, tq, Tq, col, C);
-  W::store(a.dk, a.lddk, tk, Tk, col, A);
-  W::store(a.dv, a.lddv, tk, Tk, col, B);
+  W::store(a.dq, a.pdq, tq, Tq, col, C);
+  W::store(a.dk, a.pdk, tk, Tk, col, A);
+  W::store(a.dv, a.pdv, tk, Tk, col, B);
 }
 
 // Windows of up to 16 NT tokens; without a work list (NT = 4) every window, empty ones included.  Two waves per SIMD as the bound: 256
@@ -659,33 +674,33 @@ template <int DH, int NT, bool BWD> __device__ __forceinline__ void window_role(
   using W = Window<DH, NT>;
   const int lane = threadIdx.x & 63;
   if (head >= a.nhead) return;
-  const int64_t col = (int64_t)head * DH * 2;
+  const int col = head * DH * 2;
   for (Walk walk(a, NT == 4 ? 3 : 2, NT == 4 ? 3 : 2, first, step); walk.next(a);) {
     int Tq, Tk;
     walk.tokens(toks, NT * 16, Tq, Tk);
     if (Tq == 0 || Tk == 0) {
       const uint4 z = make_uint4(0u, 0u, 0u, 0u);
       if (lane < Tq) {
-        uint4* o = reinterpret_cast<uint4*>(BWD ? (char*)a.dq + toks[0][lane] * a.lddq * 2 + col : (char*)a.o + toks[0][lane] * a.ldo * 2 + col);
+        uint4* o = reinterpret_cast<uint4*>(BWD ? row_of(a.dq, toks[0][lane], a.pdq) + col : row_of(a.o, toks[0][lane], a.po) + col);
         for (int c = 0; c < DH / 8; ++c) o[c] = z;
       }
       if (BWD && lane < Tk) {
-        uint4 *p = reinterpret_cast<uint4*>((char*)a.dk + toks[1][lane] * a.lddk * 2 + col),
-              *r = reinterpret_cast<uint4*>((char*)a.dv + toks[1][lane] * a.lddv * 2 + col);
+        uint4 *p = reinterpret_cast<uint4*>(row_of(a.dk, toks[1][lane], a.pdk) + col),
+              *r = reinterpret_cast<uint4*>(row_of(a.dv, toks[1][lane], a.pdv) + col);
         for (int c = 0; c < DH / 8; ++c) { p[c] = z; r[c] = z; }
       }
       continue;
     }
-    const typename W::Loaded krows = W::request(a.k, a.ldk, toks[1], col), vrows = W::request(a.v, a.ldv, toks[1], col),
-                             qrows = W::request(a.q, a.ldq, toks[0], col);
+    const typename W::Loaded krows = W::request(a.k, a.pk, toks[1], col), vrows = W::request(a.v, a.pv, toks[1], col),
+                             qrows = W::request(a.q, a.pq, toks[0], col);
     constexpr bool LATE = DH * NT >= 128;                // registers: dO is requested when K and V have left theirs
     typename W::Loaded grows;
-    if constexpr (BWD && !LATE) grows = W::request(a.g, a.ldg, toks[0], col);
+    if constexpr (BWD && !LATE) grows = W::request(a.g, a.pg, toks[0], col);
     W::lay(A, krows);
-    W::lay(A + W::IMAGE, vrows);
+    W::lay(A + W::IMAGE, vrows, Tk);
     if constexpr (BWD) W::lay(A + 2 * W::IMAGE, qrows);
     order_lds();
-    if constexpr (BWD && LATE) grows = W::request(a.g, a.ldg, toks[0], col);
+    if constexpr (BWD && LATE) grows = W::request(a.g, a.pg, toks[0], col);
     const int nk = (Tk + 15) >> 4;
 #define ONE(NK)                                                                                                                            \
   if constexpr (BWD) bwd_window<DH, NT, NK>(a, toks[0], toks[1], Tq, Tk, head, A, grows, A + 3 * W::IMAGE);                                \
@@ -715,19 +730,26 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   const int r8 = lane >> 3, ch = lane & 7;
   const bool in_row = head0 * DH + ch * 8 < a.nhead * DH;
-  const int64_t col = in_row ? (int64_t)head0 * DH * 2 + ch * 16 : 0;
+  int col = in_row ? head0 * DH * 2 + ch * 16 : 0;
+  asm volatile("" : "+v"(col));             // (seven tensors' addresses of this lane are not worth 14 registers from window to window)
   u32x4 rows[NI][2];
 #pragma unroll
   for (int u = 0; u < (HALF ? 1 : 2); ++u) {
-    const int64_t tk = toks[1][r8 + 8 * u], tq = toks[0][r8 + 8 * u];
-    rows[0][u] = *reinterpret_cast<const u32x4*>((const char*)a.k + tk * a.ldk * 2 + col);
-    rows[1][u] = *reinterpret_cast<const u32x4*>((const char*)a.v + tk * a.ldv * 2 + col);
-    rows[2][u] = *reinterpret_cast<const u32x4*>((const char*)a.q + tq * a.ldq * 2 + col);
-    if constexpr (BWD) rows[3][u] = *reinterpret_cast<const u32x4*>((const char*)a.g + tq * a.ldg * 2 + col);
+    const int tk = toks[1][r8 + 8 * u], tq = toks[0][r8 + 8 * u];
+    rows[0][u] = *reinterpret_cast<const u32x4*>(row_of(a.k, tk, a.pk) + col);
+    rows[1][u] = *reinterpret_cast<const u32x4*>(row_of(a.v, tk, a.pv) + col);
+    rows[2][u] = *reinterpret_cast<const u32x4*>(row_of(a.q, tq, a.pq) + col);
+    if constexpr (BWD) rows[3][u] = *reinterpret_cast<const u32x4*>(row_of(a.g, tq, a.pg) + col);
   }
+  const u32x4 none = {0u, 0u, 0u, 0u};
   if constexpr (HALF) {
+    rows[0][1] = rows[0][0]; rows[2][1] = rows[2][0];
+  }
+  // slots without a token: zero rows of V and dO, so that a probability of 0 stays one beside an infinity
 #pragma unroll
-    for (int t = 0; t < NI; ++t) rows[t][1] = rows[t][0];
+  for (int u = 0; u < 2; ++u) {
+    rows[1][u] = (HALF && u) || r8 + 8 * u >= Tk ? none : rows[1][u];
+    if constexpr (BWD) rows[3][u] = (HALF && u) || r8 + 8 * u >= Tq ? none : rows[3][u];
   }
 #pragma unroll
   for (int t = 0; t < NI; ++t)
@@ -749,7 +771,7 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
     }
 #pragma unroll
     for (int h = 0; h < HG; ++h) {
-      mx[h] = column_max(fmaxf(fmaxf(st[h][0], st[h][1]), fmaxf(st[h][2], st[h][3]))) * c;
+      mx[h] = column_max(larger(larger(st[h][0], st[h][1]), larger(st[h][2], st[h][3]))) * c;
       l[h] = 0.f;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -763,15 +785,17 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
       f32x4 o[CT];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) o[ct] = over_tokens(vc[h][ct], p[h], zero);
-      const float s = column_sum(l[h]);
-      R::put(Q + h * DH * 2, g, i, o, __builtin_amdgcn_rcpf(s));
+      const float il = __builtin_amdgcn_rcpf(column_sum(l[h]));
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) o[ct] *= il;
+      R::put(Q + h * DH * 2, g, i, o);
     }
     order_lds();
     if (in_row) {
 #pragma unroll
       for (int u = 0; u < (HALF ? 1 : 2); ++u) {
         const int r = r8 + 8 * u;
-        if (r < Tq) *reinterpret_cast<uint4*>((char*)a.o + toks[0][r] * a.ldo * 2 + col) = *reinterpret_cast<const uint4*>(Q + r * PITCH + ch * 16);
+        if (r < Tq) *reinterpret_cast<uint4*>(row_of(a.o, toks[0][r], a.po) + col) = *reinterpret_cast<const uint4*>(Q + r * PITCH + ch * 16);
       }
     }
   } else {
@@ -792,7 +816,7 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
     order_lds();
 #pragma unroll
     for (int h = 0; h < HG; ++h) {
-      const float mx = column_max(fmaxf(fmaxf(p[h][0], p[h][1]), fmaxf(p[h][2], p[h][3]))) * c;
+      const float mx = column_max(larger(larger(p[h][0], p[h][1]), larger(p[h][2], p[h][3]))) * c;
       float d = 0.f, l = 0.f;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -800,13 +824,13 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
         l += p[h][r];
         d = __builtin_fmaf(p[h][r], dp[h][r], d);
       }
-      const float il = i < Tq ? __builtin_amdgcn_rcpf(column_sum(l)) : 0.f;                   // no query: P = 0
-      d = column_sum(d) * il;
+      const float il = __builtin_amdgcn_rcpf(column_sum(i < Tq ? l : INFINITY));              // no query: P = 0
+      d = column_sum(d) * il * -a.scale;
       f32x4 t;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         p[h][r] *= il;
-        t[r] = p[h][r] * (dp[h][r] - d);
+        t[r] = p[h][r] * __builtin_fmaf(dp[h][r], a.scale, d);
       }
       ds[h] = pack4(t);
       char* tile = K + h * 2 * TILE_BYTES;
@@ -831,9 +855,9 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
         dv[ct] = over_tokens(gc[h][ct], pt[h], zero);
         dk[ct] = over_tokens(qc[h][ct], dt[h], zero);
       }
-      R::put(Q + h * DH * 2, g, i, dq, a.scale);
-      R::put(K + h * DH * 2, g, i, dk, a.scale);
-      R::put(V + h * DH * 2, g, i, dv, 1.f);
+      R::put(Q + h * DH * 2, g, i, dq);
+      R::put(K + h * DH * 2, g, i, dk);
+      R::put(V + h * DH * 2, g, i, dv);
     }
     order_lds();
     if (in_row) {
@@ -841,10 +865,10 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
       for (int u = 0; u < (HALF ? 1 : 2); ++u) {
         const int r = r8 + 8 * u;
         const char* at = K + r * PITCH + ch * 16;
-        if (r < Tq) *reinterpret_cast<uint4*>((char*)a.dq + toks[0][r] * a.lddq * 2 + col) = *reinterpret_cast<const uint4*>(at + 2 * IMAGE);
+        if (r < Tq) *reinterpret_cast<uint4*>(row_of(a.dq, toks[0][r], a.pdq) + col) = *reinterpret_cast<const uint4*>(at + 2 * IMAGE);
         if (r < Tk) {
-          *reinterpret_cast<uint4*>((char*)a.dk + toks[1][r] * a.lddk * 2 + col) = *reinterpret_cast<const uint4*>(at);
-          *reinterpret_cast<uint4*>((char*)a.dv + toks[1][r] * a.lddv * 2 + col) = *reinterpret_cast<const uint4*>(at + IMAGE);
+          *reinterpret_cast<uint4*>(row_of(a.dk, toks[1][r], a.pdk) + col) = *reinterpret_cast<const uint4*>(at);
+          *reinterpret_cast<uint4*>(row_of(a.dv, toks[1][r], a.pdv) + col) = *reinterpret_cast<const uint4*>(at + IMAGE);
         }
       }
     }
@@ -907,9 +931,11 @@ __global__ __launch_bounds__(256, (kernel_waves<DH, BWD, ROLES>())) void dot_ker
   }
 }
 
-// Workgroups along the windows: what the windows can need, at most `per_cu` per CU in all -- a few times what is resident at
-// once.  Fewer leave the last windows to a few workgroups; more spend their time on workgroups that find no window.
-unsigned walkers(int64_t windows, int per_group, unsigned gx, int per_cu = 12) {
+// Workgroups along the windows: what the windows can need, at most `per_cu` per CU in all -- a little more than what is resident at
+// once.  Fewer leave the last windows to a few workgroups (4: the backward of the large windows 84 us, not 75, at stage 1); more spend
+// their time on workgroups that find no window (12: that of the others 51 us, not 46, at stage 2).  Neighbouring windows on the same die
+// would share the grids' lines in its L2, but the dense windows are neighbours too: one die would have them all (49 us, not 39).
+unsigned walkers(int64_t windows, int per_group, unsigned gx, int per_cu = 6) {
   const int64_t need = (windows + per_group - 1) / per_group;
   int64_t most = (int64_t)tmae_num_cus() * per_cu / gx;
   if (most < 1) most = 1;
@@ -922,7 +948,7 @@ int64_t class_windows(const DotArgs& a, int cls) {
 }
 
 bool rows_ok(const void* p, int64_t ld, int width, int es) {
-  return p && ((uintptr_t)p & 15) == 0 && ld >= width && (ld * es) % 16 == 0;
+  return p && ((uintptr_t)p & 15) == 0 && ld >= width && ld < (1 << 28) && (ld * es) % 16 == 0;
 }
 
 int fill(DotArgs& a, int dtype, int64_t mq, int64_t mk, int nhead, int dh, const int32_t* grid_q, const int32_t* grid_k, int batch, int ny,
@@ -1003,9 +1029,10 @@ int tmae_win_attn_dot_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk
   if (mq == 0) return TMAE_OK;
   const int es = dtype == TMAE_BF16 ? 2 : 4, d = nhead * dh;
   if (!rows_ok(q, ldq, d, es) || !rows_ok(out, ldo, d, es) || (mk && (!rows_ok(k, ldk, d, es) || !rows_ok(v, ldv, d, es)))) return TMAE_EARG;
-  a.q = q; a.ldq = ldq; a.k = k; a.ldk = ldk; a.v = v; a.ldv = ldv; a.o = out; a.ldo = ldo;
+  a.q = q; a.k = k; a.v = v; a.o = out;
+  a.pq = (unsigned)(ldq * es); a.pk = (unsigned)(ldk * es); a.pv = (unsigned)(ldv * es); a.po = (unsigned)(ldo * es);
   Orphans z = {};
-  if (worklist && grid_q != grid_k) z = Orphans{(char*)out, ldo * es, nullptr, nullptr, 0, 0, d * es / 16};
+  if (worklist && (grid_q != grid_k || mq != mk)) z = Orphans{(char*)out, ldo * es, nullptr, nullptr, 0, 0, d * es / 16};
   int failed = TMAE_OK;
   by_head(dh, [&](auto w) {
     constexpr int DH = decltype(w)::value;
@@ -1027,10 +1054,11 @@ int tmae_win_attn_dot_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk
   const int es = dtype == TMAE_BF16 ? 2 : 4, d = nhead * dh;
   if (mq && (!rows_ok(q, ldq, d, es) || !rows_ok(dout, lddo, d, es) || !rows_ok(dq, lddq, d, es))) return TMAE_EARG;
   if (mk && (!rows_ok(k, ldk, d, es) || !rows_ok(v, ldv, d, es) || !rows_ok(dk, lddk, d, es) || !rows_ok(dv, lddv, d, es))) return TMAE_EARG;
-  a.q = q; a.ldq = ldq; a.k = k; a.ldk = ldk; a.v = v; a.ldv = ldv; a.g = dout; a.ldg = lddo;
-  a.dq = dq; a.lddq = lddq; a.dk = dk; a.lddk = lddk; a.dv = dv; a.lddv = lddv;
+  a.q = q; a.k = k; a.v = v; a.g = dout; a.dq = dq; a.dk = dk; a.dv = dv;
+  a.pq = (unsigned)(ldq * es); a.pk = (unsigned)(ldk * es); a.pv = (unsigned)(ldv * es); a.pg = (unsigned)(lddo * es);
+  a.pdq = (unsigned)(lddq * es); a.pdk = (unsigned)(lddk * es); a.pdv = (unsigned)(lddv * es);
   Orphans z = {};
-  if (worklist && grid_q != grid_k) z = Orphans{(char*)dq, lddq * es, (char*)dk, (char*)dv, lddk * es, lddv * es, d * es / 16};
+  if (worklist && (grid_q != grid_k || mq != mk)) z = Orphans{(char*)dq, lddq * es, (char*)dk, (char*)dv, lddk * es, lddv * es, d * es / 16};
   int failed = TMAE_OK;
   by_head(dh, [&](auto w) {
     constexpr int DH = decltype(w)::value;
