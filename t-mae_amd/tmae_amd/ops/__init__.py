@@ -4,6 +4,9 @@ Mirrors the operator surface the reference reaches through sst_ops_utils / torch
 pytorch3d -- same argument meaning, but every call lands in a hand-written gfx950 kernel.
 No tensor math happens here besides allocation and dense GEMMs handed to hipBLASLt via torch.
 """
+import ctypes
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -1755,17 +1758,33 @@ def win_attn(a, b, c, tau, grid_q, grid_k, nhead, batch, ny, nx, do_shift, tau_m
 
 # ----------------------------------------------------------------------------- rotary positions, q / k norms
 
-def _launch(entry, t, *args):
-    """entry(*args, stream) on the device of `t` and that device's current stream.  One function, few steps: a backward pass runs in a
-    thread of its own, where every step costs several times what it does in the caller's."""
-    dev = t.get_device()
-    if dev == torch.cuda.current_device():
-        rc = entry(*args, _s())
+_get_device = getattr(torch._C, '_cuda_getDevice', None) or torch.cuda.current_device
+_CONTIGUOUS = torch.contiguous_format
+_BF16 = torch.bfloat16
+
+
+def _launch(entry, dev, *args):
+    """entry(*args, stream) on device number `dev` and its current stream.  Few steps, here and in the functions around it: a backward
+    pass runs in a thread of its own, where each of them costs several times what it does in the caller's."""
+    if dev == _get_device():
+        rc = entry.raw(*args, _raw_stream(dev) if _raw_stream is not None else _s())
     else:
         with torch.cuda.device(dev):
-            rc = entry(*args, _s())
+            rc = entry.raw(*args, _s())
     if rc != 0:
         check(rc, entry.__name__)
+
+
+def _once(backward):
+    """A backward pass without a derivative of its own: differentiating its results is an error, whether or not the incoming gradient
+    depends on anything (the results depend on the saved tensors too).  Gradients are on there only under create_graph."""
+    checked = once_differentiable(backward)
+
+    def call(ctx, *grads):
+        if torch.is_grad_enabled():
+            return checked(ctx, *(None if g is None else g.detach().requires_grad_() for g in grads))
+        return backward(ctx, *grads)
+    return call
 
 
 def _grad_on(*tensors):
@@ -1783,23 +1802,28 @@ def rotary_freqs(sections, base=10000.0, device=None):
     return torch.cat([float(base) ** (-torch.arange(int(p), dtype=torch.float64) / int(p)) for p in sections]).to(device)
 
 
+@functools.lru_cache(maxsize=64)
+def _rotary_sections(sections):
+    """(the sections as whole numbers, as a C array, channel pairs in all)"""
+    sections = tuple(int(p) for p in sections)
+    return sections, (ctypes.c_int32 * len(sections))(*sections), sum(sections)
+
+
 def _rotary_args(name, x, positions, inv_freq, sections):
     """Checks the arguments the two rotary operators share; returns (x, positions, inv_freq, C array of the sections, P)."""
-    import ctypes as C
     if x.dim() != 3:
         raise ValueError(f'{name}: x [tokens, heads, channels] expected, got {tuple(x.shape)}')
     _dt(x)
     n, h, dh = x.shape
-    sections = tuple(int(p) for p in sections)
-    P = sum(sections)
+    sections, arr, P = _rotary_sections(tuple(sections))
     if not 1 <= len(sections) <= 4 or min(sections) < 1 or 2 * P > dh or dh > 512 or not 1 <= h <= 65535:
         raise ValueError(f'{name}: sections {sections} for {h} heads of {dh} channels (1 to 4 axes, at most {dh // 2} pairs, at most '
                          f'512 channels)')
-    if tuple(positions.shape) != (n, len(sections)):
+    if positions.shape != (n, len(sections)):
         raise ValueError(f'{name}: positions {tuple(positions.shape)}, expected {(n, len(sections))}')
     if positions.dtype not in _POS_KIND:
         raise TypeError(f'{name}: positions are int32, int64 or float32, got {positions.dtype}')
-    if inv_freq.dtype != torch.float64 or tuple(inv_freq.shape) != (P,):
+    if inv_freq.dtype != torch.float64 or inv_freq.shape != (P,):
         raise ValueError(f'{name}: inv_freq [{P}] float64 expected, got {tuple(inv_freq.shape)} {inv_freq.dtype}')
     if positions.device != x.device or inv_freq.device != x.device:
         raise ValueError(f'{name}: x on {x.device}, positions on {positions.device}, inv_freq on {inv_freq.device}')
@@ -1809,13 +1833,14 @@ def _rotary_args(name, x, positions, inv_freq, sections):
         x = x.contiguous()
     if positions.stride(1) != 1 and len(sections) > 1 or positions.stride(0) < len(sections):
         positions = positions.contiguous()
-    return x, positions, inv_freq.contiguous(), (C.c_int32 * len(sections))(*sections), P
+    return x, positions, inv_freq.contiguous(), arr, P
 
 
 def _rotary_launch(x, positions, inv_freq, arr, interleaved, inverse):
     n, h, dh = x.shape
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    _launch(lib.tmae_rotary_axes, x, x.data_ptr(), x.stride(0), x.stride(1), _dt(x), n, h, dh, positions.data_ptr(),
+    ldx, hpx, _ = x.stride()
+    y = torch.empty_like(x, memory_format=_CONTIGUOUS)
+    _launch(lib.tmae_rotary_axes, x.get_device(), x.data_ptr(), ldx, hpx, 1 if x.dtype is _BF16 else 0, n, h, dh, positions.data_ptr(),
             _POS_KIND[positions.dtype], positions.stride(0), inv_freq.data_ptr(), arr, len(arr), interleaved, inverse, y.data_ptr())
     return y
 
@@ -1828,11 +1853,11 @@ class _RotaryAxes(torch.autograd.Function):
         return _rotary_launch(x, positions, inv_freq, arr, interleaved, inverse)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         positions, inv_freq = ctx.saved_tensors
         arr, interleaved, inverse = ctx.meta
-        if dy.stride(2) != 1 and dy.shape[2] > 1:
+        if dy.stride(2) != 1:
             dy = dy.contiguous()
         return _rotary_launch(dy, positions, inv_freq, arr, interleaved, 1 - inverse), None, None, None, None, None
 
@@ -1853,10 +1878,11 @@ def rotary_axes(x, positions, inv_freq, sections, interleaved=False, inverse=Fal
 
 def _qk_norm_launch(x, q_gain, k_gain, positions, inv_freq, arr, q_heads, per_head, eps, interleaved):
     n, h, dh = x.shape
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    _launch(lib.tmae_qk_norm_rotary_fwd, x, x.data_ptr(), x.stride(0), x.stride(1), _dt(x), n, h, q_heads, dh, _p(q_gain), _p(k_gain),
-            per_head, eps, positions.data_ptr(), _POS_KIND[positions.dtype], positions.stride(0), inv_freq.data_ptr(), arr, len(arr),
-            interleaved, y.data_ptr())
+    ldx, hpx, _ = x.stride()
+    y = torch.empty_like(x, memory_format=_CONTIGUOUS)
+    _launch(lib.tmae_qk_norm_rotary_fwd, x.get_device(), x.data_ptr(), ldx, hpx, 1 if x.dtype is _BF16 else 0, n, h, q_heads, dh,
+            _p(q_gain), _p(k_gain), per_head, eps, positions.data_ptr(), _POS_KIND[positions.dtype], positions.stride(0),
+            inv_freq.data_ptr(), arr, len(arr), interleaved, y.data_ptr())
     return y
 
 
@@ -1871,19 +1897,20 @@ class _QkNormRotary(torch.autograd.Function):
         return _qk_norm_launch(x, q_gain, k_gain, positions, inv_freq, arr, q_heads, per_head, eps, interleaved)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         x, q_gain, k_gain, positions, inv_freq = ctx.saved_tensors
         arr, q_heads, per_head, eps, interleaved, want_q, want_k, wsb = ctx.meta
         n, h, dh = x.shape
+        ldx, hpx, _ = x.stride()
         dy = dy.contiguous()
         dx = torch.empty_like(dy)
         dq = torch.empty_like(q_gain) if want_q else None
         dk = torch.empty_like(k_gain) if want_k else None
         ws = _ws(wsb, x.device) if want_q or want_k else None
-        _launch(lib.tmae_qk_norm_rotary_bwd, x, x.data_ptr(), x.stride(0), x.stride(1), dy.data_ptr(), _dt(x), n, h, q_heads, dh,
-                _p(q_gain), _p(k_gain), per_head, eps, positions.data_ptr(), _POS_KIND[positions.dtype], positions.stride(0),
-                inv_freq.data_ptr(), arr, len(arr), interleaved, dx.data_ptr(), _p(dq), _p(dk), _p(ws), wsb)
+        _launch(lib.tmae_qk_norm_rotary_bwd, x.get_device(), x.data_ptr(), ldx, hpx, dy.data_ptr(), 1 if x.dtype is _BF16 else 0, n, h,
+                q_heads, dh, _p(q_gain), _p(k_gain), per_head, eps, positions.data_ptr(), _POS_KIND[positions.dtype],
+                positions.stride(0), inv_freq.data_ptr(), arr, len(arr), interleaved, dx.data_ptr(), _p(dq), _p(dk), _p(ws), wsb)
         return dx, dq, dk, None, None, None, None, None, None, None, None
 
 
@@ -1933,27 +1960,26 @@ class _WinAttnDot(torch.autograd.Function):
         return _win_attn_dot_launch(a, b, c, grid_q, grid_k, worklist, meta)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
         a, b, c, grid_q, grid_k, worklist = ctx.saved_tensors
-        c = 'kv' if ctx.packed_kv else c
-        d, nhead, batch, ny, nx, do_shift, scale, covered = ctx.meta
-        mq, mk = a.shape[0], (a if b is None else b).shape[0]
+        if ctx.packed_kv:
+            c = 'kv'
+        d, nhead, batch, ny, nx, do_shift, scale, covered, dtype, mq, mk, dh = ctx.meta
         dout = dout.contiguous()
         alloc = torch.empty_like if covered else torch.zeros_like
         da = alloc(a)
         db = alloc(b) if b is not None else None
         dc = alloc(c) if torch.is_tensor(c) else c
-        _launch(lib.tmae_win_attn_dot_bwd, a, *_WinAttn._ptrs(a, b, c, d), dout.data_ptr(), d, _dt(a), mq, mk, nhead, d // nhead,
+        _launch(lib.tmae_win_attn_dot_bwd, a.get_device(), *_WinAttn._ptrs(a, b, c, d), dout.data_ptr(), d, dtype, mq, mk, nhead, dh,
                 grid_q.data_ptr(), grid_k.data_ptr(), batch, ny, nx, do_shift, scale, *_WinAttn._ptrs(da, db, dc, d), _p(worklist))
         return da, db, (dc if torch.is_tensor(dc) else None), None, None, None, None
 
 
 def _win_attn_dot_launch(a, b, c, grid_q, grid_k, worklist, meta):
-    d, nhead, batch, ny, nx, do_shift, scale, covered = meta
-    mq, mk = a.shape[0], (a if b is None else b).shape[0]
+    d, nhead, batch, ny, nx, do_shift, scale, covered, dtype, mq, mk, dh = meta
     out = (torch.empty if covered else torch.zeros)((mq, d), dtype=a.dtype, device=a.device)
-    _launch(lib.tmae_win_attn_dot_fwd, a, *_WinAttn._ptrs(a, b, c, d), _dt(a), mq, mk, nhead, d // nhead, grid_q.data_ptr(),
+    _launch(lib.tmae_win_attn_dot_fwd, a.get_device(), *_WinAttn._ptrs(a, b, c, d), dtype, mq, mk, nhead, dh, grid_q.data_ptr(),
             grid_k.data_ptr(), batch, ny, nx, do_shift, scale, out.data_ptr(), d, _p(worklist))
     return out
 
@@ -2000,7 +2026,8 @@ def win_attn_dot(a, b, c, grid_q, grid_k, nhead, batch, ny, nx, do_shift, scale=
     a = a.contiguous()
     b = None if b is None else b.contiguous()
     c = c.contiguous() if torch.is_tensor(c) else c
-    meta = (d, nhead, batch, ny, nx, 1 if do_shift else 0, scale, bool(covered))
+    meta = (d, nhead, batch, ny, nx, 1 if do_shift else 0, scale, bool(covered), _dt(a), a.shape[0], (a if b is None else b).shape[0],
+            d // nhead)
     if _grad_on(*tensors):
         return _WinAttnDot.apply(a, b, c, grid_q, grid_k, worklist, meta)
     return _win_attn_dot_launch(a, b, c, grid_q, grid_k, worklist, meta)

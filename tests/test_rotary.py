@@ -353,3 +353,34 @@ def test_gradients_are_the_same_every_time_and_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, step(fresh))), k
+
+
+@pytest.mark.gpu
+def test_a_second_derivative_is_refused():
+    from tmae_amd import ops
+    x = torch.randn(9, 2, 16, device='cuda', requires_grad=True)
+    pos, f = torch.randint(0, 99, (9, 1), device='cuda'), ops.rotary_freqs((8,), device='cuda')
+    for y in (ops.rotary_axes(x, pos, f, (8,)), ops.qk_norm_rotary(x, None, None, pos, f, (8,))):
+        dx, = torch.autograd.grad(y.sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match='once_differentiable'):
+            (y.sum() + dx.sum()).backward()
+
+
+@pytest.mark.gpu
+def test_rows_beyond_32_bits():
+    """9 M tokens of 8 + 8 heads of 16 in bfloat16, 2^31 elements and more: the last tokens' results are those of the last tokens alone."""
+    from tmae_amd import ops
+    n, h, dh, sec, last = 9_000_000, 16, 16, (4, 4), 1000
+    g = torch.Generator(device='cuda').manual_seed(1)
+    x, dy = (torch.randn(n, h, dh, generator=g, device='cuda', dtype=torch.bfloat16) for _ in range(2))
+    assert x.numel() > 2 ** 31
+    pos = torch.randint(0, 468, (n, 2), generator=g, device='cuda', dtype=torch.int32)
+    f = ops.rotary_freqs(sec, device='cuda')
+    gain = torch.rand(dh, generator=g, device='cuda') + 0.5
+
+    def run(x, dy, pos):
+        x = x.detach().requires_grad_()
+        r, y = ops.rotary_axes(x, pos, f, sec), ops.qk_norm_rotary(x, gain, gain, pos, f, sec)
+        return [t.detach() for t in (r, y, *torch.autograd.grad(r, x, dy), *torch.autograd.grad(y, x, dy))]
+    for a, b in zip(run(x, dy, pos), run(x[-last:], dy[-last:], pos[-last:])):
+        assert torch.equal(a[-last:], b)

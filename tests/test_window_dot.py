@@ -465,3 +465,64 @@ def test_model_step_with_the_options(amp):
             # (a bias of all keys moves every logit of a query alike where no rotation stands between: not so here)
             assert p.grad.abs().max() > 0, n
     assert seen >= 16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_an_infinite_value_stays_an_infinity(dtype):
+    """v_j = inf in a channel: that channel of every query of the window is inf (all probabilities are above 0), the others are finite;
+    dO_i = inf: the same of dV.  The bad token is the first of its window, which the slots behind the last one stand for."""
+    from tmae_amd import ops
+    g = torch.Generator().manual_seed(6)
+    for dh, h in ((16, 5), (32, 2), (64, 2)):
+        for count in (40, 300, 900, 1600):                                              # 1 to 64 tokens a window
+            grid, at = place([count], 1, 40, 40, g)
+            gr = grid.cuda()
+            win = window_of(at, False)
+            first = torch.stack([(win == w).nonzero()[0, 0] for w in win.unique()])
+            touched = torch.zeros(count, h * dh, dtype=torch.bool)
+            touched[:, dh + 3] = True
+            q, k, v, do = (torch.randn(count, h * dh, generator=g).to(dtype) for _ in range(4))
+            bad_v, bad_do = v.clone(), do.clone()
+            bad_v[first, dh + 3] = float('inf')
+            bad_do[first, dh + 3] = float('inf')
+            for worklist in (None, ops.window_worklist(gr, gr, 1, 40, 40, False)):
+                run = lambda v: ops.win_attn_dot(q.cuda(), k.cuda(), v, gr, gr, h, 1, 40, 40, False, worklist=worklist, covered=True)  # noqa: E731
+                o = run(bad_v.cuda()).cpu().float()
+                assert (o[touched] == float('inf')).all() and torch.isfinite(o[~touched]).all()
+                leaf = v.cuda().requires_grad_()
+                dv = torch.autograd.grad(run(leaf), leaf, bad_do.cuda())[0].cpu().float()
+                assert (dv[touched] == float('inf')).all() and torch.isfinite(dv[~touched]).all()
+
+
+@pytest.mark.gpu
+def test_a_second_derivative_is_refused():
+    from tmae_amd import ops
+    grid = torch.arange(64, dtype=torch.int32, device='cuda')
+    x = torch.randn(64, 48, device='cuda', requires_grad=True)
+    o = ops.win_attn_dot(x, None, None, grid, grid, 1, 1, 8, 8, False)
+    dx, = torch.autograd.grad(o.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match='once_differentiable'):
+        (o.sum() + dx.sum()).backward()
+
+
+@pytest.mark.gpu
+def test_rows_beyond_32_bits():
+    """2.25 M rows of 2048 bytes: the last frame's results are those of the last frame alone."""
+    from tmae_amd import ops
+    batch, ny, nx, h, dh = 9, 500, 500, 8, 64
+    cells, d = ny * nx, h * dh
+    g = torch.Generator(device='cuda').manual_seed(1)
+    qk, v, do = (torch.randn(batch * cells, w, generator=g, device='cuda', dtype=torch.bfloat16) for w in (2 * d, d, d))
+    assert qk.numel() * 2 > 2 ** 32
+    grid = torch.arange(batch * cells, dtype=torch.int32, device='cuda')
+
+    def run(qk, v, do, grid, batch):
+        leaves = [t.detach().requires_grad_() for t in (qk, v)]
+        o = ops.win_attn_dot(*leaves, None, grid, grid, h, batch, ny, nx, True, covered=True,
+                             worklist=ops.window_worklist(grid, grid, batch, ny, nx, True))
+        return [t.detach() for t in (o, *torch.autograd.grad(o, leaves, do))]
+    whole = run(qk, v, do, grid, batch)
+    alone = run(qk[-cells:], v[-cells:], do[-cells:], grid[:cells], 1)
+    for a, b in zip(whole, alone):
+        assert torch.equal(a[-cells:], b)
