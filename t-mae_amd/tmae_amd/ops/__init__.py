@@ -1788,7 +1788,11 @@ def _once(backward):
 
 
 def _grad_on(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 _POS_KIND = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
@@ -1914,6 +1918,16 @@ class _QkNormRotary(torch.autograd.Function):
         return dx, dq, dk, None, None, None, None, None, None, None, None
 
 
+def _head_gain(name, side, gain, x, heads, per_head):
+    if gain.dtype is not torch.float32 or gain.device != x.device:
+        raise TypeError(f'{name}: {side} is float32 on {x.device}, got {gain.dtype} on {gain.device}')
+    dh = x.shape[2]
+    if gain.shape != ((heads, dh) if per_head else (dh,)):
+        raise ValueError(f'{name}: {side} {tuple(gain.shape)} for {heads} heads of {dh} channels; gains of one kind, [channels] or '
+                         f'[heads, channels], for both sides')
+    return gain.contiguous()
+
+
 def qk_norm_rotary(x, q_gain, k_gain, positions, inv_freq, sections, q_heads=None, eps=1e-6, interleaved=False):
     """The norm of every head of x [tokens, heads, channels] and the rotation of rotary_axes in one pass:
     rotate(gain * x * rsqrt(mean(x^2) + eps)), statistics in float32, one rounding to x's type.
@@ -1933,23 +1947,15 @@ def qk_norm_rotary(x, q_gain, k_gain, positions, inv_freq, sections, q_heads=Non
         raise ValueError(f'{name}: q_heads {q_heads} of {h} heads')
     if not 0.0 <= float(eps) < float('inf'):
         raise ValueError(f'{name}: eps {eps}')
-    per_head = {g.dim() for g in (q_gain, k_gain) if g is not None}
-    if len(per_head) > 1:
-        raise ValueError(f'{name}: gains of one kind, [channels] or [heads, channels], for both sides')
-    per_head = int(per_head == {2})
-    gains = []
-    for side, gain, heads in (('q_gain', q_gain, q_heads), ('k_gain', k_gain, h - q_heads)):
-        if gain is not None:
-            if gain.dtype != torch.float32 or gain.device != x.device:
-                raise TypeError(f'{name}: {side} is float32 on {x.device}, got {gain.dtype} on {gain.device}')
-            if tuple(gain.shape) != ((heads, dh) if per_head else (dh,)):
-                raise ValueError(f'{name}: {side} {tuple(gain.shape)} for {heads} heads of {dh} channels')
-            gain = gain.contiguous()
-        gains.append(gain)
+    per_head = int((q_gain is not None and q_gain.dim() == 2) or (k_gain is not None and k_gain.dim() == 2))
+    if q_gain is not None:
+        q_gain = _head_gain(name, 'q_gain', q_gain, x, q_heads, per_head)
+    if k_gain is not None:
+        k_gain = _head_gain(name, 'k_gain', k_gain, x, h - q_heads, per_head)
     _need_cuda(x)
-    if _grad_on(x, *gains):
-        return _QkNormRotary.apply(x, *gains, positions, inv_freq, arr, pairs, q_heads, per_head, float(eps), int(bool(interleaved)))
-    return _qk_norm_launch(x, *gains, positions, inv_freq, arr, q_heads, per_head, float(eps), int(bool(interleaved)))
+    if _grad_on(x, q_gain, k_gain):
+        return _QkNormRotary.apply(x, q_gain, k_gain, positions, inv_freq, arr, pairs, q_heads, per_head, float(eps), int(bool(interleaved)))
+    return _qk_norm_launch(x, q_gain, k_gain, positions, inv_freq, arr, q_heads, per_head, float(eps), int(bool(interleaved)))
 
 
 class _WinAttnDot(torch.autograd.Function):
@@ -1976,6 +1982,11 @@ class _WinAttnDot(torch.autograd.Function):
         return da, db, (dc if torch.is_tensor(dc) else None), None, None, None, None
 
 
+@functools.lru_cache(maxsize=64)
+def _worklist_size(batch, ny, nx):
+    return lib.tmae_window_worklist_size(batch, ny, nx)
+
+
 def _win_attn_dot_launch(a, b, c, grid_q, grid_k, worklist, meta):
     d, nhead, batch, ny, nx, do_shift, scale, covered, dtype, mq, mk, dh = meta
     out = (torch.empty if covered else torch.zeros)((mq, d), dtype=a.dtype, device=a.device)
@@ -1994,40 +2005,54 @@ def win_attn_dot(a, b, c, grid_q, grid_k, nhead, batch, ny, nx, do_shift, scale=
     in one cell.  worklist: window_worklist of the same grids and shift; without one every window is visited.  covered: the caller's
     promise that every row stands in the grids -- without it the results start from zeros and the others stay zero."""
     name = 'win_attn_dot'
-    layout = 'qkv' if b is None else 'qk_v' if c is None else 'q_kv' if isinstance(c, str) else 'q_k_v'
-    if (b is None and c is not None) or (layout == 'q_kv' and c != 'kv'):
+    if b is None:
+        layout, tensors, parts = 'q|k|v', (a,), 3
+    elif c is None:
+        layout, tensors, parts = 'q|k, v', (a, b), 2
+    elif isinstance(c, str):
+        layout, tensors, parts = 'q, k|v', (a, b), 1
+    else:
+        layout, tensors, parts = 'q, k, v', (a, b, c), 1
+    if (b is None and c is not None) or (layout == 'q, k|v' and c != 'kv'):
         raise ValueError(f'{name}: a, b and c are (q|k|v), (q|k, v), (q, k, v) or (q, k|v, "kv")')
-    tensors = [t for t in (a, b, c) if torch.is_tensor(t)]
-    if any(t.dim() != 2 or t.dtype != a.dtype or t.device != a.device for t in tensors):
-        raise ValueError(f'{name}: rows of one type on one device expected, got '
-                         f'{[(tuple(t.shape), t.dtype, str(t.device)) for t in tensors]}')
-    _dt(a)
-    d = a.shape[1] // {'qkv': 3, 'qk_v': 2}.get(layout, 1)
-    want = {'qkv': (3 * d,), 'qk_v': (2 * d, d), 'q_kv': (d, 2 * d), 'q_k_v': (d, d, d)}[layout]
-    if tuple(t.shape[1] for t in tensors) != want or (layout == 'qk_v' and a.shape[0] != b.shape[0]) or \
-            (layout == 'q_k_v' and b.shape[0] != c.shape[0]):
+    device, most = a.device, 0
+    for t in tensors:
+        if t.dim() != 2 or t.dtype is not a.dtype or t.device != device:
+            raise ValueError(f'{name}: rows of one type on one device expected, got '
+                             f'{[(tuple(t.shape), t.dtype, str(t.device)) for t in tensors]}')
+        most = max(most, t.shape[0])
+    dtype = _dt(a)
+    mq, d = a.shape
+    if d % parts == 0:
+        d //= parts
+    mk = mq if b is None else b.shape[0]
+    if (a.shape[1] != parts * d or (b is not None and b.shape[1] != (2 * d if layout == 'q, k|v' else d)) or
+            (layout == 'q|k, v' and mk != mq) or (layout == 'q, k, v' and c.shape != b.shape)):
         raise ValueError(f'{name}: {[tuple(t.shape) for t in tensors]} are not the rows of {layout}')
     nhead, batch, ny, nx = int(nhead), int(batch), int(ny), int(nx)
-    if nhead < 1 or nhead > 4096 or d not in (16 * nhead, 32 * nhead, 64 * nhead):
+    dh = d // nhead if nhead > 0 else 0
+    if nhead < 1 or nhead > 4096 or dh not in (16, 32, 64) or d != dh * nhead:
         raise ValueError(f'{name}: {d} channels for {nhead} heads; heads have 16, 32 or 64')
-    scale = float((d // nhead) ** -0.5 if scale is None else scale)
+    scale = float(dh ** -0.5 if scale is None else scale)
     if not 0.0 < scale <= 3e38:
         raise ValueError(f'{name}: scale {scale}')
-    if batch < 1 or ny < 1 or nx < 1 or batch * ny * nx >= 1 << 31 or max(t.shape[0] for t in tensors) >= 1 << 31:
+    cells = batch * ny * nx
+    if batch < 1 or ny < 1 or nx < 1 or cells >= 1 << 31 or most >= 1 << 31:
         raise ValueError(f'{name}: batch {batch}, grid {ny} x {nx}')
     for g, what in ((grid_q, 'grid_q'), (grid_k, 'grid_k')):
-        if g.dtype != torch.int32 or g.numel() != batch * ny * nx or not g.is_contiguous() or g.device != a.device:
-            raise ValueError(f'{name}: {what} [{batch * ny * nx}] int32 on {a.device} expected, got {tuple(g.shape)} {g.dtype} on {g.device}')
+        if g.dtype is not torch.int32 or g.numel() != cells or not g.is_contiguous() or g.device != device:
+            raise ValueError(f'{name}: {what} [{cells}] int32 on {device} expected, got {tuple(g.shape)} {g.dtype} on {g.device}')
     if worklist is not None:
-        if worklist.dtype != torch.int32 or not worklist.is_contiguous() or worklist.device != a.device or \
-                worklist.numel() != lib.tmae_window_worklist_size(batch, ny, nx):
+        if worklist.dtype is not torch.int32 or not worklist.is_contiguous() or worklist.device != device or \
+                worklist.numel() != _worklist_size(batch, ny, nx):
             raise ValueError(f'{name}: the work list is not one of {batch} grids of {ny} x {nx}')
     _need_cuda(a)
     a = a.contiguous()
-    b = None if b is None else b.contiguous()
-    c = c.contiguous() if torch.is_tensor(c) else c
-    meta = (d, nhead, batch, ny, nx, 1 if do_shift else 0, scale, bool(covered), _dt(a), a.shape[0], (a if b is None else b).shape[0],
-            d // nhead)
+    if b is not None:
+        b = b.contiguous()
+        if layout == 'q, k, v':
+            c = c.contiguous()
+    meta = (d, nhead, batch, ny, nx, 1 if do_shift else 0, scale, bool(covered), dtype, mq, mk, dh)
     if _grad_on(*tensors):
         return _WinAttnDot.apply(a, b, c, grid_q, grid_k, worklist, meta)
     return _win_attn_dot_launch(a, b, c, grid_q, grid_k, worklist, meta)
