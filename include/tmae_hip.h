@@ -637,8 +637,8 @@ int tmae_qk_norm_rotary_bwd(const void* x, int64_t ldx, int64_t hpx, const void*
                             float* dq_gain, float* dk_gain, void* ws, size_t ws_bytes, void* stream);
 
 /* ---- scaled-dot-product attention inside 8x8 windows -- layouts, grids, shift and work list of tmae_win_attn_fwd / _bwd; the logits
- * are scale * q . k (scale > 0), any number of heads, dh in {16, 32, 64}.  Every
- * base and row pitch is a multiple of 16 bytes.  The backward needs the forward's inputs only.
+ * are scale * q . k (scale > 0), up to 4096 heads, dh in {16, 32, 64}.  Every base and row pitch is a multiple of 16 bytes, a pitch
+ * below 2^28 elements.  The backward needs the forward's inputs only.
  * Every row that stands in a grid is written: zero rows where its window has no key (for dk / dv: no query).  A grid entry that is no
  * row of its tensor counts as an empty cell.  worklist (may be NULL: every window is visited) is of these grids and this shift. */
 int tmae_win_attn_dot_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, int dtype, int64_t mq,

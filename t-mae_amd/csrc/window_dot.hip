@@ -5,12 +5,19 @@
 //   rows that lie apart, took longer to write and read than the row maxima and sums take to compute again):
 //   dV_j = sum_i P_ij dO_i,  dP_ij = dO_i . v_j,  dS_ij = scale P_ij (dP_ij - sum_j P_ij dP_ij),  dQ_i = sum_j dS_ij k_j,  dK_j = sum_i dS_ij q_i
 //
-// One wavefront per (window, head), tiles of 16 tokens on the float32 matrix instruction 16x16x4.  Its accumulator layout -- lane
-// (g, i) = (lane >> 4, lane & 15) holds rows 4g .. 4g+3 of column i -- is also what its B operand takes, row 4g + r in step r: the
-// probabilities go from one product into the next without leaving the registers.  Which of the two products' orders is wanted (the
-// query or the key in the column) is had by exchanging the operands.
+// Tiles of 16 tokens.  A logit tile is computed with the keys as its rows and the queries as its columns: the accumulators' layout --
+// lane (g, i) = (lane >> 4, lane & 15) holds rows 4g .. 4g+3 of column i -- is also what the next product takes as its B operand, row
+// 4g + r in step r, so that the probabilities go into it without leaving the registers (float32 whole, bfloat16 rounded once).
 //
-// A slot without a token stands for the window's first one: it is read, its probability is set to 0, and nothing is stored for it.
+// Bound: HBM, at 8 to 20 FLOPs a byte; but rows lie apart and windows are small, so what costs is getting rows in and out.  The lanes of an
+// operand stand in 16 rows: read straight into that layout, an instruction touches some 44 lines.  Rows therefore travel in 16-byte
+// pieces, whole pieces of a line by neighbouring lanes, through LDS images; all of a window's rows are requested at once.  Padding rows to
+// tiles is what the matrix unit pays for; three sizes of windows (up to 16, 32 and 64 tokens) keep it small.  Eight frames at stage 1
+// (375 k tokens, 8 heads of 16, bfloat16): forward 108 us, backward 75 + 120 us -- 4.0, 3.4 and 4.2 TB/s of counted HBM traffic; the
+// movement alone, without the arithmetic, takes 59 + 99 us of the backward.
+//
+// A slot behind a window's last token stands for its first one: it is read, its probability is set to 0 (and V and dO are zeros there,
+// which an infinity next to them needs), and nothing is stored for it.
 #include "common.h"
 #include <type_traits>
 
@@ -38,8 +45,8 @@ __device__ __forceinline__ char* row_of(const void* base, int token, unsigned pi
   return (char*)base + (unsigned long long)(unsigned)token * pitch;
 }
 
-// LDS operations of a wave execute in order: this keeps the compiler to the order they are written in.  Every wave works in a piece of
-// LDS of its own; no workgroup barrier is needed anywhere.
+// LDS operations of a wave execute in order: this keeps the compiler to the order they are written in.  In bfloat16 every wave works in
+// a piece of LDS of its own, without a workgroup barrier.
 __device__ __forceinline__ void order_lds() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
@@ -135,7 +142,8 @@ struct Walk {
 // Four waves of a workgroup share the windows of up to 16 NT tokens: NT of them the tiles of one head, 4 / NT heads at a time -- 64 rows
 // of each tensor in LDS whatever the window's size.  A wave takes one tile of queries (out, dQ and the rows' maxima, sums and sum_j P dP),
 // then, in the backward, one tile of keys (dK, dV).  Operands come from LDS: pieces of rows for the products over the channels, single
-// values of four rows for those over the tokens.
+// values of four rows for those over the tokens.  One frame of stage 2 (16 k tokens, 8 heads of 32): forward 21 us, backward 47 us; a wave
+// for a whole (window, head), its rows read straight into the operands' layout, took 125 us for both.
 __device__ __forceinline__ float lanes4_sum(float v) { v += __shfl_xor(v, 16, 64); return v + __shfl_xor(v, 32, 64); }
 __device__ __forceinline__ float lanes4_max(float v) { v = fmaxf(v, __shfl_xor(v, 16, 64)); return fmaxf(v, __shfl_xor(v, 32, 64)); }
 
@@ -991,8 +999,8 @@ template <int DH, bool BWD, int ROLES> int launch_roles(const DotArgs& a, const 
 }
 // One launch for all windows, or one for those of more than 32 tokens and one for the others.  One overlaps the ends of the parts and
 // costs a launch less, but every workgroup then has the registers and LDS of the largest part.  Eight frames at stage 1 (375 k tokens, 8
-// heads of 16): forward 109 us in one launch against 114, backward 206 against 193; stage 2 (8 heads of 32): forward 45 against 42,
-// backward 90 against 84.  Few tokens: the launch counts.
+// heads of 16): forward 109 us in one launch against 114, backward 206 against 193; stage 2 (33 k queries, 131 k keys, 8 heads of 32):
+// forward 45 against 42, backward 90 against 84.  Few tokens: the launch counts.
 template <int DH, bool BWD> int launch_bf16(const DotArgs& a, const Orphans& z, hipStream_t stream) {
   if (!a.wl) return launch_roles<DH, BWD, ROLE4>(a, z, a.nwin, 0, 0, stream);
   const int64_t w4 = class_windows(a, 3), w2 = class_windows(a, 2), w1 = class_windows(a, 0);

@@ -3,7 +3,7 @@ q/k norms + rotation -> attention as an encoder layer runs it.
 
 Tolerances (u = 2^-24, e = eps / 2 of the stored type, bf16 2^-8; T = 64 tokens of a window at most).  Per query, A = the largest
 scale * sum |q_c k_c| of its keys:
- * a logit is off by (dh + 4) u A; the exponent's argument and the saved logarithm round once more each (of a size up to A + 6): a
+ * a logit is off by (dh + 4) u A; the exponent's argument and the sum's reciprocal round once more each (of a size up to A + 6): a
    probability is off by rho = 2 (dh + 8) u (A + 6) + (T + 16) u of itself, and by e more where it is rounded to the type for a product;
  * out: (rho + e + 4 T u) sum_j P |v| + e |out|;          dv: the same with sum_i P |dO|;
  * dS = scale P (dP - D), with G = sum |dO v| per pair and Dm = sum_j P G: off by
