@@ -441,14 +441,77 @@ template <int DH, int PITCH> struct Rows {
     return c;
   }
 };
-// c += A B over the 16 tokens of one tile, or over the 32 of two (a third tile rides with zeros: one accumulator goes through products
-// of one shape only -- a 16x16x16 right behind the 16x16x32 that it continues has read wrong values)
-__device__ __forceinline__ f32x4 over_tokens(const s16x4& a, const s16x4& b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
+// Probabilities and their gradients on the way into the products over the tokens.  Rounded: to bfloat16 once, an error of the size of the
+// result's own rounding.  Split: as the sum of two bfloat16, 16 bits and more; the instruction takes 32 tokens, and where a tile has 16 the
+// low parts ride in its second half.  Probabilities are split towards 0 and the low part stays above it, so that an infinity in V or dO
+// meets two positive numbers.
+struct Rounded { s16x4 v; };
+struct Split { s16x4 hi, lo; };
+template <bool SPLIT> using Weights = typename std::conditional<SPLIT, Split, Rounded>::type;
+template <bool SPLIT> __device__ __forceinline__ Weights<SPLIT> probabilities(const f32x4& p) {
+  if constexpr (SPLIT) {
+    u32x4 cut;
+    f32x4 rest;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      cut[r] = __float_as_uint(p[r]) & 0xffff0000u;
+      rest[r] = larger(p[r] - __uint_as_float(cut[r]), 1e-37f);
+    }
+    return Split{__builtin_bit_cast(s16x4, u32x2{cut[0] >> 16 | cut[1], cut[2] >> 16 | cut[3]}), pack4(rest)};
+  } else {
+    return Rounded{pack4(p)};
+  }
 }
-__device__ __forceinline__ f32x4 over_tokens(const s16x4& a0, const s16x4& a1, const s16x4& b0, const s16x4& b1, f32x4 c) {
+template <bool SPLIT> __device__ __forceinline__ Weights<SPLIT> gradients(const f32x4& d) {
+  if constexpr (SPLIT) {
+    const u32x2 h = {pack2(d[0], d[1]), pack2(d[2], d[3])};
+    const f32x4 near = {__uint_as_float(h[0] << 16), __uint_as_float(h[0] & 0xffff0000u), __uint_as_float(h[1] << 16), __uint_as_float(h[1] & 0xffff0000u)};
+    return Split{__builtin_bit_cast(s16x4, h), pack4(d - near)};
+  } else {
+    return Rounded{pack4(d)};
+  }
+}
+__device__ __forceinline__ f32x4 product32(const s16x4& a0, const s16x4& a1, const s16x4& b0, const s16x4& b1, f32x4 c) {
   const s16x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7), b = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// c += A B over the tokens of one tile
+__device__ __forceinline__ f32x4 over_tokens(const s16x4& a, const Rounded& b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b.v, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 over_tokens(const s16x4& a, const Split& b, f32x4 c) { return product32(a, a, b.hi, b.lo, c); }
+// A B over those of NK tiles (a third tile rides with zeros where nothing else does: one accumulator goes through products of one shape
+// only -- a 16x16x16 right behind the 16x16x32 that it continues has read wrong values)
+template <int NK> __device__ __forceinline__ f32x4 over_tiles(const s16x4* a, const Rounded* b) {
+  const s16x4 none = {0, 0, 0, 0};
+  f32x4 c = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (NK == 1) c = over_tokens(a[0], b[0], c);
+  else
+#pragma unroll
+    for (int k = 0; k < NK; k += 2) c = k + 1 < NK ? product32(a[k], a[k + 1], b[k].v, b[k + 1].v, c) : product32(a[k], none, b[k].v, none, c);
+  return c;
+}
+template <int NK> __device__ __forceinline__ f32x4 over_tiles(const s16x4* a, const Split* b) {
+  f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k + 1 < NK; k += 2) {
+    c = product32(a[k], a[k + 1], b[k].hi, b[k + 1].hi, c);
+    c = product32(a[k], a[k + 1], b[k].lo, b[k + 1].lo, c);
+  }
+  if constexpr (NK % 2 == 1) c = over_tokens(a[NK - 1], b[NK - 1], c);
+  return c;
+}
+// a tile of them, one column a lane, into LDS and out of it with rows and columns exchanged
+template <bool SPLIT> constexpr int WEIGHT_BYTES = SPLIT ? 2 * TILE_BYTES : TILE_BYTES;
+__device__ __forceinline__ void put_tile(char* tile, int g, int i, const Rounded& v) { *reinterpret_cast<s16x4*>(tile + i * TILE_PITCH + 8 * g) = v.v; }
+__device__ __forceinline__ void put_tile(char* tile, int g, int i, const Split& v) {
+  put_tile(tile, g, i, Rounded{v.hi});
+  put_tile(tile + TILE_BYTES, g, i, Rounded{v.lo});
+}
+template <bool SPLIT> __device__ __forceinline__ Weights<SPLIT> turned_tile(const char* tile, int g, int i) {
+  const char* at = tile + (4 * g + (i >> 2)) * TILE_PITCH + 8 * (i & 3);
+  if constexpr (SPLIT) return Split{read_columns(at), read_columns(at + TILE_BYTES)};
+  else return Rounded{read_columns(at)};
 }
 
 // ---- windows of more than 16 tokens: a wave per (window, head), four heads in a workgroup so that their pieces of a line meet in the cache.
@@ -496,7 +559,7 @@ template <int DH, int NT> struct Window {
 };
 
 // NK key tiles against nq query tiles.  NK is a template parameter, so that no branch stands between a matrix instruction and its reader.
-template <int DH, int NT, int NK>
+template <int DH, int NT, int NK, bool SPLIT>
 __device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq, const int* tk, int Tq, int Tk, int head, char* A,
                                            typename Window<DH, NT>::Loaded qrows) {
   using W = Window<DH, NT>;
@@ -506,12 +569,12 @@ __device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq, cons
   const int col = head * DH * 2;
   const char* V = A + W::IMAGE;
   typename R::Piece kf[NK];
-  s16x4 vc[NK][CT];
+  s16x4 vc[CT][NK];
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt) {
     kf[kt] = R::piece(A + kt * TILE, g, i);
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) vc[kt][ct] = R::columns(V + kt * TILE, g, i, ct);
+    for (int ct = 0; ct < CT; ++ct) vc[ct][kt] = R::columns(V + kt * TILE, g, i, ct);
   }
   order_lds();
   W::lay(A, qrows);
@@ -533,7 +596,7 @@ __device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq, cons
       for (int r = 0; r < 4; ++r) mx = larger(mx, st[kt][r]);
     mx = column_max(mx) * c;
     float l = 0.f;
-    s16x4 p[NK];
+    Weights<SPLIT> p[NK];
 #pragma unroll
     for (int kt = 0; kt < NK; ++kt) {
 #pragma unroll
@@ -541,18 +604,12 @@ __device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq, cons
         st[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[kt][r], c, -mx));
         l += st[kt][r];
       }
-      p[kt] = pack4(st[kt]);
+      p[kt] = probabilities<SPLIT>(st[kt]);
     }
     l = column_sum(l);
     f32x4 o[CT];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      o[ct] = zero;
-      if constexpr (NK >= 2) o[ct] = over_tokens(vc[0][ct], vc[1][ct], p[0], p[1], o[ct]);
-      if constexpr (NK == 4) o[ct] = over_tokens(vc[2][ct], vc[3][ct], p[2], p[3], o[ct]);
-      if constexpr (NK == 3) o[ct] = over_tokens(vc[2][ct], s16x4{0, 0, 0, 0}, p[2], s16x4{0, 0, 0, 0}, o[ct]);
-      if constexpr (NK == 1) o[ct] = over_tokens(vc[0][ct], p[0], o[ct]);
-    }
+    for (int ct = 0; ct < CT; ++ct) o[ct] = over_tiles<NK>(vc[ct], p);
     const float il = __builtin_amdgcn_rcpf(l);
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) o[ct] *= il;
@@ -562,12 +619,12 @@ __device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq, cons
   W::store(a.o, a.po, tq, Tq, col, A);
 }
 
-template <int DH, int NT, int NK>
+template <int DH, int NT, int NK, bool SPLIT>
 __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, const int* tk, int Tq, int Tk, int head, char* A,
                                            typename Window<DH, NT>::Loaded grows, char* tiles) {
   using W = Window<DH, NT>;
   using R = typename W::R;
-  constexpr int CT = W::CT, TILE = W::TILE, TP = TILE_PITCH;
+  constexpr int CT = W::CT, TILE = W::TILE;
   const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15, nq = (Tq + 15) >> 4;
   const int col = head * DH * 2;
   char *B = A + W::IMAGE, *C = B + W::IMAGE;
@@ -620,27 +677,28 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
       }
     const float il = __builtin_amdgcn_rcpf(column_sum(qt * 16 + i < Tq ? l : INFINITY));        // no query: P = 0
     d = column_sum(d) * il * -a.scale;
-    s16x4 ds[NK];
+    Weights<SPLIT> ds[NK];
+    constexpr int AT_ONCE = SPLIT ? 1 : 2, WB = WEIGHT_BYTES<SPLIT>;                // key tiles that the LDS tiles hold
 #pragma unroll
-    for (int k0 = 0; k0 < NK; k0 += 2) {
+    for (int k0 = 0; k0 < NK; k0 += AT_ONCE) {
 #pragma unroll
-      for (int kt = k0; kt < (k0 + 2 < NK ? k0 + 2 : NK); ++kt) {
+      for (int kt = k0; kt < (k0 + AT_ONCE < NK ? k0 + AT_ONCE : NK); ++kt) {
         f32x4 t;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           p[kt][r] *= il;
           t[r] = p[kt][r] * __builtin_fmaf(dp[kt][r], a.scale, d);
         }
-        ds[kt] = pack4(t);
-        char* tile = tiles + (kt - k0) * 2 * TILE_BYTES;
-        *reinterpret_cast<s16x4*>(tile + i * TP + 8 * g) = pack4(p[kt]);
-        *reinterpret_cast<s16x4*>(tile + TILE_BYTES + i * TP + 8 * g) = ds[kt];
+        ds[kt] = gradients<SPLIT>(t);
+        char* tile = tiles + (kt - k0) * 2 * WB;
+        put_tile(tile, g, i, probabilities<SPLIT>(p[kt]));
+        put_tile(tile + WB, g, i, ds[kt]);
       }
       order_lds();
 #pragma unroll
-      for (int kt = k0; kt < (k0 + 2 < NK ? k0 + 2 : NK); ++kt) {
-        const char* tile = tiles + (kt - k0) * 2 * TILE_BYTES + (4 * g + (i >> 2)) * TP + 8 * (i & 3);
-        const s16x4 pt = read_columns(tile), dt = read_columns(tile + TILE_BYTES);               // queries 4g .. of key i
+      for (int kt = k0; kt < (k0 + AT_ONCE < NK ? k0 + AT_ONCE : NK); ++kt) {
+        const char* tile = tiles + (kt - k0) * 2 * WB;
+        const Weights<SPLIT> pt = turned_tile<SPLIT>(tile, g, i), dt = turned_tile<SPLIT>(tile + WB, g, i);      // queries 4g .. of key i
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
           dv[kt][ct] = over_tokens(gc[ct], pt, dv[kt][ct]);
@@ -652,14 +710,10 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
     f32x4 dq[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      dq[ct] = zero;
       s16x4 kc[NK];
 #pragma unroll
       for (int kt = 0; kt < NK; ++kt) kc[kt] = R::columns(A + kt * TILE, g, i, ct);
-      if constexpr (NK >= 2) dq[ct] = over_tokens(kc[0], kc[1], ds[0], ds[1], dq[ct]);
-      if constexpr (NK == 4) dq[ct] = over_tokens(kc[2], kc[3], ds[2], ds[3], dq[ct]);
-      if constexpr (NK == 3) dq[ct] = over_tokens(kc[2], s16x4{0, 0, 0, 0}, ds[2], s16x4{0, 0, 0, 0}, dq[ct]);
-      if constexpr (NK == 1) dq[ct] = over_tokens(kc[0], ds[0], dq[ct]);
+      dq[ct] = over_tiles<NK>(kc, ds);
     }
     R::put(C + qt * TILE, g, i, dq);
   }
@@ -678,7 +732,7 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
 // Windows of up to 16 NT tokens; without a work list (NT = 4) every window, empty ones included.  Two waves per SIMD as the bound: 256
 // registers at most, and the matrix instructions then write plain vector registers (the backward of 64 channels by 64 tokens needs more).
 template <int DH, int NT, bool BWD> constexpr int window_lds() { return (BWD ? 3 : 2) * Window<DH, NT>::IMAGE + (BWD ? 4 * TILE_BYTES : 0); }
-template <int DH, int NT, bool BWD> __device__ __forceinline__ void window_role(const DotArgs& a, int first, int step, int head, int (*toks)[64], char* A) {
+template <int DH, int NT, bool BWD, bool SPLIT> __device__ __forceinline__ void window_role(const DotArgs& a, int first, int step, int head, int (*toks)[64], char* A) {
   using W = Window<DH, NT>;
   const int lane = threadIdx.x & 63;
   if (head >= a.nhead) return;
@@ -711,8 +765,8 @@ template <int DH, int NT, bool BWD> __device__ __forceinline__ void window_role(
     if constexpr (BWD && LATE) grows = W::request(a.g, a.pg, toks[0], col);
     const int nk = (Tk + 15) >> 4;
 #define ONE(NK)                                                                                                                            \
-  if constexpr (BWD) bwd_window<DH, NT, NK>(a, toks[0], toks[1], Tq, Tk, head, A, grows, A + 3 * W::IMAGE);                                \
-  else fwd_window<DH, NT, NK>(a, toks[0], toks[1], Tq, Tk, head, A, qrows)
+  if constexpr (BWD) bwd_window<DH, NT, NK, SPLIT>(a, toks[0], toks[1], Tq, Tk, head, A, grows, A + 3 * W::IMAGE);                                \
+  else fwd_window<DH, NT, NK, SPLIT>(a, toks[0], toks[1], Tq, Tk, head, A, qrows)
     if (nk == 1) { ONE(1); }
     else if (NT == 2 || nk == 2) { ONE(2); }
     else if constexpr (NT == 4) {
@@ -728,8 +782,8 @@ template <int DH, int NT, bool BWD> __device__ __forceinline__ void window_role(
 constexpr int SMALL_PITCH = 144;           // 128 bytes of a row
 
 // HALF: at most 8 tokens, one load brings a tensor's rows (rows 8 .. 15 then hold them once more)
-template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_window(const DotArgs& a, const int (*toks)[64], int Tq, int Tk, int head0, char* K) {
-  constexpr int HG = 64 / DH, PITCH = SMALL_PITCH, IMAGE = 16 * PITCH, NI = BWD ? 4 : 3, TP = TILE_PITCH;
+template <int DH, bool BWD, bool SPLIT, bool HALF> __device__ __forceinline__ void small_window(const DotArgs& a, const int (*toks)[64], int Tq, int Tk, int head0, char* K) {
+  constexpr int HG = 64 / DH, PITCH = SMALL_PITCH, IMAGE = 16 * PITCH, NI = BWD ? 4 : 3;
   using R = Rows<DH, PITCH>;
   constexpr int CT = R::CT;
   const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
@@ -768,7 +822,8 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
 #pragma unroll
   for (int r = 0; r < 4; ++r) absent[r] = 4 * g + r < Tk ? 0.f : -INFINITY;
   if constexpr (!BWD) {
-    s16x4 vc[HG][CT], p[HG];
+    s16x4 vc[HG][CT];
+    Weights<SPLIT> p[HG];
     f32x4 st[HG];
     float mx[HG], l[HG];
 #pragma unroll
@@ -786,7 +841,7 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
         st[h][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[h][r], c, -mx[h]));
         l[h] += st[h][r];
       }
-      p[h] = pack4(st[h]);
+      p[h] = probabilities<SPLIT>(st[h]);
     }
 #pragma unroll
     for (int h = 0; h < HG; ++h) {
@@ -807,8 +862,10 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
       }
     }
   } else {
-    s16x4 kc[HG][CT], qc[HG][CT], gc[HG][CT], ds[HG];
+    s16x4 kc[HG][CT], qc[HG][CT], gc[HG][CT];
+    Weights<SPLIT> ds[HG], pt[HG], dt[HG];
     f32x4 p[HG], dp[HG];
+    constexpr int WB = WEIGHT_BYTES<SPLIT>, APART = SPLIT ? 1 : 2;                 // split, the two kinds of tiles share their place
 #pragma unroll
     for (int h = 0; h < HG; ++h) {
       const int at = h * DH * 2;
@@ -840,20 +897,25 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
         p[h][r] *= il;
         t[r] = p[h][r] * __builtin_fmaf(dp[h][r], a.scale, d);
       }
-      ds[h] = pack4(t);
-      char* tile = K + h * 2 * TILE_BYTES;
-      *reinterpret_cast<s16x4*>(tile + i * TP + 8 * g) = pack4(p[h]);
-      *reinterpret_cast<s16x4*>(tile + TILE_BYTES + i * TP + 8 * g) = ds[h];
+      ds[h] = gradients<SPLIT>(t);
+      put_tile(K + h * APART * WB, g, i, probabilities<SPLIT>(p[h]));
+      if constexpr (!SPLIT) put_tile(K + (h * APART + 1) * WB, g, i, ds[h]);
     }
     order_lds();
-    s16x4 pt[HG], dt[HG];
 #pragma unroll
     for (int h = 0; h < HG; ++h) {
-      const char* tile = K + h * 2 * TILE_BYTES + (4 * g + (i >> 2)) * TP + 8 * (i & 3);
-      pt[h] = read_columns(tile);
-      dt[h] = read_columns(tile + TILE_BYTES);
+      pt[h] = turned_tile<SPLIT>(K + h * APART * WB, g, i);
+      if constexpr (!SPLIT) dt[h] = turned_tile<SPLIT>(K + (h * APART + 1) * WB, g, i);
     }
     order_lds();
+    if constexpr (SPLIT) {
+#pragma unroll
+      for (int h = 0; h < HG; ++h) put_tile(K + h * WB, g, i, ds[h]);
+      order_lds();
+#pragma unroll
+      for (int h = 0; h < HG; ++h) dt[h] = turned_tile<SPLIT>(K + h * WB, g, i);
+      order_lds();
+    }
 #pragma unroll
     for (int h = 0; h < HG; ++h) {
       f32x4 dq[CT], dk[CT], dv[CT];
@@ -884,14 +946,14 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
 }
 
 template <int DH, bool BWD> constexpr int small_lds() { return (BWD ? 4 : 3) * 16 * SMALL_PITCH; }             // of one wave
-template <int DH, bool BWD> __device__ __forceinline__ void small_role(const DotArgs& a, int first, int step, int head0, int (*toks)[64], char* lds) {
+template <int DH, bool BWD, bool SPLIT> __device__ __forceinline__ void small_role(const DotArgs& a, int first, int step, int head0, int (*toks)[64], char* lds) {
   static_assert(64 / DH * 2 * TILE_BYTES <= small_lds<DH, BWD>() || !BWD, "the P and dS tiles take the images' place");
   for (Walk walk(a, 1, 0, first, step); walk.next(a);) {
     int Tq, Tk;
     walk.tokens(toks, 16, Tq, Tk);
     if (Tq == 0 || Tk == 0) continue;                    // (in no list: the rows are zeroed elsewhere)
-    if (Tq <= 8 && Tk <= 8) small_window<DH, BWD, true>(a, toks, Tq, Tk, head0, lds);
-    else small_window<DH, BWD, false>(a, toks, Tq, Tk, head0, lds);
+    if (Tq <= 8 && Tk <= 8) small_window<DH, BWD, SPLIT, true>(a, toks, Tq, Tk, head0, lds);
+    else small_window<DH, BWD, SPLIT, false>(a, toks, Tq, Tk, head0, lds);
     order_lds();
   }
 }
@@ -905,11 +967,13 @@ template <int DH, bool BWD, int ROLES> constexpr int kernel_lds() {
             l1 = ROLES & ROLE1 ? small_lds<DH, BWD>() : 0;
   return 4 * (l4 > l2 ? (l4 > l1 ? l4 : l1) : (l2 > l1 ? l2 : l1));
 }
-template <int DH, bool BWD, int ROLES> constexpr int kernel_waves() {    // waves per SIMD that the registers allow
-  return ROLES & ROLE4 ? (DH == 16 ? (BWD ? 3 : 5) : DH == 32 ? (BWD ? 2 : 4) : BWD ? 1 : 2) : (DH == 16 ? (BWD ? 4 : 6) : DH == 32 ? (BWD ? 3 : 5) : BWD ? 2 : 4);
+template <int DH, bool BWD, int ROLES, bool SPLIT> constexpr int kernel_waves() {        // waves per SIMD that the registers allow
+  const int waves = ROLES & ROLE4 ? (DH == 16 ? (BWD ? 3 : 5) : DH == 32 ? (BWD ? 2 : 4) : BWD ? 1 : 2)
+                                  : (DH == 16 ? (BWD ? 4 : 6) : DH == 32 ? (BWD ? 3 : 5) : BWD ? 2 : 4);
+  return SPLIT && waves > 1 ? waves - 1 : waves;
 }
-template <int DH, bool BWD, int ROLES>
-__global__ __launch_bounds__(256, (kernel_waves<DH, BWD, ROLES>())) void dot_kernel(DotArgs a, Roles n, Orphans z) {
+template <int DH, bool BWD, int ROLES, bool SPLIT>
+__global__ __launch_bounds__(256, (kernel_waves<DH, BWD, ROLES, SPLIT>())) void dot_kernel(DotArgs a, Roles n, Orphans z) {
   extern __shared__ __attribute__((aligned(16))) char lds_[];
   __shared__ int toks_[4][2][64];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -917,21 +981,21 @@ __global__ __launch_bounds__(256, (kernel_waves<DH, BWD, ROLES>())) void dot_ker
   int u = blockIdx.x;
   if constexpr (ROLES & ROLE4) {
     if (u < n.n4 * n.heads) {
-      window_role<DH, 4, BWD>(a, u / n.heads, n.n4, u % n.heads * 4 + w, toks, lds_ + w * window_lds<DH, 4, BWD>());
+      window_role<DH, 4, BWD, SPLIT>(a, u / n.heads, n.n4, u % n.heads * 4 + w, toks, lds_ + w * window_lds<DH, 4, BWD>());
       return;
     }
     u -= n.n4 * n.heads;
   }
   if constexpr (ROLES & ROLE2) {
     if (u < n.n2 * n.heads) {
-      window_role<DH, 2, BWD>(a, u / n.heads, n.n2, u % n.heads * 4 + w, toks, lds_ + w * window_lds<DH, 2, BWD>());
+      window_role<DH, 2, BWD, SPLIT>(a, u / n.heads, n.n2, u % n.heads * 4 + w, toks, lds_ + w * window_lds<DH, 2, BWD>());
       return;
     }
     u -= n.n2 * n.heads;
   }
   if constexpr (ROLES & ROLE1) {
     if (u < n.n1 * n.columns) {
-      small_role<DH, BWD>(a, u / n.columns * 4 + w, n.n1 * 4, u % n.columns * (64 / DH), toks, lds_ + w * small_lds<DH, BWD>());
+      small_role<DH, BWD, SPLIT>(a, u / n.columns * 4 + w, n.n1 * 4, u % n.columns * (64 / DH), toks, lds_ + w * small_lds<DH, BWD>());
       return;
     }
     u -= n.n1 * n.columns;
@@ -981,11 +1045,11 @@ template <class F> void by_head(int dh, F&& f) {
   else if (dh == 32) f(std::integral_constant<int, 32>());
   else f(std::integral_constant<int, 64>());
 }
-template <int DH, bool BWD, int ROLES> int launch_roles(const DotArgs& a, const Orphans& z, int64_t w4, int64_t w2, int64_t w1, hipStream_t stream) {
+template <int DH, bool BWD, int ROLES, bool SPLIT = false> int launch_roles(const DotArgs& a, const Orphans& z, int64_t w4, int64_t w2, int64_t w1, hipStream_t stream) {
   constexpr int LDS = kernel_lds<DH, BWD, ROLES>();
   static TmaeLdsAttr attr;
   if (LDS + 2048 > 65536)
-    if (int e = tmae_allow_lds(attr, (const void*)dot_kernel<DH, BWD, ROLES>, LDS)) return e;
+    if (int e = tmae_allow_lds(attr, (const void*)dot_kernel<DH, BWD, ROLES, SPLIT>, LDS)) return e;
   Roles n;
   n.heads = (a.nhead + 3) / 4;
   n.columns = (a.nhead * DH + 63) / 64;
@@ -994,7 +1058,7 @@ template <int DH, bool BWD, int ROLES> int launch_roles(const DotArgs& a, const 
   n.n1 = ROLES & ROLE1 ? (int)walkers(w1, 4, n.columns) : 0;
   n.n0 = ROLES & ROLE1 && z.row16 ? (int)walkers(a.nwin, 16, 1, 1) : 0;
   const int64_t blocks = (int64_t)(n.n4 + n.n2) * n.heads + (int64_t)n.n1 * n.columns + n.n0;
-  if (blocks > 0) hipLaunchKernelGGL((dot_kernel<DH, BWD, ROLES>), dim3((unsigned)blocks), dim3(256), LDS, stream, a, n, z);
+  if (blocks > 0) hipLaunchKernelGGL((dot_kernel<DH, BWD, ROLES, SPLIT>), dim3((unsigned)blocks), dim3(256), LDS, stream, a, n, z);
   return TMAE_OK;
 }
 // One launch for all windows, or one for those of more than 32 tokens and one for the others.  One overlaps the ends of the parts and
@@ -1002,9 +1066,11 @@ template <int DH, bool BWD, int ROLES> int launch_roles(const DotArgs& a, const 
 // heads of 16): forward 109 us in one launch against 114, backward 206 against 193; stage 2 (33 k queries, 131 k keys, 8 heads of 32):
 // forward 45 against 42, backward 90 against 84.  Few tokens: the launch counts.
 template <int DH, bool BWD> int launch_bf16(const DotArgs& a, const Orphans& z, hipStream_t stream) {
-  if (!a.wl) return launch_roles<DH, BWD, ROLE4>(a, z, a.nwin, 0, 0, stream);
+  const bool few = a.mq + a.mk <= 32768;
+  if (!a.wl) return few ? launch_roles<DH, BWD, ROLE4, true>(a, z, a.nwin, 0, 0, stream) : launch_roles<DH, BWD, ROLE4>(a, z, a.nwin, 0, 0, stream);
   const int64_t w4 = class_windows(a, 3), w2 = class_windows(a, 2), w1 = class_windows(a, 0);
-  if ((DH == 16 && !BWD) || a.mq + a.mk <= 32768) return launch_roles<DH, BWD, ROLE4 | ROLE2 | ROLE1>(a, z, w4, w2, w1, stream);
+  if (few) return launch_roles<DH, BWD, ROLE4 | ROLE2 | ROLE1, true>(a, z, w4, w2, w1, stream);
+  if constexpr (DH == 16 && !BWD) return launch_roles<DH, BWD, ROLE4 | ROLE2 | ROLE1>(a, z, w4, w2, w1, stream);
   const int rc = launch_roles<DH, BWD, ROLE4>(a, z, w4, w2, w1, stream);
   return rc != TMAE_OK ? rc : launch_roles<DH, BWD, ROLE2 | ROLE1>(a, z, w4, w2, w1, stream);
 }

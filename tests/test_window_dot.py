@@ -526,3 +526,34 @@ def test_rows_beyond_32_bits():
     alone = run(qk[-cells:], v[-cells:], do[-cells:], grid[:cells], 1)
     for a, b in zip(whole, alone):
         assert torch.equal(a[-cells:], b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('worklist', [True, False])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('heads,dh,shift,cross', [(8, 16, False, False), (3, 16, True, True), (4, 32, True, False), (3, 32, False, True),
+                                                  (2, 64, False, False), (1, 64, True, True)])
+def test_many_frames(heads, dh, shift, cross, dtype, worklist):
+    """More tokens than the variants for few of them take, of every size of window: the first and the last frame against the definition."""
+    from tmae_amd import ops
+    g = torch.Generator().manual_seed(dh + heads)
+    batch, ny, nx, d, e = 25, 40, 41, heads * dh, half_step(dtype)
+    counts = [(60, 300, 700, 1300, 1640)[b % 5] for b in range(batch)]
+    grid_q, at_q = place(counts, batch, ny, nx, g)
+    grid_k, at_k = place(counts[::-1], batch, ny, nx, g) if cross else (grid_q, at_q)
+    mq, mk = at_q.shape[0], at_k.shape[0]
+    assert mq + mk > 32768
+    q, do = (torch.randn(mq, d, generator=g).to(dtype) for _ in range(2))
+    k, v = (torch.randn(mk, d, generator=g).to(dtype) for _ in range(2))
+    gq = grid_q.cuda()
+    gk = grid_k.cuda() if cross else gq
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    wl = ops.window_worklist(gq, gk, batch, ny, nx, shift) if worklist else None
+    o = ops.win_attn_dot(*leaves, gq, gk, heads, batch, ny, nx, shift, worklist=wl, covered=True)
+    got = [o, *torch.autograd.grad(o, leaves, do.cuda())]
+    for frame in (0, batch - 1):
+        fq, fk = at_q[:, 0] == frame, at_k[:, 0] == frame
+        same = window_of(at_q[fq], shift)[:, None] == window_of(at_k[fk], shift)[None]
+        want, tolerances = reference(q[fq].double(), k[fk].double(), v[fk].double(), do[fq].double(), same, heads, dh ** -0.5)
+        for what, t, rows, w, tol in zip(('out', 'dq', 'dk', 'dv'), got, (fq, fq, fk, fk), want, tolerances(e)):
+            within(t[rows.cuda()], w, tol, f'{what} of frame {frame}')
