@@ -13,7 +13,7 @@
 // operand stand in 16 rows: read straight into that layout, an instruction touches some 44 lines.  Rows therefore travel in 16-byte
 // pieces, whole pieces of a line by neighbouring lanes, through LDS images; all of a window's rows are requested at once.  Padding rows to
 // tiles is what the matrix unit pays for; three sizes of windows (up to 16, 32 and 64 tokens) keep it small.  Eight frames at stage 1
-// (375 k tokens, 8 heads of 16, bfloat16): forward 108 us, backward 75 + 120 us -- 4.0, 3.4 and 4.2 TB/s of counted HBM traffic; the
+// (375 k tokens, 8 heads of 16, bfloat16): forward 114 us, backward 75 + 121 us -- 3.9, 3.4 and 4.2 TB/s of counted HBM traffic; the
 // movement alone, without the arithmetic, takes 59 + 99 us of the backward.
 //
 // A slot behind a window's last token stands for its first one: it is read, its probability is set to 0 (and V and dO are zeros there,
@@ -968,9 +968,9 @@ template <int DH, bool BWD, int ROLES> constexpr int kernel_lds() {
   return 4 * (l4 > l2 ? (l4 > l1 ? l4 : l1) : (l2 > l1 ? l2 : l1));
 }
 template <int DH, bool BWD, int ROLES, bool SPLIT> constexpr int kernel_waves() {        // waves per SIMD that the registers allow
-  const int waves = ROLES & ROLE4 ? (DH == 16 ? (BWD ? 3 : 5) : DH == 32 ? (BWD ? 2 : 4) : BWD ? 1 : 2)
-                                  : (DH == 16 ? (BWD ? 4 : 6) : DH == 32 ? (BWD ? 3 : 5) : BWD ? 2 : 4);
-  return SPLIT && waves > 1 ? waves - 1 : waves;
+  if (!BWD) return DH == 16 ? 4 : DH == 32 ? 3 : 2;
+  if (SPLIT) return DH == 16 ? 2 : 1;
+  return ROLES & ROLE4 ? (DH == 16 ? 3 : DH == 32 ? 2 : 1) : (DH == 16 ? 4 : DH == 32 ? 3 : 2);
 }
 template <int DH, bool BWD, int ROLES, bool SPLIT>
 __global__ __launch_bounds__(256, (kernel_waves<DH, BWD, ROLES, SPLIT>())) void dot_kernel(DotArgs a, Roles n, Orphans z) {
@@ -1045,7 +1045,7 @@ template <class F> void by_head(int dh, F&& f) {
   else if (dh == 32) f(std::integral_constant<int, 32>());
   else f(std::integral_constant<int, 64>());
 }
-template <int DH, bool BWD, int ROLES, bool SPLIT = false> int launch_roles(const DotArgs& a, const Orphans& z, int64_t w4, int64_t w2, int64_t w1, hipStream_t stream) {
+template <int DH, bool BWD, int ROLES, bool SPLIT> int launch_roles(const DotArgs& a, const Orphans& z, int64_t w4, int64_t w2, int64_t w1, hipStream_t stream) {
   constexpr int LDS = kernel_lds<DH, BWD, ROLES>();
   static TmaeLdsAttr attr;
   if (LDS + 2048 > 65536)
@@ -1061,18 +1061,21 @@ template <int DH, bool BWD, int ROLES, bool SPLIT = false> int launch_roles(cons
   if (blocks > 0) hipLaunchKernelGGL((dot_kernel<DH, BWD, ROLES, SPLIT>), dim3((unsigned)blocks), dim3(256), LDS, stream, a, n, z);
   return TMAE_OK;
 }
-// One launch for all windows, or one for those of more than 32 tokens and one for the others.  One overlaps the ends of the parts and
-// costs a launch less, but every workgroup then has the registers and LDS of the largest part.  Eight frames at stage 1 (375 k tokens, 8
-// heads of 16): forward 109 us in one launch against 114, backward 206 against 193; stage 2 (33 k queries, 131 k keys, 8 heads of 32):
-// forward 45 against 42, backward 90 against 84.  Few tokens: the launch counts.
+// Forward: one launch, the probabilities split: eight frames at stage 1 (375 k tokens, 8 heads of 16) 114 us, 109 us rounded, 114 us
+// rounded in two launches; stage 2 (33 k queries, 131 k keys, 8 heads of 32) 44, 45 and 42 us.  Backward: split, the tiles that turn in LDS
+// are twice as many, and in one launch every workgroup has the registers and LDS of the largest windows: 199 and 85 us rounded in two
+// launches, 271 and 144 us split in one.  So only few tokens take that, whose time is the launch, and whose few results would show a
+// rounding as large as their own.
 template <int DH, bool BWD> int launch_bf16(const DotArgs& a, const Orphans& z, hipStream_t stream) {
-  const bool few = a.mq + a.mk <= 32768;
-  if (!a.wl) return few ? launch_roles<DH, BWD, ROLE4, true>(a, z, a.nwin, 0, 0, stream) : launch_roles<DH, BWD, ROLE4>(a, z, a.nwin, 0, 0, stream);
-  const int64_t w4 = class_windows(a, 3), w2 = class_windows(a, 2), w1 = class_windows(a, 0);
-  if (few) return launch_roles<DH, BWD, ROLE4 | ROLE2 | ROLE1, true>(a, z, w4, w2, w1, stream);
-  if constexpr (DH == 16 && !BWD) return launch_roles<DH, BWD, ROLE4 | ROLE2 | ROLE1>(a, z, w4, w2, w1, stream);
-  const int rc = launch_roles<DH, BWD, ROLE4>(a, z, w4, w2, w1, stream);
-  return rc != TMAE_OK ? rc : launch_roles<DH, BWD, ROLE2 | ROLE1>(a, z, w4, w2, w1, stream);
+  const int64_t w4 = a.wl ? class_windows(a, 3) : a.nwin, w2 = class_windows(a, 2), w1 = class_windows(a, 0);
+  constexpr int ALL = ROLE4 | ROLE2 | ROLE1;
+  if constexpr (BWD) {
+    if (a.mq + a.mk > 8192) {
+      const int rc = launch_roles<DH, BWD, ROLE4, false>(a, z, w4, w2, w1, stream);
+      return rc != TMAE_OK || !a.wl ? rc : launch_roles<DH, BWD, ROLE2 | ROLE1, false>(a, z, w4, w2, w1, stream);
+    }
+  }
+  return a.wl ? launch_roles<DH, BWD, ALL, true>(a, z, w4, w2, w1, stream) : launch_roles<DH, BWD, ROLE4, true>(a, z, w4, w2, w1, stream);
 }
 template <int DH, bool BWD> int launch_f32(const DotArgs& a, const Orphans& z, hipStream_t stream) {
   if (z.row16) hipLaunchKernelGGL(dot_orphan_kernel, dim3(walkers(a.nwin, 4, 1)), dim3(256), 0, stream, a, z);
