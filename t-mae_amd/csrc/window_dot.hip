@@ -7,7 +7,7 @@
 //
 // Tiles of 16 tokens.  A logit tile is computed with the keys as its rows and the queries as its columns: the accumulators' layout --
 // lane (g, i) = (lane >> 4, lane & 15) holds rows 4g .. 4g+3 of column i -- is also what the next product takes as its B operand, row
-// 4g + r in step r, so that the probabilities go into it without leaving the registers (float32 whole, bfloat16 rounded once).
+// 4g + r in step r, so that the probabilities go into it without leaving the registers (float32 whole, bfloat16 rounded or as a sum of two).
 //
 // Bound: HBM, at 8 to 20 FLOPs a byte; but rows lie apart and windows are small, so what costs is getting rows in and out.  The lanes of an
 // operand stand in 16 rows: read straight into that layout, an instruction touches some 44 lines.  Rows therefore travel in 16-byte
@@ -1028,7 +1028,7 @@ int fill(DotArgs& a, int dtype, int64_t mq, int64_t mk, int nhead, int dh, const
   if (dtype != TMAE_F32 && dtype != TMAE_BF16) return TMAE_EDTYPE;
   if (mq < 0 || mk < 0 || mq > 0x7fffffff || mk > 0x7fffffff || nhead < 1 || nhead > 4096 || (dh != 16 && dh != 32 && dh != 64)) return TMAE_EARG;
   if (!grid_q || !grid_k || batch < 1 || ny < 1 || nx < 1 || (int64_t)ny * nx >= ((int64_t)1 << 31) ||
-      (int64_t)batch * ny * nx >= ((int64_t)1 << 31) || !(scale > 0.f) || scale > 3e38f)
+      (int64_t)batch * ny * nx >= ((int64_t)1 << 31) || !(scale > 0.f) || scale > 2e38f)
     return TMAE_EARG;
   a.Wy = (ny + WIN - 1) / WIN + 1; a.Wx = (nx + WIN - 1) / WIN + 1;
   if (worklist && (a.Wy > 255 || a.Wx > 255 || batch > 32767)) return TMAE_EARG;

@@ -1958,6 +1958,12 @@ def qk_norm_rotary(x, q_gain, k_gain, positions, inv_freq, sections, q_heads=Non
     return _qk_norm_launch(x, q_gain, k_gain, positions, inv_freq, arr, q_heads, per_head, float(eps), int(bool(interleaved)))
 
 
+def _rows16(t):
+    """t as contiguous rows from a 16-byte boundary on (a piece of a flat buffer may begin anywhere)"""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 class _WinAttnDot(torch.autograd.Function):
     @staticmethod
     def forward(ctx, a, b, c, grid_q, grid_k, worklist, meta):
@@ -1972,7 +1978,7 @@ class _WinAttnDot(torch.autograd.Function):
         if ctx.packed_kv:
             c = 'kv'
         d, nhead, batch, ny, nx, do_shift, scale, covered, dtype, mq, mk, dh = ctx.meta
-        dout = dout.contiguous()
+        dout = _rows16(dout)
         alloc = torch.empty_like if covered else torch.zeros_like
         da = alloc(a)
         db = alloc(b) if b is not None else None
@@ -2034,7 +2040,7 @@ def win_attn_dot(a, b, c, grid_q, grid_k, nhead, batch, ny, nx, do_shift, scale=
     if nhead < 1 or nhead > 4096 or dh not in (16, 32, 64) or d != dh * nhead:
         raise ValueError(f'{name}: {d} channels for {nhead} heads; heads have 16, 32 or 64')
     scale = float(dh ** -0.5 if scale is None else scale)
-    if not 0.0 < scale <= 3e38:
+    if not 0.0 < scale <= 2e38:
         raise ValueError(f'{name}: scale {scale}')
     cells = batch * ny * nx
     if batch < 1 or ny < 1 or nx < 1 or cells >= 1 << 31 or most >= 1 << 31:
@@ -2047,11 +2053,11 @@ def win_attn_dot(a, b, c, grid_q, grid_k, nhead, batch, ny, nx, do_shift, scale=
                 worklist.numel() != _worklist_size(batch, ny, nx):
             raise ValueError(f'{name}: the work list is not one of {batch} grids of {ny} x {nx}')
     _need_cuda(a)
-    a = a.contiguous()
+    a = _rows16(a)
     if b is not None:
-        b = b.contiguous()
+        b = _rows16(b)
         if layout == 'q, k, v':
-            c = c.contiguous()
+            c = _rows16(c)
     meta = (d, nhead, batch, ny, nx, 1 if do_shift else 0, scale, bool(covered), dtype, mq, mk, dh)
     if _grad_on(*tensors):
         return _WinAttnDot.apply(a, b, c, grid_q, grid_k, worklist, meta)

@@ -57,3 +57,16 @@ def test_no_unpadded_mfma_hazard_in_any_kernel():
     files = sorted(glob.glob(os.path.join(ROOT, 't-mae_amd', 'csrc', '*.hip')))
     bad = t.check_files(files)
     assert not bad, [(os.path.basename(b[0]), b[1][:50], b[3], b[6], b[8]) for b in bad[:10]]
+
+
+def test_checker_sees_accumulation_registers_and_other_shapes():
+    """An accumulation register read too early, an accumulator that goes on in an instruction of another shape at once (both flagged),
+    and the same with the wait states in between (clean)."""
+    t = _tool()
+    kernel = 'kern:\n\tv_mfma_f32_16x16x32_bf16 %s, v[30:33], v[34:37], 0\n%s\ts_endpgm\n.Lfunc_end0:\n'
+    for dst, reader in (('a[0:3]', '\tv_accvgpr_read_b32 v1, a2\n'),
+                        ('v[70:73]', '\tv_mfma_f32_16x16x16_bf16 v[70:73], v[38:39], v[40:41], v[70:73]\n')):
+        probs = t.check_asm(kernel % (dst, reader))
+        assert len(probs) == 1 and probs[0][7] == 0, probs
+        assert t.check_asm(kernel % (dst, '\ts_nop 7\n' + reader)) == []
+    assert t.check_asm(kernel % ('a[0:3]', '\tv_mov_b32_e32 v2, v1\n')) == []

@@ -557,3 +557,30 @@ def test_many_frames(heads, dh, shift, cross, dtype, worklist):
         want, tolerances = reference(q[fq].double(), k[fk].double(), v[fk].double(), do[fq].double(), same, heads, dh ** -0.5)
         for what, t, rows, w, tol in zip(('out', 'dq', 'dk', 'dv'), got, (fq, fq, fk, fk), want, tolerances(e)):
             within(t[rows.cuda()], w, tol, f'{what} of frame {frame}')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_rows_from_any_address(dtype):
+    """Pieces of flat buffers that begin beside a 16-byte boundary, rows apart and a broadcast gradient: the same bits as aligned ones."""
+    from tmae_amd import ops
+    g = torch.Generator(device='cuda').manual_seed(8)
+    grid = torch.arange(24 * 24, dtype=torch.int32, device='cuda')
+    qk, v, row = (torch.randn(n, generator=g, device='cuda').to(dtype) for n in (576 * 64, 576 * 32, 32))
+
+    def run(qk, v, do):
+        leaves = [t.detach().requires_grad_() for t in (qk, v)]
+        o = ops.win_attn_dot(*leaves, None, grid, grid, 2, 1, 24, 24, True, covered=True)
+        return [t.detach() for t in (o, *torch.autograd.grad(o, leaves, do))]
+
+    def beside(t):
+        flat = torch.zeros(t.numel() + 1, device='cuda', dtype=dtype)
+        flat[1:] = t.reshape(-1)
+        return flat[1:].view(t.shape)
+    qk, v, do = qk.view(576, 64), v.view(576, 32), row.expand(576, 32)
+    want = run(qk, v, do.contiguous())
+    wide = torch.zeros(576, 100, device='cuda', dtype=dtype)
+    wide[:, 3:67] = qk
+    for args in ((beside(qk), beside(v), beside(do)), (wide[:, 3:67], v, do)):
+        for a, b in zip(run(*args), want):
+            assert torch.equal(a, b)
