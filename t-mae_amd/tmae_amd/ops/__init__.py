@@ -1808,9 +1808,8 @@ def rotary_freqs(sections, base=10000.0, device=None):
 
 @functools.lru_cache(maxsize=64)
 def _rotary_sections(sections):
-    """(the sections as whole numbers, as a C array, channel pairs in all)"""
-    sections = tuple(int(p) for p in sections)
-    return sections, (ctypes.c_int32 * len(sections))(*sections), sum(sections)
+    """(the sections as a C array, channel pairs in all)"""
+    return (ctypes.c_int32 * len(sections))(*sections), sum(sections)
 
 
 def _rotary_args(name, x, positions, inv_freq, sections):
@@ -1819,7 +1818,8 @@ def _rotary_args(name, x, positions, inv_freq, sections):
         raise ValueError(f'{name}: x [tokens, heads, channels] expected, got {tuple(x.shape)}')
     _dt(x)
     n, h, dh = x.shape
-    sections, arr, P = _rotary_sections(tuple(sections))
+    sections = tuple(map(int, sections))
+    arr, P = _rotary_sections(sections)
     if not 1 <= len(sections) <= 4 or min(sections) < 1 or 2 * P > dh or dh > 512 or not 1 <= h <= 65535:
         raise ValueError(f'{name}: sections {sections} for {h} heads of {dh} channels (1 to 4 axes, at most {dh // 2} pairs, at most '
                          f'512 channels)')
@@ -2004,7 +2004,7 @@ def _win_attn_dot_launch(a, b, c, grid_q, grid_k, worklist, meta):
 def win_attn_dot(a, b, c, grid_q, grid_k, nhead, batch, ny, nx, do_shift, scale=None, worklist=None, covered=False):
     """Scaled-dot-product attention inside the 8x8 windows of win_attn, over projected rows (float32 / bfloat16) in its layouts:
     a = packed [m, 3 d] (q|k|v), b and c None; a = packed [m, 2 d] (q|k), b = v [m, d], c None; a = q [mq, d], b = k and c = v [mk, d];
-    a = q, b = packed [mk, 2 d] (k|v), c = 'kv'.  Heads of 16, 32 or 64 channels, any number of them; the logits are scale * q . k
+    a = q, b = packed [mk, 2 d] (k|v), c = 'kv'.  Up to 4096 heads of 16, 32 or 64 channels; the logits are scale * q . k
     (default: channels ** -0.5).  Queries whose window holds no key get zero rows.
 
     grid_q, grid_k [batch * ny * nx] int32: row numbers of the queries and keys, -1 where a cell is empty (index_grid); a row stands
