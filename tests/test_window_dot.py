@@ -584,3 +584,78 @@ def test_rows_from_any_address(dtype):
     for args in ((beside(qk), beside(v), beside(do)), (wide[:, 3:67], v, do)):
         for a, b in zip(run(*args), want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_large_calls_in_a_graph_and_side_by_side():
+    """Norms, rotation and attention over more tokens than the variants for few of them take: replays on new inputs, with eager work
+    between them, and calls at once on two streams give the bits of a call alone."""
+    from tmae_amd import ops
+    g = torch.Generator(device='cuda').manual_seed(3)
+    batch, ny, nx, h, dh, sec = 4, 100, 99, 8, 16, (2, 3, 3)
+    n, d = batch * ny * nx, h * dh
+    grid = torch.arange(n, dtype=torch.int32, device='cuda')
+    wl = ops.window_worklist(grid, grid, batch, ny, nx, True)
+    pos = torch.randint(0, 99, (n, 3), generator=g, device='cuda', dtype=torch.int32)
+    f = ops.rotary_freqs(sec, 100.0, 'cuda')
+
+    def inputs():
+        return [torch.randn(s, generator=g, device='cuda').to(t) for s, t in (((n, 2 * d), torch.bfloat16), ((n, d), torch.bfloat16),
+                                                                              ((dh,), torch.float32), ((dh,), torch.float32))]
+
+    def run(qk, v, gq, gk, do):
+        leaves = [t.detach().requires_grad_() for t in (qk, v, gq, gk)]
+        turned = ops.qk_norm_rotary(leaves[0].view(n, 2 * h, dh), *leaves[2:], pos, f, sec).view(n, 2 * d)
+        o = ops.win_attn_dot(turned, leaves[1], None, grid, grid, h, batch, ny, nx, True, worklist=wl, covered=True)
+        return [o.detach(), *torch.autograd.grad(o, leaves, do)]
+    do = torch.randn(n, d, generator=g, device='cuda').bfloat16()
+    held = inputs()
+    run(*held, do)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(*held, do)
+    for k in range(3):
+        fresh = inputs()
+        for a, b in zip(held, fresh):
+            a.copy_(b)
+        graph.replay()
+        want = run(*fresh, do)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+    sets = [inputs() for _ in range(2)]
+    alone = [run(*s, do) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(3):
+        both = []
+        for stream, s in zip(streams, sets):
+            with torch.cuda.stream(stream):
+                both.append(run(*s, do))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(both, alone) for a, b in zip(x, y))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('heads,dh', [(4, 16), (2, 32), (1, 64)])
+def test_infinities_in_large_calls(heads, dh):
+    """As in small ones: an infinite dO of a window's first token makes that channel of dV infinite in its window, and nothing else."""
+    from tmae_amd import ops
+    g = torch.Generator().manual_seed(dh)
+    batch, ny, nx = 12, 40, 41
+    grid, at = place([(60, 300, 700, 1300, 1640)[b % 5] for b in range(batch)], batch, ny, nx, g)
+    n = at.shape[0]
+    assert 2 * n > 8192
+    win = window_of(at, False)
+    order = torch.argsort(win, stable=True)
+    first = order[torch.cat([torch.ones(1, dtype=torch.bool), win[order][1:] != win[order][:-1]])]
+    touched = torch.zeros(n, heads * dh, dtype=torch.bool)
+    touched[:, 5] = True
+    q, k, v, do = (torch.randn(n, heads * dh, generator=g).bfloat16() for _ in range(4))
+    do[first, 5] = float('inf')
+    gr = grid.cuda()
+    for worklist in (None, ops.window_worklist(gr, gr, batch, ny, nx, False)):
+        leaf = v.cuda().requires_grad_()
+        o = ops.win_attn_dot(q.cuda(), k.cuda(), leaf, gr, gr, heads, batch, ny, nx, False, worklist=worklist, covered=True)
+        dv = torch.autograd.grad(o, leaf, do.cuda())[0].cpu().float()
+        assert torch.isfinite(o).all() and (dv[touched] == float('inf')).all() and torch.isfinite(dv[~touched]).all()
