@@ -13,8 +13,8 @@
 // operand stand in 16 rows: read straight into that layout, an instruction touches some 44 lines.  Rows therefore travel in 16-byte
 // pieces, whole pieces of a line by neighbouring lanes, through LDS images; all of a window's rows are requested at once.  Padding rows to
 // tiles is what the matrix unit pays for; three sizes of windows (up to 16, 32 and 64 tokens) keep it small.  Eight frames at stage 1
-// (375 k tokens, 8 heads of 16, bfloat16): forward 114 us, backward 75 + 121 us -- 3.9, 3.4 and 4.2 TB/s of counted HBM traffic; the
-// movement alone, without the arithmetic, takes 59 + 99 us of the backward.
+// (375 k tokens, 8 heads of 16, bfloat16): forward 112 us, backward 73 + 111 us -- about 4 TB/s of counted HBM traffic; the movement alone,
+// without the arithmetic, took 59 + 99 us of the backward.
 //
 // A slot behind a window's last token stands for its first one: it is read, its probability is set to 0 (and V and dO are zeros there,
 // which an infinity next to them needs), and nothing is stored for it.
@@ -46,11 +46,18 @@ __device__ __forceinline__ char* row_of(const void* base, int token, unsigned pi
 }
 
 // LDS operations of a wave execute in order: this keeps the compiler to the order they are written in.  In bfloat16 every wave works in
-// a piece of LDS of its own, without a workgroup barrier.
+// images of its own; the waves of a workgroup meet where they move rows for each other.
 __device__ __forceinline__ void order_lds() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// A barrier of the workgroup for what is in LDS alone: rows on their way from or to memory stay on their way.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // The windows of a launch: those of the work list's classes `from`, `from` - 1, ... `to` one after the other (larger windows first), or
@@ -220,13 +227,13 @@ template <int DH, int NT, bool BWD> __device__ __forceinline__ void f32_role(con
       if (slot >= Tk) rows[0][p] = rows[1][p] = zero;
       if (slot >= Tq) { rows[2][p] = zero; if constexpr (BWD) rows[3][p] = zero; }
     }
-    __syncthreads();                         // the window before is done with
+    lds_barrier();                         // the window before is done with
 #pragma unroll
     for (int p = 0; p < PASSES; ++p)
 #pragma unroll
       for (int n = 0; n < NI; ++n)
         *reinterpret_cast<f32x4*>(lds + n * R::IMAGE + (p * RP + (int)threadIdx.x / LPR) * R::PITCH + (int)threadIdx.x % LPR * 4) = rows[n][p];
-    __syncthreads();
+    lds_barrier();
     const int nq = (Tq + 15) >> 4, nk = (Tk + 15) >> 4;
     const float *K = lds + hh * ROWS * R::PITCH, *V = K + R::IMAGE, *Q = K + 2 * R::IMAGE, *G = K + 3 * R::IMAGE;
     const bool mine = head < a.nhead;
@@ -284,7 +291,7 @@ template <int DH, int NT, bool BWD> __device__ __forceinline__ void f32_role(con
       }
     }
     if constexpr (BWD) {
-      __syncthreads();
+      lds_barrier();
       if (mine && t < nk) {
         const typename R::Piece kf = R::piece(K + t * TILE, g, i), vf = R::piece(V + t * TILE, g, i);
         f32x4 dk[CT], dv[CT];
@@ -514,59 +521,62 @@ template <bool SPLIT> __device__ __forceinline__ Weights<SPLIT> turned_tile(cons
   else return Rounded{read_columns(at)};
 }
 
-// ---- windows of more than 16 tokens: a wave per (window, head), four heads in a workgroup so that their pieces of a line meet in the cache.
-// All rows of the window are requested at once.  Forward: K and V go through the wave's two images into registers, Q takes K's place, the
-// output Q's.  Backward: K, V and Q have images; V goes into registers and dO takes its place; at the end dQ, dK and dV stand where Q, K
-// and dO stood.
+// ---- windows of more than 16 tokens: a workgroup per window and four heads, a wave for each of them.  The four move the rows together,
+// whole 128-byte lines at a time, and past the cache on the way out (stage 1: 72 + 111 us backward, 74 + 119 us where each wave moves its
+// own 32 bytes of a row, 147 + 133 us where those go past the cache; stage 2 across frames 35 + 44 and 39 + 46 us).  All rows of the window
+// are requested at once.  Forward: K and V go through the wave's two images into registers, Q takes K's place, the output Q's.  Backward:
+// K, V and Q have images; V goes into registers and dO takes its place; at the end dQ, dK and dV stand where Q, K and dO stood.
 template <int DH, int NT> struct Window {
   static constexpr int PITCH = DH * 2 + 16, TILE = 16 * PITCH, IMAGE = NT * TILE;
-  static constexpr int CHUNKS = DH / 8, RPI = 64 / CHUNKS, LOADS = NT * 16 / RPI;             // 16-byte chunks of a row, rows of a load
+  static constexpr int CHUNKS = DH / 8, LINE = 4 * CHUNKS, LOADS = NT * 16 * LINE / 256;      // 16-byte chunks of a head's row, of the four heads'
   using R = Rows<DH, PITCH>;
   static constexpr int CT = R::CT;
 
+  // chunk s * 256 + threadIdx.x of the window's rows
+  struct Place { int row, head, chunk; };
+  static __device__ __forceinline__ Place place(int s) {
+    const int q = s * 256 + (int)threadIdx.x, c = q % LINE;
+    return Place{q / LINE, c / CHUNKS, c % CHUNKS};
+  }
   struct Loaded { u32x4 row[LOADS]; };
-  static __device__ __forceinline__ Loaded request(const void* base, unsigned pitch, const int* toks, int col) {
-    const int lane = threadIdx.x & 63;
+  // head0: the first of the four; of heads that do not exist the last one's rows
+  static __device__ __forceinline__ Loaded request(const void* base, unsigned pitch, const int* toks, int head0, int nhead) {
     Loaded l;
 #pragma unroll
-    for (int s = 0; s < LOADS; ++s)
-      l.row[s] = *reinterpret_cast<const u32x4*>(row_of(base, toks[s * RPI + lane / CHUNKS], pitch) + col + (lane % CHUNKS) * 16);
+    for (int s = 0; s < LOADS; ++s) {
+      const Place p = place(s);
+      const int head = head0 + p.head < nhead ? head0 + p.head : nhead - 1;
+      l.row[s] = *reinterpret_cast<const u32x4*>(row_of(base, toks[p.row], pitch) + head * DH * 2 + p.chunk * 16);
+    }
     return l;
   }
-  // the rows from `T` on as zeros: a probability of 0 stays one beside an infinity
-  static __device__ __forceinline__ void lay(char* image, Loaded l, int T) {
-    const int lane = threadIdx.x & 63;
+  // into an image of every head (per_head bytes apart); the rows from `T` on as zeros: a probability of 0 stays one beside an infinity
+  static __device__ __forceinline__ void lay(char* images, int per_head, Loaded l, int T) {
     const u32x4 none = {0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int s = 0; s < LOADS; ++s) l.row[s] = s * RPI + lane / CHUNKS < T ? l.row[s] : none;
-    lay(image, l);
+    for (int s = 0; s < LOADS; ++s) {
+      const Place p = place(s);
+      *reinterpret_cast<u32x4*>(images + p.head * per_head + p.row * PITCH + p.chunk * 16) = p.row < T ? l.row[s] : none;
+    }
   }
-  static __device__ __forceinline__ void lay(char* image, Loaded l) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int s = 0; s < LOADS; ++s) *reinterpret_cast<u32x4*>(image + (s * RPI + lane / CHUNKS) * PITCH + (lane % CHUNKS) * 16) = l.row[s];
-  }
-  static __device__ __forceinline__ void store(void* base, unsigned pitch, const int* toks, int T, int col, const char* image) {
-    const int lane = threadIdx.x & 63;
+  static __device__ __forceinline__ void store(void* base, unsigned pitch, const int* toks, int T, int head0, int nhead, const char* images, int per_head) {
 #pragma unroll
     for (int s = 0; s < LOADS; ++s) {
-      const int r = s * RPI + lane / CHUNKS;
-      if (r < T)
-        *reinterpret_cast<uint4*>(row_of(base, toks[r], pitch) + col + (lane % CHUNKS) * 16) =
-            *reinterpret_cast<const uint4*>(image + r * PITCH + (lane % CHUNKS) * 16);
+      const Place p = place(s);
+      if (p.row < T && head0 + p.head < nhead)
+        __builtin_nontemporal_store(*reinterpret_cast<const u32x4*>(images + p.head * per_head + p.row * PITCH + p.chunk * 16),
+                                    reinterpret_cast<u32x4*>(row_of(base, toks[p.row], pitch) + (head0 + p.head) * DH * 2 + p.chunk * 16));
     }
   }
 };
 
 // NK key tiles against nq query tiles.  NK is a template parameter, so that no branch stands between a matrix instruction and its reader.
 template <int DH, int NT, int NK, bool SPLIT>
-__device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq, const int* tk, int Tq, int Tk, int head, char* A,
-                                           typename Window<DH, NT>::Loaded qrows) {
+__device__ __forceinline__ void fwd_window(const DotArgs& a, int Tq, int Tk, char* images, int per_head, char* A, typename Window<DH, NT>::Loaded qrows) {
   using W = Window<DH, NT>;
   using R = typename W::R;
   constexpr int CT = W::CT, TILE = W::TILE;
   const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15, nq = (Tq + 15) >> 4;
-  const int col = head * DH * 2;
   const char* V = A + W::IMAGE;
   typename R::Piece kf[NK];
   s16x4 vc[CT][NK];
@@ -576,9 +586,9 @@ __device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq, cons
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) vc[ct][kt] = R::columns(V + kt * TILE, g, i, ct);
   }
-  order_lds();
-  W::lay(A, qrows);
-  order_lds();
+  lds_barrier();
+  W::lay(images, per_head, qrows, Tq);
+  lds_barrier();
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   f32x4 absent;                              // of the last key tile: -inf where there is no key
 #pragma unroll
@@ -615,18 +625,15 @@ __device__ __forceinline__ void fwd_window(const DotArgs& a, const int* tq, cons
     for (int ct = 0; ct < CT; ++ct) o[ct] *= il;
     R::put(A + qt * TILE, g, i, o);
   }
-  order_lds();
-  W::store(a.o, a.po, tq, Tq, col, A);
 }
 
 template <int DH, int NT, int NK, bool SPLIT>
-__device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, const int* tk, int Tq, int Tk, int head, char* A,
-                                           typename Window<DH, NT>::Loaded grows, char* tiles) {
+__device__ __forceinline__ void bwd_window(const DotArgs& a, int Tq, int Tk, char* images, int per_head, char* A, typename Window<DH, NT>::Loaded grows,
+                                           char* tiles) {
   using W = Window<DH, NT>;
   using R = typename W::R;
   constexpr int CT = W::CT, TILE = W::TILE;
   const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15, nq = (Tq + 15) >> 4;
-  const int col = head * DH * 2;
   char *B = A + W::IMAGE, *C = B + W::IMAGE;
   typename R::Piece kf[NK], vf[NK];
 #pragma unroll
@@ -634,9 +641,9 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
     kf[kt] = R::piece(A + kt * TILE, g, i);
     vf[kt] = R::piece(B + kt * TILE, g, i);
   }
-  order_lds();
-  W::lay(B, grows, Tq);
-  order_lds();
+  lds_barrier();
+  W::lay(images + W::IMAGE, per_head, grows, Tq);
+  lds_barrier();
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   f32x4 absent;
 #pragma unroll
@@ -723,25 +730,23 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, const int* tq, cons
     R::put(A + kt * TILE, g, i, dk[kt]);
     R::put(B + kt * TILE, g, i, dv[kt]);
   }
-  order_lds();
-  W::store(a.dq, a.pdq, tq, Tq, col, C);
-  W::store(a.dk, a.pdk, tk, Tk, col, A);
-  W::store(a.dv, a.pdv, tk, Tk, col, B);
 }
 
 // Windows of up to 16 NT tokens; without a work list (NT = 4) every window, empty ones included.  Two waves per SIMD as the bound: 256
 // registers at most, and the matrix instructions then write plain vector registers (the backward of 64 channels by 64 tokens needs more).
 template <int DH, int NT, bool BWD> constexpr int window_lds() { return (BWD ? 3 : 2) * Window<DH, NT>::IMAGE + (BWD ? 4 * TILE_BYTES : 0); }
-template <int DH, int NT, bool BWD, bool SPLIT> __device__ __forceinline__ void window_role(const DotArgs& a, int first, int step, int head, int (*toks)[64], char* A) {
+template <int DH, int NT, bool BWD, bool SPLIT> __device__ __forceinline__ void window_role(const DotArgs& a, int first, int step, int head0, int (*toks)[64], char* images) {
   using W = Window<DH, NT>;
-  const int lane = threadIdx.x & 63;
-  if (head >= a.nhead) return;
-  const int col = head * DH * 2;
+  constexpr int PER_HEAD = window_lds<DH, NT, BWD>();
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  char* const A = images + w * PER_HEAD;
   for (Walk walk(a, NT == 4 ? 3 : 2, NT == 4 ? 3 : 2, first, step); walk.next(a);) {
     int Tq, Tk;
     walk.tokens(toks, NT * 16, Tq, Tk);
-    if (Tq == 0 || Tk == 0) {
+    if (Tq == 0 || Tk == 0) {                            // of all four waves at once: they walk the same windows
       const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+      const int col = (head0 + w) * DH * 2;
+      if (head0 + w >= a.nhead) continue;
       if (lane < Tq) {
         uint4* o = reinterpret_cast<uint4*>(BWD ? row_of(a.dq, toks[0][lane], a.pdq) + col : row_of(a.o, toks[0][lane], a.po) + col);
         for (int c = 0; c < DH / 8; ++c) o[c] = z;
@@ -753,27 +758,35 @@ template <int DH, int NT, bool BWD, bool SPLIT> __device__ __forceinline__ void 
       }
       continue;
     }
-    const typename W::Loaded krows = W::request(a.k, a.pk, toks[1], col), vrows = W::request(a.v, a.pv, toks[1], col),
-                             qrows = W::request(a.q, a.pq, toks[0], col);
+    const typename W::Loaded krows = W::request(a.k, a.pk, toks[1], head0, a.nhead), vrows = W::request(a.v, a.pv, toks[1], head0, a.nhead),
+                             qrows = W::request(a.q, a.pq, toks[0], head0, a.nhead);
     constexpr bool LATE = DH * NT >= 128;                // registers: dO is requested when K and V have left theirs
     typename W::Loaded grows;
-    if constexpr (BWD && !LATE) grows = W::request(a.g, a.pg, toks[0], col);
-    W::lay(A, krows);
-    W::lay(A + W::IMAGE, vrows, Tk);
-    if constexpr (BWD) W::lay(A + 2 * W::IMAGE, qrows);
-    order_lds();
-    if constexpr (BWD && LATE) grows = W::request(a.g, a.pg, toks[0], col);
+    if constexpr (BWD && !LATE) grows = W::request(a.g, a.pg, toks[0], head0, a.nhead);
+    lds_barrier();                                     // the window before is stored
+    W::lay(images, PER_HEAD, krows, Tk);
+    W::lay(images + W::IMAGE, PER_HEAD, vrows, Tk);
+    if constexpr (BWD) W::lay(images + 2 * W::IMAGE, PER_HEAD, qrows, Tq);
+    lds_barrier();
+    if constexpr (BWD && LATE) grows = W::request(a.g, a.pg, toks[0], head0, a.nhead);
     const int nk = (Tk + 15) >> 4;
 #define ONE(NK)                                                                                                                            \
-  if constexpr (BWD) bwd_window<DH, NT, NK, SPLIT>(a, toks[0], toks[1], Tq, Tk, head, A, grows, A + 3 * W::IMAGE);                                \
-  else fwd_window<DH, NT, NK, SPLIT>(a, toks[0], toks[1], Tq, Tk, head, A, qrows)
+  if constexpr (BWD) bwd_window<DH, NT, NK, SPLIT>(a, Tq, Tk, images, PER_HEAD, A, grows, A + 3 * W::IMAGE);                              \
+  else fwd_window<DH, NT, NK, SPLIT>(a, Tq, Tk, images, PER_HEAD, A, qrows)
     if (nk == 1) { ONE(1); }
     else if (NT == 2 || nk == 2) { ONE(2); }
     else if constexpr (NT == 4) {
       if (nk == 3) { ONE(3); } else { ONE(4); }
     }
 #undef ONE
-    order_lds();
+    lds_barrier();
+    if constexpr (BWD) {
+      W::store(a.dq, a.pdq, toks[0], Tq, head0, a.nhead, images + 2 * W::IMAGE, PER_HEAD);
+      W::store(a.dk, a.pdk, toks[1], Tk, head0, a.nhead, images, PER_HEAD);
+      W::store(a.dv, a.pdv, toks[1], Tk, head0, a.nhead, images + W::IMAGE, PER_HEAD);
+    } else {
+      W::store(a.o, a.po, toks[0], Tq, head0, a.nhead, images, PER_HEAD);
+    }
   }
 }
 
@@ -858,7 +871,7 @@ template <int DH, bool BWD, bool SPLIT, bool HALF> __device__ __forceinline__ vo
 #pragma unroll
       for (int u = 0; u < (HALF ? 1 : 2); ++u) {
         const int r = r8 + 8 * u;
-        if (r < Tq) *reinterpret_cast<uint4*>(row_of(a.o, toks[0][r], a.po) + col) = *reinterpret_cast<const uint4*>(Q + r * PITCH + ch * 16);
+        if (r < Tq) *reinterpret_cast<u32x4*>(row_of(a.o, toks[0][r], a.po) + col) = *reinterpret_cast<const u32x4*>(Q + r * PITCH + ch * 16);
       }
     }
   } else {
@@ -935,10 +948,10 @@ template <int DH, bool BWD, bool SPLIT, bool HALF> __device__ __forceinline__ vo
       for (int u = 0; u < (HALF ? 1 : 2); ++u) {
         const int r = r8 + 8 * u;
         const char* at = K + r * PITCH + ch * 16;
-        if (r < Tq) *reinterpret_cast<uint4*>(row_of(a.dq, toks[0][r], a.pdq) + col) = *reinterpret_cast<const uint4*>(at + 2 * IMAGE);
+        if (r < Tq) *reinterpret_cast<u32x4*>(row_of(a.dq, toks[0][r], a.pdq) + col) = *reinterpret_cast<const u32x4*>(at + 2 * IMAGE);
         if (r < Tk) {
-          *reinterpret_cast<uint4*>(row_of(a.dk, toks[1][r], a.pdk) + col) = *reinterpret_cast<const uint4*>(at);
-          *reinterpret_cast<uint4*>(row_of(a.dv, toks[1][r], a.pdv) + col) = *reinterpret_cast<const uint4*>(at + IMAGE);
+          *reinterpret_cast<u32x4*>(row_of(a.dk, toks[1][r], a.pdk) + col) = *reinterpret_cast<const u32x4*>(at);
+          *reinterpret_cast<u32x4*>(row_of(a.dv, toks[1][r], a.pdv) + col) = *reinterpret_cast<const u32x4*>(at + IMAGE);
         }
       }
     }
@@ -981,14 +994,14 @@ __global__ __launch_bounds__(256, (kernel_waves<DH, BWD, ROLES, SPLIT>())) void 
   int u = blockIdx.x;
   if constexpr (ROLES & ROLE4) {
     if (u < n.n4 * n.heads) {
-      window_role<DH, 4, BWD, SPLIT>(a, u / n.heads, n.n4, u % n.heads * 4 + w, toks, lds_ + w * window_lds<DH, 4, BWD>());
+      window_role<DH, 4, BWD, SPLIT>(a, u / n.heads, n.n4, u % n.heads * 4, toks, lds_);
       return;
     }
     u -= n.n4 * n.heads;
   }
   if constexpr (ROLES & ROLE2) {
     if (u < n.n2 * n.heads) {
-      window_role<DH, 2, BWD, SPLIT>(a, u / n.heads, n.n2, u % n.heads * 4 + w, toks, lds_ + w * window_lds<DH, 2, BWD>());
+      window_role<DH, 2, BWD, SPLIT>(a, u / n.heads, n.n2, u % n.heads * 4, toks, lds_);
       return;
     }
     u -= n.n2 * n.heads;
