@@ -13,8 +13,7 @@
 // operand stand in 16 rows: read straight into that layout, an instruction touches some 44 lines.  Rows therefore travel in 16-byte
 // pieces, whole pieces of a line by neighbouring lanes, through LDS images; all of a window's rows are requested at once.  Padding rows to
 // tiles is what the matrix unit pays for; three sizes of windows (up to 16, 32 and 64 tokens) keep it small.  Eight frames at stage 1
-// (375 k tokens, 8 heads of 16, bfloat16): forward 112 us, backward 73 + 111 us -- about 4 TB/s of counted HBM traffic; the movement alone,
-// without the arithmetic, took 59 + 99 us of the backward.
+// (375 k tokens, 8 heads of 16, bfloat16): forward 111 us, backward 217 us.
 //
 // A slot behind a window's last token stands for its first one: it is read, its probability is set to 0 (and V and dO are zeros there,
 // which an infinity next to them needs), and nothing is stored for it.
@@ -373,8 +372,9 @@ __global__ __launch_bounds__(256) void dot_orphan_kernel(DotArgs a, Orphans z) {
 // (logits, dP), columns (ds_read_b64_tr_b16 returns four rows of one column) for the products over tokens.  Results go back the same
 // way: into the image, and out in whole rows.
 //
-// P and dS enter their products rounded to bfloat16 (2^-8 of each; sums, maxima and everything else stay float32): their error is
-// that of the results' own rounding.
+// P and dS enter their products as the sum of two bfloat16 each (2^-15 of a probability, 2^-16 of dS; sums, maxima and everything else stay
+// float32): the results' error is that of their own rounding.  Rounded to one bfloat16 they would add as much again (2-norms: 0.0024 of the
+// gradients, not 0.0017) and save 30 of 217 us of the backward at stage 1, 5 of 85 across frames of stage 2.
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -448,56 +448,33 @@ template <int DH, int PITCH> struct Rows {
     return c;
   }
 };
-// Probabilities and their gradients on the way into the products over the tokens.  Rounded: to bfloat16 once, an error of the size of the
-// result's own rounding.  Split: as the sum of two bfloat16, 16 bits and more; the instruction takes 32 tokens, and where a tile has 16 the
-// low parts ride in its second half.  Probabilities are split towards 0 and the low part stays above it, so that an infinity in V or dO
-// meets two positive numbers.
-struct Rounded { s16x4 v; };
+// Probabilities and their gradients on the way into the products over the tokens: as the sum of two bfloat16, 16 bits and more.  The
+// instruction takes 32 tokens; where a tile has 16 the low parts ride in its second half.  Probabilities are split towards 0 and the low
+// part stays above it, so that an infinity in V or dO meets two positive numbers.
 struct Split { s16x4 hi, lo; };
-template <bool SPLIT> using Weights = typename std::conditional<SPLIT, Split, Rounded>::type;
-template <bool SPLIT> __device__ __forceinline__ Weights<SPLIT> probabilities(const f32x4& p) {
-  if constexpr (SPLIT) {
-    u32x4 cut;
-    f32x4 rest;
+__device__ __forceinline__ Split probabilities(const f32x4& p) {
+  u32x4 cut;
+  f32x4 rest;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      cut[r] = __float_as_uint(p[r]) & 0xffff0000u;
-      rest[r] = larger(p[r] - __uint_as_float(cut[r]), 1e-37f);
-    }
-    return Split{__builtin_bit_cast(s16x4, u32x2{cut[0] >> 16 | cut[1], cut[2] >> 16 | cut[3]}), pack4(rest)};
-  } else {
-    return Rounded{pack4(p)};
+  for (int r = 0; r < 4; ++r) {
+    cut[r] = __float_as_uint(p[r]) & 0xffff0000u;
+    rest[r] = larger(p[r] - __uint_as_float(cut[r]), 1e-37f);
   }
+  return Split{__builtin_bit_cast(s16x4, u32x2{cut[0] >> 16 | cut[1], cut[2] >> 16 | cut[3]}), pack4(rest)};
 }
-template <bool SPLIT> __device__ __forceinline__ Weights<SPLIT> gradients(const f32x4& d) {
-  if constexpr (SPLIT) {
-    const u32x2 h = {pack2(d[0], d[1]), pack2(d[2], d[3])};
-    const f32x4 near = {__uint_as_float(h[0] << 16), __uint_as_float(h[0] & 0xffff0000u), __uint_as_float(h[1] << 16), __uint_as_float(h[1] & 0xffff0000u)};
-    return Split{__builtin_bit_cast(s16x4, h), pack4(d - near)};
-  } else {
-    return Rounded{pack4(d)};
-  }
+__device__ __forceinline__ Split gradients(const f32x4& d) {
+  const u32x2 h = {pack2(d[0], d[1]), pack2(d[2], d[3])};
+  const f32x4 near = {__uint_as_float(h[0] << 16), __uint_as_float(h[0] & 0xffff0000u), __uint_as_float(h[1] << 16), __uint_as_float(h[1] & 0xffff0000u)};
+  return Split{__builtin_bit_cast(s16x4, h), pack4(d - near)};
 }
 __device__ __forceinline__ f32x4 product32(const s16x4& a0, const s16x4& a1, const s16x4& b0, const s16x4& b1, f32x4 c) {
   const s16x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7), b = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 // c += A B over the tokens of one tile
-__device__ __forceinline__ f32x4 over_tokens(const s16x4& a, const Rounded& b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b.v, c, 0, 0, 0);
-}
 __device__ __forceinline__ f32x4 over_tokens(const s16x4& a, const Split& b, f32x4 c) { return product32(a, a, b.hi, b.lo, c); }
-// A B over those of NK tiles (a third tile rides with zeros where nothing else does: one accumulator goes through products of one shape
-// only -- a 16x16x16 right behind the 16x16x32 that it continues has read wrong values)
-template <int NK> __device__ __forceinline__ f32x4 over_tiles(const s16x4* a, const Rounded* b) {
-  const s16x4 none = {0, 0, 0, 0};
-  f32x4 c = {0.f, 0.f, 0.f, 0.f};
-  if constexpr (NK == 1) c = over_tokens(a[0], b[0], c);
-  else
-#pragma unroll
-    for (int k = 0; k < NK; k += 2) c = k + 1 < NK ? product32(a[k], a[k + 1], b[k].v, b[k + 1].v, c) : product32(a[k], none, b[k].v, none, c);
-  return c;
-}
+// A B over those of NK tiles (one accumulator goes through products of one shape only: a 16x16x16 right behind the 16x16x32 that it
+// continues has read wrong values)
 template <int NK> __device__ __forceinline__ f32x4 over_tiles(const s16x4* a, const Split* b) {
   f32x4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -509,21 +486,20 @@ template <int NK> __device__ __forceinline__ f32x4 over_tiles(const s16x4* a, co
   return c;
 }
 // a tile of them, one column a lane, into LDS and out of it with rows and columns exchanged
-template <bool SPLIT> constexpr int WEIGHT_BYTES = SPLIT ? 2 * TILE_BYTES : TILE_BYTES;
-__device__ __forceinline__ void put_tile(char* tile, int g, int i, const Rounded& v) { *reinterpret_cast<s16x4*>(tile + i * TILE_PITCH + 8 * g) = v.v; }
+constexpr int WEIGHT_BYTES = 2 * TILE_BYTES;
 __device__ __forceinline__ void put_tile(char* tile, int g, int i, const Split& v) {
-  put_tile(tile, g, i, Rounded{v.hi});
-  put_tile(tile + TILE_BYTES, g, i, Rounded{v.lo});
+  *reinterpret_cast<s16x4*>(tile + i * TILE_PITCH + 8 * g) = v.hi;
+  *reinterpret_cast<s16x4*>(tile + TILE_BYTES + i * TILE_PITCH + 8 * g) = v.lo;
 }
-template <bool SPLIT> __device__ __forceinline__ Weights<SPLIT> turned_tile(const char* tile, int g, int i) {
+__device__ __forceinline__ Split turned_tile(const char* tile, int g, int i) {
   const char* at = tile + (4 * g + (i >> 2)) * TILE_PITCH + 8 * (i & 3);
-  if constexpr (SPLIT) return Split{read_columns(at), read_columns(at + TILE_BYTES)};
-  else return Rounded{read_columns(at)};
+  return Split{read_columns(at), read_columns(at + TILE_BYTES)};
 }
 
 // ---- windows of more than 16 tokens: a workgroup per window and four heads, a wave for each of them.  The four move the rows together,
-// whole 128-byte lines at a time, and past the cache on the way out (stage 1: 72 + 111 us backward, 74 + 119 us where each wave moves its
-// own 32 bytes of a row, 147 + 133 us where those go past the cache; stage 2 across frames 35 + 44 and 39 + 46 us).  All rows of the window
+// whole 128-byte lines at a time, and past the cache on the way out (with P and dS rounded once, backward of the large windows + the others
+// in two launches, stage 1: 72 + 111 us; 74 + 119 where each wave moves its own 32 bytes of a row, 147 + 133 where those go past the cache;
+// stage 2 across frames 35 + 44 and 39 + 46).  All rows of the window
 // are requested at once.  Forward: K and V go through the wave's two images into registers, Q takes K's place, the output Q's.  Backward:
 // K, V and Q have images; V goes into registers and dO takes its place; at the end dQ, dK and dV stand where Q, K and dO stood.
 template <int DH, int NT> struct Window {
@@ -571,7 +547,7 @@ template <int DH, int NT> struct Window {
 };
 
 // NK key tiles against nq query tiles.  NK is a template parameter, so that no branch stands between a matrix instruction and its reader.
-template <int DH, int NT, int NK, bool SPLIT>
+template <int DH, int NT, int NK>
 __device__ __forceinline__ void fwd_window(const DotArgs& a, int Tq, int Tk, char* images, int per_head, char* A, typename Window<DH, NT>::Loaded qrows) {
   using W = Window<DH, NT>;
   using R = typename W::R;
@@ -606,7 +582,7 @@ __device__ __forceinline__ void fwd_window(const DotArgs& a, int Tq, int Tk, cha
       for (int r = 0; r < 4; ++r) mx = larger(mx, st[kt][r]);
     mx = column_max(mx) * c;
     float l = 0.f;
-    Weights<SPLIT> p[NK];
+    Split p[NK];
 #pragma unroll
     for (int kt = 0; kt < NK; ++kt) {
 #pragma unroll
@@ -614,7 +590,7 @@ __device__ __forceinline__ void fwd_window(const DotArgs& a, int Tq, int Tk, cha
         st[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[kt][r], c, -mx));
         l += st[kt][r];
       }
-      p[kt] = probabilities<SPLIT>(st[kt]);
+      p[kt] = probabilities(st[kt]);
     }
     l = column_sum(l);
     f32x4 o[CT];
@@ -627,7 +603,7 @@ __device__ __forceinline__ void fwd_window(const DotArgs& a, int Tq, int Tk, cha
   }
 }
 
-template <int DH, int NT, int NK, bool SPLIT>
+template <int DH, int NT, int NK>
 __device__ __forceinline__ void bwd_window(const DotArgs& a, int Tq, int Tk, char* images, int per_head, char* A, typename Window<DH, NT>::Loaded grows,
                                            char* tiles) {
   using W = Window<DH, NT>;
@@ -684,33 +660,24 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, int Tq, int Tk, cha
       }
     const float il = __builtin_amdgcn_rcpf(column_sum(qt * 16 + i < Tq ? l : INFINITY));        // no query: P = 0
     d = column_sum(d) * il * -a.scale;
-    Weights<SPLIT> ds[NK];
-    constexpr int AT_ONCE = SPLIT ? 1 : 2, WB = WEIGHT_BYTES<SPLIT>;                // key tiles that the LDS tiles hold
+    Split ds[NK];
 #pragma unroll
-    for (int k0 = 0; k0 < NK; k0 += AT_ONCE) {
+    for (int kt = 0; kt < NK; ++kt) {
+      f32x4 t;
 #pragma unroll
-      for (int kt = k0; kt < (k0 + AT_ONCE < NK ? k0 + AT_ONCE : NK); ++kt) {
-        f32x4 t;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          p[kt][r] *= il;
-          t[r] = p[kt][r] * __builtin_fmaf(dp[kt][r], a.scale, d);
-        }
-        ds[kt] = gradients<SPLIT>(t);
-        char* tile = tiles + (kt - k0) * 2 * WB;
-        put_tile(tile, g, i, probabilities<SPLIT>(p[kt]));
-        put_tile(tile + WB, g, i, ds[kt]);
+      for (int r = 0; r < 4; ++r) {
+        p[kt][r] *= il;
+        t[r] = p[kt][r] * __builtin_fmaf(dp[kt][r], a.scale, d);
       }
+      ds[kt] = gradients(t);
+      put_tile(tiles, g, i, probabilities(p[kt]));
+      put_tile(tiles + WEIGHT_BYTES, g, i, ds[kt]);
       order_lds();
+      const Split pt = turned_tile(tiles, g, i), dt = turned_tile(tiles + WEIGHT_BYTES, g, i);      // queries 4g .. of key i
 #pragma unroll
-      for (int kt = k0; kt < (k0 + AT_ONCE < NK ? k0 + AT_ONCE : NK); ++kt) {
-        const char* tile = tiles + (kt - k0) * 2 * WB;
-        const Weights<SPLIT> pt = turned_tile<SPLIT>(tile, g, i), dt = turned_tile<SPLIT>(tile + WB, g, i);      // queries 4g .. of key i
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          dv[kt][ct] = over_tokens(gc[ct], pt, dv[kt][ct]);
-          dk[kt][ct] = over_tokens(qc[ct], dt, dk[kt][ct]);
-        }
+      for (int ct = 0; ct < CT; ++ct) {
+        dv[kt][ct] = over_tokens(gc[ct], pt, dv[kt][ct]);
+        dk[kt][ct] = over_tokens(qc[ct], dt, dk[kt][ct]);
       }
       order_lds();
     }
@@ -734,8 +701,8 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, int Tq, int Tk, cha
 
 // Windows of up to 16 NT tokens; without a work list (NT = 4) every window, empty ones included.  Two waves per SIMD as the bound: 256
 // registers at most, and the matrix instructions then write plain vector registers (the backward of 64 channels by 64 tokens needs more).
-template <int DH, int NT, bool BWD> constexpr int window_lds() { return (BWD ? 3 : 2) * Window<DH, NT>::IMAGE + (BWD ? 4 * TILE_BYTES : 0); }
-template <int DH, int NT, bool BWD, bool SPLIT> __device__ __forceinline__ void window_role(const DotArgs& a, int first, int step, int head0, int (*toks)[64], char* images) {
+template <int DH, int NT, bool BWD> constexpr int window_lds() { return (BWD ? 3 : 2) * Window<DH, NT>::IMAGE + (BWD ? 2 * WEIGHT_BYTES : 0); }
+template <int DH, int NT, bool BWD> __device__ __forceinline__ void window_role(const DotArgs& a, int first, int step, int head0, int (*toks)[64], char* images) {
   using W = Window<DH, NT>;
   constexpr int PER_HEAD = window_lds<DH, NT, BWD>();
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -771,8 +738,8 @@ template <int DH, int NT, bool BWD, bool SPLIT> __device__ __forceinline__ void 
     if constexpr (BWD && LATE) grows = W::request(a.g, a.pg, toks[0], head0, a.nhead);
     const int nk = (Tk + 15) >> 4;
 #define ONE(NK)                                                                                                                            \
-  if constexpr (BWD) bwd_window<DH, NT, NK, SPLIT>(a, Tq, Tk, images, PER_HEAD, A, grows, A + 3 * W::IMAGE);                              \
-  else fwd_window<DH, NT, NK, SPLIT>(a, Tq, Tk, images, PER_HEAD, A, qrows)
+  if constexpr (BWD) bwd_window<DH, NT, NK>(a, Tq, Tk, images, PER_HEAD, A, grows, A + 3 * W::IMAGE);                              \
+  else fwd_window<DH, NT, NK>(a, Tq, Tk, images, PER_HEAD, A, qrows)
     if (nk == 1) { ONE(1); }
     else if (NT == 2 || nk == 2) { ONE(2); }
     else if constexpr (NT == 4) {
@@ -795,7 +762,7 @@ template <int DH, int NT, bool BWD, bool SPLIT> __device__ __forceinline__ void 
 constexpr int SMALL_PITCH = 144;           // 128 bytes of a row
 
 // HALF: at most 8 tokens, one load brings a tensor's rows (rows 8 .. 15 then hold them once more)
-template <int DH, bool BWD, bool SPLIT, bool HALF> __device__ __forceinline__ void small_window(const DotArgs& a, const int (*toks)[64], int Tq, int Tk, int head0, char* K) {
+template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_window(const DotArgs& a, const int (*toks)[64], int Tq, int Tk, int head0, char* K) {
   constexpr int HG = 64 / DH, PITCH = SMALL_PITCH, IMAGE = 16 * PITCH, NI = BWD ? 4 : 3;
   using R = Rows<DH, PITCH>;
   constexpr int CT = R::CT;
@@ -836,7 +803,7 @@ template <int DH, bool BWD, bool SPLIT, bool HALF> __device__ __forceinline__ vo
   for (int r = 0; r < 4; ++r) absent[r] = 4 * g + r < Tk ? 0.f : -INFINITY;
   if constexpr (!BWD) {
     s16x4 vc[HG][CT];
-    Weights<SPLIT> p[HG];
+    Split p[HG];
     f32x4 st[HG];
     float mx[HG], l[HG];
 #pragma unroll
@@ -854,7 +821,7 @@ template <int DH, bool BWD, bool SPLIT, bool HALF> __device__ __forceinline__ vo
         st[h][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[h][r], c, -mx[h]));
         l[h] += st[h][r];
       }
-      p[h] = probabilities<SPLIT>(st[h]);
+      p[h] = probabilities(st[h]);
     }
 #pragma unroll
     for (int h = 0; h < HG; ++h) {
@@ -876,9 +843,8 @@ template <int DH, bool BWD, bool SPLIT, bool HALF> __device__ __forceinline__ vo
     }
   } else {
     s16x4 kc[HG][CT], qc[HG][CT], gc[HG][CT];
-    Weights<SPLIT> ds[HG], pt[HG], dt[HG];
+    Split ds[HG], pt[HG], dt[HG];            // (the tiles of both kinds share their place in LDS)
     f32x4 p[HG], dp[HG];
-    constexpr int WB = WEIGHT_BYTES<SPLIT>, APART = SPLIT ? 1 : 2;                 // split, the two kinds of tiles share their place
 #pragma unroll
     for (int h = 0; h < HG; ++h) {
       const int at = h * DH * 2;
@@ -910,25 +876,19 @@ template <int DH, bool BWD, bool SPLIT, bool HALF> __device__ __forceinline__ vo
         p[h][r] *= il;
         t[r] = p[h][r] * __builtin_fmaf(dp[h][r], a.scale, d);
       }
-      ds[h] = gradients<SPLIT>(t);
-      put_tile(K + h * APART * WB, g, i, probabilities<SPLIT>(p[h]));
-      if constexpr (!SPLIT) put_tile(K + (h * APART + 1) * WB, g, i, ds[h]);
+      ds[h] = gradients(t);
+      put_tile(K + h * WEIGHT_BYTES, g, i, probabilities(p[h]));
     }
     order_lds();
 #pragma unroll
-    for (int h = 0; h < HG; ++h) {
-      pt[h] = turned_tile<SPLIT>(K + h * APART * WB, g, i);
-      if constexpr (!SPLIT) dt[h] = turned_tile<SPLIT>(K + (h * APART + 1) * WB, g, i);
-    }
+    for (int h = 0; h < HG; ++h) pt[h] = turned_tile(K + h * WEIGHT_BYTES, g, i);
     order_lds();
-    if constexpr (SPLIT) {
 #pragma unroll
-      for (int h = 0; h < HG; ++h) put_tile(K + h * WB, g, i, ds[h]);
-      order_lds();
+    for (int h = 0; h < HG; ++h) put_tile(K + h * WEIGHT_BYTES, g, i, ds[h]);
+    order_lds();
 #pragma unroll
-      for (int h = 0; h < HG; ++h) dt[h] = turned_tile<SPLIT>(K + h * WB, g, i);
-      order_lds();
-    }
+    for (int h = 0; h < HG; ++h) dt[h] = turned_tile(K + h * WEIGHT_BYTES, g, i);
+    order_lds();
 #pragma unroll
     for (int h = 0; h < HG; ++h) {
       f32x4 dq[CT], dk[CT], dv[CT];
@@ -959,14 +919,14 @@ template <int DH, bool BWD, bool SPLIT, bool HALF> __device__ __forceinline__ vo
 }
 
 template <int DH, bool BWD> constexpr int small_lds() { return (BWD ? 4 : 3) * 16 * SMALL_PITCH; }             // of one wave
-template <int DH, bool BWD, bool SPLIT> __device__ __forceinline__ void small_role(const DotArgs& a, int first, int step, int head0, int (*toks)[64], char* lds) {
-  static_assert(64 / DH * 2 * TILE_BYTES <= small_lds<DH, BWD>() || !BWD, "the P and dS tiles take the images' place");
+template <int DH, bool BWD> __device__ __forceinline__ void small_role(const DotArgs& a, int first, int step, int head0, int (*toks)[64], char* lds) {
+  static_assert(64 / DH * WEIGHT_BYTES <= small_lds<DH, BWD>() || !BWD, "the P and dS tiles take the images' place");
   for (Walk walk(a, 1, 0, first, step); walk.next(a);) {
     int Tq, Tk;
     walk.tokens(toks, 16, Tq, Tk);
     if (Tq == 0 || Tk == 0) continue;                    // (in no list: the rows are zeroed elsewhere)
-    if (Tq <= 8 && Tk <= 8) small_window<DH, BWD, SPLIT, true>(a, toks, Tq, Tk, head0, lds);
-    else small_window<DH, BWD, SPLIT, false>(a, toks, Tq, Tk, head0, lds);
+    if (Tq <= 8 && Tk <= 8) small_window<DH, BWD, true>(a, toks, Tq, Tk, head0, lds);
+    else small_window<DH, BWD, false>(a, toks, Tq, Tk, head0, lds);
     order_lds();
   }
 }
@@ -980,13 +940,12 @@ template <int DH, bool BWD, int ROLES> constexpr int kernel_lds() {
             l1 = ROLES & ROLE1 ? small_lds<DH, BWD>() : 0;
   return 4 * (l4 > l2 ? (l4 > l1 ? l4 : l1) : (l2 > l1 ? l2 : l1));
 }
-template <int DH, bool BWD, int ROLES, bool SPLIT> constexpr int kernel_waves() {        // waves per SIMD that the registers allow
+template <int DH, bool BWD, int ROLES> constexpr int kernel_waves() {        // waves per SIMD that the registers allow
   if (!BWD) return DH == 16 ? 4 : DH == 32 ? 3 : 2;
-  if (SPLIT) return DH == 16 ? 2 : 1;
   return ROLES & ROLE4 ? (DH == 16 ? 3 : DH == 32 ? 2 : 1) : (DH == 16 ? 4 : DH == 32 ? 3 : 2);
 }
-template <int DH, bool BWD, int ROLES, bool SPLIT>
-__global__ __launch_bounds__(256, (kernel_waves<DH, BWD, ROLES, SPLIT>())) void dot_kernel(DotArgs a, Roles n, Orphans z) {
+template <int DH, bool BWD, int ROLES>
+__global__ __launch_bounds__(256, (kernel_waves<DH, BWD, ROLES>())) void dot_kernel(DotArgs a, Roles n, Orphans z) {
   extern __shared__ __attribute__((aligned(16))) char lds_[];
   __shared__ int toks_[4][2][64];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -994,21 +953,21 @@ __global__ __launch_bounds__(256, (kernel_waves<DH, BWD, ROLES, SPLIT>())) void 
   int u = blockIdx.x;
   if constexpr (ROLES & ROLE4) {
     if (u < n.n4 * n.heads) {
-      window_role<DH, 4, BWD, SPLIT>(a, u / n.heads, n.n4, u % n.heads * 4, toks, lds_);
+      window_role<DH, 4, BWD>(a, u / n.heads, n.n4, u % n.heads * 4, toks, lds_);
       return;
     }
     u -= n.n4 * n.heads;
   }
   if constexpr (ROLES & ROLE2) {
     if (u < n.n2 * n.heads) {
-      window_role<DH, 2, BWD, SPLIT>(a, u / n.heads, n.n2, u % n.heads * 4, toks, lds_);
+      window_role<DH, 2, BWD>(a, u / n.heads, n.n2, u % n.heads * 4, toks, lds_);
       return;
     }
     u -= n.n2 * n.heads;
   }
   if constexpr (ROLES & ROLE1) {
     if (u < n.n1 * n.columns) {
-      small_role<DH, BWD, SPLIT>(a, u / n.columns * 4 + w, n.n1 * 4, u % n.columns * (64 / DH), toks, lds_ + w * small_lds<DH, BWD>());
+      small_role<DH, BWD>(a, u / n.columns * 4 + w, n.n1 * 4, u % n.columns * (64 / DH), toks, lds_ + w * small_lds<DH, BWD>());
       return;
     }
     u -= n.n1 * n.columns;
@@ -1058,11 +1017,11 @@ template <class F> void by_head(int dh, F&& f) {
   else if (dh == 32) f(std::integral_constant<int, 32>());
   else f(std::integral_constant<int, 64>());
 }
-template <int DH, bool BWD, int ROLES, bool SPLIT> int launch_roles(const DotArgs& a, const Orphans& z, int64_t w4, int64_t w2, int64_t w1, hipStream_t stream) {
+template <int DH, bool BWD, int ROLES> int launch_roles(const DotArgs& a, const Orphans& z, int64_t w4, int64_t w2, int64_t w1, hipStream_t stream) {
   constexpr int LDS = kernel_lds<DH, BWD, ROLES>();
   static TmaeLdsAttr attr;
   if (LDS + 2048 > 65536)
-    if (int e = tmae_allow_lds(attr, (const void*)dot_kernel<DH, BWD, ROLES, SPLIT>, LDS)) return e;
+    if (int e = tmae_allow_lds(attr, (const void*)dot_kernel<DH, BWD, ROLES>, LDS)) return e;
   Roles n;
   n.heads = (a.nhead + 3) / 4;
   n.columns = (a.nhead * DH + 63) / 64;
@@ -1071,24 +1030,23 @@ template <int DH, bool BWD, int ROLES, bool SPLIT> int launch_roles(const DotArg
   n.n1 = ROLES & ROLE1 ? (int)walkers(w1, 4, n.columns) : 0;
   n.n0 = ROLES & ROLE1 && z.row16 ? (int)walkers(a.nwin, 16, 1, 1) : 0;
   const int64_t blocks = (int64_t)(n.n4 + n.n2) * n.heads + (int64_t)n.n1 * n.columns + n.n0;
-  if (blocks > 0) hipLaunchKernelGGL((dot_kernel<DH, BWD, ROLES, SPLIT>), dim3((unsigned)blocks), dim3(256), LDS, stream, a, n, z);
+  if (blocks > 0) hipLaunchKernelGGL((dot_kernel<DH, BWD, ROLES>), dim3((unsigned)blocks), dim3(256), LDS, stream, a, n, z);
   return TMAE_OK;
 }
-// Forward: one launch, the probabilities split: eight frames at stage 1 (375 k tokens, 8 heads of 16) 114 us, 109 us rounded, 114 us
-// rounded in two launches; stage 2 (33 k queries, 131 k keys, 8 heads of 32) 44, 45 and 42 us.  Backward: split, the tiles that turn in LDS
-// are twice as many, and in one launch every workgroup has the registers and LDS of the largest windows: 199 and 85 us rounded in two
-// launches, 271 and 144 us split in one.  So only few tokens take that, whose time is the launch, and whose few results would show a
-// rounding as large as their own.
+// One launch for all sizes of windows: its workgroups have the registers and the LDS of the largest ones, a second launch costs its own
+// tail.  Backward of heads of 16: 217 us in one launch and 219 in two for eight frames at stage 1 (375 k tokens), 11 and 17 for one of 8 k
+// tokens; heads of 32 across frames (33 k queries, 131 k keys): 85 and 85.  Of heads of 64 the largest windows leave room for one workgroup
+// a CU: 20 and 24 us with 16 k queries and keys, 27 and 27 with 32 k, 49 and 44 with 64 k, 120 and 97 with 188 k.
 template <int DH, bool BWD> int launch_bf16(const DotArgs& a, const Orphans& z, hipStream_t stream) {
   const int64_t w4 = a.wl ? class_windows(a, 3) : a.nwin, w2 = class_windows(a, 2), w1 = class_windows(a, 0);
-  constexpr int ALL = ROLE4 | ROLE2 | ROLE1;
-  if constexpr (BWD) {
-    if (a.mq + a.mk > 8192) {
-      const int rc = launch_roles<DH, BWD, ROLE4, false>(a, z, w4, w2, w1, stream);
-      return rc != TMAE_OK || !a.wl ? rc : launch_roles<DH, BWD, ROLE2 | ROLE1, false>(a, z, w4, w2, w1, stream);
+  if (!a.wl) return launch_roles<DH, BWD, ROLE4>(a, z, w4, w2, w1, stream);
+  if constexpr (BWD && DH == 64) {
+    if (a.mq + a.mk > 32768) {
+      const int rc = launch_roles<DH, BWD, ROLE4>(a, z, w4, w2, w1, stream);
+      return rc != TMAE_OK ? rc : launch_roles<DH, BWD, ROLE2 | ROLE1>(a, z, w4, w2, w1, stream);
     }
   }
-  return a.wl ? launch_roles<DH, BWD, ALL, true>(a, z, w4, w2, w1, stream) : launch_roles<DH, BWD, ROLE4, true>(a, z, w4, w2, w1, stream);
+  return launch_roles<DH, BWD, ROLE4 | ROLE2 | ROLE1>(a, z, w4, w2, w1, stream);
 }
 template <int DH, bool BWD> int launch_f32(const DotArgs& a, const Orphans& z, hipStream_t stream) {
   if (z.row16) hipLaunchKernelGGL(dot_orphan_kernel, dim3(walkers(a.nwin, 4, 1)), dim3(256), 0, stream, a, z);

@@ -659,3 +659,61 @@ def test_infinities_in_large_calls(heads, dh):
         o = ops.win_attn_dot(q.cuda(), k.cuda(), leaf, gr, gr, heads, batch, ny, nx, False, worklist=worklist, covered=True)
         dv = torch.autograd.grad(o, leaf, do.cuda())[0].cpu().float()
         assert torch.isfinite(o).all() and (dv[touched] == float('inf')).all() and torch.isfinite(dv[~touched]).all()
+
+
+TWO_PARTS = 2.0 ** -15         # a probability as two bfloat16: cut to 8 bits (the rest is below 2^-7 of it), the rest rounded (2^-8 of that)
+
+
+def two_parts(p):
+    high = (p.float().view(torch.int32) & -65536).view(torch.float32)
+    return high.double() + (p.float() - high).bfloat16().double()
+
+
+def test_the_tolerance_tells_one_rounding_of_the_probabilities_from_two_parts():
+    """The bound of the next test holds for P and dS as two bfloat16 and not for either of them rounded to one."""
+    case = [c for c in CASES if c[0] == 'ragged'][0]
+    q, k, v, do, _, _, same = (t.double() if t.is_floating_point() else t for t in make(case))
+    h, scale = 8, 0.4
+    want, tolerances = reference(q, k, v, do, same, h, scale)
+    tols = [t + half_step(torch.bfloat16) * w.abs() for t, w in zip(tolerances(TWO_PARTS), want)]
+    heads = lambda t: t.view(t.shape[0], h, -1).transpose(0, 1)                        # noqa: E731
+    rows = lambda t: t.transpose(0, 1).reshape(t.shape[1], -1)                         # noqa: E731
+    p = torch.softmax((heads(q) @ heads(k).transpose(1, 2) * scale).masked_fill(~same, -float('inf')), -1)
+    dp = heads(do) @ heads(v).transpose(1, 2)
+    ds = scale * p * (dp - (p * dp).sum(-1, keepdim=True))
+    for part, fits in ((two_parts, True), (lambda t: t.bfloat16().double(), False)):
+        results = (part(p) @ heads(v), part(ds) @ heads(k), part(ds).transpose(1, 2) @ heads(q), part(p).transpose(1, 2) @ heads(do))
+        for got, w, tol in zip(results, want, tols):
+            assert ((rows(got).bfloat16().double() - w).abs() <= tol).all() == fits
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('worklist', [True, False])
+@pytest.mark.parametrize('batch', [1, 9])
+@pytest.mark.parametrize('heads,dh,shift,cross', [(8, 16, False, False), (3, 16, True, True), (4, 32, True, False), (3, 32, False, True),
+                                                  (2, 64, False, False), (1, 64, True, True)])
+def test_probabilities_and_their_gradients_keep_two_parts(heads, dh, shift, cross, batch, worklist):
+    """bfloat16 results carry their own rounding and P and dS as two bfloat16, however many tokens the call has: the first and the last
+    frame against the definition, with 2^-15 of a probability where `test_many_frames` allows a rounding of 2^-8."""
+    from tmae_amd import ops
+    g = torch.Generator().manual_seed(dh + heads + batch)
+    ny, nx, d, e = 40, 41, heads * dh, half_step(torch.bfloat16)
+    counts = [(1300, 300, 700, 60, 1640)[b % 5] for b in range(batch)]
+    grid_q, at_q = place(counts, batch, ny, nx, g)
+    grid_k, at_k = place(counts[::-1], batch, ny, nx, g) if cross else (grid_q, at_q)
+    mq, mk = at_q.shape[0], at_k.shape[0]
+    assert (mq + mk > 8192) == (batch > 1)
+    q, do = (torch.randn(mq, d, generator=g).bfloat16() for _ in range(2))
+    k, v = (torch.randn(mk, d, generator=g).bfloat16() for _ in range(2))
+    gq = grid_q.cuda()
+    gk = grid_k.cuda() if cross else gq
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    wl = ops.window_worklist(gq, gk, batch, ny, nx, shift) if worklist else None
+    o = ops.win_attn_dot(*leaves, gq, gk, heads, batch, ny, nx, shift, worklist=wl, covered=True)
+    got = [o, *torch.autograd.grad(o, leaves, do.cuda())]
+    for frame in {0, batch - 1}:
+        fq, fk = at_q[:, 0] == frame, at_k[:, 0] == frame
+        same = window_of(at_q[fq], shift)[:, None] == window_of(at_k[fk], shift)[None]
+        want, tolerances = reference(q[fq].double(), k[fk].double(), v[fk].double(), do[fq].double(), same, heads, dh ** -0.5)
+        for what, t, rows, w, tol in zip(('out', 'dq', 'dk', 'dv'), got, (fq, fq, fk, fk), want, tolerances(TWO_PARTS)):
+            within(t[rows.cuda()], w, tol + e * w.abs(), f'{what} of frame {frame}')
