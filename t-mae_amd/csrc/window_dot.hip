@@ -924,7 +924,7 @@ template <int DH, bool BWD> __device__ __forceinline__ void small_role(const Dot
   for (Walk walk(a, 1, 0, first, step); walk.next(a);) {
     int Tq, Tk;
     walk.tokens(toks, 16, Tq, Tk);
-    if (Tq == 0 || Tk == 0) continue;                    // (in no list: the rows are zeroed elsewhere)
+    if (Tq == 0 || Tk == 0) continue;                    // (the rows are zeroed by those who look for such windows)
     if (Tq <= 8 && Tk <= 8) small_window<DH, BWD, true>(a, toks, Tq, Tk, head0, lds);
     else small_window<DH, BWD, false>(a, toks, Tq, Tk, head0, lds);
     order_lds();
@@ -985,10 +985,12 @@ unsigned walkers(int64_t windows, int per_group, unsigned gx, int per_cu = 6) {
   if (most < 1) most = 1;
   return (unsigned)(need < most ? need : most);
 }
-// windows that a class of a work list can hold: class c > 0 windows hold more than 8 * 2^(c-1) tokens of one of the two frames
+// windows that a class of a work list can hold, where the grids hold rows only: class c > 0 windows have more than 8 * 2^(c-1) tokens of one
+// of the two frames.  The list counts entries that are no row as well, so that a class may hold windows that these numbers rule out: one
+// workgroup at least walks every class, and a walk goes through the whole of it.
 int64_t class_windows(const DotArgs& a, int cls) {
   const int64_t most = (a.mq + a.mk) / (cls == 0 ? 2 : cls == 1 ? 9 : cls == 2 ? 17 : 33);
-  return most < a.nwin ? most : a.nwin;
+  return most < 1 ? 1 : most < a.nwin ? most : a.nwin;
 }
 
 bool rows_ok(const void* p, int64_t ld, int width, int es) {

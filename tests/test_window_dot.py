@@ -717,3 +717,33 @@ def test_probabilities_and_their_gradients_keep_two_parts(heads, dh, shift, cros
         want, tolerances = reference(q[fq].double(), k[fk].double(), v[fk].double(), do[fq].double(), same, heads, dh ** -0.5)
         for what, t, rows, w, tol in zip(('out', 'dq', 'dk', 'dv'), got, (fq, fq, fk, fk), want, tolerances(TWO_PARTS)):
             within(t[rows.cuda()], w, tol + e * w.abs(), f'{what} of frame {frame}')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('cross', [False, True])
+@pytest.mark.parametrize('cells', [12, 20, 64])
+def test_windows_listed_for_more_cells_than_there_are_rows(cells, cross, dtype):
+    """Five rows in a window whose other cells hold numbers that are no rows, and the work list of that very grid: the list puts the
+    window among those of `cells` tokens, and every row of it is written."""
+    from tmae_amd import ops
+    g = torch.Generator().manual_seed(cells)
+    m, d = 5, 64
+
+    def window():
+        grid = torch.full((64,), -1, dtype=torch.int32)
+        at = torch.randperm(64, generator=g)[:cells]
+        grid[at] = torch.arange(cells, dtype=torch.int32) + m
+        grid[at[:m]] = torch.arange(m, dtype=torch.int32)
+        return grid.cuda()
+    gq = window()
+    gk = window() if cross else gq
+    q, k, v, do = (torch.randn(m, d, generator=g).to(dtype) for _ in range(4))
+    want, tolerances = reference(q.double(), k.double(), v.double(), do.double(), torch.ones(m, m, dtype=torch.bool), 4, 0.25)
+    wl = ops.window_worklist(gq, gk, 1, 8, 8, False)
+    for covered in (False, True):
+        leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+        o = ops.win_attn_dot(*leaves, gq, gk, 4, 1, 8, 8, False, worklist=wl, covered=covered)
+        grads = torch.autograd.grad(o, leaves, do.cuda())
+        for what, got, w, t in zip(('out', 'dq', 'dk', 'dv'), (o, *grads), want, tolerances(half_step(dtype))):
+            within(got, w, t, what)
