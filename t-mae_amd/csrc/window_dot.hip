@@ -450,7 +450,8 @@ template <int DH, int PITCH> struct Rows {
 };
 // Probabilities and their gradients on the way into the products over the tokens: as the sum of two bfloat16, 16 bits and more.  The
 // instruction takes 32 tokens; where a tile has 16 the low parts ride in its second half.  Probabilities are split towards 0 and the low
-// part stays above it, so that an infinity in V or dO meets two positive numbers.
+// part of one above 0 stays above it (the median of the rest, the smallest normal number and the probability), so that an infinity in V or
+// dO meets two positive numbers; of 0 both parts are 0.
 struct Split { s16x4 hi, lo; };
 __device__ __forceinline__ Split probabilities(const f32x4& p) {
   u32x4 cut;
@@ -458,7 +459,7 @@ __device__ __forceinline__ Split probabilities(const f32x4& p) {
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     cut[r] = __float_as_uint(p[r]) & 0xffff0000u;
-    rest[r] = larger(p[r] - __uint_as_float(cut[r]), 1e-37f);
+    rest[r] = __builtin_amdgcn_fmed3f(p[r] - __uint_as_float(cut[r]), 0x1p-126f, p[r]);
   }
   return Split{__builtin_bit_cast(s16x4, u32x2{cut[0] >> 16 | cut[1], cut[2] >> 16 | cut[3]}), pack4(rest)};
 }

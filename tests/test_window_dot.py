@@ -747,3 +747,40 @@ def test_windows_listed_for_more_cells_than_there_are_rows(cells, cross, dtype):
         grads = torch.autograd.grad(o, leaves, do.cuda())
         for what, got, w, t in zip(('out', 'dq', 'dk', 'dv'), (o, *grads), want, tolerances(half_step(dtype))):
             within(got, w, t, what)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('heads,dh', [(5, 16), (2, 32), (1, 64)])
+def test_a_key_of_probability_zero_adds_nothing(heads, dh, dtype):
+    """One key of every window has logits of -2^17 and less, so that its probabilities are 0, and V of the type's largest and lowest
+    values: out is that of the other keys, and its own dV is 0."""
+    from tmae_amd import ops
+    g = torch.Generator().manual_seed(heads)
+    ny, d = 40, heads * dh
+    for count in (300, 900, 1600):
+        grid, at = place([count], 1, ny, ny, g)
+        win = window_of(at, False)
+        masked = torch.zeros(count, dtype=torch.bool)
+        for w in win.unique():
+            rows = (win == w).nonzero()[:, 0]
+            if rows.numel() > 1:
+                masked[rows[torch.randint(rows.numel(), (1,), generator=g)]] = True
+        q, k, v, do = (torch.randn(count, d, generator=g).to(dtype) for _ in range(4))
+        q.view(count, heads, dh)[..., 3] = -2.0 ** 10
+        k.view(count, heads, dh)[..., 3] = 0.0
+        k.view(count, heads, dh)[masked, :, 3] = 2.0 ** 10
+        v[masked] = torch.where(torch.rand(int(masked.sum()), d, generator=g) < 0.5, 1, -1).to(dtype) * torch.finfo(dtype).max
+        gr = grid.cuda()
+        same = (win[:, None] == win[None]) & ~masked[None]
+        clean = v.double()
+        clean[masked] = 0.0
+        want, tolerances = reference(q.double(), k.double(), clean, do.double(), same, heads, dh ** -0.5)
+        tols = tolerances(half_step(dtype))
+        for worklist in (None, ops.window_worklist(gr, gr, 1, ny, ny, False)):
+            leaf = v.cuda().requires_grad_()
+            o = ops.win_attn_dot(q.cuda(), k.cuda(), leaf, gr, gr, heads, 1, ny, ny, False, worklist=worklist, covered=True)
+            dv, = torch.autograd.grad(o, leaf, do.cuda())
+            within(o, want[0], tols[0], 'out')
+            within(dv, want[3], tols[3], 'dv')
+            assert not dv[masked.cuda()].any()
