@@ -275,7 +275,7 @@ template <int DH, int NT, bool BWD> __device__ __forceinline__ void f32_role(con
       if constexpr (BWD) {
         d = lanes4_sum(d) * il;
         const int row = hh * ROWS + t * 16 + i;
-        if (g == 0) { top[row] = mx; inv[row] = t * 16 + i < Tq ? il : 0.f; dot[row] = d; }          // no query: P = 0
+        if (g == 0) { top[row] = mx; inv[row] = t * 16 + i < Tq ? il : 0.f; dot[row] = d; }          // no query: P = dS = 0
 #pragma unroll
         for (int kt = 0; kt < NT; ++kt) {
           if (kt < nk) {
@@ -301,8 +301,9 @@ template <int DH, int NT, bool BWD> __device__ __forceinline__ void f32_role(con
           const int row = hh * ROWS + qt * 16 + 4 * g;                              // rows = queries, column = key i
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            p[r] = inv[row + r] != 0.f ? __builtin_amdgcn_exp2f(fmaf(p[r], c, -top[row + r])) * inv[row + r] : 0.f;
-            ds[r] = p[r] * (ds[r] - dot[row + r]);
+            const bool present = inv[row + r] != 0.f;
+            p[r] = present ? __builtin_amdgcn_exp2f(fmaf(p[r], c, -top[row + r])) * inv[row + r] : 0.f;
+            ds[r] = present ? p[r] * (ds[r] - dot[row + r]) : 0.f;
           }
           R::over_tokens(G + qt * TILE, p, dv, g, i);
           R::over_tokens(Q + qt * TILE, ds, dk, g, i);
@@ -659,7 +660,8 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, int Tq, int Tk, cha
         l += p[kt][r];
         d = __builtin_fmaf(p[kt][r], dp[kt][r], d);
       }
-    const float il = __builtin_amdgcn_rcpf(column_sum(qt * 16 + i < Tq ? l : INFINITY));        // no query: P = 0
+    const bool present = qt * 16 + i < Tq;                                         // no query: P = dS = 0, whatever the keys hold
+    const float il = __builtin_amdgcn_rcpf(column_sum(l));
     d = column_sum(d) * il * -a.scale;
     Split ds[NK];
 #pragma unroll
@@ -667,8 +669,8 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, int Tq, int Tk, cha
       f32x4 t;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        p[kt][r] *= il;
-        t[r] = p[kt][r] * __builtin_fmaf(dp[kt][r], a.scale, d);
+        p[kt][r] = present ? p[kt][r] * il : 0.f;
+        t[r] = present ? p[kt][r] * __builtin_fmaf(dp[kt][r], a.scale, d) : 0.f;
       }
       ds[kt] = gradients(t);
       put_tile(tiles, g, i, probabilities(p[kt]));
@@ -869,13 +871,13 @@ template <int DH, bool BWD, bool HALF> __device__ __forceinline__ void small_win
         l += p[h][r];
         d = __builtin_fmaf(p[h][r], dp[h][r], d);
       }
-      const float il = __builtin_amdgcn_rcpf(column_sum(i < Tq ? l : INFINITY));              // no query: P = 0
+      const float il = __builtin_amdgcn_rcpf(column_sum(l));
       d = column_sum(d) * il * -a.scale;
       f32x4 t;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        p[h][r] *= il;
-        t[r] = p[h][r] * __builtin_fmaf(dp[h][r], a.scale, d);
+        p[h][r] = i < Tq ? p[h][r] * il : 0.f;                                       // no query: P = dS = 0, whatever the keys hold
+        t[r] = i < Tq ? p[h][r] * __builtin_fmaf(dp[h][r], a.scale, d) : 0.f;
       }
       ds[h] = gradients(t);
       put_tile(K + h * WEIGHT_BYTES, g, i, probabilities(p[h]));

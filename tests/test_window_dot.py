@@ -784,3 +784,45 @@ def test_a_key_of_probability_zero_adds_nothing(heads, dh, dtype):
             within(o, want[0], tols[0], 'out')
             within(dv, want[3], tols[3], 'dv')
             assert not dv[masked.cuda()].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('heads,dh', [(5, 16), (2, 32), (1, 64)])
+def test_a_key_that_infinity_masks(heads, dh, dtype):
+    """One key of every window holds an infinity where all queries are negative: its logits are -inf, its probabilities 0.  The results are
+    those of the other keys: nothing of it reaches them over the slots behind a window's last query (0 times an infinity).  Its own dK and
+    dV are 0, and only that channel of dQ (0 times the infinity) has no value."""
+    from tmae_amd import ops
+    g = torch.Generator().manual_seed(heads)
+    ny, d = 40, heads * dh
+    for count in (300, 900, 1600, 9 * 900):                                             # 1 to 64 tokens a window; one frame, or nine
+        batch = max(1, count // 1600)
+        count = count // batch
+        grid, at = place([count] * batch, batch, ny, ny, g)
+        win = window_of(at, False)
+        n = at.shape[0]
+        masked = torch.zeros(n, dtype=torch.bool)
+        for w in win.unique():
+            rows = (win == w).nonzero()[:, 0]
+            if rows.numel() > 1:
+                masked[rows[torch.randint(rows.numel(), (1,), generator=g)]] = True
+        q, k, v, do = (torch.randn(n, d, generator=g).to(dtype) for _ in range(4))
+        q[:, 3] = -q[:, 3].abs() - 0.125
+        k[masked, 3] = float('inf')
+        gr = grid.cuda()
+        tail = at[:, 0] == batch - 1                                                    # a frame of them against the definition
+        same = (win[tail][:, None] == win[tail][None]) & ~masked[tail][None]
+        clean = k[tail].double()
+        clean[masked[tail], 3] = 0.0
+        # (of heads without the infinity the key is not masked: the first head alone)
+        want, tolerances = reference(q[tail, :dh].double(), clean[:, :dh], v[tail, :dh].double(), do[tail, :dh].double(), same, 1, dh ** -0.5)
+        for worklist in (None, ops.window_worklist(gr, gr, batch, ny, ny, False)):
+            leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+            o = ops.win_attn_dot(*leaves, gr, gr, heads, batch, ny, ny, False, worklist=worklist, covered=True)
+            grads = torch.autograd.grad(o, leaves, do.cuda())
+            for what, got, w, t in zip(('out', 'dq', 'dk', 'dv'), (o, *grads), want, tolerances(half_step(dtype))):
+                got = got.detach().cpu()
+                channels = torch.arange(dh) if what != 'dq' else torch.tensor([c for c in range(dh) if c != 3])
+                assert torch.isfinite(got[:, [c for c in range(d) if what != 'dq' or c != 3]]).all(), what
+                within(got[tail][:, channels], w[:, channels], t[:, channels], what)
