@@ -24,7 +24,8 @@ namespace {
 constexpr int MAX_AXES = 4;
 constexpr int TABLE_PAIRS = 2048;          // cos / sin pairs of a tile: 16 KB of LDS
 
-enum { MODE_ADJACENT = 0, MODE_SPLIT = 1, MODE_SPLIT_ANY = 2 };
+// how the pairs lie: (2i, 2i+1) or (i, i + P); P a multiple of 4 or any (the selects that another P takes cost 5 % where they are not needed)
+enum { MODE_ADJACENT = 0, MODE_SPLIT = 1, MODE_SPLIT_ANY = 2, MODE_ADJACENT_ANY = 3 };
 
 struct RotaryArgs {
   const void* x; int64_t ldx, hpx;         // [n, h, dh]: row pitch and head pitch in elements, channels contiguous
@@ -32,7 +33,7 @@ struct RotaryArgs {
   void* y;                                 // contiguous [n, h, dh] (dx in the backward)
   int64_t n; int h, q_heads, dh;
   const void* pos; int64_t ldpos; int pos_kind;                     // 0 int32, 1 int64, 2 float32
-  const double* inv_freq; int P, PT;       // PT: pairs of a table row, P rounded up to 4 (the padding turns by nothing)
+  const double* inv_freq; int P, PT;       // PT: pairs of a table row, P rounded up to 4
   int sec_end[MAX_AXES];                   // pairs [sec_end[a-1], sec_end[a]) turn by axis a
   float sign;                              // -1: the inverse rotation
   const float* q_gain; const float* k_gain; int gain_pitch;         // 0: one gain for all heads
@@ -174,14 +175,15 @@ __device__ __forceinline__ float turned_second(float p, float q, float2 w) { ret
 // turns the unit's channels in place; cs: the token's row of the table, xch: the 8 floats of every lane of the wave (MODE_SPLIT_ANY)
 template <int MODE>
 __device__ __forceinline__ void turn_unit(const RotaryArgs& a, int u, const float2* cs, float* v, float* xch) {
-  if constexpr (MODE == MODE_ADJACENT) {
+  if constexpr (MODE == MODE_ADJACENT || MODE == MODE_ADJACENT_ANY) {
     if (4 * u < a.P) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 w = cs[4 * u + j];
         const float p = v[2 * j], q = v[2 * j + 1];
-        v[2 * j] = turned_first(p, q, w);
-        v[2 * j + 1] = turned_second(p, q, w);
+        const bool turns = MODE == MODE_ADJACENT || 4 * u + j < a.P;          // the padding turns by 0: no way past an infinity
+        v[2 * j] = turns ? turned_first(p, q, w) : p;
+        v[2 * j + 1] = turns ? turned_second(p, q, w) : q;
       }
     }
   } else if constexpr (MODE == MODE_SPLIT) {
@@ -455,11 +457,15 @@ int fill_args(RotaryArgs& a, const void* x, int64_t ldx, int64_t hpx, int dtype,
 }
 
 // (MODE, VEC): vector accesses need 16-byte rows and whole units; pairs (i, i + P) can then stay in one lane when P is a multiple of 4
+template <int MODE, class F> void by_access(bool vec, F&& f) {
+  if (vec) f(std::integral_constant<int, MODE>(), std::true_type());
+  else f(std::integral_constant<int, MODE>(), std::false_type());
+}
 template <class F> void by_layout(const RotaryArgs& a, bool interleaved, bool vec, F&& f) {
-  if (interleaved) { if (vec) f(std::integral_constant<int, MODE_ADJACENT>(), std::true_type()); else f(std::integral_constant<int, MODE_ADJACENT>(), std::false_type()); }
+  if (interleaved && a.P % 4 == 0) by_access<MODE_ADJACENT>(vec, f);
+  else if (interleaved) by_access<MODE_ADJACENT_ANY>(vec, f);
   else if (vec && a.P % 4 == 0) f(std::integral_constant<int, MODE_SPLIT>(), std::true_type());
-  else if (vec) f(std::integral_constant<int, MODE_SPLIT_ANY>(), std::true_type());
-  else f(std::integral_constant<int, MODE_SPLIT_ANY>(), std::false_type());
+  else by_access<MODE_SPLIT_ANY>(vec, f);
 }
 
 template <class T, bool NORM> void launch_fwd(const RotaryArgs& a, bool interleaved, bool vec, hipStream_t stream) {

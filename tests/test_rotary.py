@@ -384,3 +384,43 @@ def test_rows_beyond_32_bits():
         return [t.detach() for t in (r, y, *torch.autograd.grad(r, x, dy), *torch.autograd.grad(y, x, dy))]
     for a, b in zip(run(x, dy, pos), run(x[-last:], dy[-last:], pos[-last:])):
         assert torch.equal(a[-last:], b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('value', [float('inf'), -float('inf'), float('nan')])
+@pytest.mark.parametrize('interleaved', [False, True])
+@pytest.mark.parametrize('sections,dh,dtype', [((3,), 16, torch.bfloat16), ((2, 3), 24, torch.float32), ((1,), 7, torch.float32), ((3, 4), 24, torch.bfloat16)])
+def test_a_bad_value_that_does_not_turn_stays_in_its_channel(sections, dh, dtype, interleaved, value):
+    """Channels from 2 P on pass as they are, whatever stands beside them: in rotary_axes, in the gains of qk_norm_rotary, and in the
+    gradient that comes back to it."""
+    from tmae_amd import ops
+    n, h, p = 67, 3, sum(sections)
+    f = ops.rotary_freqs(sections, device='cuda')
+    g = torch.Generator(device='cuda').manual_seed(dh)
+    pos = torch.randint(0, 99, (n, len(sections)), device='cuda', generator=g)
+    x = torch.randn(n, h, dh, device='cuda', generator=g).to(dtype)
+    clean = ops.rotary_axes(x, pos, f, sections, interleaved=interleaved)
+    gain = torch.rand(dh, device='cuda', generator=g) + 0.5
+    normed = ops.qk_norm_rotary(x, gain, gain, pos, f, sections, q_heads=h, interleaved=interleaved)
+
+    def others(c):
+        return [e for e in range(dh) if e != c]
+    for c in range(2 * p, dh):
+        bad = x.clone()
+        bad[..., c] = value
+        leaf = bad.clone().requires_grad_()
+        y = ops.rotary_axes(leaf, pos, f, sections, interleaved=interleaved)
+        back = ops.rotary_axes(bad, pos, f, sections, interleaved=interleaved, inverse=True)
+        dx, = torch.autograd.grad(y, leaf, bad)
+        for t in (y, back, dx):
+            assert torch.equal(t[..., 2 * p:].isnan(), bad[..., 2 * p:].isnan())
+            assert torch.equal(t[..., 2 * p:].nan_to_num(7.0), bad[..., 2 * p:].nan_to_num(7.0))
+        assert torch.equal(y[..., others(c)], clean[..., others(c)])
+        wrong = gain.clone()
+        wrong[c] = value
+        y = ops.qk_norm_rotary(x, wrong, wrong, pos, f, sections, q_heads=h, interleaved=interleaved)
+        assert torch.equal(y[..., others(c)], normed[..., others(c)])
+        leaves = [gain.clone().requires_grad_(), x.clone().requires_grad_()]
+        y = ops.qk_norm_rotary(leaves[1], leaves[0], None, pos, f, sections, interleaved=interleaved)
+        dg, = torch.autograd.grad(y, leaves[:1], bad)
+        assert torch.isfinite(dg[others(c)]).all() and not torch.isfinite(dg[c])
