@@ -8,6 +8,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
@@ -1781,6 +1782,8 @@ def _once(backward):
     checked = once_differentiable(backward)
 
     def call(ctx, *grads):
+        if forward_ad._current_level >= 0 and any(g is not None and forward_ad.unpack_dual(g).tangent is not None for g in grads):
+            raise NotImplementedError('tmae_amd: forward-mode derivatives of this backward pass are not there')
         if torch.is_grad_enabled():
             return checked(ctx, *(None if g is None else g.detach().requires_grad_() for g in grads))
         return backward(ctx, *grads)
@@ -1788,6 +1791,10 @@ def _once(backward):
 
 
 def _grad_on(*tensors):
+    """Whether the call goes through its autograd Function: gradients are recorded, or a level of forward-mode derivatives is open (the
+    Function refuses a tensor that has a tangent; past it, the tangent would be lost)."""
+    if forward_ad._current_level >= 0:
+        return True
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:

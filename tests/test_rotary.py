@@ -424,3 +424,34 @@ def test_a_bad_value_that_does_not_turn_stays_in_its_channel(sections, dh, dtype
         y = ops.qk_norm_rotary(leaves[1], leaves[0], None, pos, f, sections, interleaved=interleaved)
         dg, = torch.autograd.grad(y, leaves[:1], bad)
         assert torch.isfinite(dg[others(c)]).all() and not torch.isfinite(dg[c])
+
+
+def test_forward_mode_derivatives_are_refused(monkeypatch):
+    """None of these operators has one: a tensor with a tangent is an error, with and without recorded gradients, and so is a tangent on
+    the gradient that comes back.  (The launches are left out: this is the host's side.)"""
+    from torch.autograd import forward_ad
+    from tmae_amd import ops
+    monkeypatch.setattr(ops, '_need_cuda', lambda t: None)
+    monkeypatch.setattr(ops, '_launch', lambda *a: None)
+    pos, f, grid = torch.zeros(64, 2, dtype=torch.int32), ops.rotary_freqs((4, 4)), torch.arange(64, dtype=torch.int32)
+    gain = torch.ones(16)
+    calls = [(lambda t: ops.rotary_axes(t.view(64, 3, 16), pos, f, (4, 4)), (64, 48)),
+             (lambda t: ops.qk_norm_rotary(t.view(64, 3, 16), gain, gain, pos, f, (4, 4), q_heads=2), (64, 48)),
+             (lambda t: ops.qk_norm_rotary(torch.ones(64, 3, 16), t, gain, pos, f, (4, 4), q_heads=2), (16,)),
+             (lambda t: ops.win_attn_dot(t, None, None, grid, grid, 1, 1, 8, 8, False), (64, 48)),
+             (lambda t: ops.win_attn_dot(torch.ones(64, 32), t, None, grid, grid, 1, 1, 8, 8, False), (64, 16))]
+    for call, shape in calls:
+        plain = torch.ones(shape)
+        assert call(plain) is not None
+        with forward_ad.dual_level():
+            assert call(plain) is not None
+            for leaf in (plain, plain.clone().requires_grad_()):
+                with pytest.raises((RuntimeError, NotImplementedError), match='forward'):
+                    call(forward_ad.make_dual(leaf, plain))
+                with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError), match='forward'):
+                    call(forward_ad.make_dual(leaf, plain))
+            leaf = plain.clone().requires_grad_()
+            y = call(leaf)
+            torch.autograd.grad(y, leaf, torch.ones_like(y), retain_graph=True)
+            with pytest.raises((RuntimeError, NotImplementedError), match='forward'):
+                torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
