@@ -1843,7 +1843,8 @@ def _rotary_args(name, x, positions, inv_freq, sections):
     if x.stride(2) != 1 and dh > 1:
         x = x.contiguous()
     if positions.stride(1) != 1 and len(sections) > 1 or positions.stride(0) < len(sections):
-        positions = positions.contiguous()
+        # one token (or none) is contiguous whatever the stride over it, which goes on as the pitch
+        positions = positions.contiguous() if n > 1 else positions.flatten().contiguous().view(n, len(sections))
     return x, positions, inv_freq.contiguous(), arr, P
 
 

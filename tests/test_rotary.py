@@ -455,3 +455,34 @@ def test_forward_mode_derivatives_are_refused(monkeypatch):
             torch.autograd.grad(y, leaf, torch.ones_like(y), retain_graph=True)
             with pytest.raises((RuntimeError, NotImplementedError), match='forward'):
                 torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+def test_the_pitch_of_one_tokens_positions(monkeypatch):
+    """The stride over a single token (or none) says nothing: transposed positions of one token have 1 there."""
+    from tmae_amd import ops
+    monkeypatch.setattr(ops, '_need_cuda', lambda t: None)
+    seen = []
+    monkeypatch.setattr(ops, '_launch', lambda entry, dev, *a: seen.append((entry.__name__, a)))
+    f, parts = ops.rotary_freqs((4, 5, 7)), [torch.tensor([t], dtype=torch.int32) for t in (3, 1, 4)]
+    for n, pos in ((1, torch.stack(parts).t()), (1, torch.stack(parts, 1)), (1, torch.arange(9).view(1, 9)[:, ::4]),
+                   (0, torch.zeros(3, 0, dtype=torch.int32).t())):
+        assert pos.shape == (n, 3)
+        x = torch.ones(n, 2, 32, requires_grad=True)
+        for y in (ops.rotary_axes(x, pos, f, (4, 5, 7)), ops.qk_norm_rotary(x, None, None, pos, f, (4, 5, 7))):
+            torch.autograd.grad(y, x, torch.ones_like(y))
+        at = {'tmae_rotary_axes': 9, 'tmae_qk_norm_rotary_fwd': 14, 'tmae_qk_norm_rotary_bwd': 15}         # ldpos
+        assert len(seen) == 4 and all(a[at[name]] >= 3 for name, a in seen), [(name, a[at[name]]) for name, a in seen]
+        seen.clear()
+
+
+@pytest.mark.gpu
+def test_one_tokens_positions_transposed():
+    from tmae_amd import ops
+    f = ops.rotary_freqs((4, 5, 7), device='cuda')
+    x = torch.randn(1, 2, 32, device='cuda')
+    parts = [torch.tensor([t], dtype=torch.int32, device='cuda') for t in (3, 1, 4)]
+    apart = torch.arange(9, device='cuda').view(1, 9)[:, ::4]
+    for pos in (torch.stack(parts).t(), apart):
+        plain = pos.clone(memory_format=torch.contiguous_format).reshape(-1).clone().view(1, 3)
+        assert torch.equal(ops.rotary_axes(x, pos, f, (4, 5, 7)), ops.rotary_axes(x, plain, f, (4, 5, 7)))
+        assert torch.equal(ops.qk_norm_rotary(x, None, None, pos, f, (4, 5, 7)), ops.qk_norm_rotary(x, None, None, plain, f, (4, 5, 7)))
