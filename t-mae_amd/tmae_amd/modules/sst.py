@@ -89,7 +89,8 @@ class CosineMultiheadAttention(nn.Module):
         """rows [m, d] (queries or keys) or [m, 2 d] (both) of plan's voxels, normalised and turned by their positions."""
         f = self._freqs.get(rows.device)
         if f is None:
-            f = self._freqs[rows.device] = ops.rotary_freqs(self.sections, self.base, rows.device)
+            with torch.inference_mode(False):        # (kept from the first call on: a training step's backward takes it as well)
+                f = self._freqs[rows.device] = ops.rotary_freqs(self.sections, self.base, rows.device)
         heads = rows.view(rows.shape[0], rows.shape[1] // self.head_dim, self.head_dim)
         pos = plan.positions(len(self.sections), time)
         if not self.qk_norm:

@@ -826,3 +826,19 @@ def test_a_key_that_infinity_masks(heads, dh, dtype):
                 channels = torch.arange(dh) if what != 'dq' else torch.tensor([c for c in range(dh) if c != 3])
                 assert torch.isfinite(got[:, [c for c in range(d) if what != 'dq' or c != 3]]).all(), what
                 within(got[tail][:, channels], w[:, channels], t[:, channels], what)
+
+
+def test_frequencies_made_in_inference_mode_serve_training(monkeypatch):
+    """The layer keeps its frequencies from the first call on; made in inference mode they would be refused by the first recorded one."""
+    from types import SimpleNamespace
+    from tmae_amd import ops
+    from tmae_amd.modules.sst import WindowAttention
+    seen = []
+    monkeypatch.setattr(ops, 'rotary_axes', lambda heads, pos, f, sections: seen.append(f) or heads)
+    a = WindowAttention(128, 8, 0.0, {'cosine': False, 'rotary': {'SECTIONS': [4, 4]}}).self_attn
+    plan = SimpleNamespace(positions=lambda axes, time=0: torch.zeros(3, axes, dtype=torch.int32))
+    with torch.inference_mode():
+        a.turn(torch.zeros(3, 256), plan, True, True)
+    a.turn(torch.zeros(3, 256, requires_grad=True), plan, True, True)
+    assert len(seen) == 2 and not any(f.is_inference() for f in seen)
+    assert torch.equal(seen[0], ops.rotary_freqs((4, 4), 100.0))
