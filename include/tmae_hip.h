@@ -616,7 +616,7 @@ int tmae_frame_prepare_boxes(const float* points, int row, int64_t n, const doub
 /* ---- rotary positions with several axes; norms of queries and keys for each head with the rotation in the same pass -----------
  * x [n, h, dh] (row pitch ldx, head pitch hpx, in elements; channels contiguous), y / dy / dx contiguous [n, h, dh].  Channel pair i
  * < P = sum of `sections` (host array of `axes` <= 4 counts, 2 P <= dh <= 512) turns by theta = positions[n, axis(i)] * inv_freq[i]
- * (inv_freq [P] float64, the product and its reduction in float64): pair i = channels (2i, 2i+1) if `interleaved`, else (i, i + P);
+ * (inv_freq [P] float64, the product in float64, reduced whatever its size): pair i = channels (2i, 2i+1) if `interleaved`, else (i, i + P);
  * axis(i) by the sections in order; channels >= 2 P pass.  positions [n, axes] with row pitch ldpos: pos_kind 0 int32, 1 int64,
  * 2 float32.  inverse: by -theta (the gradient of the rotation).  x and y do not overlap. */
 int tmae_rotary_axes(const void* x, int64_t ldx, int64_t hpx, int dtype, int64_t n, int h, int dh, const void* positions, int pos_kind,

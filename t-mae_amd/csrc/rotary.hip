@@ -1,6 +1,6 @@
 // Rotary positions with several axes, and the norms of queries and keys for each head with the rotation in the same pass.
 //
-//   theta[n, i] = positions[n, axis(i)] * inv_freq[i]                 (double: positions may be far, the angle is reduced exactly)
+//   theta[n, i] = positions[n, axis(i)] * inv_freq[i]                 (double: positions may be far)
 //   rotation of pair i:  a' = a cos - b sin,  b' = a sin + b cos      (a, b) = channels (2i, 2i+1) or (i, i + P); the rest passes
 //   norm of a head:      xh = x * rsqrt(mean_c x^2 + eps),  y = rotate(gain * xh)
 //   its gradient, with dz = rotate^-1(dy), t = gain * dz, r = rsqrt(mean_c x^2 + eps):
@@ -42,13 +42,51 @@ struct RotaryArgs {
   float* part;                             // backward: partial rows of the gain gradient
 };
 
-// cos and sin of pos * w to float32 accuracy whatever the size of the product: k = the nearest multiple of pi/2, the remainder by two
-// fused multiply-adds with the two halves of pi/2, Taylor series on [-pi/4, pi/4] (first dropped terms 2e-9 and 2e-9).
+// 2 / pi, the 32 bits before the binary point and 1120 behind it
+__constant__ uint32_t TWO_OVER_PI[36] = {
+    0x00000000u, 0xa2f9836eu, 0x4e441529u, 0xfc2757d1u, 0xf534ddc0u, 0xdb629599u, 0x3c439041u, 0xfe5163abu, 0xdebbc561u,
+    0xb7246e3au, 0x424dd2e0u, 0x06492eeau, 0x09d1921cu, 0xfe1deb1cu, 0xb129a73eu, 0xe88235f5u, 0x2ebb4484u, 0xe99c7026u,
+    0xb45f7e41u, 0x3991d639u, 0x835339f4u, 0x9c845f8bu, 0xbdf9283bu, 0x1ff897ffu, 0xde05980fu, 0xef2f118bu, 0x5a0a6d1fu,
+    0x6d367ecfu, 0x27cb09b7u, 0x4f463f66u, 0x9e5fea2du, 0x7527bac7u, 0xebe5f17bu, 0x3d0739f7u, 0x8a5292eau, 0x6bfb5fb1u};
+// theta = m 2^e in multiples of pi/2, for 2^22 <= |theta| (Payne and Hanek's reduction): bits of 2 / pi that make multiples of 4 with m 2^e are
+// left out, the 128 behind them hold the multiple's last two bits and, after the product with m, 70 bits and more of its fraction.  Sets
+// k to the multiple modulo 4 and returns the rest as an angle; no angle for infinities and NaN.
+__device__ __forceinline__ double far_angle(double theta, int& k) {
+  const uint64_t bits = (uint64_t)__double_as_longlong(theta);
+  const int exponent = (int)(bits >> 52) & 0x7ff;
+  if (exponent == 0x7ff) return __longlong_as_double(0x7ff8000000000000ll);
+  const uint64_t m = (bits & 0xfffffffffffffull) | 0x10000000000000ull;
+  const int first = exponent - 1075 + 30, word = first >> 5, shift = first & 31;       // the first bit that counts: at most 1001
+  uint64_t hi = (uint64_t)TWO_OVER_PI[word] << 32 | TWO_OVER_PI[word + 1], lo = (uint64_t)TWO_OVER_PI[word + 2] << 32 | TWO_OVER_PI[word + 3];
+  const uint64_t next = (uint64_t)TWO_OVER_PI[word + 4] << 32;
+  if (shift) {
+    hi = hi << shift | lo >> (64 - shift);
+    lo = lo << shift | next >> (64 - shift);
+  }
+  hi = __umul64hi(m, lo) + m * hi;
+  lo = m * lo;
+  const int64_t fraction = (int64_t)(hi << 2 | lo >> 62);                            // above a half: the next multiple, and back from it
+  const int n = (int)(hi >> 62) + (fraction < 0 ? 1 : 0);
+  const double angle = (double)fraction * (1.57079632679489661923 * 0x1p-64);
+  k = (theta < 0 ? -n : n) & 3;
+  return theta < 0 ? -angle : angle;
+}
+
+// cos and sin of the float64 product pos * w to float32 accuracy, Taylor series on [-pi/4, pi/4] (first dropped terms 2e-9 and 1e-10).  Up to
+// 2^45: k = the nearest multiple of pi/2 (near enough: the remainder leaves that interval by less than 0.01), the remainder by two fused
+// multiply-adds with the two halves of pi/2, of which 2^-108 is missing.  Beyond, a double has no place for k.
 __device__ __forceinline__ float2 cos_sin(double pos, double w) {
   const double theta = pos * w;
-  const double k = rint(theta * 0.63661977236758134308);
-  double rem = fma(-k, 1.57079632679489661923, theta);
-  rem = fma(-k, 6.12323399573676603587e-17, rem);
+  double rem;
+  int q = 0;
+  if (fabs(theta) <= 0x1p45) {
+    const double k = rint(theta * 0.63661977236758134308);
+    rem = fma(-k, 1.57079632679489661923, theta);
+    rem = fma(-k, 6.12323399573676603587e-17, rem);
+    q = (int)(k - 4.0 * floor(k * 0.25));
+  } else {
+    rem = far_angle(theta, q);
+  }
   const float x = (float)rem, x2 = x * x;
   float s = fmaf(x2, 2.755731922e-6f, -1.984126984e-4f);
   s = fmaf(x2, s, 8.333333333e-3f);
@@ -58,7 +96,6 @@ __device__ __forceinline__ float2 cos_sin(double pos, double w) {
   c = fmaf(x2, c, -1.388888889e-3f);
   c = fmaf(x2, c, 4.166666667e-2f);
   c = fmaf(x2 * x2, c, fmaf(x2, -0.5f, 1.0f));
-  const int q = (int)(k - 4.0 * floor(k * 0.25));
   const float cc = (q & 1) ? s : c, ss = (q & 1) ? c : s;
   return make_float2((q == 1 || q == 2) ? -cc : cc, (q >= 2) ? -ss : ss);
 }

@@ -1880,7 +1880,8 @@ def rotary_axes(x, positions, inv_freq, sections, interleaved=False, inverse=Fal
 
     Channel pair i < P = sum(sections) turns by positions[:, axis(i)] * inv_freq[i]; the first sections[0] pairs belong to axis 0
     and so on.  Pair i is channels (2i, 2i+1) if `interleaved`, else (i, i + P); channels from 2 P on pass unchanged.
-    positions [tokens, len(sections)] int32 / int64 / float32, inv_freq [P] float64 (rotary_freqs).  inverse: turns back."""
+    positions [tokens, len(sections)] int32 / int64 / float32, inv_freq [P] float64 (rotary_freqs); the angle is their product in float64 (an
+    int64 beyond 2^53 is rounded to it), of any size.  inverse: turns back."""
     x, positions, inv_freq, arr, _ = _rotary_args('rotary_axes', x, positions, inv_freq, sections)
     _need_cuda(x)
     if _grad_on(x):

@@ -486,3 +486,36 @@ def test_one_tokens_positions_transposed():
         plain = pos.clone(memory_format=torch.contiguous_format).reshape(-1).clone().view(1, 3)
         assert torch.equal(ops.rotary_axes(x, pos, f, (4, 5, 7)), ops.rotary_axes(x, plain, f, (4, 5, 7)))
         assert torch.equal(ops.qk_norm_rotary(x, None, None, pos, f, (4, 5, 7)), ops.qk_norm_rotary(x, None, None, plain, f, (4, 5, 7)))
+
+
+@pytest.mark.gpu
+def test_angles_of_any_size():
+    """Positions up to the ends of their types: the pair (1, 0) turns into the cosine and sine of the float64 product.  Their error is that
+    of any angle (2 u); infinities and NaN have no angle."""
+    import math
+    from tmae_amd import ops
+    g = torch.Generator().manual_seed(12)
+    sections = (3, 2)
+    f = ops.rotary_freqs(sections, 100.0)
+    f[4] = 3e5                                                                          # (the frequencies are the caller's)
+    big = torch.randint(-(1 << 62), 1 << 62, (400, 2), generator=g)
+    stamps = 1_700_000_000_000_000_000 + torch.randint(0, 1 << 50, (400, 2), generator=g)
+    ends = torch.tensor([[(1 << 63) - 1, -(1 << 63)], [1 << 53, (1 << 53) + 2], [0, 1], [(1 << 45) - 1, 1 << 45], [-(1 << 45), 1 << 46]])
+    ladder = torch.tensor([[1 << s, -(1 << s) - 1] for s in range(63)])
+    sizes = torch.rand(900, 2, generator=g) * 38
+    floats = (10.0 ** sizes).float() * (torch.randint(0, 2, (900, 2), generator=g) * 2 - 1)
+    edges = torch.tensor([[3.4028234e38, -3.4028234e38], [1e-30, 0.0], [2.0 ** 45, 2.0 ** 44], [1e30, 1.765e18]])
+    for pos in (torch.cat([big, stamps, ends, ladder]), torch.cat([floats, edges])):
+        n = pos.shape[0]
+        theta = (pos.double()[:, [0, 0, 0, 1, 1]] * f[None]).tolist()
+        want = torch.tensor([[[math.cos(t), math.sin(t)] for t in row] for row in theta], dtype=torch.float64)
+        for interleaved in (False, True):
+            x = torch.zeros(n, 1, 10)
+            x[..., 0::2 if interleaved else 1][..., :5] = 1.0
+            y = ops.rotary_axes(x.cuda(), pos.cuda(), f.cuda(), sections, interleaved=interleaved).cpu()[:, 0].double()
+            got = torch.stack([y[:, 0::2], y[:, 1::2]], -1) if interleaved else torch.stack([y[:, :5], y[:, 5:]], -1)
+            assert (got.abs() <= 1 + 2 * U).all()
+            assert ((got - want).abs() <= 2 * U).all(), float((got - want).abs().max() / U)
+    pos = torch.tensor([[float('inf'), 1.0], [1.0, -float('inf')], [float('nan'), 1.0], [1.0, 1.0]])
+    y = ops.rotary_axes(torch.ones(4, 1, 10, device='cuda'), pos.cuda(), f.cuda(), sections, interleaved=True).cpu()[:, 0]
+    assert torch.equal(y.isnan(), torch.tensor([[True] * 6 + [False] * 4, [False] * 6 + [True] * 4, [True] * 6 + [False] * 4, [False] * 10]))
