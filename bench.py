@@ -66,11 +66,12 @@ def parse():
 
 
 def _pmc_files():
-    """Committed counter passes of `bench.py --probe-hbm-only` (profiles/roundN_pmc.json), latest round first."""
+    """Committed counter passes of `bench.py --probe-hbm-only`: profiles/probe_pmc.json, then the older roundN_pmc.json, latest first."""
     import glob
     import re
     fs = glob.glob(os.path.join(ROOT, 'profiles', 'round*_pmc.json'))
-    return sorted(fs, key=lambda f: -int(re.search(r'round(\d+)_pmc', f).group(1)))
+    fs = sorted(fs, key=lambda f: -int(re.search(r'round(\d+)_pmc', f).group(1)))
+    return glob.glob(os.path.join(ROOT, 'profiles', 'probe_pmc.json')) + fs
 
 
 _PMC_FILES = {'token_gemm': 'token_gemm_wreg.hip', 'token_gemm_gelu': 'token_gemm_wreg.hip', 'wgrad': 'wgrad.hip',
