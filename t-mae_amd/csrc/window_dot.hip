@@ -7,13 +7,14 @@
 //
 // Tiles of 16 tokens.  A logit tile is computed with the keys as its rows and the queries as its columns: the accumulators' layout --
 // lane (g, i) = (lane >> 4, lane & 15) holds rows 4g .. 4g+3 of column i -- is also what the next product takes as its B operand, row
-// 4g + r in step r, so that the probabilities go into it without leaving the registers (float32 whole, bfloat16 rounded or as a sum of two).
+// 4g + r in step r, so that the probabilities go into it without leaving the registers (float32 whole, bfloat16 as the sum of two).
 //
-// Bound: HBM, at 8 to 20 FLOPs a byte; but rows lie apart and windows are small, so what costs is getting rows in and out.  The lanes of an
-// operand stand in 16 rows: read straight into that layout, an instruction touches some 44 lines.  Rows therefore travel in 16-byte
-// pieces, whole pieces of a line by neighbouring lanes, through LDS images; all of a window's rows are requested at once.  Padding rows to
-// tiles is what the matrix unit pays for; three sizes of windows (up to 16, 32 and 64 tokens) keep it small.  Eight frames at stage 1
-// (375 k tokens, 8 heads of 16, bfloat16): forward 111 us, backward 217 us.
+// Bound: HBM, at 14 to 24 FLOPs a byte; but rows lie apart and windows are small, so what costs is getting rows in and out.  The lanes of an
+// operand stand in 16 rows: read straight into that layout, an instruction touches a line for every few lanes.  Rows therefore travel in
+// 16-byte pieces, whole pieces of a line by neighbouring lanes, through LDS images; all of a window's rows are requested at once.  Padding
+// rows to tiles is what the matrix unit pays for; three sizes of windows (up to 16, 32 and 64 tokens) keep it small.  Eight frames at stage 1
+// (375 k tokens, 8 heads of 16, bfloat16): forward 104 us, backward 187 us, 4.2 and 3.9 TB/s of counted HBM traffic (110 and 223 us with a
+// profiler's trace around every launch; the comparisons below are of traced launches).
 //
 // A slot behind a window's last token stands for its first one: it is read, its probability is set to 0 (and V and dO are zeros there,
 // which an infinity next to them needs), and nothing is stored for it.
@@ -367,15 +368,14 @@ __global__ __launch_bounds__(256) void dot_orphan_kernel(DotArgs a, Orphans z) {
 
 // ------------------------------------------------------------------------------------------------------------------ bfloat16
 // The same products on the bfloat16 matrix instructions.  Their operands want the 16 rows of a tile in 16 neighbouring lanes: loaded that
-// way straight from the tensors, each instruction touches 16 lines per 16 lanes and the cache's tag port is what the kernels wait for
-// (44 accesses per instruction, busy 2/3 of the time; 8-byte pieces of 16 rows).  So rows travel in 16-byte chunks, neighbouring lanes
-// on neighbouring chunks, into row images in LDS, and the operands are read there: pieces of a row for the products over the channels
-// (logits, dP), columns (ds_read_b64_tr_b16 returns four rows of one column) for the products over tokens.  Results go back the same
-// way: into the image, and out in whole rows.
+// way straight from the tensors, each instruction touches 16 lines per 16 lanes, and the first kernels waited for that.  So rows travel in
+// 16-byte chunks, neighbouring lanes on neighbouring chunks, into row images in LDS, and the operands are read there: pieces of a row for
+// the products over the channels (logits, dP), columns (ds_read_b64_tr_b16 returns four rows of one column) for the products over tokens.
+// Results go back the same way: into the image, and out in whole rows.
 //
 // P and dS enter their products as the sum of two bfloat16 each (2^-15 of a probability, 2^-16 of dS; sums, maxima and everything else stay
 // float32): the results' error is that of their own rounding.  Rounded to one bfloat16 they would add as much again (2-norms: 0.0024 of the
-// gradients, not 0.0017) and save 30 of 217 us of the backward at stage 1, 5 of 85 across frames of stage 2.
+// gradients, not 0.0017) and save 35 of 220 us of the backward at stage 1, 6 of 85 across frames of stage 2.
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -702,8 +702,8 @@ __device__ __forceinline__ void bwd_window(const DotArgs& a, int Tq, int Tk, cha
   }
 }
 
-// Windows of up to 16 NT tokens; without a work list (NT = 4) every window, empty ones included.  Two waves per SIMD as the bound: 256
-// registers at most, and the matrix instructions then write plain vector registers (the backward of 64 channels by 64 tokens needs more).
+// Windows of up to 16 NT tokens; without a work list (NT = 4) every window, empty ones included.  From two waves per SIMD on, 256 registers at
+// most, the matrix instructions write plain vector registers (the backward of 64 channels by 64 tokens needs more: kernel_waves).
 template <int DH, int NT, bool BWD> constexpr int window_lds() { return (BWD ? 3 : 2) * Window<DH, NT>::IMAGE + (BWD ? 2 * WEIGHT_BYTES : 0); }
 template <int DH, int NT, bool BWD> __device__ __forceinline__ void window_role(const DotArgs& a, int first, int step, int head0, int (*toks)[64], char* images) {
   using W = Window<DH, NT>;
@@ -979,9 +979,10 @@ __global__ __launch_bounds__(256, (kernel_waves<DH, BWD, ROLES>())) void dot_ker
 }
 
 // Workgroups along the windows: what the windows can need, at most `per_cu` per CU in all -- a little more than what is resident at
-// once.  Fewer leave the last windows to a few workgroups (4: the backward of the large windows 84 us, not 75, at stage 1); more spend
-// their time on workgroups that find no window (12: that of the others 51 us, not 46, at stage 2).  Neighbouring windows on the same die
-// would share the grids' lines in its L2, but the dense windows are neighbours too: one die would have them all (49 us, not 39).
+// once.  In bfloat16 6 take 111 + 223 us forward and backward at stage 1, 4 take 114 + 228 (the last windows are left to few workgroups),
+// 12 take 114 + 230 (some find no window); across frames of stage 2 43 + 86, 41 + 83 and 50 + 96.  Neighbouring windows on the same die
+// would share the grids' lines in its L2, but the dense windows are neighbours too: one die would have them all (49 us, not 39, for the
+// small and middle windows of stage 2's backward).
 unsigned walkers(int64_t windows, int per_group, unsigned gx, int per_cu = 6) {
   const int64_t need = (windows + per_group - 1) / per_group;
   int64_t most = (int64_t)tmae_num_cus() * per_cu / gx;
