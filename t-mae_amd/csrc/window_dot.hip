@@ -452,7 +452,8 @@ template <int DH, int PITCH> struct Rows {
 // Probabilities and their gradients on the way into the products over the tokens: as the sum of two bfloat16, 16 bits and more.  The
 // instruction takes 32 tokens; where a tile has 16 the low parts ride in its second half.  Probabilities are split towards 0 and the low
 // part of one above 0 stays above it (the median of the rest, the smallest normal number and the probability), so that an infinity in V or
-// dO meets two positive numbers; of 0 both parts are 0.
+// dO meets two positive numbers; of 0 both parts are 0.  dS is rounded to the nearest, and the rest of an infinity (a NaN, of which the median
+// makes a finite number) leaves it one.
 struct Split { s16x4 hi, lo; };
 __device__ __forceinline__ Split probabilities(const f32x4& p) {
   u32x4 cut;
@@ -467,7 +468,10 @@ __device__ __forceinline__ Split probabilities(const f32x4& p) {
 __device__ __forceinline__ Split gradients(const f32x4& d) {
   const u32x2 h = {pack2(d[0], d[1]), pack2(d[2], d[3])};
   const f32x4 near = {__uint_as_float(h[0] << 16), __uint_as_float(h[0] & 0xffff0000u), __uint_as_float(h[1] << 16), __uint_as_float(h[1] & 0xffff0000u)};
-  return Split{__builtin_bit_cast(s16x4, h), pack4(d - near)};
+  f32x4 rest = d - near;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) rest[r] = __builtin_amdgcn_fmed3f(rest[r], -0x1p120f, 0x1p120f);           // finite beside an infinity
+  return Split{__builtin_bit_cast(s16x4, h), pack4(rest)};
 }
 __device__ __forceinline__ f32x4 product32(const s16x4& a0, const s16x4& a1, const s16x4& b0, const s16x4& b1, f32x4 c) {
   const s16x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7), b = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);

@@ -842,3 +842,40 @@ def test_frequencies_made_in_inference_mode_serve_training(monkeypatch):
     a.turn(torch.zeros(3, 256, requires_grad=True), plan, True, True)
     assert len(seen) == 2 and not any(f.is_inference() for f in seen)
     assert torch.equal(seen[0], ops.rotary_freqs((4, 4), 100.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('heads,dh', [(5, 16), (2, 32), (1, 64)])
+def test_an_infinite_gradient_of_a_probability_stays_one(heads, dh, dtype):
+    """One query a window, V of one of its keys infinite in one channel: dP of that key is infinite, so is sum_j P dP, and dS of every other
+    key is the opposite infinity: dK of those is that times the query, an infinity of a known sign in every channel of the head."""
+    from tmae_amd import ops
+    g = torch.Generator().manual_seed(heads)
+    batch, ny, d = 2, 40, heads * dh
+    for count in (300, 900, 1600):
+        grid_k, at_k = place([count] * batch, batch, ny, ny, g)
+        win = window_of(at_k, False)
+        homes = win.unique()
+        homes = homes[torch.tensor([int((win == w).sum()) > 1 for w in homes])]
+        first = torch.stack([(win == w).nonzero()[0, 0] for w in homes])                # the query stands in the cell of a key
+        grid_q = torch.full_like(grid_k, -1)
+        grid_q[at_k[first, 0] * ny * ny + at_k[first, 1] * ny + at_k[first, 2]] = torch.arange(len(homes), dtype=torch.int32)
+        mq, mk = len(homes), at_k.shape[0]
+        q, do = (torch.randn(mq, d, generator=g).to(dtype) for _ in range(2))
+        k, v = (torch.randn(mk, d, generator=g).to(dtype) for _ in range(2))
+        bad = torch.stack([(win == w).nonzero()[-1, 0] for w in homes])
+        v[bad, 3] = float('inf')
+        of = torch.full((mk,), -1, dtype=torch.long)
+        for i, w in enumerate(homes):
+            of[win == w] = i
+        rest = of >= 0
+        rest[bad] = False
+        sign = -torch.sign(do[of[rest], 3].float())[:, None] * torch.sign(q[of[rest], :dh].float())
+        gq, gk = grid_q.cuda(), grid_k.cuda()
+        for worklist in (None, ops.window_worklist(gq, gk, batch, ny, ny, False)):
+            leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+            o = ops.win_attn_dot(*leaves, gq, gk, heads, batch, ny, ny, False, worklist=worklist, covered=True)
+            dk, dv = (t.cpu().float() for t in torch.autograd.grad(o, leaves[1:], do.cuda()))
+            assert torch.equal(dk[rest][:, :dh], sign * float('inf'))
+            assert torch.isfinite(dk[:, dh:]).all() and torch.isfinite(dv).all()
